@@ -362,6 +362,131 @@ int se12_encode_bitmap(const uint8_t* tile_fallback_dev, int tiles, uint8_t* bit
 int se12_encode_raw(const uint16_t* w_dev, int rows, int cols, int ldw, const int32_t* fallback_index_dev,
                     int16_t* raw_dev, void* stream);
 
+/*
+ * The decode step around the GEMVs: a paged 8-bit key/value cache, attention
+ * over it, and log probabilities of the LM head's logits. No counterpart in
+ * the reference, which has the GEMV only. All of them are asynchronous on
+ * `stream`, allocate nothing and can be captured in a graph; lengths, page
+ * tables and token ids are read on the device, so a captured call follows
+ * their contents. What a kernel finds out of range there (a page id, a
+ * position beyond the page table or the rotation table, a token id beyond the
+ * vocabulary) is skipped and sets bit 1 of se12_device_status.
+ *
+ * A cache holds one layer's keys and values. A block is one page of one KV
+ * head: page_size codes rows of head_dim bytes and one fp32 scale; a value is
+ * code * scale. page_size: 16, 32, 64, 128 or 256; head_dim: a multiple of 16
+ * up to 256; kind: int8 (codes -127..127) or e4m3 bit patterns.
+ *   codes:  [pages][kv_heads][page_size][head_dim] u8, 16-byte aligned
+ *   scales: [pages][kv_heads] fp32
+ * The handle keeps the pointers and TMA descriptors; it holds no device memory.
+ */
+#define SE12_KV_INT8 0
+#define SE12_KV_E4M3 1
+#define SE12_KV_MAX_SEQS 2048
+
+typedef struct se12_kv_pages {
+  int32_t pages, page_size, kv_heads, head_dim;
+  int32_t kind;
+  void* k_codes;
+  void* v_codes;
+  float* k_scales;
+  float* v_scales;
+} se12_kv_pages;
+
+typedef struct se12_kv_cache se12_kv_cache;
+
+int se12_kv_cache_create(const se12_kv_pages* pages, se12_kv_cache** out);
+void se12_kv_cache_destroy(se12_kv_cache* cache);
+
+/* A ragged batch of new tokens. Sequence b's are the rows query_start[b] ..
+ * query_start[b + 1] - 1 of the token arrays, at positions lens[b] - count ..
+ * lens[b] - 1 of its sequence: lens counts the new tokens. query_start null:
+ * one token per sequence (tokens == seqs). A row at a negative position is
+ * inactive (a padding row: lens[b] == 0): nothing is stored for it and its
+ * outputs are zero. Position p is slot p % page_size of page
+ * block_table[b][p / page_size]; entries past the length are not read.
+ * seqs <= SE12_KV_MAX_SEQS. */
+typedef struct se12_kv_batch {
+  int32_t seqs, tokens;
+  const int32_t* lens;         /* device [seqs] */
+  const int32_t* query_start;  /* device [seqs + 1], or null */
+  const int32_t* block_table;  /* device [seqs][table_stride] */
+  int64_t table_stride;
+  int32_t max_pages;           /* columns of block_table */
+} se12_kv_batch;
+
+/* Appends the batch's keys and values (fp32 or BF16, rows of head_dim values
+ * at k + token * k_token_stride + head * k_head_stride) and, with q, writes
+ * the queries, rotated, as BF16. Keys and queries are rotated by their
+ * positions: cos and sin are fp32 [rope_rows][rope_stride], rotary_dim / 2
+ * columns used; the pair (x1, x2) becomes (x1 cos - x2 sin, x2 cos + x1 sin),
+ * pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved. cos null:
+ * no rotation. A block's scale is the least power of two, 2^-100 at least,
+ * that holds its tokens; when a token raises it, the block's older codes are
+ * rounded again at the new scale. A block that receives a value that is not
+ * finite gets the scale NaN, which attention over it returns, until the page
+ * starts anew. Two sequences of a call must not append to one page. */
+typedef struct se12_kv_append_args {
+  int32_t bf16;                /* 0: q, k, v are fp32; 1: BF16 */
+  int32_t q_heads;
+  const void* q;               /* or null */
+  const void* k;
+  const void* v;
+  int64_t q_token_stride, q_head_stride;  /* elements */
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  const float* cos;
+  const float* sin;
+  int64_t rope_stride;
+  int32_t rope_rows, rotary_dim, interleaved;
+  uint16_t* q_out;             /* BF16 */
+  int64_t q_out_token_stride, q_out_head_stride;
+} se12_kv_append_args;
+
+int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_append_args* args, void* stream);
+
+/* Attention of the batch's rows over their sequences:
+ *   out_i = sum_j softmax_j(s_ij) v_j, s_ij = scale q_i . k_j, then, with
+ *   softcap > 0, softcap * tanh(s_ij / softcap);
+ * a row at position p sees the positions j <= p, with window > 0 only those
+ * with p - j < window. A row that sees nothing is zero. q and out: BF16
+ * [tokens][q_heads][head_dim] with token and head strides; query head h uses
+ * KV head h / (q_heads / kv_heads). max_query: the largest number of rows of a
+ * sequence. The workspace is zeroed once (se12_workspace_clear); every
+ * completed call leaves it ready for the next, and calls that may overlap on
+ * the GPU need separate ones. */
+typedef struct se12_kv_attend_args {
+  const uint16_t* q;
+  int64_t q_token_stride, q_head_stride;  /* elements */
+  uint16_t* out;
+  int64_t out_token_stride, out_head_stride;
+  int32_t q_heads, max_query, window;
+  float scale, softcap;
+} se12_kv_attend_args;
+
+size_t se12_kv_attend_workspace_bytes(const se12_kv_cache* cache);
+int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_attend_args* args,
+                   void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* Pages read back as BF16 (exact): page ids pages_dev[0 .. count - 1], or the
+ * first `count` pages where it is null, into k_out and v_out
+ * [count][kv_heads][page_size][head_dim], 16-byte aligned. */
+int se12_kv_decode(const se12_kv_cache* cache, const int32_t* pages_dev, int count, uint16_t* k_out, uint16_t* v_out,
+                   void* stream);
+
+/* Log probabilities over rows of logits (fp32 or BF16, `ld` elements apart):
+ * logprob[i] of token tokens[i] (a negative id: none, NaN), the entropy of the
+ * row's distribution, and the `top` (0 .. SE12_LOGPROBS_MAX_TOP) largest
+ * logits' ids and log probabilities, ties to the lowest id. With softcap > 0
+ * the logits are softcap * tanh(x / softcap), -inf staying -inf. A NaN or +inf
+ * in a row, or nothing but -inf, makes its log probabilities and entropy NaN.
+ * Workspace as for se12_kv_attend. */
+#define SE12_LOGPROBS_MAX_TOP 32
+size_t se12_token_logprobs_workspace_bytes(void);
+int se12_token_logprobs(const void* logits_dev, int bf16, int rows, int vocab, int64_t ld, const int64_t* tokens_dev,
+                        int top, float softcap, float* logprob_dev, float* entropy_dev, int64_t* top_ids_dev,
+                        float* top_logprobs_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+
 /* Device status word (bit 0: a bounded wait timed out, bit 1: bad argument
  * seen by a kernel). Reading it synchronises with the device. While bit 0 is
  * set, the waits on other CTAs' and other GPUs' progress give up at once

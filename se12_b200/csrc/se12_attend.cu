@@ -1,0 +1,715 @@
+// Attention over the paged 8-bit cache for few query rows per KV head (next
+// tokens, drafted tokens): split over the tokens, joined in the same launch.
+//
+//   s_ij = scale * ks_j * (q_i . kc_j)          kc, vc: codes; ks, vs: scales
+//   o_i  = sum_j exp(s_ij) vs_j vc_j / sum_j exp(s_ij)
+//
+// The codes never become values: a code is exact in FP16, the scales
+// multiply the logits and the probabilities, and q enters as FP16 times a
+// power of two per row (a BF16 row fits without loss but for elements below
+// 2^-16 of its largest).
+//
+// Work is the list of all (sequence, KV head, row tile, chunk of tokens), a
+// chunk being 8 KB of keys and values, cut into equal runs, one per CTA; the
+// list comes from the lengths in device memory, so that the launch does not
+// depend on them (a captured graph follows the lengths) and a ragged batch
+// is balanced to a chunk. A CTA's 8 warps take its chunks in turn, each
+// with a pipeline of its own (3 stages filled by TMA, 192 KB per SM in
+// flight or in work: no CTA-wide barrier inside a run) and its own running
+// maxima and sums; a pair's warps are joined in shared memory, its CTAs
+// through global memory by the CTA that finishes last, in CTA order.
+//
+// Layout of the products (mma.sync m16n8k16, tokens or dimensions as M,
+// query rows as N = 8): with a group of up to 8 query rows per KV head the
+// tensor pipe needs half of what rows-as-M would, and every lane reads whole
+// 16-byte vectors of codes: S^T = K Q^T takes the contraction in the order
+// the bytes lie in, O^T = V^T P^T interleaves two tokens' bytes with one
+// byte permute per pair. P^T is S^T's accumulator transposed by movmatrix.
+// The bound is HBM; tcgen05 would need the codes widened into shared memory
+// first and pads the rows to 64 or more.
+//
+// Two running maxima: m over s, for the sum l; and mp over s + log2 vs, for
+// the weights p * vs that multiply the codes. So the FP16 weights stay in
+// [0, 1] with the largest term near 1 whatever the blocks' scales are.
+#include "se12_device.cuh"
+#include "se12_serve.h"
+
+#include <cuda_fp16.h>
+
+namespace se12 {
+
+constexpr int kAttendWarps = 8;
+constexpr int kAttendThreads = kAttendWarps * 32;
+constexpr int kAttendStages = 3;
+constexpr int kAttendBox = 2048;         // 16 tokens x 128 bytes
+constexpr int kAttendStageBytes = 8192;  // keys and values of a chunk
+constexpr int kAttendDeposit = 16384;    // joining the warps' sums
+constexpr int kAttendMaxSeqs = 2048;
+constexpr int kAttendMinChunks = 8;      // per CTA: one per warp
+constexpr int kAttendSlotRows = 16;
+constexpr int kAttendSlotFloats = kAttendSlotRows * (256 + 4);  // sums, then (m, l, mp) per row
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// Four codes (bytes) as two FP16 pairs, bytes (0, 1) and (2, 3).
+// int8: byte ^ 0x80 is code + 128; as the low byte of 0x6400 it makes the
+// FP16 number 1024 + code + 128, from which 1152 is taken exactly.
+template <int KIND>
+__device__ __forceinline__ void widen(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  if constexpr (KIND == kKvInt8) {
+    const uint32_t u = codes ^ 0x80808080u;
+    const uint32_t bias = 0x64806480u;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(prmt(u, 0x64646464u, 0x4140u)), "r"(bias));
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(prmt(u, 0x64646464u, 0x4342u)), "r"(bias));
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(codes));
+  }
+}
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ void cp_async_4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// A sequence's part of the work list.
+struct SeqWork {
+  int tokens;   // new tokens
+  int first;    // position of the first one (may be negative: inactive tokens)
+  int length;   // tokens in the cache
+  int low;      // first chunk's first token: a multiple of the chunk, at or below the first visible token
+  int chunks;   // per pair
+  int tiles;    // row tiles
+};
+
+template <int CHUNK, int ROWS>
+__device__ __forceinline__ SeqWork sequence_work(const AttendArgs& a, int b) {
+  SeqWork w;
+  if (a.t.query_start) {
+    const int q0 = max(a.t.query_start[b], 0), q1 = min(a.t.query_start[b + 1], a.t.tokens);
+    w.tokens = max(q1 - q0, 0);
+  } else {
+    w.tokens = 1;
+  }
+  w.length = max(a.t.lens[b], 0);
+  w.first = w.length - w.tokens;
+  const int visible = a.window ? max(w.first - a.window + 1, 0) : 0;
+  w.low = visible / CHUNK * CHUNK;
+  // an empty sequence keeps one chunk, whose CTA writes its rows' zeros
+  w.chunks = max((w.length - w.low + CHUNK - 1) / CHUNK, 1);
+  w.tiles = (w.tokens * a.group + ROWS - 1) / ROWS;
+  return w;
+}
+
+// A place in the work list: chunk `chunk` of pair `pair` (KV head x row
+// tile) of sequence b, whose pairs start at `base`.
+struct Place {
+  int b, pair, chunk;
+  int base;
+  SeqWork w;
+};
+
+template <int KIND, int DP, int NT>
+struct AttendShape {
+  static constexpr int kBoxes = DP / 128;                           // boxes per 16 tokens
+  static constexpr int kChunk = kAttendStageBytes / 2 / DP;         // tokens per chunk: 16 or 32
+  static constexpr int kSubs = kChunk / 16;
+  static constexpr int kRows = 8 * NT;
+};
+
+struct AttendSmem {
+  // after the pipelines (1024-byte aligned)
+  float deposit[kAttendDeposit / 4];
+  float stat[kAttendWarps][kAttendSlotRows][3];   // m, l, mp of each warp
+  float factor[kAttendWarps][kAttendSlotRows];
+  float out_scale[kAttendSlotRows];
+  float scales[kAttendWarps][kAttendStages][2][2];  // [sub][keys, values]
+  int usable[kAttendWarps][kAttendStages][2];
+  uint64_t full[kAttendWarps][kAttendStages];
+  int last;
+  int before[1];  // [seqs + 1] chunks x tiles of the sequences before (per KV head)
+};
+
+template <int KIND, int DP, int NT>
+__global__ void __launch_bounds__(kAttendThreads, 1)
+    attend_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                       const AttendArgs a) {
+  using Shape = AttendShape<KIND, DP, NT>;
+  constexpr int HB = Shape::kBoxes, CHUNK = Shape::kChunk, SUBS = Shape::kSubs, ROWS = Shape::kRows;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* pipes = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  AttendSmem& sm = *reinterpret_cast<AttendSmem*>(pipes + kAttendWarps * kAttendStages * kAttendStageBytes);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = lane >> 2, c = lane & 3;
+
+  if (lane == 0) {
+    for (int s = 0; s < kAttendStages; ++s) mbar_init(&sm.full[warp][s], 1);
+    fence_barrier_init();
+    if (warp == 0) {
+      prefetch_tmap(&kmap);
+      prefetch_tmap(&vmap);
+    }
+  }
+  grid_launch_dependents();
+  grid_dependency_wait();
+
+  // ---- the work list
+  const int heads = a.c.heads;
+  for (int b = threadIdx.x; b < a.t.seqs; b += kAttendThreads) {
+    const SeqWork w = sequence_work<CHUNK, ROWS>(a, b);
+    sm.before[b + 1] = w.chunks * w.tiles;
+  }
+  if (threadIdx.x == 0) sm.before[0] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    int carry = 0;
+    for (int i = 1; i <= a.t.seqs; i += 32) {
+      int v = i + lane <= a.t.seqs ? sm.before[i + lane] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        if (lane >= d) v += u;
+      }
+      v += carry;
+      if (i + lane <= a.t.seqs) sm.before[i + lane] = v;
+      carry = __shfl_sync(0xFFFFFFFFu, v, 31);
+    }
+  }
+  __syncthreads();
+  const int total = sm.before[a.t.seqs] * heads;
+  const int per = max(kAttendMinChunks, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  const int g0 = static_cast<int>(min(static_cast<long long>(blockIdx.x) * per, static_cast<long long>(total)));
+  const int g1 = min(g0 + per, total);
+  if (g0 >= g1) return;
+
+  auto locate = [&](int g) {
+    int lo = 0, hi = a.t.seqs - 1;  // last b with before[b] * heads <= g
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (static_cast<long long>(sm.before[mid]) * heads <= g) lo = mid;
+      else hi = mid - 1;
+    }
+    Place p;
+    p.b = lo;
+    p.base = sm.before[lo] * heads;
+    p.w = sequence_work<CHUNK, ROWS>(a, lo);
+    p.pair = (g - p.base) / p.w.chunks;
+    p.chunk = (g - p.base) - p.pair * p.w.chunks;
+    return p;
+  };
+  auto advance = [&](Place& p, int by) {  // to the place `by` chunks on (before total)
+    p.chunk += by;
+    while (p.chunk >= p.w.chunks) {
+      p.chunk -= p.w.chunks;
+      if (++p.pair == p.w.tiles * heads) {
+        p.pair = 0;
+        do {
+          ++p.b;
+        } while (sm.before[p.b + 1] == sm.before[p.b]);
+        p.base = sm.before[p.b] * heads;
+        // (chunks left over continue in the next sequence)
+        p.w = sequence_work<CHUNK, ROWS>(a, p.b);
+      }
+    }
+  };
+
+  // ---- this warp's pipeline: chunks g0 + warp, + 8, ...
+  unsigned char* pipe = pipes + warp * (kAttendStages * kAttendStageBytes);
+  const uint32_t pipe_addr = smem_addr(pipe);
+  const uint64_t policy = policy_evict_first();
+  Place next{};
+  int next_g = g0 + warp;
+  int next_page = -1;  // this lane's (lane < SUBS) page for the next chunk to issue
+  auto fetch_page = [&]() {
+    next_page = -1;
+    if (lane < SUBS) {
+      const int t0 = next.w.low + next.chunk * CHUNK + lane * 16;
+      const int visible = a.window ? next.w.first - a.window + 1 : 0;
+      if (t0 < next.w.length && t0 + 16 > visible) {
+        const int i = t0 >> a.c.page_shift;
+        next_page = i < a.t.max_pages ? a.t.table[next.b * a.t.table_stride + i] : -1;
+        if (next_page < 0 || next_page >= a.c.pages) {
+          raise_status(kStatusBadArgument);
+          next_page = -1;
+        }
+      }
+    }
+  };
+  auto issue = [&](int stage) {  // the chunk at `next`, then move on
+    uint64_t* bar = &sm.full[warp][stage];
+    const bool use = next_page >= 0;
+    const int head = next.pair / next.w.tiles;
+    const long long block = static_cast<long long>(next_page) * heads + head;
+    if (lane < SUBS) {
+      sm.usable[warp][stage][lane] = use;
+      if (use) {
+        cp_async_4(&sm.scales[warp][stage][lane][0], a.c.k_scales + block);
+        cp_async_4(&sm.scales[warp][stage][lane][1], a.c.v_scales + block);
+        cp_async_mbar_arrive(bar);
+      }
+    }
+    const int boxes = __popc(__ballot_sync(0xFFFFFFFFu, use)) * 2 * HB;
+    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * kAttendBox);
+    __syncwarp();
+    if (use) {
+      const int t0 = next.w.low + next.chunk * CHUNK + lane * 16;
+      const int row = static_cast<int>(block * a.c.page_size + (t0 & (a.c.page_size - 1)));
+      unsigned char* dst = pipe + stage * kAttendStageBytes + lane * HB * kAttendBox;
+#pragma unroll
+      for (int hb = 0; hb < HB; ++hb) {
+        tma_load_2d(dst + hb * kAttendBox, &kmap, hb * 128, row, bar, policy);
+        tma_load_2d(dst + kAttendStageBytes / 2 + hb * kAttendBox, &vmap, hb * 128, row, bar, policy);
+      }
+    }
+    next_g += kAttendWarps;
+    if (next_g < g1) {
+      advance(next, kAttendWarps);
+      fetch_page();
+    }
+  };
+  if (next_g < g1) {
+    next = locate(next_g);
+    fetch_page();
+  }
+#pragma unroll
+  for (int s = 0; s < kAttendStages; ++s)
+    if (next_g < g1) issue(s);
+
+  int stage = 0;
+  uint32_t phase = 0;
+  bool dead = false;  // a wait ran out: skip the rest (status raised)
+
+  // ---- the pairs of this CTA's run
+  Place at = locate(g0);
+  for (int g = g0; g < g1;) {
+    const int run = min(at.w.chunks - at.chunk, g1 - g);  // chunks of this pair here
+    const int head = at.pair / at.w.tiles, tile = at.pair % at.w.tiles;
+    const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
+    const int rows_all = at.w.tokens * a.group;
+
+    // queries: lane (r, c) holds, of rows r (+ 8 per n-tile), the dimensions
+    // 128 hb + 32 c .. + 31 in byte order
+    uint32_t qf[NT][HB][8][2];
+    float row_scale[NT][2];  // of rows 2c, 2c + 1
+    int row_pos[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = tile * ROWS + n * 8 + r;
+      uint32_t raw[HB][16];
+      unsigned big = 0;
+      const bool live = row < rows_all;
+      const int i = live ? row / a.group : 0;
+      const uint16_t* src = a.q + (token0 + i) * a.q_ts + (head * a.group + (live ? row - i * a.group : 0)) * a.q_hs;
+#pragma unroll
+      for (int hb = 0; hb < HB; ++hb) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int d = hb * 128 + c * 32 + j * 8;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (live && d < a.c.dim) {  // dim is a multiple of 16
+            if (a.q_vec) {
+              v = *reinterpret_cast<const uint4*>(src + d);
+            } else {
+              const uint16_t* s = src + d;
+              v = make_uint4(s[0] | (static_cast<uint32_t>(s[1]) << 16), s[2] | (static_cast<uint32_t>(s[3]) << 16),
+                             s[4] | (static_cast<uint32_t>(s[5]) << 16), s[6] | (static_cast<uint32_t>(s[7]) << 16));
+            }
+          }
+          raw[hb][4 * j] = v.x, raw[hb][4 * j + 1] = v.y, raw[hb][4 * j + 2] = v.z, raw[hb][4 * j + 3] = v.w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t w = word_of(v, k);
+            big = max(big, max((w << 16) & 0x7FFFFFFFu, w & 0x7FFF0000u));
+          }
+        }
+      }
+      big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+      big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+      // the row times 2^-e, largest in [1, 2) (zero rows and infinities: e clamped)
+      int e = static_cast<int>(big >> 23) - 127;
+      e = max(min(e, 120), -120);
+      const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+#pragma unroll
+      for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t w = raw[hb][2 * j + k];
+            qf[n][hb][j][k] = half2_bits(
+                __floats2half2_rn(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down));
+          }
+        }
+      const float up = __uint_as_float(static_cast<unsigned>(127 + e) << 23) * a.scale;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        row_scale[n][k] = __shfl_sync(0xFFFFFFFFu, up, (2 * c + k) * 4);
+        const int rr = tile * ROWS + n * 8 + 2 * c + k;
+        row_pos[n][k] = at.w.first + min(rr, rows_all - 1) / a.group;
+      }
+    }
+    const int pos_min = at.w.first + min(tile * ROWS, rows_all - 1) / a.group;
+    const int pos_max = at.w.first + min(tile * ROWS + ROWS - 1, rows_all - 1) / a.group;
+
+    float m[NT][2], l[NT][2], mp[NT][2];
+    float acc[HB][4][2][NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        m[n][k] = mp[n][k] = kNegInf;
+        l[n][k] = 0.f;
+      }
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[hb][w][h][n][k] = 0.f;
+
+    // this warp's first chunk of the pair: the run's chunks are g .. g + run - 1
+    int mine = (warp - (g - g0)) & (kAttendWarps - 1);
+    for (; mine < run; mine += kAttendWarps) {
+      if (!dead) dead = !__all_sync(0xFFFFFFFFu, mbar_wait(&sm.full[warp][stage], phase));
+      if (dead) break;
+      const uint32_t base = pipe_addr + stage * kAttendStageBytes;
+#pragma unroll
+      for (int sub = 0; sub < SUBS; ++sub) {
+        if (!sm.usable[warp][stage][sub]) continue;
+        const float ks = sm.scales[warp][stage][sub][0];
+        const float vs = sm.scales[warp][stage][sub][1];
+        const int t0 = at.w.low + (at.chunk + mine) * CHUNK + sub * 16;
+        // S^T: 16 tokens x 8 rows
+        float s[NT][2][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[n][h][k] = 0.f;
+        const uint32_t kbase = base + sub * HB * kAttendBox + r * 128;
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t off = kbase + hb * kAttendBox + (((2 * c + i) ^ r) << 4);
+            const uint4 x = lds128(off), y = lds128(off + 1024);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t a0, a1, a2, a3;
+              widen<KIND>(word_of(x, w), a0, a2);
+              widen<KIND>(word_of(y, w), a1, a3);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                mma_f16_16816(s[n][w & 1], a0, a1, a2, a3, qf[n][hb][4 * i + w][0], qf[n][hb][4 * i + w][1]);
+            }
+          }
+        // logits in units of log 2, masks, running maxima
+        const bool masked = t0 + 15 > pos_min || (a.window && pos_max - t0 >= a.window);
+        const float lv = lg2(vs);
+        float p[NT][4];
+        uint32_t pf[NT][2];
+        bool grew = false;
+        float shrink[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float x = (s[n][0][k] + s[n][1][k]) * (row_scale[n][k & 1] * ks);
+            if (a.softcap != 0.f) {
+              // cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1)
+              const float e = ex2(x * (2.f * kLog2e / a.softcap));
+              x = a.softcap * kLog2e - __fdividef(2.f * kLog2e * a.softcap, e + 1.f);
+            } else {
+              x *= kLog2e;
+            }
+            if (masked) {
+              const int j = t0 + r + (k >> 1) * 8, pos = row_pos[n][k & 1];
+              if (j > pos || (a.window && pos - j >= a.window)) x = kNegInf;
+            }
+            p[n][k] = x;
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float top = fmaxf(p[n][k], p[n][k + 2]);
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+            const float m_new = fmaxf(m[n][k], top), mp_new = fmaxf(mp[n][k], top + lv);
+            const float m_ref = m_new == kNegInf ? 0.f : m_new, mp_ref = mp_new == kNegInf ? 0.f : mp_new;
+            l[n][k] *= ex2(m[n][k] - m_ref);
+            shrink[n][k] = ex2(mp[n][k] - mp_ref);
+            grew |= mp_new != mp[n][k];
+            m[n][k] = m_new;
+            mp[n][k] = mp_new;
+            const float x0 = p[n][k], x1 = p[n][k + 2];
+            l[n][k] += ex2(x0 - m_ref) + ex2(x1 - m_ref);
+            // a masked token weighs nothing, whatever its block's scale holds
+            p[n][k] = x0 == kNegInf ? 0.f : ex2(x0 + lv - mp_ref);
+            p[n][k + 2] = x1 == kNegInf ? 0.f : ex2(x1 + lv - mp_ref);
+          }
+          pf[n][0] = transpose_8x8(half2_bits(__floats2half2_rn(p[n][0], p[n][1])));
+          pf[n][1] = transpose_8x8(half2_bits(__floats2half2_rn(p[n][2], p[n][3])));
+        }
+        if (__any_sync(0xFFFFFFFFu, grew)) {
+#pragma unroll
+          for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) acc[hb][w][h][n][k] *= shrink[n][k & 1];
+        }
+        // O^T += V^T P^T: lane (r, c) reads dimensions 128 hb + 16 r .. + 15
+        // of tokens 2c, 2c + 1, 2c + 8, 2c + 9
+        const uint32_t vbase = base + kAttendStageBytes / 2 + sub * HB * kAttendBox + 2 * c * 128;
+        const bool clip = t0 + 16 > at.w.length;  // codes past the sequence may be anything
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb) {
+          uint4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[i] = lds128(vbase + hb * kAttendBox + (i & 1) * 128 + (i >> 1) * 1024 + ((r ^ (2 * c + (i & 1))) << 4));
+            if (clip && t0 + 2 * c + (i & 1) + (i >> 1) * 8 >= at.w.length) v[i] = make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t x0 = word_of(v[0], w), x1 = word_of(v[1], w), y0 = word_of(v[2], w), y1 = word_of(v[3], w);
+            uint32_t a0, a1, a2, a3;
+            widen<KIND>(prmt(x0, x1, 0x5140u), a0, a1);
+            widen<KIND>(prmt(y0, y1, 0x5140u), a2, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16_16816(acc[hb][w][0][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+            widen<KIND>(prmt(x0, x1, 0x7362u), a0, a1);
+            widen<KIND>(prmt(y0, y1, 0x7362u), a2, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16_16816(acc[hb][w][1][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the stage
+      if (next_g < g1) issue(stage);
+      if (++stage == kAttendStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+
+    // ---- join the warps
+    const int rows = min(ROWS, rows_all - tile * ROWS);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float v = l[n][k];
+        v += __shfl_xor_sync(0xFFFFFFFFu, v, 4);
+        v += __shfl_xor_sync(0xFFFFFFFFu, v, 8);
+        v += __shfl_xor_sync(0xFFFFFFFFu, v, 16);
+        if (r == 0) {
+          float* st = sm.stat[warp][n * 8 + 2 * c + k];
+          st[0] = m[n][k];
+          st[1] = v;
+          st[2] = mp[n][k];
+        }
+      }
+    __syncthreads();
+    const int pair_start = g - at.chunk;  // work-list places of this pair
+    const int pair_end = pair_start + at.w.chunks;
+    const int cta_first = pair_start / per, cta_last = (pair_end - 1) / per;
+    const bool whole = cta_first == cta_last;
+    const int slot = pair_start > g0 ? 1 : 0;
+    float* part = a.partials + (static_cast<size_t>(blockIdx.x) * 2 + slot) * kAttendSlotFloats;
+    if (threadIdx.x < rows) {
+      const int row = threadIdx.x;
+      float mm = kNegInf, mmp = kNegInf;
+      for (int w = 0; w < kAttendWarps; ++w) {
+        mm = fmaxf(mm, sm.stat[w][row][0]);
+        mmp = fmaxf(mmp, sm.stat[w][row][2]);
+      }
+      const float mr = mm == kNegInf ? 0.f : mm, mpr = mmp == kNegInf ? 0.f : mmp;
+      float sum = 0.f;
+      for (int w = 0; w < kAttendWarps; ++w) {
+        sum += sm.stat[w][row][1] * ex2(sm.stat[w][row][0] - mr);
+        sm.factor[w][row] = ex2(sm.stat[w][row][2] - mpr);
+      }
+      if (whole) {
+        sm.out_scale[row] = sum == 0.f ? 0.f : ex2(mpr - mr) / sum;
+      } else {
+        float* st = part + kAttendSlotRows * 256 + row * 4;
+        st[0] = mm;
+        st[1] = sum;
+        st[2] = mmp;
+      }
+    }
+    __syncthreads();
+    // words (of 4 dimensions per lane: 32 in all) joined at a time
+    const int words = max(1, min(HB * 4, kAttendDeposit / (kAttendWarps * 32 * 4) / rows));
+    for (int w0 = 0; w0 < HB * 4; w0 += words) {
+      const int nw = min(words, HB * 4 - w0);
+#pragma unroll
+      for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int word = hb * 4 + w - w0;
+          if (word >= 0 && word < nw) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int row = n * 8 + 2 * c + k;
+                if (row < rows) {
+                  const float f = sm.factor[warp][row];
+                  float4 v = make_float4(acc[hb][w][0][n][k] * f, acc[hb][w][0][n][k + 2] * f, acc[hb][w][1][n][k] * f,
+                                         acc[hb][w][1][n][k + 2] * f);
+                  *reinterpret_cast<float4*>(&sm.deposit[((warp * rows + row) * nw + word) * 32 + r * 4]) = v;
+                }
+              }
+          }
+        }
+      __syncthreads();
+      const int count = rows * nw * 8;  // vectors of 4 dimensions
+      for (int i = threadIdx.x; i < count; i += kAttendThreads) {
+        const int row = i / (nw * 8), word = i / 8 % nw, rr = i & 7;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kAttendWarps; ++w) {
+          const float4 u = *reinterpret_cast<const float4*>(&sm.deposit[((w * rows + row) * nw + word) * 32 + rr * 4]);
+          v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        const int wd = w0 + word;
+        const int d = (wd >> 2) * 128 + rr * 16 + (wd & 3) * 4;
+        if (whole) {
+          if (d < a.c.dim) {
+            const float f = sm.out_scale[row];
+            const int all = tile * ROWS + row, i_tok = all / a.group;
+            uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (head * a.group + all - i_tok * a.group) * a.o_hs + d;
+            out[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v.x * f));
+            out[1] = __bfloat16_as_ushort(__float2bfloat16_rn(v.y * f));
+            out[2] = __bfloat16_as_ushort(__float2bfloat16_rn(v.z * f));
+            out[3] = __bfloat16_as_ushort(__float2bfloat16_rn(v.w * f));
+          }
+        } else {
+          *reinterpret_cast<float4*>(part + row * 256 + d) = v;
+        }
+      }
+      __syncthreads();
+    }
+    if (!whole) {
+      // ---- join the CTAs of the pair: the last to arrive adds all in order
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const int arrived = atomic_add_acq_rel_gpu(a.counters + cta_first, 1);
+        sm.last = arrived == cta_last - cta_first;
+        if (sm.last) a.counters[cta_first] = 0;
+      }
+      __syncthreads();
+      if (sm.last) {
+        __threadfence();
+        const int parts = cta_last - cta_first + 1;
+        const float* first = a.partials + (static_cast<size_t>(cta_first) * 2 + (pair_start > cta_first * per ? 1 : 0)) * kAttendSlotFloats;
+        const float* rest = a.partials + static_cast<size_t>(cta_first) * 2 * kAttendSlotFloats;  // + 2 slots per CTA
+        auto part_of = [&](int i) { return i == 0 ? first : rest + static_cast<size_t>(i) * 2 * kAttendSlotFloats; };
+        if (threadIdx.x < rows) {
+          float mm = kNegInf, mmp = kNegInf;
+          for (int i = 0; i < parts; ++i) {
+            const float* st = part_of(i) + kAttendSlotRows * 256 + threadIdx.x * 4;
+            mm = fmaxf(mm, __ldcg(st));
+            mmp = fmaxf(mmp, __ldcg(st + 2));
+          }
+          const float mr = mm == kNegInf ? 0.f : mm, mpr = mmp == kNegInf ? 0.f : mmp;
+          float sum = 0.f;
+          for (int i = 0; i < parts; ++i) {
+            const float* st = part_of(i) + kAttendSlotRows * 256 + threadIdx.x * 4;
+            sum += __ldcg(st + 1) * ex2(__ldcg(st) - mr);
+          }
+          sm.factor[0][threadIdx.x] = mpr;
+          sm.out_scale[threadIdx.x] = sum == 0.f ? 0.f : ex2(mpr - mr) / sum;
+        }
+        __syncthreads();
+        const int vectors = a.c.dim / 4;
+        for (int i = threadIdx.x; i < rows * vectors; i += kAttendThreads) {
+          const int row = i / vectors, d = (i - row * vectors) * 4;
+          const float mpr = sm.factor[0][row], f = sm.out_scale[row];
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int j = 0; j < parts; ++j) {
+            const float* pt = part_of(j);
+            const float4 u = __ldcg(reinterpret_cast<const float4*>(pt + row * 256 + d));
+            const float w = ex2(__ldcg(pt + kAttendSlotRows * 256 + row * 4 + 2) - mpr);
+            v.x += u.x * w, v.y += u.y * w, v.z += u.z * w, v.w += u.w * w;
+          }
+          const int all = tile * ROWS + row, i_tok = all / a.group;
+          uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (head * a.group + all - i_tok * a.group) * a.o_hs + d;
+          out[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v.x * f));
+          out[1] = __bfloat16_as_ushort(__float2bfloat16_rn(v.y * f));
+          out[2] = __bfloat16_as_ushort(__float2bfloat16_rn(v.z * f));
+          out[3] = __bfloat16_as_ushort(__float2bfloat16_rn(v.w * f));
+        }
+      }
+      __syncthreads();
+    }
+    g += run;
+    if (g < g1) advance(at, run);
+  }
+}
+
+// ------------------------------------------------------------------ launch
+
+size_t kv_attend_partial_bytes(int sm_count) { return static_cast<size_t>(sm_count) * 2 * kAttendSlotFloats * 4; }
+
+template <int KIND, int DP, int NT>
+cudaError_t launch_attend_rows(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int sm_count,
+                               cudaStream_t stream) {
+  const size_t smem = 1024 + kAttendWarps * kAttendStages * kAttendStageBytes + sizeof(AttendSmem) + a.t.seqs * sizeof(int);
+  return launch_overlapped(attend_rows_kernel<KIND, DP, NT>, dim3(sm_count), kAttendThreads, smem, stream, kmap, vmap, a);
+}
+
+template <int KIND>
+cudaError_t launch_attend_kind(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int max_query,
+                               int sm_count, cudaStream_t stream) {
+  const bool one = static_cast<long long>(max_query) * a.group <= 8;  // query rows per KV head in one n-tile
+  if (a.c.dim <= 128)
+    return one ? launch_attend_rows<KIND, 128, 1>(kmap, vmap, a, sm_count, stream)
+               : launch_attend_rows<KIND, 128, 2>(kmap, vmap, a, sm_count, stream);
+  return one ? launch_attend_rows<KIND, 256, 1>(kmap, vmap, a, sm_count, stream)
+             : launch_attend_rows<KIND, 256, 2>(kmap, vmap, a, sm_count, stream);
+}
+
+cudaError_t launch_kv_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int max_query,
+                             int sm_count, cudaStream_t stream) {
+  return a.c.kind == kKvInt8 ? launch_attend_kind<kKvInt8>(kmap, vmap, a, max_query, sm_count, stream)
+                             : launch_attend_kind<kKvE4m3>(kmap, vmap, a, max_query, sm_count, stream);
+}
+
+}  // namespace se12

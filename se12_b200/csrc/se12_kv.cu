@@ -1,0 +1,481 @@
+// The paged 8-bit key/value cache: appending new tokens, with the position
+// rotation applied on the way, and reading pages back.
+//
+// A block (one page of one KV head, keys and values separately) holds codes
+// c and one scale s = 2^e; a value is c * s. e is the smallest integer >=
+// kMinScaleExponent with amax <= qmax * 2^e over the block's tokens (qmax 127
+// for int8, 448 for e4m3). Powers of two cost int8 up to one of its seven
+// bits, and buy two things: when a later token raises the block's scale, the
+// older codes shrink by an exact power of two and are rounded once more (for
+// e4m3 that only touches subnormals), so that the rounding errors of
+// repeated growth form a geometric series below one step; and code * scale
+// is exact in BF16 and in every product with a query, whatever order the
+// kernels apply the scale in.
+//
+// Both kernels are bound by memory: the new tokens are read once from HBM
+// (the second pass of a prompt block hits L2) and the codes written once.
+#include "se12_device.cuh"
+#include "se12_serve.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+namespace se12 {
+
+constexpr int kMinScaleExponent = -100;
+constexpr unsigned kInfBits = 0x7F800000u;
+constexpr unsigned kNanBits = 0x7FC00000u;
+
+// Bits of the least admissible scale for a block whose largest magnitude has
+// the fp32 bits `amax`; NaN where that is not finite.
+template <int KIND>
+__device__ __forceinline__ float fit_scale(unsigned amax) {
+  if (amax >= kInfBits) return __uint_as_float(kNanBits);
+  // qmax = 1.984375 * 2^6 (127) or 1.75 * 2^8 (448)
+  constexpr int q_exponent = KIND == kKvInt8 ? 6 : 8;
+  constexpr unsigned q_mantissa = KIND == kKvInt8 ? 0x7E0000u : 0x600000u;
+  int e = static_cast<int>(amax >> 23) - 127 - q_exponent + ((amax & 0x7FFFFFu) > q_mantissa ? 1 : 0);
+  if (e < kMinScaleExponent) e = kMinScaleExponent;
+  return __uint_as_float(static_cast<unsigned>(e + 127) << 23);
+}
+
+// Scaled value to code, rounded to nearest, ties to even. |x| <= qmax.
+template <int KIND>
+__device__ __forceinline__ uint32_t to_code(float x) {
+  if constexpr (KIND == kKvInt8) return static_cast<uint32_t>(__float2int_rn(x)) & 0xFFu;
+  return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+}
+
+template <int KIND>
+__device__ __forceinline__ float code_value(uint32_t c) {
+  if constexpr (KIND == kKvInt8) return static_cast<float>(static_cast<int8_t>(c));
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(c), __NV_E4M3)));
+}
+
+__device__ __forceinline__ float load_value(const float* p) { return *p; }
+__device__ __forceinline__ float load_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// VP consecutive elements (VP > 1: the address is a multiple of their size).
+template <int VP>
+__device__ __forceinline__ void load_vector(float (&x)[VP], const float* p) {
+  if constexpr (VP == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else if constexpr (VP == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x, x[1] = v.y;
+  } else {
+    x[0] = *p;
+  }
+}
+
+template <int VP>
+__device__ __forceinline__ void load_vector(float (&x)[VP], const __nv_bfloat16* p) {
+  if constexpr (VP == 4) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xFFFF0000u);
+    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xFFFF0000u);
+  } else if constexpr (VP == 2) {
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+    x[0] = __uint_as_float(v << 16), x[1] = __uint_as_float(v & 0xFFFF0000u);
+  } else {
+    x[0] = load_value(p);
+  }
+}
+
+// A row of `dim` values as dim / 2 pairs (a, b): the pairs the rotation turns
+// together first, then neighbours. A lane takes VP consecutive pairs at a
+// time, so that both members stay in one lane.
+struct PairMap {
+  int pairs;   // dim / 2
+  int turned;  // pairs below this are rotated
+  int split;   // pairs below this have members p and p + half, the others 2p and 2p + 1
+  int half;
+
+  __device__ __forceinline__ void at(int p, int& a, int& b) const {
+    if (p < split) {
+      a = p;
+      b = p + half;
+    } else {
+      a = 2 * p;
+      b = 2 * p + 1;
+    }
+  }
+};
+
+// (a, b) turned by the angle whose cosine and sine are c and s; each product
+// and each sum is rounded by itself, as elementary tensor operations do.
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+  const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+  b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+  a = x;
+}
+
+// Calls f(a index, b index, values a, values b) for this lane's pairs of one row.
+template <int VP, typename T, typename F>
+__device__ __forceinline__ void for_row(const T* row, const PairMap& map, const float* cos, const float* sin, int lane,
+                                        F&& f) {
+  for (int p = lane * VP; p < map.pairs; p += 32 * VP) {
+    float a[VP], b[VP];
+    int ia, ib;
+    map.at(p, ia, ib);
+    load_vector<VP>(a, row + ia);
+    load_vector<VP>(b, row + ib);
+    if (p < map.turned) {
+      float c[VP], s[VP];
+      load_vector<VP>(c, cos + p);
+      load_vector<VP>(s, sin + p);
+#pragma unroll
+      for (int j = 0; j < VP; ++j) turn(a[j], b[j], c[j], s[j]);
+    }
+    f(ia, ib, a, b);
+  }
+}
+
+template <int VP>
+__device__ __forceinline__ unsigned magnitude_bits(const float (&x)[VP], unsigned m) {
+#pragma unroll
+  for (int j = 0; j < VP; ++j) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+  return m;
+}
+
+template <int KIND, int VP>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[VP], float inv) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < VP; ++j) w |= to_code<KIND>(x[j] * inv) << (8 * j);
+  if constexpr (VP == 4)
+    *reinterpret_cast<uint32_t*>(p) = w;
+  else if constexpr (VP == 2)
+    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w);
+  else
+    *p = static_cast<uint8_t>(w);
+}
+
+template <int VP>
+__device__ __forceinline__ void store_bf16(uint16_t* p, const float (&x)[VP]) {
+  uint16_t h[VP];
+#pragma unroll
+  for (int j = 0; j < VP; ++j) h[j] = __bfloat16_as_ushort(__float2bfloat16_rn(x[j]));
+  if constexpr (VP == 4)
+    *reinterpret_cast<uint2*>(p) = make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
+  else if constexpr (VP == 2)
+    *reinterpret_cast<uint32_t*>(p) = h[0] | (static_cast<uint32_t>(h[1]) << 16);
+  else
+    *p = h[0];
+}
+
+// Rounds `bytes` codes (a multiple of 16) again after the scale grew by 1 / ratio.
+template <int KIND>
+__device__ __forceinline__ void shrink_codes(uint8_t* codes, int bytes, float ratio, int thread, int threads) {
+  for (int i = thread * 16; i < bytes; i += threads * 16) {
+    uint4 v = *reinterpret_cast<const uint4*>(codes + i);
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t r = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) r |= to_code<KIND>(code_value<KIND>((w[j] >> (8 * b)) & 0xFFu) * ratio) << (8 * b);
+      w[j] = r;
+    }
+    *reinterpret_cast<uint4*>(codes + i) = v;
+  }
+}
+
+// Page of position `pos` of sequence b, or -1 (and the status word raised)
+// where the table has none for it.
+__device__ __forceinline__ int page_of(const TokenBatch& t, const KvView& c, int b, int pos) {
+  const int i = pos >> c.page_shift;
+  if (i < t.max_pages) {
+    const int page = t.table[b * t.table_stride + i];
+    if (page >= 0 && page < c.pages) return page;
+  }
+  raise_status(kStatusBadArgument);
+  return -1;
+}
+
+// Scale of a block once tokens with largest magnitude `amax` have joined it;
+// `ratio` = what the older codes shrink by.
+template <int KIND>
+__device__ __forceinline__ float joined_scale(const float* scale, bool older, unsigned amax, float& ratio) {
+  const float need = fit_scale<KIND>(amax);
+  ratio = 1.f;
+  if (!older) return need;
+  const float before = *scale;
+  if (!(before >= need)) {  // grows, or one of the two is not finite
+    if (before < need) {
+      ratio = before * __frcp_rn(need);
+      return need;
+    }
+    return __uint_as_float(kNanBits);
+  }
+  return before;
+}
+
+// How a row of queries or keys (turned) or values (not) splits into pairs.
+// Vector lanes (vp > 1) serve rows that are turned in halves, whole or not
+// at all, and split both kinds in halves.
+__device__ __forceinline__ PairMap pair_map(const AppendArgs& a, bool turned, int vp) {
+  PairMap m;
+  m.pairs = a.c.dim / 2;
+  m.turned = turned && a.cos ? a.rotary / 2 : 0;
+  m.split = vp > 1 ? m.pairs : a.interleaved ? 0 : m.turned;
+  m.half = vp > 1 ? m.pairs : m.turned;
+  return m;
+}
+
+// One query row (token t, head h), rotated, as BF16. `pos` < 0: an inactive
+// row, written as zeros.
+template <typename T, int VP>
+__device__ __forceinline__ void rotate_query(const AppendArgs& a, int token, int head, int pos, int lane) {
+  uint16_t* out = a.q_out + token * a.o_ts + head * a.o_hs;
+  const bool bad = a.cos && pos >= a.rope_rows;
+  if (pos < 0 || bad) {
+    if (bad) raise_status(kStatusBadArgument);
+    for (int i = lane; i < a.c.dim; i += 32) out[i] = 0;
+    return;
+  }
+  const T* row = static_cast<const T*>(a.q) + token * a.q_ts + head * a.q_hs;
+  PairMap map = pair_map(a, true, VP);
+  for_row<VP>(row, map, a.cos + pos * a.rope_stride, a.sin + pos * a.rope_stride, lane,
+              [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
+                store_bf16<VP>(out + ia, x);
+                store_bf16<VP>(out + ib, y);
+              });
+}
+
+// One token per sequence: a warp per (sequence, KV head, keys or values) and
+// one per (sequence, query head).
+template <typename T, int KIND, int VP>
+__global__ void __launch_bounds__(128) kv_append_step_kernel(const AppendArgs a) {
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int per_seq = 2 * a.c.heads + (a.q ? a.q_heads : 0);
+  const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int b = static_cast<int>(item / per_seq);
+  const int what = static_cast<int>(item % per_seq);
+  grid_dependency_wait();
+  if (b >= a.t.seqs) return;
+  const int pos = a.t.lens[b] - 1;
+  if (what >= 2 * a.c.heads) {
+    rotate_query<T, VP>(a, b, what - 2 * a.c.heads, pos, lane);
+    return;
+  }
+  if (pos < 0) return;
+  const bool keys = what < a.c.heads;
+  const int head = keys ? what : what - a.c.heads;
+  if (keys && a.cos && pos >= a.rope_rows) {
+    raise_status(kStatusBadArgument);
+    return;
+  }
+  const T* row = static_cast<const T*>(keys ? a.k : a.v) + b * (keys ? a.k_ts : a.v_ts) + head * (keys ? a.k_hs : a.v_hs);
+  const PairMap map = pair_map(a, keys, VP);
+  const float* cos = a.cos + pos * a.rope_stride;
+  const float* sin = a.sin + pos * a.rope_stride;
+  const int page = page_of(a.t, a.c, b, pos);
+  if (page < 0) return;
+  const int slot = pos & (a.c.page_size - 1);
+  const long long block = static_cast<long long>(page) * a.c.heads + head;
+  uint8_t* codes = (keys ? a.c.k_codes : a.c.v_codes) + block * a.c.page_size * a.c.dim;
+  float* scale = (keys ? a.c.k_scales : a.c.v_scales) + block;
+  unsigned amax = 0;
+  for_row<VP>(row, map, cos, sin, lane, [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
+    amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
+  });
+  amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+  float ratio;
+  const float now = joined_scale<KIND>(scale, slot > 0, amax, ratio);
+  const bool finite = now == now;
+  if (ratio != 1.f) shrink_codes<KIND>(codes, slot * a.c.dim, ratio, lane, 32);
+  const float inv = finite ? __frcp_rn(now) : 0.f;  // exact for the powers of two stored here
+  uint8_t* to = codes + slot * a.c.dim;
+  for_row<VP>(row, map, cos, sin, lane, [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
+    if (finite) {
+      store_codes<KIND, VP>(to + ia, x, inv);
+      store_codes<KIND, VP>(to + ib, y, inv);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VP; ++j) to[ia + j] = to[ib + j] = 0;
+    }
+  });
+  __syncwarp();
+  if (lane == 0) *scale = now;
+}
+
+// The sequence token t belongs to: the number of sequences 1 .. seqs - 1
+// that start at or before it, counted 32 at a time by one warp.
+__device__ __forceinline__ int sequence_of(const TokenBatch& t, int token, int lane) {
+  if (!t.query_start) return token;
+  int n = 0;
+  for (int i = 1; i < t.seqs; i += 32) {
+    const int b = i + lane;
+    n += __popc(__ballot_sync(0xFFFFFFFFu, b < t.seqs && t.query_start[b] <= token));
+  }
+  return n;
+}
+
+// Any number of tokens per sequence. CTAs with blockIdx.y < 2 * heads: each
+// looks through `span` consecutive tokens for the first new token of a block
+// (of its sequence, or of a page) and stores that block's new tokens, a warp
+// per token: one pass for the largest magnitude, one for the codes. The
+// other CTAs rotate queries, a warp per row.
+template <typename T, int KIND, int VP>
+__global__ void __launch_bounds__(256) kv_append_prompt_kernel(const AppendArgs a, const int span) {
+  __shared__ unsigned s_amax[8];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = blockIdx.x * span, end = min(first + span, a.t.tokens);
+  int b = sequence_of(a.t, first, lane);
+  const int what = blockIdx.y;
+  if (what >= 2 * a.c.heads) {
+    // span tokens x 8 heads per CTA
+    const int head = (what - 2 * a.c.heads) * 8 + warp;
+    if (head >= a.q_heads) return;
+    for (int t = first; t < end; ++t) {
+      while (b + 1 < a.t.seqs && a.t.query_start[b + 1] <= t) ++b;
+      const bool owned = t >= a.t.query_start[b] && t < a.t.query_start[b + 1];
+      rotate_query<T, VP>(a, t, head, owned ? a.t.lens[b] - (a.t.query_start[b + 1] - t) : -1, lane);
+    }
+    return;
+  }
+  const bool keys = what < a.c.heads;
+  const int head = keys ? what : what - a.c.heads;
+  const T* src = static_cast<const T*>(keys ? a.k : a.v) + head * (keys ? a.k_hs : a.v_hs);
+  const long long ts = keys ? a.k_ts : a.v_ts;
+  const PairMap map = pair_map(a, keys, VP);
+  for (int t = first; t < end; ++t) {
+    while (b + 1 < a.t.seqs && a.t.query_start[b + 1] <= t) ++b;
+    const int start = a.t.query_start[b], stop = min(a.t.query_start[b + 1], a.t.tokens);
+    const int pos = a.t.lens[b] - (a.t.query_start[b + 1] - t);
+    if (t < start || t >= stop || pos < 0) continue;  // not a sequence's token, or an inactive one
+    const int slot = pos & (a.c.page_size - 1);
+    if (t != start && slot != 0) continue;
+    const int page = page_of(a.t, a.c, b, pos);
+    if (page < 0) continue;
+    const int count = min(a.c.page_size - slot, stop - t);
+    if (keys && a.cos && pos + count > a.rope_rows) {
+      raise_status(kStatusBadArgument);
+      continue;
+    }
+    const long long block = static_cast<long long>(page) * a.c.heads + head;
+    uint8_t* codes = (keys ? a.c.k_codes : a.c.v_codes) + block * a.c.page_size * a.c.dim;
+    float* scale = (keys ? a.c.k_scales : a.c.v_scales) + block;
+    unsigned amax = 0;
+    for (int i = warp; i < count; i += 8)
+      for_row<VP>(src + (t + i) * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
+                  [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
+                    amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
+                  });
+    amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+    if (lane == 0) s_amax[warp] = amax;
+    __syncthreads();
+    amax = s_amax[lane & 7];
+    amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+    float ratio;
+    const float now = joined_scale<KIND>(scale, slot > 0, amax, ratio);
+    __syncthreads();  // every thread has read the old scale and the maxima
+    const bool finite = now == now;
+    if (ratio != 1.f) shrink_codes<KIND>(codes, slot * a.c.dim, ratio, threadIdx.x, 256);
+    const float inv = finite ? __frcp_rn(now) : 0.f;  // exact for the powers of two stored here
+    for (int i = warp; i < count; i += 8) {
+      uint8_t* to = codes + (slot + i) * a.c.dim;
+      for_row<VP>(src + (t + i) * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
+                  [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
+                    if (finite) {
+                      store_codes<KIND, VP>(to + ia, x, inv);
+                      store_codes<KIND, VP>(to + ib, y, inv);
+                    } else {
+#pragma unroll
+                      for (int j = 0; j < VP; ++j) to[ia + j] = to[ib + j] = 0;
+                    }
+                  });
+    }
+    if (threadIdx.x == 0) *scale = now;
+  }
+}
+
+// Pages read back as BF16 (exact: a code has at most 8 significant bits).
+template <int KIND>
+__global__ void __launch_bounds__(256) kv_decode_kernel(const KvView c, const int32_t* pages, int count, uint16_t* k_out,
+                                                        uint16_t* v_out) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int block_codes = c.page_size * c.dim;  // a multiple of 256
+  const long long per_page = static_cast<long long>(c.heads) * block_codes;
+  const long long total = count * per_page;
+  const uint8_t* codes = blockIdx.y ? c.v_codes : c.k_codes;
+  const float* scales = blockIdx.y ? c.v_scales : c.k_scales;
+  uint16_t* out = blockIdx.y ? v_out : k_out;
+  for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 8; i < total; i += gridDim.x * 2048ll) {
+    const long long n = i / per_page, rest = i - n * per_page;
+    const int page = pages ? pages[n] : static_cast<int>(n);
+    uint32_t w[4] = {};
+    if (page >= 0 && page < c.pages) {
+      const uint2 v = *reinterpret_cast<const uint2*>(codes + page * per_page + rest);
+      const float s = scales[static_cast<long long>(page) * c.heads + rest / block_codes];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t pair = (j < 2 ? v.x : v.y) >> (16 * (j & 1));
+        const float lo = code_value<KIND>(pair & 0xFFu) * s, hi = code_value<KIND>((pair >> 8) & 0xFFu) * s;
+        w[j] = __bfloat16_as_ushort(__float2bfloat16_rn(lo)) |
+               (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(hi))) << 16);
+      }
+    } else {
+      raise_status(kStatusBadArgument);
+    }
+    *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+
+template <typename T, int KIND, int VP>
+cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t stream) {
+  if (!a.t.query_start) {
+    const long long warps = static_cast<long long>(a.t.seqs) * (2 * a.c.heads + (a.q ? a.q_heads : 0));
+    return launch_overlapped(kv_append_step_kernel<T, KIND, VP>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0,
+                             stream, a);
+  }
+  // few tokens: one per CTA, so that short sequences' blocks run side by side
+  const int span = a.t.tokens <= 256 ? 1 : 16;
+  const dim3 grid((a.t.tokens + span - 1) / span, 2 * a.c.heads + (a.q ? (a.q_heads + 7) / 8 : 0));
+  return launch_overlapped(kv_append_prompt_kernel<T, KIND, VP>, grid, 256, 0, stream, a, span);
+}
+
+template <typename T, int KIND>
+cudaError_t launch_append_kind(const AppendArgs& a, cudaStream_t stream) {
+  // vector lanes: whole rows turned in halves (or not at all), 32 * VP pairs
+  // a step, and every row and table address a multiple of VP elements
+  const int vp = a.c.dim % 256 == 0 ? 4 : a.c.dim % 128 == 0 ? 2 : 1;
+  bool vec = vp > 1 && (!a.cos || (!a.interleaved && a.rotary == a.c.dim && a.rope_stride % vp == 0 &&
+                                   reinterpret_cast<uintptr_t>(a.cos) % (vp * 4) == 0 &&
+                                   reinterpret_cast<uintptr_t>(a.sin) % (vp * 4) == 0));
+  const void* ptr[3] = {a.k, a.v, a.q};
+  const long long stride[6] = {a.k_ts, a.k_hs, a.v_ts, a.v_hs, a.q_ts, a.q_hs};
+  for (int i = 0; i < 3; ++i)
+    if (ptr[i] && (reinterpret_cast<uintptr_t>(ptr[i]) % (vp * sizeof(T)) || stride[2 * i] % vp || stride[2 * i + 1] % vp))
+      vec = false;
+  if (a.q && (reinterpret_cast<uintptr_t>(a.q_out) % (vp * 2) || a.o_ts % vp || a.o_hs % vp)) vec = false;
+  if (!vec) return launch_append_as<T, KIND, 1>(a, stream);
+  return vp == 4 ? launch_append_as<T, KIND, 4>(a, stream) : launch_append_as<T, KIND, 2>(a, stream);
+}
+
+cudaError_t launch_kv_append(bool bf16, const AppendArgs& a, cudaStream_t stream) {
+  if (bf16)
+    return a.c.kind == kKvInt8 ? launch_append_kind<__nv_bfloat16, kKvInt8>(a, stream)
+                               : launch_append_kind<__nv_bfloat16, kKvE4m3>(a, stream);
+  return a.c.kind == kKvInt8 ? launch_append_kind<float, kKvInt8>(a, stream) : launch_append_kind<float, kKvE4m3>(a, stream);
+}
+
+cudaError_t launch_kv_decode(const KvView& c, const int32_t* pages, int count, uint16_t* k_out, uint16_t* v_out,
+                             cudaStream_t stream) {
+  const long long vectors = static_cast<long long>(count) * c.heads * c.page_size * c.dim / 8;
+  const long long blocks = (vectors + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), 2);
+  return launch_overlapped(c.kind == kKvInt8 ? kv_decode_kernel<kKvInt8> : kv_decode_kernel<kKvE4m3>, grid, 256, 0, stream, c,
+                           pages, count, k_out, v_out);
+}
+
+}  // namespace se12

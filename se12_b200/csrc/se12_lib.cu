@@ -4,3 +4,7 @@
 #include "se12_gemv.cu"
 #include "se12_chain.cu"
 #include "se12_abi.cu"
+#include "se12_kv.cu"
+#include "se12_attend.cu"
+#include "se12_logprobs.cu"
+#include "se12_serve_abi.cu"

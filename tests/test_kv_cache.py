@@ -1,0 +1,686 @@
+"""The paged 8-bit key/value cache and attention over it, against plain
+implementations: the stored codes and scales bit for bit (the store's
+arithmetic is elementary fp32 operations), attention against 64-bit sums
+over the stored values.
+
+Attention's tolerance, elementwise: the output is rounded to BF16 (half a
+unit in the last place of o); a weight carries an FP16 rounding (2^-11) and the fp32 errors of the
+logits, the exponential and the sum (together below 2^-12 for the logits
+here, |s| < 100), so 2^-10 of sum_j p_j |v_j|; a weight below FP16's normal
+range is off by 2^-25 of the largest, so 2^-24 of the length times the
+largest |v|.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+QMAX = {"int8": 127.0, "e4m3": 448.0}
+
+
+# ------------------------------------------------------------------ plain implementation (CPU)
+
+
+def value_of(codes: torch.Tensor, kind: str) -> torch.Tensor:
+    return codes.float() if kind == "int8" else codes.view(torch.float8_e4m3fn).float()
+
+
+def code_of(x: torch.Tensor, kind: str) -> torch.Tensor:
+    return torch.round(x).to(torch.int8) if kind == "int8" else x.to(torch.float8_e4m3fn).view(torch.int8)
+
+
+def least_scale(amax: float, kind: str) -> float:
+    if not math.isfinite(amax):
+        return math.nan
+    e = -100
+    while amax > QMAX[kind] * 2.0**e:
+        e += 1
+    return 2.0**e
+
+
+def rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool) -> torch.Tensor:
+    """x [..., dim] fp32 turned by cos, sin [rotary / 2]."""
+    n = cos.shape[-1]
+    out = x.clone()
+    a, b = (x[..., 0 : 2 * n : 2], x[..., 1 : 2 * n : 2]) if interleaved else (x[..., :n], x[..., n : 2 * n])
+    first, second = a * cos - b * sin, b * cos + a * sin
+    if interleaved:
+        out[..., 0 : 2 * n : 2], out[..., 1 : 2 * n : 2] = first, second
+    else:
+        out[..., :n], out[..., n : 2 * n] = first, second
+    return out
+
+
+class PlainCache:
+    """The same cache in elementary CPU operations, one block at a time."""
+
+    def __init__(self, pages, page_size, heads, dim, kind):
+        self.page_size, self.kind, self.heads, self.dim = page_size, kind, heads, dim
+        self.codes = {w: torch.zeros(pages, heads, page_size, dim, dtype=torch.int8) for w in "kv"}
+        self.scales = {w: torch.ones(pages, heads) for w in "kv"}
+
+    def append(self, k, v, table, lens, starts, cos=None, sin=None, interleaved=False, q=None):
+        out = None if q is None else torch.zeros(q.shape, dtype=torch.bfloat16)
+        for b, ln in enumerate(lens):
+            n = starts[b + 1] - starts[b]
+            blocks: dict = {}
+            for i in range(n):
+                pos, t = ln - n + i, starts[b] + i
+                if pos < 0:
+                    continue
+                turn = (lambda x: x) if cos is None else (lambda x, p=pos: rotate(x, cos[p], sin[p], interleaved))
+                if q is not None:
+                    out[t] = turn(q[t].float()).to(torch.bfloat16)
+                blocks.setdefault(pos // self.page_size, []).append((pos % self.page_size, turn(k[t].float()), v[t].float()))
+            for column, rows in blocks.items():
+                page, first = int(table[b, column]), rows[0][0]
+                for w, which in (("k", 1), ("v", 2)):
+                    for h in range(self.heads):
+                        new = torch.stack([r[which][h] for r in rows])
+                        need = least_scale(float(new.abs().max()) if bool(torch.isfinite(new).all()) else math.inf, self.kind)
+                        before = float(self.scales[w][page, h])
+                        now = need if first == 0 else math.nan if math.isnan(need) or math.isnan(before) else max(need, before)
+                        block = self.codes[w][page, h]
+                        if first and now > before:
+                            block[:first] = code_of(value_of(block[:first], self.kind) * (before / now), self.kind)
+                        self.scales[w][page, h] = now
+                        for r, x in zip(rows, new):
+                            block[r[0]] = 0 if math.isnan(now) else code_of(x / now, self.kind)
+        return out
+
+    def values(self, w):
+        return value_of(self.codes[w], self.kind).double() * self.scales[w].double()[:, :, None, None]
+
+
+def plain_attend(q, keys, values, table, lens, starts, scale, softcap, window):
+    """(output, sum of p |v|, largest |v|) in 64 bits; keys, values [pages, heads, page, dim]."""
+    tokens, q_heads, dim = q.shape
+    heads, page = keys.shape[1], keys.shape[2]
+    out, size = torch.zeros(tokens, q_heads, dim, dtype=torch.float64), torch.zeros(tokens, q_heads, dim, dtype=torch.float64)
+    biggest = torch.zeros(tokens, q_heads, 1, dtype=torch.float64)
+    for b, ln in enumerate(lens):
+        n = starts[b + 1] - starts[b]
+        if ln == 0 or n == 0:
+            continue
+        ids = [int(p) for p in table[b, : (ln + page - 1) // page]]
+        for h in range(heads):
+            k = torch.cat([keys[p, h] for p in ids])[:ln]
+            v = torch.cat([values[p, h] for p in ids])[:ln]
+            for i in range(n):
+                pos, t = ln - n + i, starts[b] + i
+                low = max(0, pos - window + 1) if window else 0
+                if pos < 0:
+                    continue
+                for g in range(h * q_heads // heads, (h + 1) * q_heads // heads):
+                    s = k[low : pos + 1] @ q[t, g].double() * scale
+                    if softcap:
+                        s = softcap * torch.tanh(s / softcap)
+                    p = torch.softmax(s, 0)
+                    out[t, g] = p @ v[low : pos + 1]
+                    size[t, g] = p @ v[low : pos + 1].abs()
+                    biggest[t, g] = v[low : pos + 1].abs().max()
+    return out, size, biggest
+
+
+def check_attend(got, want, size, biggest, length):
+    half_unit = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=1e-300))) - 8)
+    tol = half_unit + 2.0**-10 * size + 2.0**-24 * length * biggest
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= tol).all()), f"worst {float((err / tol.clamp(min=1e-300)).max()):.2f} of the tolerance"
+
+
+# ------------------------------------------------------------------ CPU: refusals
+
+
+@pytest.mark.parametrize("args", [
+    dict(pages=0), dict(kv_heads=0), dict(page_size=8), dict(page_size=48), dict(page_size=512), dict(head_dim=8),
+    dict(head_dim=264), dict(head_dim=100), dict(kind="fp8"),
+])
+def test_cache_refuses_bad_shapes(args):
+    from se12_b200.kv_cache import PagedKvCache
+
+    full = dict(pages=4, page_size=16, kv_heads=2, head_dim=64, kind="int8")
+    full.update(args)
+    with pytest.raises(ValueError):
+        PagedKvCache(**full)
+
+
+def test_abi_refuses_bad_arguments_without_a_device():
+    from se12_b200 import _build, _lib
+
+    _build.build()
+    lib = _lib.load()
+    handle = ctypes.c_void_p()
+    good = dict(pages=4, page_size=16, kv_heads=2, head_dim=64, kind=0, k_codes=256, v_codes=256, k_scales=256, v_scales=256)
+
+    def create(**changed):
+        return lib.se12_kv_cache_create(ctypes.byref(_lib.Se12KvPagesStruct(**{**good, **changed})), ctypes.byref(handle))
+
+    assert lib.se12_kv_cache_create(None, ctypes.byref(handle)) == 1
+    assert create(pages=0) == 1 and create(page_size=24) == 1 and create(head_dim=24) == 1 and create(k_codes=None) == 1
+    assert create(kind=2) == 2  # SE12_ERR_UNSUPPORTED_FORMAT
+    assert create(v_codes=257) == 3  # SE12_ERR_MISALIGNED
+    assert create(pages=1 << 27) == 1 and b"31 bits" in lib.se12_last_error()
+    assert lib.se12_kv_append(None, None, None, None) == 1
+    assert lib.se12_kv_attend(None, None, None, None, 0, None) == 1
+    assert lib.se12_kv_decode(None, None, 1, None, None, None) == 1
+    assert lib.se12_kv_attend_workspace_bytes(None) == 0
+    lib.se12_kv_cache_destroy(None)
+
+
+def test_least_scale_holds_the_largest_magnitude():
+    for kind in QMAX:
+        for x in (0.0, 1e-40, 1e-30, 0.7, 127.0, 127.00001, 448.0, 449.0, 3e38):
+            s = least_scale(x, kind)
+            assert x <= QMAX[kind] * s and (s == 2.0**-100 or x > QMAX[kind] * s / 2)
+
+
+# ------------------------------------------------------------------ GPU helpers
+
+
+def random_tables(g, lens, page, spare=3):
+    """A page table with the sequences' pages in random order, and the pool's size."""
+    need = [(ln + page - 1) // page for ln in lens]
+    pool = sum(need) + spare
+    order = torch.randperm(pool, generator=g)
+    table = torch.full((len(lens), max(max(need), 1) + 1), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at : at + n]
+        at += n
+    table[:, -1] = 1 << 30  # entries past a sequence's pages may hold anything
+    return table, pool
+
+
+def starts_of(counts):
+    starts = [0]
+    for n in counts:
+        starts.append(starts[-1] + n)
+    return starts
+
+
+def make_pair(pages, page, heads, dim, kind):
+    from se12_b200.kv_cache import PagedKvCache
+
+    return PagedKvCache(pages, page, heads, dim, kind), PlainCache(pages, page, heads, dim, kind)
+
+
+def same_cache(cache, plain):
+    for w, codes, scales in (("k", cache.k_codes, cache.k_scales), ("v", cache.v_codes, cache.v_scales)):
+        assert torch.equal(scales.cpu().view(torch.int32), plain.scales[w].view(torch.int32)) or (
+            torch.equal(scales.cpu().isnan(), plain.scales[w].isnan())
+            and torch.equal(scales.cpu().nan_to_num(), plain.scales[w].nan_to_num()))
+        assert torch.equal(codes.cpu(), plain.codes[w]), f"{w} codes"
+
+
+def rope(g, rows, half):
+    angle = torch.rand(rows, half, generator=g) * 6.3
+    return torch.cos(angle), torch.sin(angle)
+
+
+# ------------------------------------------------------------------ append
+
+
+APPEND = [
+    # kind, dtype, page, heads, q_heads, dim, rotary (0: none), interleaved
+    ("int8", torch.float32, 16, 2, 4, 256, 256, False),
+    ("e4m3", torch.float32, 32, 2, 6, 128, 128, False),
+    ("int8", torch.bfloat16, 64, 3, 3, 128, 128, False),
+    ("e4m3", torch.bfloat16, 16, 1, 8, 256, 256, False),
+    ("int8", torch.float32, 16, 2, 2, 64, 64, False),
+    ("int8", torch.float32, 16, 2, 2, 96, 32, False),    # partial rotation
+    ("e4m3", torch.bfloat16, 16, 2, 2, 80, 80, True),    # neighbouring pairs
+    ("int8", torch.bfloat16, 128, 1, 2, 192, 64, True),
+    ("e4m3", torch.float32, 16, 1, 1, 16, 2, False),
+    ("int8", torch.float32, 256, 2, 2, 128, 0, False),   # no rotation
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype,page,heads,q_heads,dim,rotary,interleaved", APPEND)
+@pytest.mark.parametrize("steps", [
+    [[1, 1, 1, 1, 1]] * 3,                                    # next tokens
+    [[40, 1, 0, 17, 3], [1, 16, 33, 0, 2], [5, 5, 5, 5, 5]],  # prompts, continued
+    [[300, 0, 0, 0, 1], [1, 1, 1, 1, 1]],
+])
+def test_append_stores_the_same_codes(kind, dtype, page, heads, q_heads, dim, rotary, interleaved, steps):
+    g = torch.Generator().manual_seed(dim + page)
+    counts = [sum(s[b] for s in steps) for b in range(5)]
+    table, pool = random_tables(g, counts, page)
+    cache, plain = make_pair(pool, page, heads, dim, kind)
+    cos, sin = rope(g, max(counts), rotary // 2) if rotary else (None, None)
+    dev_table = table.cuda()
+    lens = [0] * 5
+    for step, new in enumerate(steps):
+        lens = [a + b for a, b in zip(lens, new)]
+        starts = starts_of(new)
+        # q, k and v side by side; magnitudes grow, so that blocks' scales do
+        y = torch.randn(starts[-1], q_heads + 2 * heads, dim, generator=g) * 3.0**step * (1 + 9 * torch.rand(dim, generator=g))
+        y = y.to(dtype)
+        q, k, v = y[:, :q_heads], y[:, q_heads : q_heads + heads], y[:, q_heads + heads :]
+        want = plain.append(k, v, table, lens, starts, cos, sin, interleaved, q)
+        d = y.cuda()
+        start = None if all(n == 1 for n in new) else torch.tensor(starts, dtype=torch.int32).cuda()
+        got = cache.append(d[:, q_heads : q_heads + heads], d[:, q_heads + heads :], dev_table,
+                           torch.tensor(lens, dtype=torch.int32).cuda(), q=d[:, :q_heads], query_start=start,
+                           cos=None if cos is None else cos.cuda(), sin=None if sin is None else sin.cuda(),
+                           interleaved=interleaved)
+        assert torch.equal(got.cpu().view(torch.int16), want.view(torch.int16))
+        same_cache(cache, plain)
+    keys, values = cache.decode()
+    assert torch.equal(keys.double().cpu(), plain.values("k")) and torch.equal(values.double().cpu(), plain.values("v"))
+    some = torch.tensor([int(table[0, 0]), 0, int(table[0, 0])], dtype=torch.int32)
+    keys, values = cache.decode(some.cuda())
+    assert torch.equal(keys.double().cpu(), plain.values("k")[some.long()])
+    assert torch.equal(values.double().cpu(), plain.values("v")[some.long()])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens_each", [1, 3])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_append_takes_any_strides(tokens_each, dim):
+    """Rows at odd offsets, heads far apart, an output with its own strides,
+    a rotation table cut from a wider one: the scalar path, the same codes."""
+    g = torch.Generator().manual_seed(5)
+    heads, q_heads, seqs, page = 2, 4, 3, 16
+    lens = [20, 7, 33]
+    table, pool = random_tables(g, lens, page)
+    cache, plain = make_pair(pool, page, heads, dim, "int8")
+    cos, sin = rope(g, 40, dim // 2)
+    starts = starts_of([tokens_each] * seqs)
+    t = starts[-1]
+    start = None if tokens_each == 1 else torch.tensor(starts, dtype=torch.int32).cuda()
+
+    def odd(x):  # the same values, one element past an aligned address, head stride dim + 3
+        wide = torch.zeros(t, x.shape[1], dim + 3)
+        wide[:, :, 1 : dim + 1] = x
+        return wide.cuda()[:, :, 1 : dim + 1]
+
+    q, k, v = torch.randn(t, q_heads, dim, generator=g), torch.randn(t, heads, dim, generator=g), torch.randn(t, heads, dim, generator=g)
+    want = plain.append(k, v, table, lens, starts, cos, sin, False, q)
+    out = torch.full((t, q_heads, dim + 5), 7.0, dtype=torch.bfloat16, device="cuda")
+    wide = torch.zeros(2, 40, dim // 2 + 1)
+    wide[0, :, 1:], wide[1, :, 1:] = cos, sin
+    wide = wide.cuda()
+    got = cache.append(odd(k), odd(v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), q=odd(q), query_start=start,
+                       cos=wide[0][:, 1:], sin=wide[1][:, 1:], q_out=out[:, :, 2 : dim + 2])
+    assert torch.equal(got.cpu().view(torch.int16), want.view(torch.int16))
+    assert bool((out[:, :, :2] == 7).all()) and bool((out[:, :, dim + 2 :] == 7).all())
+    same_cache(cache, plain)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_repeated_growth_stays_below_a_step(kind):
+    """Tokens whose magnitudes double again and again, appended one by one:
+    the older values stay within the sum of the roundings. int8: each growth
+    by 2^g rounds to half of the new step, and the steps at least double, so
+    below one step of the last scale. e4m3: a relative 2^-4 at most once
+    (exponent shifts are exact) plus half of the subnormal step 2^-9 each time."""
+    g = torch.Generator().manual_seed(2)
+    page, dim = 64, 128
+    x = torch.randn(page, 1, dim, generator=g) * 2.0 ** (torch.arange(page) / 5.0)[:, None, None]
+    cache, plain = make_pair(2, page, 1, dim, kind)
+    table = torch.tensor([[1]], dtype=torch.int32)
+    for i in range(page):
+        lens = torch.tensor([i + 1], dtype=torch.int32).cuda()
+        cache.append(x[i : i + 1].cuda(), x[i : i + 1].cuda(), table.cuda(), lens)
+        plain.append(x[i : i + 1], x[i : i + 1], table, [i + 1], [0, 1])
+    same_cache(cache, plain)
+    keys, _ = cache.decode()
+    step = float(cache.k_scales[1, 0])
+    err = (keys[1, 0].double().cpu() - x[:, 0].double()).abs()
+    assert float(err.max()) <= step if kind == "int8" else bool((err <= 2.0**-4 * x[:, 0].abs() + 2.0**-9 * step).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_value_that_is_not_finite_poisons_its_block(prompt, bad):
+    page, dim = 16, 128
+    cache, plain = make_pair(3, page, 2, dim, "int8")
+    table = torch.tensor([[2, 0]], dtype=torch.int32)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(17, 2, dim, generator=g)
+    x[9, 1, 5] = bad
+
+    def feed(a, b):
+        cache.append(x[a:b].cuda(), x[a:b].cuda(), table.cuda(), torch.tensor([b], dtype=torch.int32).cuda(),
+                     query_start=torch.tensor([0, b - a], dtype=torch.int32).cuda() if prompt else None)
+        plain.append(x[a:b], x[a:b], table, [b], [0, b - a])
+
+    for a, b in [(0, 5), (5, 12), (12, 17)] if prompt else [(i, i + 1) for i in range(17)]:
+        feed(a, b)
+    same_cache(cache, plain)
+    assert bool(cache.k_scales[2, 1].isnan()) and not bool(cache.k_scales[2, 0].isnan()) and not bool(cache.k_scales[0].isnan().any())
+    q = torch.randn(1, 4, dim, generator=g).to(torch.bfloat16)
+    out = cache.attend(q.cuda(), table.cuda(), torch.tensor([17], dtype=torch.int32).cuda()).cpu()
+    assert bool(out[0, 2:].isnan().all()) and not bool(out[0, :2].isnan().any())
+    # outside the window the poisoned block does not count
+    out = cache.attend(q.cuda(), table.cuda(), torch.tensor([17], dtype=torch.int32).cuda(), window=1).cpu()
+    assert not bool(out.isnan().any())
+    # a page that starts anew is clean again
+    cache.append(x[:1].cuda(), x[:1].cuda(), table.cuda(), torch.tensor([1], dtype=torch.int32).cuda())
+    assert not bool(cache.k_scales.isnan().any())
+
+
+@pytest.mark.gpu
+def test_padding_rows_store_nothing():
+    cache, _ = make_pair(3, 16, 2, 128, "int8")
+    before = cache.k_codes.clone()
+    table = torch.full((2, 1), -1, dtype=torch.int32, device="cuda")
+    x = torch.randn(2, 2, 128, device="cuda")
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    cos = torch.ones(1, 64, device="cuda")
+    for start in (None, torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")):
+        q = cache.append(x, x, table, lens, q=x, cos=cos, sin=cos, query_start=start)
+        assert bool((q == 0).all()) and torch.equal(cache.k_codes, before)
+        assert bool((cache.attend(q, table, lens, query_start=start) == 0).all())
+    # more new rows than the sequence is long: the first ones are padding
+    q = cache.append(x, x, torch.tensor([[1]], dtype=torch.int32, device="cuda"), lens[:1] + 1, q=x,
+                     query_start=torch.tensor([0, 2], dtype=torch.int32, device="cuda"))
+    assert bool((q[0] == 0).all()) and bool((q[1] == x[1].to(torch.bfloat16)).all())
+    assert bool((cache.k_codes[1, :, 0] != 0).any()) and bool((cache.k_codes[1, :, 1:] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prompt", [False, True])
+def test_indexes_out_of_range_set_the_status(prompt):
+    from se12_b200.device import device_status
+
+    cache, _ = make_pair(3, 16, 2, 128, "int8")
+    x = torch.randn(1, 2, 128, device="cuda")
+    start = torch.tensor([0, 1], dtype=torch.int32, device="cuda") if prompt else None
+    cos = torch.ones(4, 64, device="cuda")
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for table, lens, table_cos in ((ints([[3]]), ints([1]), None), (ints([[-1]]), ints([1]), None), (ints([[0]]), ints([17]), None),
+                                   (ints([[0]]), ints([5]), cos)):
+        q = cache.append(x, x, table, lens, q=x, cos=table_cos, sin=table_cos, query_start=start)
+        assert device_status() == 2
+        assert bool((cache.k_codes == 0).all()) and (table_cos is None or bool((q == 0).all()))
+        if table_cos is None:
+            out = cache.attend(x.to(torch.bfloat16), table, lens, query_start=start)
+            assert device_status() == 2 and bool(torch.isfinite(out).all())
+    keys, _ = cache.decode(ints([0, 7]))
+    assert device_status() == 2 and bool((keys[1] == 0).all())
+
+
+# ------------------------------------------------------------------ attention
+
+
+def filled(g, pool, page, heads, dim, kind, spread=1.0):
+    """A cache whose blocks hold random codes, with scales 2^(+-spread)."""
+    from se12_b200.kv_cache import PagedKvCache
+
+    tensors = []
+    for _ in range(2):
+        x = torch.randn(pool, heads, page, dim, generator=g)
+        x *= 2.0 ** ((torch.rand(pool, heads, 1, 1, generator=g) * 2 - 1) * spread)
+        s = torch.tensor([[least_scale(float(x[p, h].abs().max()), kind) for h in range(heads)] for p in range(pool)])
+        tensors.append((code_of(x / s[:, :, None, None], kind), s))
+    (k, ks), (v, vs) = tensors
+    cache = PagedKvCache.from_tensors(k.cuda(), v.cuda(), ks.cuda(), vs.cuda(), kind)
+    return cache, value_of(k, kind).double() * ks.double()[:, :, None, None], value_of(v, kind).double() * vs.double()[:, :, None, None]
+
+
+def attend_case(seed, kind, page, heads, q_heads, dim, lens, counts, softcap=0.0, window=0, spread=1.0, q_scale=1.0,
+                max_query=None, scale=None):
+    g = torch.Generator().manual_seed(seed)
+    table, pool = random_tables(g, lens, page)
+    cache, keys, values = filled(g, pool, page, heads, dim, kind, spread)
+    starts = starts_of(counts)
+    q = (torch.randn(starts[-1], q_heads, dim, generator=g) * q_scale).to(torch.bfloat16)
+    start = None if all(n == 1 for n in counts) and max_query is None else torch.tensor(starts, dtype=torch.int32).cuda()
+    args = (table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    got = cache.attend(q.cuda(), *args, query_start=start, softcap=softcap, window=window, scale=scale, max_query=max_query)
+    want = plain_attend(q, keys, values, table, lens, starts, dim**-0.5 if scale is None else scale, softcap, window)
+    check_attend(got, *want, max(lens))
+    again = cache.attend(q.cuda(), *args, query_start=start, softcap=softcap, window=window, scale=scale, max_query=max_query)
+    assert torch.equal(got.view(torch.int16), again.view(torch.int16))
+    return cache, q, args, got
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_attend_lengths_around_pages_and_tiles(kind, page, dim):
+    attend_case(page + dim, kind, page, 2, 4, dim, [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 255, 256, 257, 700], [1] * 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [16, 48, 64, 80, 96, 112, 144, 192, 240])
+def test_attend_head_dimensions(dim):
+    attend_case(dim, "int8" if dim % 32 else "e4m3", 32, 2, 2, dim, [5, 100], [1, 1], softcap=20.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,q_heads", [(1, 1), (1, 8), (2, 6), (4, 20), (1, 16), (2, 34), (3, 3), (1, 64)])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_attend_head_layouts(heads, q_heads, dim):
+    attend_case(heads * 100 + q_heads, "int8", 16, heads, q_heads, dim, [77, 3], [1, 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("window", [0, 1, 7, 16, 100])
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+def test_attend_windows_and_several_queries(kind, dim, window, softcap):
+    """Drafted tokens and prompt chunks, idle sequences, and more rows than
+    the sequence is long (the first ones see nothing)."""
+    counts = [1, 4, 0, 19, 33, 3, 0]
+    cache, q, args, got = attend_case(window + dim, kind, 16, 2, 6, dim, [40, 4, 9, 200, 33, 2, 0], counts, softcap=softcap,
+                                      window=window)
+    start = torch.tensor(starts_of(counts), dtype=torch.int32).cuda()
+    bound = cache.attend(q.cuda(), *args, query_start=start, softcap=softcap, window=window, max_query=33)
+    assert torch.allclose(bound.float(), got.float(), rtol=2.0**-6, atol=2.0**-7)
+    assert bool((got[starts_of(counts)[5]] == 0).all())  # position -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,q_heads,heads", [(128, 8, 1), (256, 4, 2), (128, 12, 1), (256, 12, 1)])
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 8, 17, 70])
+def test_attend_query_counts(dim, q_heads, heads, n):
+    attend_case(n, "e4m3", 64, heads, q_heads, dim, [300, n], [n, n], max_query=n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [5000, 20011])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_attend_one_long_sequence_is_split(length, dim):
+    attend_case(length, "int8", 128, 1, 4, dim, [length], [1], softcap=30.0)
+    attend_case(length, "e4m3", 16, 2, 2, dim, [length, 1, 3, length // 2], [1, 1, 1, 1], window=length // 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_attend_blocks_of_very_different_scales(kind):
+    """Scales from 2^-40 to 2^40: a weight's precision does not depend on
+    what other blocks hold."""
+    attend_case(9, kind, 16, 2, 4, 128, [200, 45], [1, 1], spread=40.0, q_scale=2.0**-41)
+    attend_case(10, kind, 16, 2, 4, 256, [200, 45], [2, 2], spread=18.0, scale=2.0**-20)
+
+
+@pytest.mark.gpu
+def test_attend_weights_of_zero_values_count():
+    """Tokens whose values are all zero still take their share."""
+    from se12_b200.kv_cache import PagedKvCache
+
+    cache = PagedKvCache(2, 16, 1, 128)
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    k = torch.zeros(32, 1, 128, device="cuda")
+    v = torch.zeros(32, 1, 128, device="cuda")
+    v[16:] = 8.0
+    lens = torch.tensor([32], dtype=torch.int32, device="cuda")
+    cache.append(k, v, table, lens, query_start=torch.tensor([0, 32], dtype=torch.int32, device="cuda"))
+    out = cache.attend(torch.ones(1, 2, 128, dtype=torch.bfloat16, device="cuda"), table, lens)
+    assert bool((out == 4.0).all())
+
+
+@pytest.mark.gpu
+def test_attend_ignores_what_lies_past_the_length():
+    """NaN codes and scales of other pages and slots do not reach the output."""
+    g = torch.Generator().manual_seed(4)
+    cache, keys, values = filled(g, 4, 32, 1, 128, "e4m3")
+    table = torch.tensor([[1, 3, 2]], dtype=torch.int32).cuda()
+    lens = torch.tensor([41], dtype=torch.int32).cuda()
+    q = torch.randn(1, 4, 128, generator=g).to(torch.bfloat16).cuda()
+    want = cache.attend(q, table, lens)
+    for codes in (cache.k_codes, cache.v_codes):
+        codes[3, :, 9:] = 0x7F  # NaN
+        codes[2] = -1
+    for scales in (cache.k_scales, cache.v_scales):
+        scales[2] = math.nan
+        scales[0] = math.inf
+    assert torch.equal(cache.attend(q, table, lens).view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.gpu
+def test_attend_queries_that_are_not_finite_stay_in_their_rows():
+    cache, q, args, got = attend_case(6, "int8", 16, 1, 4, 128, [50, 9], [1, 1])
+    q[0, 1, 3] = math.nan
+    q[0, 2, 7] = math.inf
+    out = cache.attend(q.cuda(), *args)
+    assert bool(out[0, 1].isnan().all()) and bool(out[0, 2].isnan().all())
+    for t, h in ((0, 0), (0, 3), (1, 0), (1, 1), (1, 2), (1, 3)):
+        assert torch.equal(out[t, h].view(torch.int16), got[t, h].view(torch.int16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [128, 256])
+def test_attend_takes_any_strides(dim):
+    cache, q, args, got = attend_case(7, "int8", 16, 2, 4, dim, [50, 9, 130], [1, 1, 1])
+    wide = torch.zeros(3, 4, dim + 3, dtype=torch.bfloat16)
+    wide[:, :, 1 : dim + 1] = q
+    out = torch.full((3, 4, dim + 2), 5.0, dtype=torch.bfloat16, device="cuda")
+    res = cache.attend(wide.cuda()[:, :, 1 : dim + 1], *args, out=out[:, :, 1 : dim + 1])
+    assert torch.equal(res.contiguous().view(torch.int16), got.view(torch.int16))
+    assert bool((out[:, :, 0] == 5).all()) and bool((out[:, :, -1] == 5).all())
+    # a column of a wider table
+    table = torch.cat([args[0], args[0]], dim=1)[:, : args[0].shape[1]]
+    assert torch.equal(cache.attend(q.cuda(), table, args[1]).view(torch.int16), got.view(torch.int16))
+
+
+@pytest.mark.gpu
+def test_attend_many_sequences():
+    lens = [(i * 37) % 70 for i in range(600)]
+    attend_case(8, "int8", 16, 1, 2, 128, lens, [1] * 600)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A pool of more than 2^32 codes: the last pages are the last pages."""
+    from se12_b200.kv_cache import PagedKvCache
+
+    page, heads, dim = 256, 8, 256
+    pages = (1 << 32) // (page * heads * dim) + 40
+    cache = PagedKvCache(pages, page, heads, dim)
+    g = torch.Generator().manual_seed(1)
+    n = 300
+    x, y = torch.randn(n, heads, dim, generator=g), torch.randn(n, heads, dim, generator=g)
+    ids = [pages - 1, pages - 7]
+    table = torch.tensor([ids], dtype=torch.int32)
+    lens = torch.tensor([n], dtype=torch.int32).cuda()
+    cache.append(x.cuda(), y.cuda(), table.cuda(), lens, query_start=torch.tensor([0, n], dtype=torch.int32).cuda())
+    small = PlainCache(2, page, heads, dim, "int8")
+    small.append(x, y, torch.tensor([[0, 1]]), [n], [0, n])
+    assert torch.equal(cache.k_codes[ids].cpu(), small.codes["k"]) and torch.equal(cache.v_codes[ids].cpu(), small.codes["v"])
+    assert bool((cache.k_codes[:2] == 0).all())
+    q = torch.randn(1, heads, dim, generator=g).to(torch.bfloat16)
+    got = cache.attend(q.cuda(), table.cuda(), lens)
+    want = plain_attend(q, small.values("k"), small.values("v"), torch.tensor([[0, 1]]), [n], [0, 1], dim**-0.5, 0.0, 0)
+    check_attend(got, *want, n)
+    keys, _ = cache.decode(torch.tensor(ids, dtype=torch.int32).cuda())
+    assert torch.equal(keys.double().cpu(), small.values("k"))
+
+
+@pytest.mark.gpu
+def test_a_captured_step_follows_lengths_and_tables():
+    """append + attend in one graph, replayed with other lengths and pages:
+    the bits of the eager calls; also on a stream of its own."""
+    from se12_b200.kv_cache import PagedKvCache
+
+    g = torch.Generator().manual_seed(11)
+    heads, q_heads, dim, page, seqs = 2, 4, 128, 16, 3
+    pool = 3 * 40
+    caches = [PagedKvCache(pool, page, heads, dim, "int8") for _ in range(2)]
+    table = torch.randperm(pool, generator=g).to(torch.int32).view(seqs, 40).cuda()
+    cos, sin = (t.cuda() for t in rope(g, 700, dim // 2))
+    lens = torch.ones(seqs, dtype=torch.int32, device="cuda")
+    y = torch.randn(seqs, q_heads + 2 * heads, dim, generator=g).cuda()
+
+    def step(cache):
+        q = cache.append(y[:, q_heads : q_heads + heads], y[:, q_heads + heads :], table, lens, q=y[:, :q_heads], cos=cos, sin=sin)
+        return cache.attend(q, table, lens)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(caches[1])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(caches[1])
+    torch.cuda.synchronize()
+    for i in range(60):
+        fresh = torch.randn(seqs, q_heads + 2 * heads, dim, generator=g)
+        y.copy_(fresh.cuda())
+        lens.copy_(torch.tensor([i + 1, 10 * i + 1, 0 if i < 30 else i - 29], dtype=torch.int32))
+        want = step(caches[0])
+        with torch.cuda.stream(stream):
+            stream.wait_stream(torch.cuda.default_stream())
+            graph.replay()
+        torch.cuda.default_stream().wait_stream(stream)
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16)), i
+    assert torch.equal(caches[0].k_codes, caches[1].k_codes) and torch.equal(caches[0].v_scales, caches[1].v_scales)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    from se12_b200.kv_cache import PagedKvCache
+
+    cache = PagedKvCache(4, 16, 2, 64)
+    x = torch.randn(2, 2, 64, device="cuda")
+    q = x.to(torch.bfloat16)
+    table = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    lens = torch.ones(2, dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    cos = torch.ones(4, 32, device="cuda")
+    for call in (
+        lambda: cache.append(x[:, :1], x, table, lens),
+        lambda: cache.append(x, x[:1], table, lens),
+        lambda: cache.append(x[:, :, :32], x, table, lens),
+        lambda: cache.append(x, x, table, lens[:1]),
+        lambda: cache.append(x, x, table.long(), lens),
+        lambda: cache.append(x, x, table, lens.long()),
+        lambda: cache.append(x, x, table, lens, cos=cos),
+        lambda: cache.append(x, x, table, lens, cos=cos, sin=cos[:3]),
+        lambda: cache.append(x, x, table, lens, cos=cos.repeat(1, 2), sin=cos.repeat(1, 2)),
+        lambda: cache.append(x, x, table, lens, query_start=start[:2]),
+        lambda: cache.append(x, x, table, lens, q_out=q),
+        lambda: cache.append(x.cpu(), x, table, lens),
+        lambda: cache.append(x.transpose(1, 2).contiguous().transpose(1, 2), x, table, lens),
+        lambda: cache.attend(q[:, :1], table, lens),
+        lambda: cache.attend(q, table, lens, query_start=start.long()),
+        lambda: cache.attend(q, table.cpu(), lens),
+        lambda: cache.attend(q, table, lens, out=torch.empty(2, 2, 32, dtype=torch.bfloat16, device="cuda")),
+        lambda: cache.decode(lens.long()),
+        lambda: PagedKvCache.from_tensors(cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales[:2]),
+        lambda: PagedKvCache.from_tensors(cache.k_codes.float(), cache.v_codes.float(), cache.k_scales, cache.v_scales),
+    ):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: cache.append(x.half(), x.half(), table, lens), lambda: cache.append(x, x.to(torch.bfloat16), table, lens),
+                 lambda: cache.attend(x, table, lens)):
+        with pytest.raises(TypeError):
+            call()
+    for args in (dict(window=-1), dict(softcap=-1.0), dict(softcap=math.inf), dict(scale=math.nan), dict(max_query=0),
+                 dict(max_query=2)):
+        with pytest.raises(RuntimeError):
+            cache.attend(q, table, lens, **args)
+    assert cache.append(x[:0], x[:0], table, lens, q=x[:0]).shape == (0, 2, 64)
+    assert cache.attend(q[:0], table, lens).shape == (0, 2, 64)

@@ -1,0 +1,255 @@
+"""Token log probabilities against 64-bit sums over the same logits.
+
+Tolerance of a log probability or an entropy, absolute: a term exp(z - M)
+carries 2^-22 (the exponential) and the rounding of (z - M) log2(e) (2^-24 of
+at most 200), sums of a few dozen roundings of 2^-24, so below 1e-5 of the
+sum, plus 2^-21 of the result; capped logits are off by at most 2^-20 of the
+cap (the exponential's and the quotient's 2^-22 and the argument's rounding).
+Ids are exact.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from se12_b200.logprobs import MAX_TOP, token_logprobs
+
+
+def plain(x: torch.Tensor, tokens: torch.Tensor, top: int, softcap: float):
+    x64 = x.double()
+    z = x64 if not softcap else torch.where(x64 == -math.inf, x64, softcap * torch.tanh(x64 / softcap))
+    logp = torch.log_softmax(z, -1)
+    p = logp.exp()
+    entropy = -torch.where(p == 0, torch.zeros_like(p), p * logp).sum(-1)
+    safe = tokens.clamp(0, x.shape[1] - 1)
+    lp = logp.gather(1, safe[:, None])[:, 0]
+    lp = torch.where((tokens < 0) | (tokens >= x.shape[1]), torch.full_like(lp, math.nan), lp)
+    order = torch.where(x64.isnan(), torch.full_like(x64, math.inf), x64.clamp(-1e308, 1e307))  # NaN above +inf
+    ids = torch.sort(order, dim=-1, descending=True, stable=True).indices[:, :top]
+    return lp, entropy, ids, logp.gather(1, ids)
+
+
+def check(x: torch.Tensor, tokens: torch.Tensor, top: int, softcap: float = 0.0, device_logits=None):
+    got = token_logprobs(x.cuda() if device_logits is None else device_logits, tokens.cuda(), top=top, softcap=softcap)
+    want = plain(x, tokens, top, softcap)
+    assert got.top_ids.shape == (x.shape[0], top) and got.top_ids.dtype == torch.int64
+    assert torch.equal(got.top_ids.cpu(), want[2])
+    for g, w in ((got.logprob, want[0]), (got.entropy, want[1]), (got.top_logprobs, want[3])):
+        g = g.double().cpu()
+        assert torch.equal(g.isnan(), w.isnan()) and torch.equal(g.isinf(), w.isinf())
+        fine = torch.isfinite(w)
+        tol = 1e-5 + 2.0**-20 * softcap + 2.0**-21 * w.abs()
+        assert bool(((g - w).abs() <= tol)[fine].all()), float(((g - w).abs() / tol)[fine].max())
+    return got
+
+
+def logits(seed: int, rows: int, vocab: int, dtype=torch.float32, spread: float = 3.0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(rows, vocab, generator=g) * spread).to(dtype)
+    return x, torch.randint(0, vocab, (rows,), generator=g)
+
+
+# ------------------------------------------------------------------ CPU: refusals
+
+
+def test_refusals():
+    x, t = torch.zeros(2, 10), torch.zeros(2, dtype=torch.int64)
+    for call in (
+        lambda: token_logprobs(x[0], t),
+        lambda: token_logprobs(x.half(), t),
+        lambda: token_logprobs(x.double(), t),
+        lambda: token_logprobs(x.t().contiguous().t(), t),
+        lambda: token_logprobs(x, t.int()),
+        lambda: token_logprobs(x, t[:1]),
+        lambda: token_logprobs(x, t, top=-1),
+        lambda: token_logprobs(x, t, top=11),
+        lambda: token_logprobs(torch.zeros(2, 100), t, top=MAX_TOP + 1),
+        lambda: token_logprobs(x, t, softcap=-1.0),
+        lambda: token_logprobs(x, t, softcap=math.inf),
+        lambda: token_logprobs(x, t, softcap=math.nan),
+        lambda: token_logprobs(x, t),  # not on a GPU
+    ):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_abi_refuses_bad_arguments_without_a_device():
+    from se12_b200 import _build, _lib
+
+    _build.build()
+    lib = _lib.load()
+    need = lib.se12_token_logprobs_workspace_bytes()
+
+    def call(logits=256, rows=2, vocab=10, ld=10, tokens=256, top=2, softcap=0.0, ids=256, ws=256, size=need):
+        return lib.se12_token_logprobs(logits, 0, rows, vocab, ld, tokens, top, softcap, 256, 256, ids, 256, ws, size, None)
+
+    assert call(logits=None) == 1 and call(tokens=None) == 1 and call(rows=0) == 1 and call(ld=9) == 1 and call(top=33) == 1
+    assert call(top=11) == 1 and call(ids=None) == 1 and call(softcap=-1.0) == 1 and call(softcap=math.nan) == 1
+    assert call(ws=None) == 4 and call(size=need - 1) == 4 and call(ws=264) == 3
+
+
+# ------------------------------------------------------------------ GPU
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 2), (3, 31), (2, 33), (5, 1000), (4, 8191), (4, 8192), (4, 8193), (1, 100003),
+                                        (2, 256000), (700, 4099), (301, 16384), (1, 1000000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_sizes(rows, vocab, dtype, softcap):
+    x, t = logits(rows + vocab, rows, vocab, dtype)
+    for top in sorted({0, min(1, vocab), min(5, vocab), min(32, vocab)}):
+        check(x, t, top, softcap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [50, 9000, 70000])
+def test_equal_values_go_to_the_lowest_id(vocab):
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randint(-3, 3, (6, vocab), generator=g).to(torch.float32)
+    x[0] = 1.0                       # a constant row
+    x[1] = torch.where(torch.rand(vocab, generator=g) < 0.5, 0.0, -0.0)  # zeros of both signs are equal
+    x[2, 7:] = -math.inf
+    t = torch.randint(0, vocab, (6,), generator=g)
+    check(x, t, 20)
+    check(x.to(torch.bfloat16), t, 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [300, 40000])
+def test_sorted_rows(vocab):
+    """Every value of an ascending row enters the list."""
+    x = torch.linspace(-20, 20, vocab)[None].repeat(3, 1)
+    x[1] = x[1].flip(0)
+    x[2] = x[2].roll(vocab // 2)
+    check(x, torch.tensor([0, 1, vocab - 1]), 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("vocab", [40, 20000, 200000])
+def test_banned_tokens(vocab, softcap):
+    g = torch.Generator().manual_seed(1)
+    x, t = logits(3, 6, vocab)
+    x[0, torch.rand(vocab, generator=g) < 0.9] = -math.inf
+    x[1] = -math.inf
+    x[1, vocab // 2] = 2.0               # one token left
+    x[2] = -math.inf
+    x[2, -3:] = torch.tensor([1.0, 1.0, -4.0])
+    x[3, : vocab // 2] = -math.inf
+    x[4, 5:] = -math.inf                 # fewer tokens than alternatives
+    t[0] = int((x[0] == -math.inf).nonzero()[0, 0])  # a banned token: -inf
+    check(x, t, 20, softcap)
+    check(x.to(torch.bfloat16), t, 20, softcap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [40, 20000])
+def test_masks_of_the_lowest_value_and_empty_rows(vocab):
+    low = torch.finfo(torch.float32).min
+    x, t = logits(4, 7, vocab)
+    x[0, ::2] = low
+    x[1] = low                           # uniform
+    x[2] = -math.inf                     # nothing left: NaN
+    x[3] = low
+    x[3, 3] = -math.inf
+    x[4] = low
+    x[4, 9] = 0.5
+    x[5] = -3.0e38
+    x[6, 11] = 3.0e38                    # forced
+    got = check(x, t, 5)
+    assert bool(got.logprob[2].isnan()) and got.top_ids[2].tolist() == [0, 1, 2, 3, 4]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("vocab", [100, 20000])
+def test_values_that_are_not_finite_stay_in_their_rows(vocab, bad):
+    x, t = logits(5, 4, vocab)
+    x[1, vocab - 1] = bad
+    x[2, 0] = bad
+    x[2, 60] = bad
+    got = check(x, t, 8)
+    assert bool(got.logprob[1].isnan()) and bool(got.entropy[2].isnan()) and not bool(got.logprob[0].isnan())
+    assert int(got.top_ids[1, 0]) == vocab - 1 and got.top_ids[2, :2].tolist() == [0, 60]
+
+
+@pytest.mark.gpu
+def test_tokens_outside_the_vocabulary():
+    from se12_b200.device import device_status
+
+    x, _ = logits(6, 3, 500)
+    check(x, torch.tensor([-1, 5, -100]), 3)
+    assert device_status() == 0
+    check(x, torch.tensor([499, 500, 1 << 40]), 3)
+    assert device_status() == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pad,offset", [(8, 0), (3, 0), (5, 1), (0, 3)])
+def test_strides_and_alignment(dtype, pad, offset):
+    x, t = logits(7, 5, 9001, dtype)
+    wide = torch.full((5, 9001 + pad + offset), 99.0, dtype=dtype)
+    wide[:, offset : offset + 9001] = x
+    check(x, t, 10, device_logits=wide.cuda()[:, offset : offset + 9001])
+
+
+@pytest.mark.gpu
+def test_large_and_small_logits():
+    for spread in (1e-3, 100.0, 1e4):
+        x, t = logits(8, 3, 30000, spread=spread)
+        check(x, t, 5)
+    x, t = logits(9, 3, 30000)
+    check(x + 1000.0, t, 5)
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    x, t = logits(10, 2, 150000)
+    dx, dt = x.cuda(), t.cuda()
+    want = token_logprobs(dx, dt, top=7, softcap=30.0)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = token_logprobs(dx, dt, top=7, softcap=30.0)
+        for _ in range(3):
+            graph.replay()
+    stream.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    y, _ = logits(11, 2, 150000)
+    dx.copy_(y.cuda())
+    want = token_logprobs(dx, dt, top=7, softcap=30.0)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_rows_past_31_bits_of_values():
+    """More than 2^31 logits: the last rows are the last rows."""
+    rows, vocab = 16400, 131072
+    x = torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    y, t = logits(12, 2, vocab, torch.bfloat16)
+    x[-2:] = y.cuda()
+    tokens = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    tokens[-2:] = t.cuda()
+    got = token_logprobs(x, tokens, top=3)
+    want = plain(y, t, 3, 0.0)
+    assert torch.equal(got.top_ids[-2:].cpu(), want[2]) and got.top_ids[:-2].unique().tolist() == [0, 1, 2]
+    assert bool(((got.logprob[-2:].cpu().double() - want[0]).abs() <= 1e-5 + 2.0**-21 * want[0].abs()).all())
+    assert bool(((got.logprob[:-2].double() + math.log(vocab)).abs() < 1e-5).all())
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    got = token_logprobs(torch.zeros(0, 10, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda"), top=3)
+    assert got.logprob.shape == (0,) and got.top_ids.shape == (0, 3)
