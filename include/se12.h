@@ -383,6 +383,7 @@ int se12_encode_raw(const uint16_t* w_dev, int rows, int cols, int ldw, const in
 #define SE12_KV_INT8 0
 #define SE12_KV_E4M3 1
 #define SE12_KV_MAX_SEQS 2048
+#define SE12_COUNTER_BYTES 4096
 
 typedef struct se12_kv_pages {
   int32_t pages, page_size, kv_heads, head_dim;
@@ -452,9 +453,10 @@ int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const
  * with p - j < window. A row that sees nothing is zero. q and out: BF16
  * [tokens][q_heads][head_dim] with token and head strides; query head h uses
  * KV head h / (q_heads / kv_heads). max_query: the largest number of rows of a
- * sequence. The workspace is zeroed once (se12_workspace_clear); every
- * completed call leaves it ready for the next, and calls that may overlap on
- * the GPU need separate ones. */
+ * sequence. The first SE12_COUNTER_BYTES of the workspace (16-byte aligned)
+ * are zeroed once (se12_workspace_clear); every completed call leaves them
+ * zero for the next, and calls that may overlap on the GPU need separate
+ * workspaces. */
 typedef struct se12_kv_attend_args {
   const uint16_t* q;
   int64_t q_token_stride, q_head_stride;  /* elements */
@@ -464,7 +466,10 @@ typedef struct se12_kv_attend_args {
   float scale, softcap;
 } se12_kv_attend_args;
 
+/* Enough for any call on the cache; enough for calls of these sizes (a third
+ * for up to 16 query rows per KV head). */
 size_t se12_kv_attend_workspace_bytes(const se12_kv_cache* cache);
+size_t se12_kv_attend_call_bytes(const se12_kv_cache* cache, int q_heads, int max_query);
 int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_attend_args* args,
                    void* workspace_dev, size_t workspace_bytes, void* stream);
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 
 LIBRARY_PATH = pathlib.Path(__file__).resolve().parent / "libse12_b200.so"
 
@@ -69,31 +70,12 @@ class Se12KvPagesStruct(ctypes.Structure):
         (name, c_void_p) for name in ("k_codes", "v_codes", "k_scales", "v_scales")]
 
 
-class Se12KvBatchStruct(ctypes.Structure):
-    """Mirror of ``se12_kv_batch`` in include/se12.h."""
-
-    _fields_ = [("seqs", ctypes.c_int32), ("tokens", ctypes.c_int32), ("lens", c_void_p), ("query_start", c_void_p),
-                ("block_table", c_void_p), ("table_stride", ctypes.c_int64), ("max_pages", ctypes.c_int32)]
-
-
-class Se12KvAppendStruct(ctypes.Structure):
-    """Mirror of ``se12_kv_append_args`` in include/se12.h."""
-
-    _fields_ = [("bf16", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
-                ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64), ("k_token_stride", ctypes.c_int64),
-                ("k_head_stride", ctypes.c_int64), ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
-                ("cos", c_void_p), ("sin", c_void_p), ("rope_stride", ctypes.c_int64), ("rope_rows", ctypes.c_int32),
-                ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("q_out", c_void_p),
-                ("q_out_token_stride", ctypes.c_int64), ("q_out_head_stride", ctypes.c_int64)]
-
-
-class Se12KvAttendStruct(ctypes.Structure):
-    """Mirror of ``se12_kv_attend_args`` in include/se12.h."""
-
-    _fields_ = [("q", c_void_p), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64), ("out", c_void_p),
-                ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64), ("q_heads", ctypes.c_int32),
-                ("max_query", ctypes.c_int32), ("window", ctypes.c_int32), ("scale", ctypes.c_float),
-                ("softcap", ctypes.c_float)]
+# The argument blocks of the calls a decode step makes many of, as packed
+# bytes (a quarter of the time ctypes fields take): se12_kv_batch,
+# se12_kv_append_args and se12_kv_attend_args in include/se12.h, in order.
+KV_BATCH = struct.Struct("=2i3Qqi4x")
+KV_APPEND = struct.Struct("=2i3Q6q2Qq3i4xQ2q")
+KV_ATTEND = struct.Struct("=Q2qQ2q3i2f4x")
 
 
 # name -> (restype, argtypes)
@@ -148,10 +130,10 @@ SIGNATURES = {
     "se12_gemv_order_matched": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "se12_kv_cache_create": (c_int, [ctypes.POINTER(Se12KvPagesStruct), ctypes.POINTER(c_void_p)]),
     "se12_kv_cache_destroy": (None, [c_void_p]),
-    "se12_kv_append": (c_int, [c_void_p, ctypes.POINTER(Se12KvBatchStruct), ctypes.POINTER(Se12KvAppendStruct), c_void_p]),
+    "se12_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),  # KV_BATCH, KV_APPEND bytes
     "se12_kv_attend_workspace_bytes": (c_size_t, [c_void_p]),
-    "se12_kv_attend": (c_int, [c_void_p, ctypes.POINTER(Se12KvBatchStruct), ctypes.POINTER(Se12KvAttendStruct), c_void_p,
-                               c_size_t, c_void_p]),
+    "se12_kv_attend_call_bytes": (c_size_t, [c_void_p, c_int, c_int]),
+    "se12_kv_attend": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),  # KV_BATCH, KV_ATTEND bytes
     "se12_kv_decode": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "se12_token_logprobs_workspace_bytes": (c_size_t, []),
     "se12_token_logprobs": (c_int, [c_void_p, c_int, c_int, c_int, ctypes.c_int64, c_void_p, c_int, ctypes.c_float, c_void_p,

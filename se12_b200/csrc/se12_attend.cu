@@ -13,11 +13,13 @@
 // chunk being 8 KB of keys and values, cut into equal runs, one per CTA; the
 // list comes from the lengths in device memory, so that the launch does not
 // depend on them (a captured graph follows the lengths) and a ragged batch
-// is balanced to a chunk. A CTA's 8 warps take its chunks in turn, each
-// with a pipeline of its own (3 stages filled by TMA, 192 KB per SM in
-// flight or in work: no CTA-wide barrier inside a run) and its own running
-// maxima and sums; a pair's warps are joined in shared memory, its CTAs
-// through global memory by the CTA that finishes last, in CTA order.
+// is balanced to a chunk. A CTA's 4 warps take its chunks in turn, each with
+// a TMA pipeline of its own (no CTA-wide barrier inside a pair's chunks) and
+// its own references and sums; a pair's warps are joined in shared memory,
+// its CTAs through global memory by the CTA that finishes last, in CTA order.
+// Small CTAs, 2 to 4 per SM: 12 or 16 warps hide each other's latencies (8
+// warps in one CTA ran at half of the issue rate: 142 us against 107 for
+// 131071 tokens of 16 KV heads of 128), and short sequences' pairs run side by side.
 //
 // Layout of the products (mma.sync m16n8k16, tokens or dimensions as M,
 // query rows as N = 8): with a group of up to 8 query rows per KV head the
@@ -28,9 +30,12 @@
 // The bound is HBM; tcgen05 would need the codes widened into shared memory
 // first and pads the rows to 64 or more.
 //
-// Two running maxima: m over s, for the sum l; and mp over s + log2 vs, for
-// the weights p * vs that multiply the codes. So the FP16 weights stay in
-// [0, 1] with the largest term near 1 whatever the blocks' scales are.
+// Two references instead of one running maximum: m for the sum l of 2^(s - m),
+// and mp for the weights 2^(s + log2 vs - mp) that multiply the codes, so that
+// the FP16 weights keep their precision whatever the blocks' scales are. Both
+// are raised only when a value passes them by more than fits (2^8 of FP16's
+// 2^16; 2^30 of fp32's 2^127), which a vote per chunk decides: the usual chunk
+// pays neither the reduction over the lanes nor the scaling of the sums.
 #include "se12_device.cuh"
 #include "se12_serve.h"
 
@@ -38,16 +43,19 @@
 
 namespace se12 {
 
-constexpr int kAttendWarps = 8;
+constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = kAttendWarps * 32;
-constexpr int kAttendStages = 3;
+constexpr int kAttendStages = 2;
 constexpr int kAttendBox = 2048;         // 16 tokens x 128 bytes
 constexpr int kAttendStageBytes = 8192;  // keys and values of a chunk
-constexpr int kAttendDeposit = 16384;    // joining the warps' sums
+constexpr int kAttendDeposit = 8192;     // joining the warps' sums
 constexpr int kAttendMaxSeqs = 2048;
-constexpr int kAttendMinChunks = 8;      // per CTA: one per warp
 constexpr int kAttendSlotRows = 16;
 constexpr int kAttendSlotFloats = kAttendSlotRows * (256 + 4);  // sums, then (m, l, mp) per row
+constexpr int kAttendMaxCtas = 3;        // per SM
+constexpr float kAttendStart = -1.0e30f; // both references before the first token
+constexpr float kAttendRaise = 8.f;      // weights up to 2^8 of the reference
+constexpr float kAttendRaiseSum = 30.f;
 
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
@@ -140,9 +148,13 @@ struct AttendShape {
   static constexpr int kRows = 8 * NT;
 };
 
+// After the pipelines (1024-byte aligned).
 struct AttendSmem {
-  // after the pipelines (1024-byte aligned)
-  float deposit[kAttendDeposit / 4];
+  union {
+    uint4 queries[512];                   // FP16 fragments: [n-tile][box][4 pairs of words][lane]
+    float deposit[kAttendDeposit / 4];    // the warps' sums while they are joined
+  };
+  float row_scale[kAttendSlotRows];       // 2^e * scale of each query row
   float stat[kAttendWarps][kAttendSlotRows][3];   // m, l, mp of each warp
   float factor[kAttendWarps][kAttendSlotRows];
   float out_scale[kAttendSlotRows];
@@ -150,11 +162,12 @@ struct AttendSmem {
   int usable[kAttendWarps][kAttendStages][2];
   uint64_t full[kAttendWarps][kAttendStages];
   int last;
+  int most;                               // chunks of the longest pair
   int before[1];  // [seqs + 1] chunks x tiles of the sequences before (per KV head)
 };
 
-template <int KIND, int DP, int NT>
-__global__ void __launch_bounds__(kAttendThreads, 1)
+template <int KIND, int DP, int NT, int CTAS>
+__global__ void __launch_bounds__(kAttendThreads, CTAS)
     attend_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                        const AttendArgs a) {
   using Shape = AttendShape<KIND, DP, NT>;
@@ -178,11 +191,15 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
 
   // ---- the work list
   const int heads = a.c.heads;
+  if (threadIdx.x == 0) sm.before[0] = sm.most = 0;
+  __syncthreads();
+  int most = 0;
   for (int b = threadIdx.x; b < a.t.seqs; b += kAttendThreads) {
     const SeqWork w = sequence_work<CHUNK, ROWS>(a, b);
     sm.before[b + 1] = w.chunks * w.tiles;
+    most = max(most, w.chunks);
   }
-  if (threadIdx.x == 0) sm.before[0] = 0;
+  atomicMax(&sm.most, most);
   __syncthreads();
   if (warp == 0) {
     int carry = 0;
@@ -200,7 +217,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
   }
   __syncthreads();
   const int total = sm.before[a.t.seqs] * heads;
-  const int per = max(kAttendMinChunks, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  // short pairs are not cut below a chunk per warp
+  const int per = max(min(kAttendWarps, sm.most), (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
   const int g0 = static_cast<int>(min(static_cast<long long>(blockIdx.x) * per, static_cast<long long>(total)));
   const int g1 = min(g0 + per, total);
   if (g0 >= g1) return;
@@ -310,21 +328,20 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
     const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
     const int rows_all = at.w.tokens * a.group;
 
-    // queries: lane (r, c) holds, of rows r (+ 8 per n-tile), the dimensions
-    // 128 hb + 32 c .. + 31 in byte order
-    uint32_t qf[NT][HB][8][2];
-    float row_scale[NT][2];  // of rows 2c, 2c + 1
-    int row_pos[NT][2];
+    // queries as the second operand's fragments: lane (r, c) of an n-tile
+    // needs, of row r, the dimensions 128 hb + 32 c .. + 31 in byte order. A
+    // warp prepares every fourth n-tile.
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      if ((n & (kAttendWarps - 1)) != warp) continue;
       const int row = tile * ROWS + n * 8 + r;
-      uint32_t raw[HB][16];
+      uint4 raw[HB][4];
       unsigned big = 0;
       const bool live = row < rows_all;
       const int i = live ? row / a.group : 0;
       const uint16_t* src = a.q + (token0 + i) * a.q_ts + (head * a.group + (live ? row - i * a.group : 0)) * a.q_hs;
 #pragma unroll
-      for (int hb = 0; hb < HB; ++hb) {
+      for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int d = hb * 128 + c * 32 + j * 8;
@@ -338,39 +355,41 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
                              s[4] | (static_cast<uint32_t>(s[5]) << 16), s[6] | (static_cast<uint32_t>(s[7]) << 16));
             }
           }
-          raw[hb][4 * j] = v.x, raw[hb][4 * j + 1] = v.y, raw[hb][4 * j + 2] = v.z, raw[hb][4 * j + 3] = v.w;
+          raw[hb][j] = v;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t w = word_of(v, k);
             big = max(big, max((w << 16) & 0x7FFFFFFFu, w & 0x7FFF0000u));
           }
         }
-      }
       big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
       big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
       // the row times 2^-e, largest in [1, 2) (zero rows and infinities: e clamped)
       int e = static_cast<int>(big >> 23) - 127;
       e = max(min(e, 120), -120);
       const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+      auto halves = [&](uint32_t w) {
+        return half2_bits(__floats2half2_rn(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down));
+      };
 #pragma unroll
       for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 4; ++j)
+          sm.queries[((n * HB + hb) * 4 + j) * 32 + lane] =
+              make_uint4(halves(raw[hb][j].x), halves(raw[hb][j].y), halves(raw[hb][j].z), halves(raw[hb][j].w));
+      if (c == 0) sm.row_scale[n * 8 + r] = __uint_as_float(static_cast<unsigned>(127 + e) << 23) * a.scale;
+    }
+    __syncthreads();
+    float row_scale[NT][2];  // of rows 2c, 2c + 1
+    int row_pos[NT][2];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t w = raw[hb][2 * j + k];
-            qf[n][hb][j][k] = half2_bits(
-                __floats2half2_rn(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down));
-          }
-        }
-      const float up = __uint_as_float(static_cast<unsigned>(127 + e) << 23) * a.scale;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        row_scale[n][k] = __shfl_sync(0xFFFFFFFFu, up, (2 * c + k) * 4);
-        const int rr = tile * ROWS + n * 8 + 2 * c + k;
-        row_pos[n][k] = at.w.first + min(rr, rows_all - 1) / a.group;
+        const int row = n * 8 + 2 * c + k;
+        row_scale[n][k] = sm.row_scale[row] * (a.softcap != 0.f ? 2.f * kLog2e / a.softcap : kLog2e);
+        row_pos[n][k] = at.w.first + min(tile * ROWS + row, rows_all - 1) / a.group;
       }
-    }
     const int pos_min = at.w.first + min(tile * ROWS, rows_all - 1) / a.group;
     const int pos_max = at.w.first + min(tile * ROWS + ROWS - 1, rows_all - 1) / a.group;
 
@@ -380,7 +399,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        m[n][k] = mp[n][k] = kNegInf;
+        m[n][k] = mp[n][k] = kAttendStart;
         l[n][k] = 0.f;
       }
 #pragma unroll
@@ -400,12 +419,19 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
       if (!dead) dead = !__all_sync(0xFFFFFFFFu, mbar_wait(&sm.full[warp][stage], phase));
       if (dead) break;
       const uint32_t base = pipe_addr + stage * kAttendStageBytes;
+      const int t0 = at.w.low + (at.chunk + mine) * CHUNK;
+      bool use[SUBS];
+      float lv[SUBS];
+      float p[SUBS][NT][4];  // logits in units of log 2, then weights
 #pragma unroll
       for (int sub = 0; sub < SUBS; ++sub) {
-        if (!sm.usable[warp][stage][sub]) continue;
-        const float ks = sm.scales[warp][stage][sub][0];
-        const float vs = sm.scales[warp][stage][sub][1];
-        const int t0 = at.w.low + (at.chunk + mine) * CHUNK + sub * 16;
+        use[sub] = sm.usable[warp][stage][sub];
+        lv[sub] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) p[sub][n][k] = kNegInf;
+        if (!use[sub]) continue;
         // S^T: 16 tokens x 8 rows
         float s[NT][2][4];
 #pragma unroll
@@ -421,6 +447,11 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
           for (int i = 0; i < 2; ++i) {
             const uint32_t off = kbase + hb * kAttendBox + (((2 * c + i) ^ r) << 4);
             const uint4 x = lds128(off), y = lds128(off + 1024);
+            uint4 qf[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) qf[n][j] = sm.queries[((n * HB + hb) * 4 + 2 * i + j) * 32 + lane];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               uint32_t a0, a1, a2, a3;
@@ -428,79 +459,111 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
               widen<KIND>(word_of(y, w), a1, a3);
 #pragma unroll
               for (int n = 0; n < NT; ++n)
-                mma_f16_16816(s[n][w & 1], a0, a1, a2, a3, qf[n][hb][4 * i + w][0], qf[n][hb][4 * i + w][1]);
+                mma_f16_16816(s[n][w & 1], a0, a1, a2, a3, word_of(qf[n][w >> 1], 2 * (w & 1)),
+                              word_of(qf[n][w >> 1], 2 * (w & 1) + 1));
             }
           }
-        // logits in units of log 2, masks, running maxima
-        const bool masked = t0 + 15 > pos_min || (a.window && pos_max - t0 >= a.window);
-        const float lv = lg2(vs);
-        float p[NT][4];
+        const float ks = sm.scales[warp][stage][sub][0];
+        lv[sub] = lg2(sm.scales[warp][stage][sub][1]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float x = (s[n][0][k] + s[n][1][k]) * (row_scale[n][k & 1] * ks);
+            // cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1); the
+            // factor 2 log2(e) / cap is in row_scale
+            if (a.softcap != 0.f) x = a.softcap * kLog2e - __fdividef(2.f * kLog2e * a.softcap, ex2(x) + 1.f);
+            p[sub][n][k] = x;
+          }
+      }
+      const bool masked = t0 + CHUNK - 1 > pos_min || (a.window && pos_max - t0 >= a.window);
+      if (masked) {
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int j = t0 + sub * 16 + r + (k >> 1) * 8, pos = row_pos[n][k & 1];
+              if (j > pos || (a.window && pos - j >= a.window)) p[sub][n][k] = kNegInf;
+            }
+      }
+      // raise the references where a value passes them
+      bool passes = false;
+      float top[NT][2], top_v[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          top[n][k] = top_v[n][k] = kNegInf;
+#pragma unroll
+          for (int sub = 0; sub < SUBS; ++sub) {
+            const float t = fmaxf(p[sub][n][k], p[sub][n][k + 2]);
+            top[n][k] = fmaxf(top[n][k], t);
+            top_v[n][k] = fmaxf(top_v[n][k], t + lv[sub]);
+          }
+          passes |= top[n][k] - m[n][k] > kAttendRaiseSum || top_v[n][k] - mp[n][k] > kAttendRaise;
+        }
+      if (__any_sync(0xFFFFFFFFu, passes)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float t = top[n][k], tv = top_v[n][k];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+              t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, d));
+              tv = fmaxf(tv, __shfl_xor_sync(0xFFFFFFFFu, tv, d));
+            }
+            t = fmaxf(t, m[n][k]);
+            tv = fmaxf(tv, mp[n][k]);
+            l[n][k] *= ex2(m[n][k] - t);
+            const float f = ex2(mp[n][k] - tv);
+            m[n][k] = t;
+            mp[n][k] = tv;
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+              for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  acc[hb][w][h][n][k] *= f;
+                  acc[hb][w][h][n][k + 2] *= f;
+                }
+          }
+      }
+#pragma unroll
+      for (int sub = 0; sub < SUBS; ++sub) {
+        if (!use[sub]) continue;
         uint32_t pf[NT][2];
-        bool grew = false;
-        float shrink[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float x = (s[n][0][k] + s[n][1][k]) * (row_scale[n][k & 1] * ks);
-            if (a.softcap != 0.f) {
-              // cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1)
-              const float e = ex2(x * (2.f * kLog2e / a.softcap));
-              x = a.softcap * kLog2e - __fdividef(2.f * kLog2e * a.softcap, e + 1.f);
-            } else {
-              x *= kLog2e;
-            }
-            if (masked) {
-              const int j = t0 + r + (k >> 1) * 8, pos = row_pos[n][k & 1];
-              if (j > pos || (a.window && pos - j >= a.window)) x = kNegInf;
-            }
-            p[n][k] = x;
-          }
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float top = fmaxf(p[n][k], p[n][k + 2]);
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-            const float m_new = fmaxf(m[n][k], top), mp_new = fmaxf(mp[n][k], top + lv);
-            const float m_ref = m_new == kNegInf ? 0.f : m_new, mp_ref = mp_new == kNegInf ? 0.f : mp_new;
-            l[n][k] *= ex2(m[n][k] - m_ref);
-            shrink[n][k] = ex2(mp[n][k] - mp_ref);
-            grew |= mp_new != mp[n][k];
-            m[n][k] = m_new;
-            mp[n][k] = mp_new;
-            const float x0 = p[n][k], x1 = p[n][k + 2];
-            l[n][k] += ex2(x0 - m_ref) + ex2(x1 - m_ref);
+            const float x = p[sub][n][k];
+            l[n][k & 1] += ex2(x - m[n][k & 1]);
+            p[sub][n][k] = ex2(x + (lv[sub] - mp[n][k & 1]));
             // a masked token weighs nothing, whatever its block's scale holds
-            p[n][k] = x0 == kNegInf ? 0.f : ex2(x0 + lv - mp_ref);
-            p[n][k + 2] = x1 == kNegInf ? 0.f : ex2(x1 + lv - mp_ref);
+            if (masked && x == kNegInf) p[sub][n][k] = 0.f;
           }
-          pf[n][0] = transpose_8x8(half2_bits(__floats2half2_rn(p[n][0], p[n][1])));
-          pf[n][1] = transpose_8x8(half2_bits(__floats2half2_rn(p[n][2], p[n][3])));
-        }
-        if (__any_sync(0xFFFFFFFFu, grew)) {
-#pragma unroll
-          for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-            for (int w = 0; w < 4; ++w)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) acc[hb][w][h][n][k] *= shrink[n][k & 1];
+          pf[n][0] = transpose_8x8(half2_bits(__floats2half2_rn(p[sub][n][0], p[sub][n][1])));
+          pf[n][1] = transpose_8x8(half2_bits(__floats2half2_rn(p[sub][n][2], p[sub][n][3])));
         }
         // O^T += V^T P^T: lane (r, c) reads dimensions 128 hb + 16 r .. + 15
         // of tokens 2c, 2c + 1, 2c + 8, 2c + 9
         const uint32_t vbase = base + kAttendStageBytes / 2 + sub * HB * kAttendBox + 2 * c * 128;
-        const bool clip = t0 + 16 > at.w.length;  // codes past the sequence may be anything
+        const int ts = t0 + sub * 16;
+        const bool clip = ts + 16 > at.w.length;  // codes past the sequence may be anything
 #pragma unroll
         for (int hb = 0; hb < HB; ++hb) {
           uint4 v[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 4; ++i)
             v[i] = lds128(vbase + hb * kAttendBox + (i & 1) * 128 + (i >> 1) * 1024 + ((r ^ (2 * c + (i & 1))) << 4));
-            if (clip && t0 + 2 * c + (i & 1) + (i >> 1) * 8 >= at.w.length) v[i] = make_uint4(0, 0, 0, 0);
+          if (clip) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (ts + 2 * c + (i & 1) + (i >> 1) * 8 >= at.w.length) v[i] = make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -551,19 +614,18 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
     float* part = a.partials + (static_cast<size_t>(blockIdx.x) * 2 + slot) * kAttendSlotFloats;
     if (threadIdx.x < rows) {
       const int row = threadIdx.x;
-      float mm = kNegInf, mmp = kNegInf;
+      float mm = kAttendStart, mmp = kAttendStart;
       for (int w = 0; w < kAttendWarps; ++w) {
         mm = fmaxf(mm, sm.stat[w][row][0]);
         mmp = fmaxf(mmp, sm.stat[w][row][2]);
       }
-      const float mr = mm == kNegInf ? 0.f : mm, mpr = mmp == kNegInf ? 0.f : mmp;
       float sum = 0.f;
       for (int w = 0; w < kAttendWarps; ++w) {
-        sum += sm.stat[w][row][1] * ex2(sm.stat[w][row][0] - mr);
-        sm.factor[w][row] = ex2(sm.stat[w][row][2] - mpr);
+        sum += sm.stat[w][row][1] * ex2(sm.stat[w][row][0] - mm);
+        sm.factor[w][row] = ex2(sm.stat[w][row][2] - mmp);
       }
       if (whole) {
-        sm.out_scale[row] = sum == 0.f ? 0.f : ex2(mpr - mr) / sum;
+        sm.out_scale[row] = sum == 0.f ? 0.f : ex2(mmp - mm) / sum;
       } else {
         float* st = part + kAttendSlotRows * 256 + row * 4;
         st[0] = mm;
@@ -641,20 +703,19 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
         const float* rest = a.partials + static_cast<size_t>(cta_first) * 2 * kAttendSlotFloats;  // + 2 slots per CTA
         auto part_of = [&](int i) { return i == 0 ? first : rest + static_cast<size_t>(i) * 2 * kAttendSlotFloats; };
         if (threadIdx.x < rows) {
-          float mm = kNegInf, mmp = kNegInf;
+          float mm = kAttendStart, mmp = kAttendStart;
           for (int i = 0; i < parts; ++i) {
             const float* st = part_of(i) + kAttendSlotRows * 256 + threadIdx.x * 4;
             mm = fmaxf(mm, __ldcg(st));
             mmp = fmaxf(mmp, __ldcg(st + 2));
           }
-          const float mr = mm == kNegInf ? 0.f : mm, mpr = mmp == kNegInf ? 0.f : mmp;
           float sum = 0.f;
           for (int i = 0; i < parts; ++i) {
             const float* st = part_of(i) + kAttendSlotRows * 256 + threadIdx.x * 4;
-            sum += __ldcg(st + 1) * ex2(__ldcg(st) - mr);
+            sum += __ldcg(st + 1) * ex2(__ldcg(st) - mm);
           }
-          sm.factor[0][threadIdx.x] = mpr;
-          sm.out_scale[threadIdx.x] = sum == 0.f ? 0.f : ex2(mpr - mr) / sum;
+          sm.factor[0][threadIdx.x] = mmp;
+          sm.out_scale[threadIdx.x] = sum == 0.f ? 0.f : ex2(mmp - mm) / sum;
         }
         __syncthreads();
         const int vectors = a.c.dim / 4;
@@ -686,13 +747,23 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
 
 // ------------------------------------------------------------------ launch
 
-size_t kv_attend_partial_bytes(int sm_count) { return static_cast<size_t>(sm_count) * 2 * kAttendSlotFloats * 4; }
+// More than 16 query rows per KV head go to attend_tile_kernel.
+bool kv_attend_takes_tiles(int max_query, int group) {
+  return static_cast<long long>(max_query) * group > kAttendSlotRows;
+}
 
-template <int KIND, int DP, int NT>
+size_t kv_attend_partial_bytes(int sm_count, bool tile) {
+  if (tile) return kv_attend_tile_partial_bytes(sm_count);
+  return static_cast<size_t>(sm_count) * kAttendMaxCtas * 2 * kAttendSlotFloats * 4;
+}
+
+template <int KIND, int DP, int NT, int CTAS>
 cudaError_t launch_attend_rows(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int sm_count,
                                cudaStream_t stream) {
+  static_assert(CTAS <= kAttendMaxCtas, "workspace slots");
   const size_t smem = 1024 + kAttendWarps * kAttendStages * kAttendStageBytes + sizeof(AttendSmem) + a.t.seqs * sizeof(int);
-  return launch_overlapped(attend_rows_kernel<KIND, DP, NT>, dim3(sm_count), kAttendThreads, smem, stream, kmap, vmap, a);
+  return launch_overlapped(attend_rows_kernel<KIND, DP, NT, CTAS>, dim3(sm_count * CTAS), kAttendThreads, smem, stream, kmap,
+                           vmap, a);
 }
 
 template <int KIND>
@@ -700,14 +771,15 @@ cudaError_t launch_attend_kind(const CUtensorMap& kmap, const CUtensorMap& vmap,
                                int sm_count, cudaStream_t stream) {
   const bool one = static_cast<long long>(max_query) * a.group <= 8;  // query rows per KV head in one n-tile
   if (a.c.dim <= 128)
-    return one ? launch_attend_rows<KIND, 128, 1>(kmap, vmap, a, sm_count, stream)
-               : launch_attend_rows<KIND, 128, 2>(kmap, vmap, a, sm_count, stream);
-  return one ? launch_attend_rows<KIND, 256, 1>(kmap, vmap, a, sm_count, stream)
-             : launch_attend_rows<KIND, 256, 2>(kmap, vmap, a, sm_count, stream);
+    return one ? launch_attend_rows<KIND, 128, 1, 3>(kmap, vmap, a, sm_count, stream)
+               : launch_attend_rows<KIND, 128, 2, 3>(kmap, vmap, a, sm_count, stream);
+  return one ? launch_attend_rows<KIND, 256, 1, 3>(kmap, vmap, a, sm_count, stream)
+             : launch_attend_rows<KIND, 256, 2, 2>(kmap, vmap, a, sm_count, stream);
 }
 
 cudaError_t launch_kv_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int max_query,
                              int sm_count, cudaStream_t stream) {
+  if (kv_attend_takes_tiles(max_query, a.group)) return launch_attend_tile(a, sm_count, stream);
   return a.c.kind == kKvInt8 ? launch_attend_kind<kKvInt8>(kmap, vmap, a, max_query, sm_count, stream)
                              : launch_attend_kind<kKvE4m3>(kmap, vmap, a, max_query, sm_count, stream);
 }

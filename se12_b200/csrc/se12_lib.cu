@@ -6,5 +6,6 @@
 #include "se12_abi.cu"
 #include "se12_kv.cu"
 #include "se12_attend.cu"
+#include "se12_attend_tile.cu"
 #include "se12_logprobs.cu"
 #include "se12_serve_abi.cu"

@@ -60,6 +60,7 @@ struct AttendArgs {
   int q_vec;          // q rows are 16-byte aligned
   uint16_t* out;      // BF16
   long long o_ts, o_hs;
+  int o_vec;          // and the output's
   int q_heads, group;
   float scale;        // of the logits
   float softcap;      // 0: none
@@ -92,7 +93,10 @@ cudaError_t launch_kv_decode(const KvView& c, const int32_t* pages, int count, u
                              cudaStream_t stream);
 cudaError_t launch_kv_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int max_query,
                              int sm_count, cudaStream_t stream);
-size_t kv_attend_partial_bytes(int sm_count);
+size_t kv_attend_partial_bytes(int sm_count, bool tile);
+bool kv_attend_takes_tiles(int max_query, int group);
+cudaError_t launch_attend_tile(const AttendArgs& a, int sm_count, cudaStream_t stream);
+size_t kv_attend_tile_partial_bytes(int sm_count);
 cudaError_t launch_token_logprobs(bool bf16, LogprobArgs a, int sm_count, cudaStream_t stream);
 size_t logprob_partial_bytes(int sm_count);
 

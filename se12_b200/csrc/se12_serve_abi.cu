@@ -12,6 +12,10 @@ struct se12_kv_cache {
 
 namespace {
 
+// A launch has at most kAttendMaxCtas CTAs per SM, each with a counter.
+constexpr int kMaxSms = 160;
+static_assert(kMaxSms * se12::kAttendMaxCtas * sizeof(int) <= SE12_COUNTER_BYTES, "the counters of a launch");
+
 // Codes as [pages * heads * page_size rows][dim bytes], one box = 16 tokens x
 // 128 bytes (a page is a multiple of 16 tokens, so a box never leaves it;
 // columns past dim read as zero codes, which stand for zero).
@@ -81,7 +85,7 @@ int se12_kv_cache_create(const se12_kv_pages* p, se12_kv_cache** out) {
   v.heads = p->kv_heads;
   v.dim = p->head_dim;
   v.kind = p->kind;
-  c->sm_count = sm_count;
+  c->sm_count = std::min(sm_count, kMaxSms);
   st = encode_kv_map(&c->k_map, p->k_codes, v);
   if (st == SE12_OK) st = encode_kv_map(&c->v_map, p->v_codes, v);
   if (st != SE12_OK) {
@@ -127,10 +131,17 @@ int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const
   return SE12_OK;
 }
 
-// [partial sums][arrival counters, zero between calls]
+// [arrival counters, zero between calls][partial sums]
 size_t se12_kv_attend_workspace_bytes(const se12_kv_cache* c) {
   if (!c) return 0;
-  return se12::kv_attend_partial_bytes(c->sm_count) + (static_cast<size_t>(c->sm_count) * 4 + 255) / 256 * 256;
+  return SE12_COUNTER_BYTES + std::max(se12::kv_attend_partial_bytes(c->sm_count, false),
+                                       se12::kv_attend_partial_bytes(c->sm_count, true));
+}
+
+size_t se12_kv_attend_call_bytes(const se12_kv_cache* c, int q_heads, int max_query) {
+  if (!c || q_heads < 1 || max_query < 1) return 0;
+  const bool tiles = se12::kv_attend_takes_tiles(max_query, std::max(q_heads / c->view.heads, 1));
+  return SE12_COUNTER_BYTES + se12::kv_attend_partial_bytes(c->sm_count, tiles);
 }
 
 int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_attend_args* p, void* workspace,
@@ -154,7 +165,7 @@ int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const
                       (static_cast<double>(batch->max_pages) * v.page_size / 16 + 2) *
                       (static_cast<double>(p->max_query) * group / 8 + 1);
   if (work > 2.0e9) return fail(SE12_ERR_INVALID_ARGUMENT, "the batch is too large for one call: split it by sequences");
-  const size_t need = se12_kv_attend_workspace_bytes(cache);
+  const size_t need = se12_kv_attend_call_bytes(cache, p->q_heads, p->max_query);
   if (!workspace || workspace_bytes < need)
     return fail(SE12_ERR_WORKSPACE_TOO_SMALL, "workspace needs " + std::to_string(need) + " bytes");
   if (!aligned16(workspace)) return fail(SE12_ERR_MISALIGNED, "the workspace must be 16-byte aligned");
@@ -164,13 +175,14 @@ int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const
   a.q_vec = aligned16(p->q) && a.q_ts % 8 == 0 && a.q_hs % 8 == 0;
   a.out = p->out;
   a.o_ts = p->out_token_stride, a.o_hs = p->out_head_stride;
+  a.o_vec = aligned16(p->out) && a.o_ts % 8 == 0 && a.o_hs % 8 == 0;
   a.q_heads = p->q_heads;
   a.group = group;
   a.scale = p->scale;
   a.softcap = p->softcap;
   a.window = p->window;
-  a.partials = static_cast<float*>(workspace);
-  a.counters = reinterpret_cast<int*>(static_cast<char*>(workspace) + se12::kv_attend_partial_bytes(cache->sm_count));
+  a.counters = static_cast<int*>(workspace);
+  a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + SE12_COUNTER_BYTES);
   const cudaError_t err = se12::launch_kv_attend(cache->k_map, cache->v_map, a, p->max_query, cache->sm_count,
                                                  static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return cuda_fail(err, "se12_kv_attend launch");
@@ -189,8 +201,10 @@ int se12_kv_decode(const se12_kv_cache* cache, const int32_t* pages, int count, 
   return SE12_OK;
 }
 
-// For any B200: 148 SMs, room for 160. [partial rows][arrival counters]
-size_t se12_token_logprobs_workspace_bytes(void) { return se12::logprob_partial_bytes(160) + 160 * 2 * 4; }
+// For any B200: 148 SMs, room for kMaxSms. [arrival counters][partial rows]
+size_t se12_token_logprobs_workspace_bytes(void) {
+  return SE12_COUNTER_BYTES + se12::logprob_partial_bytes(kMaxSms);
+}
 
 int se12_token_logprobs(const void* logits, int bf16, int rows, int vocab, int64_t ld, const int64_t* tokens, int top,
                         float softcap, float* logprob, float* entropy, int64_t* top_ids, float* top_logprobs,
@@ -208,7 +222,7 @@ int se12_token_logprobs(const void* logits, int bf16, int rows, int vocab, int64
   int device = 0, sm_count = 0;
   const int st = current_device_info(&device, &sm_count);
   if (st != SE12_OK) return st;
-  if (sm_count > 160) sm_count = 160;
+  sm_count = std::min(sm_count, kMaxSms);
   se12::LogprobArgs a{};
   a.logits = logits;
   a.ld = ld;
@@ -222,8 +236,8 @@ int se12_token_logprobs(const void* logits, int bf16, int rows, int vocab, int64
   a.top_ids = reinterpret_cast<long long*>(top_ids);
   a.top_logprobs = top_logprobs;
   a.vec = aligned16(logits) && ld * (bf16 ? 2 : 4) % 16 == 0;
-  a.partials = static_cast<unsigned char*>(workspace);
-  a.counters = reinterpret_cast<int*>(static_cast<char*>(workspace) + se12::logprob_partial_bytes(160));
+  a.counters = static_cast<int*>(workspace);
+  a.partials = static_cast<unsigned char*>(workspace) + SE12_COUNTER_BYTES;
   const cudaError_t err = se12::launch_token_logprobs(bf16 != 0, a, sm_count, static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return cuda_fail(err, "se12_token_logprobs launch");
   return SE12_OK;

@@ -27,21 +27,36 @@ import weakref
 import torch
 
 from . import _lib
-from .device import _WorkspacePool, stream_handle
+from .device import _WorkspacePool
 
 KINDS = {"int8": 0, "e4m3": 1}
 PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_SEQS = 2048
+COUNTER_BYTES = 4096  # SE12_COUNTER_BYTES: the part of a workspace that must be zero before a call
 
 _WORKSPACES = _WorkspacePool()
 
 
-def _workspace(pool: _WorkspacePool, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """A zeroed workspace for this call. While a graph is captured it belongs
-    to the graph (its clearing is captured with it); otherwise the stream's."""
+def _workspace(pool: _WorkspacePool, device: torch.device, stream: int, nbytes: int) -> int:
+    """Address of a workspace for this call, its counters zero. While a graph
+    is captured it belongs to the graph (the clearing is captured with it);
+    otherwise it is the stream's, which every call leaves zeroed."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return pool.get(device, stream, nbytes)
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf[:COUNTER_BYTES].zero_()
+        return buf.data_ptr()
+    return pool.get(device, stream, nbytes).data_ptr()
+
+
+def _launch(index: int, function, name: str, *args) -> None:
+    """function(*args, current stream) on GPU ``index``."""
+    if torch.cuda.current_device() == index:
+        status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def _rows(x: torch.Tensor, name: str, heads: int | None, dim: int, tokens: int | None, dtypes, device) -> torch.Tensor:
@@ -122,6 +137,7 @@ class PagedKvCache:
         self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.kind = k_codes, v_codes, k_scales, v_scales, kind
         self.pages, self.kv_heads, self.page_size, self.head_dim = k_codes.shape
         self.device = k_codes.device
+        self._index = self.device.index
         s = _lib.Se12KvPagesStruct(self.pages, self.page_size, self.kv_heads, self.head_dim, KINDS[kind], k_codes.data_ptr(),
                                    v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
         handle = ctypes.c_void_p()
@@ -129,13 +145,13 @@ class PagedKvCache:
             _lib.check(lib.se12_kv_cache_create(ctypes.byref(s), ctypes.byref(handle)), "se12_kv_cache_create")
         self._handle = handle
         self._finalizer = weakref.finalize(self, lib.se12_kv_cache_destroy, handle)
-        self._attend_bytes = lib.se12_kv_attend_workspace_bytes(handle)
+        self._lib = lib
 
     @property
     def handle(self) -> ctypes.c_void_p:
         return self._handle
 
-    def _batch(self, tokens: int, block_table, lens, query_start) -> _lib.Se12KvBatchStruct:
+    def _batch(self, tokens: int, block_table, lens, query_start) -> bytes:
         _index(block_table, "block_table", 2, self.device)
         _index(lens, "lens", 1, self.device)
         seqs = lens.shape[0]
@@ -150,9 +166,9 @@ class PagedKvCache:
             _index(query_start, "query_start", 1, self.device)
             if query_start.shape[0] != seqs + 1:
                 raise ValueError(f"query_start must have {seqs + 1} entries, got {query_start.shape[0]}")
-        return _lib.Se12KvBatchStruct(seqs, tokens, lens.data_ptr(), None if query_start is None else query_start.data_ptr(),
-                                      block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]),
-                                      block_table.shape[1])
+        columns = block_table.shape[1]
+        return _lib.KV_BATCH.pack(seqs, tokens, lens.data_ptr(), 0 if query_start is None else query_start.data_ptr(),
+                                  block_table.data_ptr(), max(block_table.stride(0), columns), columns)
 
     # ------------------------------------------------------------------ operators
     def append(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
@@ -177,35 +193,37 @@ class PagedKvCache:
         if tokens == 0:
             return None if q is None else (q_out if q_out is not None else q.new_empty(q.shape, dtype=torch.bfloat16))
         batch = self._batch(tokens, block_table, lens, query_start)
-        a = _lib.Se12KvAppendStruct()
-        a.bf16 = int(k.dtype == torch.bfloat16)
-        a.k, a.v = k.data_ptr(), v.data_ptr()
-        a.k_token_stride, a.k_head_stride = k.stride(0), k.stride(1)
-        a.v_token_stride, a.v_head_stride = v.stride(0), v.stride(1)
+        queries, query_out, q_heads = (0, 0, 0), (0, 0, 0), 0
         if q is not None:
             _rows(q, "q", None, self.head_dim, tokens, (k.dtype,), self.device)
+            q_heads = q.shape[1]
+            if q_heads < 1:
+                raise ValueError("q has no heads")
             if q_out is None:
                 q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
             else:
-                _rows(q_out, "q_out", q.shape[1], self.head_dim, tokens, (torch.bfloat16,), self.device)
-            a.q, a.q_heads, a.q_token_stride, a.q_head_stride = q.data_ptr(), q.shape[1], q.stride(0), q.stride(1)
-            a.q_out, a.q_out_token_stride, a.q_out_head_stride = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+                _rows(q_out, "q_out", q_heads, self.head_dim, tokens, (torch.bfloat16,), self.device)
+            queries = (q.data_ptr(), q.stride(0), q.stride(1))
+            query_out = (q_out.data_ptr(), q_out.stride(0), q_out.stride(1))
         elif q_out is not None:
             raise ValueError("q_out without q")
         if (cos is None) != (sin is None):
             raise ValueError("cos and sin go together")
+        turn = (0, 0, 0, 0, 0)
         if cos is not None:
             for t, name in ((cos, "cos"), (sin, "sin")):
                 if t.dtype != torch.float32 or t.dim() != 2 or t.stride(1) != 1 or t.device != self.device:
                     raise ValueError(f"{name} must be an fp32 [positions, rotary / 2] tensor on {self.device}")
-            if cos.shape != sin.shape or cos.stride(0) != sin.stride(0):
+            rows, half = cos.shape
+            if sin.shape != cos.shape or cos.stride(0) != sin.stride(0):
                 raise ValueError("cos and sin must have the same shape and strides")
-            if not 1 <= cos.shape[1] <= self.head_dim // 2 or cos.shape[0] < 1:
+            if not 1 <= half <= self.head_dim // 2 or rows < 1:
                 raise ValueError(f"cos and sin must have 1..{self.head_dim // 2} columns and a row or more")
-            a.cos, a.sin, a.rope_stride = cos.data_ptr(), sin.data_ptr(), max(cos.stride(0), cos.shape[1])
-            a.rope_rows, a.rotary_dim, a.interleaved = cos.shape[0], 2 * cos.shape[1], int(interleaved)
-        with torch.cuda.device(self.device):
-            _lib.call("se12_kv_append", self._handle, ctypes.byref(batch), ctypes.byref(a), stream_handle(self.device))
+            turn = (cos.data_ptr(), sin.data_ptr(), max(cos.stride(0), half), rows, 2 * half)
+        args = _lib.KV_APPEND.pack(k.dtype == torch.bfloat16, q_heads, queries[0], k.data_ptr(), v.data_ptr(), queries[1],
+                                   queries[2], k.stride(0), k.stride(1), v.stride(0), v.stride(1), *turn, bool(interleaved),
+                                   *query_out)
+        _launch(self._index, self._lib.se12_kv_append, "se12_kv_append", self._handle, batch, args)
         return q_out
 
     def attend(self, q: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, query_start: torch.Tensor | None = None,
@@ -232,13 +250,12 @@ class PagedKvCache:
         batch = self._batch(tokens, block_table, lens, query_start)
         if max_query is None:
             max_query = 1 if query_start is None else tokens
-        a = _lib.Se12KvAttendStruct(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                                    q.shape[1], int(max_query), int(window),
-                                    self.head_dim ** -0.5 if scale is None else float(scale), float(softcap))
-        with torch.cuda.device(self.device):
-            stream = stream_handle(self.device)
-            ws = _workspace(_WORKSPACES, self.device, stream, self._attend_bytes)
-            _lib.call("se12_kv_attend", self._handle, ctypes.byref(batch), ctypes.byref(a), ws.data_ptr(), ws.numel(), stream)
+        max_query = int(max_query)
+        args = _lib.KV_ATTEND.pack(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                                   q.shape[1], max_query, int(window), self.head_dim ** -0.5 if scale is None else scale, softcap)
+        need = self._lib.se12_kv_attend_call_bytes(self._handle, q.shape[1], max_query)
+        ws = _workspace(_WORKSPACES, self.device, torch._C._cuda_getCurrentRawStream(self._index), need)
+        _launch(self._index, self._lib.se12_kv_attend, "se12_kv_attend", self._handle, batch, args, ws, need)
         return out
 
     def decode(self, pages: torch.Tensor | None = None) -> tuple:
@@ -249,9 +266,8 @@ class PagedKvCache:
         k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         if count:
-            with torch.cuda.device(self.device):
-                _lib.call("se12_kv_decode", self._handle, None if pages is None else pages.data_ptr(), count, k.data_ptr(),
-                          v.data_ptr(), stream_handle(self.device))
+            _launch(self._index, self._lib.se12_kv_decode, "se12_kv_decode", self._handle,
+                    None if pages is None else pages.data_ptr(), count, k.data_ptr(), v.data_ptr())
         return k, v
 
 

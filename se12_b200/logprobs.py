@@ -15,8 +15,8 @@ import typing
 import torch
 
 from . import _lib
-from .device import _WorkspacePool, stream_handle
-from .kv_cache import _workspace
+from .device import _WorkspacePool
+from .kv_cache import _launch, _workspace
 
 MAX_TOP = 32
 
@@ -52,19 +52,19 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
         raise ValueError("logits and tokens must be on one GPU")
     if tokens.stride(0) != 1 and rows > 1:
         tokens = tokens.contiguous()
-    scalars = torch.empty(2, rows, dtype=torch.float32, device=device)
+    index = device.index
+    logprob = torch.empty(rows, dtype=torch.float32, device=device)
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
     ids = torch.empty(rows, top, dtype=torch.int64, device=device)
     top_logprobs = torch.empty(rows, top, dtype=torch.float32, device=device)
-    result = TokenLogprobs(scalars[0], scalars[1], ids, top_logprobs)
-    if rows == 0:
-        return result
-    with torch.cuda.device(device):
-        stream = stream_handle(device)
-        ws = _workspace(_WORKSPACES, device, stream, _lib.load().se12_token_logprobs_workspace_bytes())
-        _lib.call("se12_token_logprobs", logits.data_ptr(), int(logits.dtype == torch.bfloat16), rows, vocab,
-                  max(logits.stride(0), vocab), tokens.data_ptr(), top, softcap, scalars.data_ptr(),
-                  scalars.data_ptr() + 4 * rows, ids.data_ptr(), top_logprobs.data_ptr(), ws.data_ptr(), ws.numel(), stream)
-    return result
+    if rows:
+        lib = _lib.load()
+        need = lib.se12_token_logprobs_workspace_bytes()
+        ws = _workspace(_WORKSPACES, device, torch._C._cuda_getCurrentRawStream(index), need)
+        _launch(index, lib.se12_token_logprobs, "se12_token_logprobs", logits.data_ptr(), logits.dtype == torch.bfloat16, rows,
+                vocab, max(logits.stride(0), vocab), tokens.data_ptr(), top, softcap, logprob.data_ptr(), entropy.data_ptr(),
+                ids.data_ptr(), top_logprobs.data_ptr(), ws, need)
+    return TokenLogprobs(logprob, entropy, ids, top_logprobs)
 
 
 __all__ = ["MAX_TOP", "TokenLogprobs", "token_logprobs"]
