@@ -11,24 +11,23 @@
 // rows of contraction, V as it lies (a transposed second operand). The
 // probabilities go back to tensor memory as P's FP16 operand.
 //
-//   warps 0-7   softmax: a thread per row, two warps per 32 rows, one for each
-//               half of the tile's tokens
-//   warps 8-11  keys, warps 12-15 values: codes to FP16 tiles, two tiles deep
-//   warp 16     one thread issues the products: S of tile j + 1 before P V of
-//               tile j, so that the tensor pipe works during the softmax
-//               (17-19 only complete its warp group)
+//   warps 0-3   softmax: a thread per row
+//   warps 4-7   keys, warps 8-11 values: codes to FP16 tiles, two tiles deep
+//   warp 12     issues the products: S of tile j + 1 before P V of tile j, so
+//               that the tensor pipe works during the softmax (13-15 only
+//               complete its warp group)
 //
-// The roles walk the CTA's run on their own and meet at mbarriers only; the
-// register file is split by role (setmaxnreg).
+// The roles walk the CTA's run on their own and meet at mbarriers only.
 //
-// As in attend_rows_kernel a row's references are raised only when a value
-// passes them by 2^8; then the row's sums in tensor memory are scaled by the
-// row's own threads, after P V of the tile before. The two warps of a row
-// agree by one barrier with a vote per tile. The sum l is taken from the weights,
-// a factor per 16 tokens, unless scales differ by more than 2^80.
-// A row's capped logits take a polynomial of tanh for |x / cap| < 0.7 (two
-// special-function calls less per logit; the unit has 16 a clock, and the
-// softmax is what bounds the kernel).
+// The softmax goes over S twice, 64 tokens in registers. First the largest
+// product of every 16 tokens, which decides whether the row's references are
+// raised (as in attend_rows_kernel; the row's sums in tensor memory are then
+// scaled by the row's own thread, after P V of the tile before) and whether
+// the tile is usual: block scales within 2^60 of each other, capped logits
+// within |x / cap| <= 0.7, where a polynomial of tanh serves (two special-
+// function calls less per logit). A usual tile's second pass takes a handful
+// of instructions per logit; the sum l comes from the weights, by a factor per
+// 16 tokens. Other tiles take the slow way, eight tokens at a time.
 //
 // The work list (sequences, KV heads, row tiles, KV tiles) is cut into equal
 // runs, one per CTA, and a tile's CTAs are joined as in attend_rows_kernel.
@@ -40,13 +39,13 @@
 namespace se12 {
 
 constexpr int kTileAttendRows = 128;  // query rows of a tile
-constexpr int kTileSoftmaxWarps = 8;
+constexpr int kTileSoftmaxWarps = 4;
 constexpr int kTileLoaderWarps = 4;   // for keys, and as many for values
 constexpr int kTileAttendThreads = (kTileSoftmaxWarps + 2 * kTileLoaderWarps + 4) * 32;
-// Registers per thread: 96 at launch (20 warps); 2 x 128 + 2 x 88 + 40 per
-// thread of the five warp groups stays below 5 x 96.
-constexpr int kTileSoftmaxRegs = 128, kTileLoaderRegs = 88, kTileIssuerRegs = 40;
-static_assert(2 * kTileSoftmaxRegs + 2 * kTileLoaderRegs + kTileIssuerRegs <= 5 * 96, "more registers than the launch has");
+// Registers per thread by role (setmaxnreg), out of the launch's 128 for each
+// of the four warp groups.
+constexpr int kTileSoftmaxRegs = 208, kTileLoaderRegs = 104, kTileIssuerRegs = 80;
+static_assert(kTileSoftmaxRegs + 2 * kTileLoaderRegs + kTileIssuerRegs <= 4 * 128, "more registers than the launch has");
 constexpr int kTileKvBytes = 32768;   // an FP16 tile of keys or values
 constexpr int kTileMeta = 4;          // tiles whose block scales are kept
 constexpr int kTileSlotFloats = kTileAttendRows * (256 + 4);
@@ -66,26 +65,52 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, int columns) {
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Arrives on the barrier once every product this thread issued is done.
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+// The product calls are made by a whole warp, in step, for one elected lane:
+// their operands are then warp-uniform registers throughout (issued by one
+// thread in a branch of its own, a product took 250 cycles to issue).
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+
+// Arrives on the barrier once every product the lane issued is done.
+__device__ __forceinline__ void tc_commit(uint64_t* bar, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+      "r"(elected)
+      : "memory");
+}
+
+// Shared-memory operand in 128-byte-swizzled atoms of 8 rows x 128 bytes.
+// Low word: address, and for a transposed operand the stride between its
+// 128-byte column panels; high word: 1024 bytes between atoms along the rows,
+// the descriptor's version and the swizzle.
+constexpr uint32_t kOperandHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t operand_low(uint32_t addr, uint32_t panel_bytes) {
+  return (addr >> 4) | ((panel_bytes >> 4) << 16);
 }
 
 // D = A B (+ D), FP16 operands from shared memory, fp32 accumulator.
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, bool add,
+                                          uint32_t elected) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "mov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(elected), "r"(kOperandHigh)
       : "memory");
 }
 
 // The same with A in tensor memory.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_low, uint32_t idesc, bool add,
+                                          uint32_t elected) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "mov.b64 b, {%2, %6};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_low), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(elected), "r"(kOperandHigh)
       : "memory");
 }
 
@@ -115,42 +140,49 @@ __device__ __forceinline__ void tmem_store_32(uint32_t addr, const uint32_t (&r)
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_store_16(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_store_8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_load_8(uint32_t (&r)[8], uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_4(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3])
+               : "memory");
+}
+
+// 16 bytes, or zeros where `use` is false (without a branch).
+__device__ __forceinline__ uint4 load_or_zero(const uint8_t* p, bool use) {
+  uint4 v;
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"(static_cast<uint32_t>(use)));
+  return v;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Shared-memory operand in 128-byte-swizzled atoms of 8 rows x 128 bytes:
-// stride between atoms along the rows (1024 bytes here) and, for a
-// transposed operand, between 128-byte column panels.
-__device__ __forceinline__ uint64_t tc_operand(uint32_t addr, uint32_t panel_bytes) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>((panel_bytes >> 4) & 0x3FFF) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-
 // FP16 operands, fp32 accumulator, M = 128; B transposed (rows of
 // contraction) or not.
 __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool transposed_b) {
   return (1u << 4) | ((transposed_b ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
-}
-
-// A barrier of `threads` threads that returns the OR of their predicates.
-__device__ __forceinline__ bool vote_barrier(int id, int threads, bool x) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %3, 0;\n\t"
-      "barrier.cta.red.or.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(x))
-      : "memory");
-  return r != 0;
 }
 
 // ------------------------------------------------------------------ work list
@@ -196,11 +228,49 @@ struct TilePlace {
   TileSpan s;
 };
 
+// The place of work-list entry g; the next pair after a place.
+template <int TT>
+__device__ __forceinline__ void tile_start(const AttendArgs& a, const int* before, int g, TilePlace* at) {
+  const int heads = a.c.heads;
+  int lo = 0, hi = a.t.seqs - 1;  // last b with before[b] * heads <= g
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (static_cast<long long>(before[mid]) * heads <= g) lo = mid;
+    else hi = mid - 1;
+  }
+  at->b = lo;
+  at->w = tile_sequence(a, lo);
+  const int x = g - before[lo] * heads, each = before[lo + 1] - before[lo];
+  at->head = x / each;
+  at->tile = 0;
+  at->chunk = x - at->head * each;
+  at->s = tile_span<TT>(a, at->w, 0);
+  while (at->chunk >= at->s.chunks) {
+    at->chunk -= at->s.chunks;
+    at->s = tile_span<TT>(a, at->w, ++at->tile);
+  }
+}
+
+template <int TT>
+__device__ __forceinline__ void tile_next_pair(const AttendArgs& a, const int* before, TilePlace* at) {  // there is one
+  at->chunk = 0;
+  if (++at->tile == at->w.tiles) {
+    at->tile = 0;
+    if (++at->head == a.c.heads) {
+      at->head = 0;
+      do {
+        ++at->b;
+      } while (before[at->b + 1] == before[at->b]);
+      at->w = tile_sequence(a, at->b);
+    }
+  }
+  at->s = tile_span<TT>(a, at->w, at->tile);
+}
+
 struct TileSmem {
   float meta[kTileMeta][8][2];        // [16 tokens of the tile][scale of keys, log2 of values' scale]
-  int meta_ok[kTileMeta];             // bit g: those tokens' page is good
+  int meta_missing[kTileMeta];        // bit g: those tokens' page is not there
   float row_scale[kTileAttendRows];
-  float exchange[2][kTileAttendRows][2];
   float out_scale[kTileAttendRows];
   float merged_ref[kTileAttendRows];
   uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
@@ -221,6 +291,189 @@ struct TileShape {
   static constexpr int kColS = 0, kColP = 2 * kTokens, kColO = 3 * kTokens;  // tensor memory columns
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kPanels) * kQueryPanel + 4 * kTileKvBytes + sizeof(TileSmem);
 };
+
+// ------------------------------------------------------------------ softmax of a tile
+
+// What a row keeps over its tiles.
+struct RowSoftmax {
+  float m, l, mp;  // reference and sum of 2^(logit - m); reference of the weights
+};
+
+struct TileLogits {
+  uint32_t from, to;        // S and P of this tile in tensor memory, this warp's lanes
+  const float (*meta)[2];   // per 16 tokens: scale of keys, log2 of values' scale
+  float row_scale;          // logits per product (capped: logits / cap)
+  float cap2;               // cap * log2(e)
+  int low, high;            // this row sees the tile's tokens low .. high
+};
+
+// The largest product of each 16 of the 64 tokens in s.
+template <bool MASK>
+__device__ __forceinline__ void group_maxima(float* t, const uint32_t (&s)[2][32], int k0, int low, int high) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      v[k] = __uint_as_float(s[q >> 1][(q & 1) * 16 + k]);
+      if (MASK && (k0 + q * 16 + k < low || k0 + q * 16 + k > high)) v[k] = kNegInf;
+    }
+    float top = max3(v[0], v[1], v[2]);
+#pragma unroll
+    for (int k = 3; k < 15; k += 2) top = max3(top, v[k], v[k + 1]);
+    t[q] = fmaxf(top, v[15]);
+  }
+}
+
+// Weights of the 64 tokens in s into P, and their sum.
+template <bool CAP, bool MASK>
+__device__ __forceinline__ void group_weights(RowSoftmax& r, const TileLogits& z, const uint32_t (&s)[2][32], int k0) {
+  // cap tanh(u) in units of log 2: u times a polynomial of u^2 of degree 4
+  // (Chebyshev fit of tanh(u) / u on |u| <= 0.7, off by 1.9e-7)
+  const float c0 = 0.999999706f * z.cap2, c1 = -0.33330266f * z.cap2, c2 = 0.132816473f * z.cap2,
+              c3 = -0.0508535559f * z.cap2, c4 = 0.0137912829f * z.cap2;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t p[8];
+      const int q = (k0 >> 4) + c * 2 + h;
+      const float f = z.row_scale * z.meta[q][0], shift = z.meta[q][1] - r.mp;
+      float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = h * 16 + 2 * k + e;
+          const float v = __uint_as_float(s[c][i]);
+          if (CAP) {
+            const float u = v * f, t = u * u;
+            float y = fmaf(c4, t, c3);
+            y = fmaf(y, t, c2);
+            y = fmaf(y, t, c1);
+            y = fmaf(y, t, c0);
+            w[e] = fmaf(y, u, shift);
+          } else {
+            w[e] = fmaf(v, f, shift);
+          }
+          w[e] = ex2(w[e]);
+          if (MASK && (k0 + c * 32 + i < z.low || k0 + c * 32 + i > z.high)) w[e] = 0.f;
+        }
+        sum0 += w[0];
+        sum1 += w[1];
+        p[k] = half2_bits(__floats2half2_rn(w[0], w[1]));
+      }
+      r.l = fmaf(sum0 + sum1, ex2(-shift - r.m), r.l);  // 2^(logit - m) = w 2^(mp - lv - m)
+      tmem_store_8(z.to + k0 / 2 + c * 16 + h * 8, p);
+    }
+  }
+}
+
+__device__ __forceinline__ void load_64(uint32_t (&s)[2][32], uint32_t from) {
+  tmem_load_32(s[0], from);
+  tmem_load_32(s[1], from + 32);
+  tmem_wait_load();
+}
+
+// A tile's weights, if it is usual. `scale_sums(f)` multiplies the row's sums
+// so far by f. False (for the whole warp): take the slow way.
+template <int TT, bool CAP, bool MASK, typename ScaleSums>
+__device__ __forceinline__ bool usual_tile(RowSoftmax& r, const TileLogits& z, ScaleSums&& scale_sums) {
+  constexpr int kHalves = TT / 64, kGroups = TT / 16;
+  uint32_t s[2][32];
+  float t[kGroups];
+  bool unusual = false;
+  float top = r.mp, top_lv = 0.f;
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h) {
+    load_64(s, z.from + h * 64);
+    group_maxima<MASK>(t + h * 4, s, h * 64, z.low, z.high);
+#pragma unroll
+    for (int q = h * 4; q < h * 4 + 4; ++q) {
+      const float f = z.row_scale * z.meta[q][0], lv = z.meta[q][1];
+      const float u = t[q] * f;
+      const bool none = MASK && t[q] == kNegInf;
+      unusual |= !(f > 0.f) || (CAP && !none && !(fabsf(u) <= 0.7f));
+      // (capped: u bounds tanh(u) above for u >= 0, and is near it below)
+      const float v = none ? kNegInf : (CAP ? u * z.cap2 : u) + lv;
+      if (v > top) {
+        top = v;
+        top_lv = lv;
+      }
+    }
+  }
+  if (__any_sync(0xFFFFFFFFu, !unusual && top - r.mp > kAttendRaise)) {
+    const bool raise = !unusual && top - r.mp > kAttendRaise;
+    const float mp = raise ? top : r.mp, m = mp - top_lv;
+    if (raise && m - r.m > kAttendRaiseSum) {
+      r.l *= ex2(r.m - m);
+      r.m = m;
+    }
+    scale_sums(ex2(r.mp - mp));
+    r.mp = mp;
+  }
+#pragma unroll
+  for (int q = 0; q < kGroups; ++q)
+    unusual |= !(fabsf(r.mp - z.meta[q][1] - r.m) <= 60.f) && !(MASK && t[q] == kNegInf && r.m == kAttendStart);
+  if (__any_sync(0xFFFFFFFFu, unusual)) return false;
+#pragma unroll
+  for (int h = kHalves - 1; h >= 0; --h) {  // the last 64 are still in registers
+    if (h < kHalves - 1) load_64(s, z.from + h * 64);
+    group_weights<CAP, MASK>(r, z, s, h * 64);
+  }
+  return true;
+}
+
+// Any tile, eight tokens at a time. `missing`: bit q set where the 16 tokens'
+// page is not there; masked and missing tokens weigh nothing.
+template <int TT, typename ScaleSums>
+__device__ __forceinline__ void any_tile(RowSoftmax& r, const TileLogits& z, int missing, ScaleSums&& scale_sums) {
+  auto logits = [&](float (&y)[8], int k0) {
+    uint32_t s[8];
+    tmem_load_8(s, z.from + k0);
+    tmem_wait_load();
+    const float f = z.row_scale * z.meta[k0 >> 4][0];
+    const bool there = !((missing >> (k0 >> 4)) & 1);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float v = __uint_as_float(s[k]) * f;
+      if (z.cap2 != 0.f) v = z.cap2 - __fdividef(2.f * z.cap2, ex2(v * (2.f * kLog2e)) + 1.f);
+      y[k] = k0 + k < z.low || k0 + k > z.high || !there ? kNegInf : v;
+    }
+  };
+  float top = r.m, top_v = r.mp;
+#pragma unroll 1
+  for (int k0 = 0; k0 < TT; k0 += 8) {
+    float y[8];
+    logits(y, k0);
+    const float lv = z.meta[k0 >> 4][1];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      top = fmaxf(top, y[k]);
+      if (y[k] != kNegInf) top_v = fmaxf(top_v, y[k] + lv);
+    }
+  }
+  r.l *= ex2(r.m - top);
+  r.m = top;
+  scale_sums(ex2(r.mp - top_v));
+  r.mp = top_v;
+#pragma unroll 1
+  for (int k0 = 0; k0 < TT; k0 += 8) {
+    float y[8];
+    logits(y, k0);
+    const float shift = z.meta[k0 >> 4][1] - r.mp;
+    uint32_t p[4];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      r.l += ex2(y[k] - r.m);
+      y[k] = y[k] == kNegInf ? 0.f : ex2(y[k] + shift);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) p[k] = half2_bits(__floats2half2_rn(y[2 * k], y[2 * k + 1]));
+    tmem_store_4(z.to + k0 / 2, p);
+  }
+}
 
 // ------------------------------------------------------------------ kernel
 
@@ -280,47 +533,14 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
     }
   }
   __syncthreads();
-  const uint32_t tmem = sm.tmem;
+  constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: they begin at 0
   const int total = sm.before[a.t.seqs] * heads;
   const int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   const int g0 = static_cast<int>(min(static_cast<long long>(blockIdx.x) * per, static_cast<long long>(total)));
   const int g1 = min(g0 + per, total);
 
   // ---- each role walks the CTA's run pair by pair
-  TilePlace at{};
-  auto start = [&]() {
-    int lo = 0, hi = a.t.seqs - 1;  // last b with before[b] * heads <= g0
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (static_cast<long long>(sm.before[mid]) * heads <= g0) lo = mid;
-      else hi = mid - 1;
-    }
-    at.b = lo;
-    at.w = tile_sequence(a, lo);
-    const int x = g0 - sm.before[lo] * heads, each = sm.before[lo + 1] - sm.before[lo];
-    at.head = x / each;
-    at.tile = 0;
-    at.chunk = x - at.head * each;
-    at.s = tile_span<TT>(a, at.w, 0);
-    while (at.chunk >= at.s.chunks) {
-      at.chunk -= at.s.chunks;
-      at.s = tile_span<TT>(a, at.w, ++at.tile);
-    }
-  };
-  auto next_pair = [&]() {  // there is one
-    at.chunk = 0;
-    if (++at.tile == at.w.tiles) {
-      at.tile = 0;
-      if (++at.head == heads) {
-        at.head = 0;
-        do {
-          ++at.b;
-        } while (sm.before[at.b + 1] == sm.before[at.b]);
-        at.w = tile_sequence(a, at.b);
-      }
-    }
-    at.s = tile_span<TT>(a, at.w, at.tile);
-  };
+  TilePlace at;
   // Once a wait has run out (status raised) a role waits no more: the results
   // are void, but every thread still meets the barriers and returns.
   bool dead = false;
@@ -333,44 +553,50 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
   } else if (warp >= kIssuer) {
     // ---- products
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTileIssuerRegs));
-    if (warp == kIssuer && lane == 0) {
-      start();
-      const uint32_t q_addr = smem_addr(q_tile), k_base = smem_addr(k_tiles), v_base = smem_addr(v_tiles);
-      auto scores = [&](int j) {  // S of tile j (of the ring)
-        const uint32_t k_addr = k_base + (j & 1) * kTileKvBytes;
-        wait(&sm.k_full[j & 1], (j >> 1) & 1);
+    if (warp == kIssuer) {
+      tile_start<TT>(a, sm.before, g0, &at);
+      const uint32_t elected = elect_lane();
+      const uint32_t q_low = operand_low(smem_addr(q_tile), 16), k_low = operand_low(smem_addr(k_tiles), 16),
+                     v_low = operand_low(smem_addr(v_tiles), Shape::kPanelBytes);
+      // (what the compiler cannot see to be uniform passes through a reduction)
+      auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+        wait(bar, parity);
+        dead = __any_sync(0xFFFFFFFFu, dead);
+      };
+      auto scores = [&](uint32_t j) {  // S of tile j (of the ring)
+        wait_warp(&sm.k_full[j & 1], (j >> 1) & 1);
         if (dead) return;
         tc_fence_after();
+        const uint32_t k_at = k_low + (j & 1) * (kTileKvBytes >> 4), s_at = Shape::kColS + (j & 1) * TT;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
-          tc_mma_ss(tmem + Shape::kColS + (j & 1) * TT, tc_operand(q_addr + (k >> 2) * Shape::kQueryPanel + (k & 3) * 32, 16),
-                    tc_operand(k_addr + (k >> 2) * Shape::kPanelBytes + (k & 3) * 32, 16), tc_idesc(TT, false), k > 0);
-        tc_commit(&sm.s_full[j & 1]);
+          tc_mma_ss(s_at, q_low + (((k >> 2) * Shape::kQueryPanel + (k & 3) * 32) >> 4),
+                    k_at + (((k >> 2) * Shape::kPanelBytes + (k & 3) * 32) >> 4), tc_idesc(TT, false), k > 0, elected);
+        tc_commit(&sm.s_full[j & 1], elected);
       };
-      int done = 0, pair = 0;  // KV tiles and pairs before: the rings' phases
+      uint32_t done = 0, pair = 0;  // KV tiles and pairs before: the rings' phases
       for (int g = g0; g < g1; ++pair) {
-        const int run = min(at.s.chunks - at.chunk, g1 - g);
-        wait(&sm.q_full, pair & 1);
+        const uint32_t run = __reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(min(at.s.chunks - at.chunk, g1 - g)));
+        wait_warp(&sm.q_full, pair & 1);
         scores(done);
-        for (int i = 0; i < run && !dead; ++i) {
-          const int j = done + i;
+        for (uint32_t i = 0; i < run && !dead; ++i) {
+          const uint32_t j = done + i;
           if (i + 1 < run) scores(j + 1);
-          wait(&sm.v_full[j & 1], (j >> 1) & 1);
-          wait(&sm.p_full[j & 1], (j >> 1) & 1);
-          if (i == 0 && pair > 0) wait(&sm.o_free, (pair - 1) & 1);
+          wait_warp(&sm.v_full[j & 1], (j >> 1) & 1);
+          wait_warp(&sm.p_full[j & 1], (j >> 1) & 1);
+          if (i == 0 && pair > 0) wait_warp(&sm.o_free, (pair - 1) & 1);
           if (dead) break;
           tc_fence_after();
-          const uint32_t v_addr = v_base + (j & 1) * kTileKvBytes;
+          const uint32_t v_at = v_low + (j & 1) * (kTileKvBytes >> 4), p_at = Shape::kColP + (j & 1) * (TT / 2);
 #pragma unroll
           for (int k = 0; k < TT / 16; ++k)
-            tc_mma_ts(tmem + Shape::kColO, tmem + Shape::kColP + (j & 1) * (TT / 2) + k * 8,
-                      tc_operand(v_addr + k * 2048, Shape::kPanelBytes), tc_idesc(DP, true), i > 0 || k > 0);
-          tc_commit(&sm.pv_done[j & 1]);
+            tc_mma_ts(Shape::kColO, p_at + k * 8, v_at + ((k * 2048) >> 4), tc_idesc(DP, true), i > 0 || k > 0, elected);
+          tc_commit(&sm.pv_done[j & 1], elected);
         }
         if (dead) break;
         done += run;
         g += run;
-        if (g < g1) next_pair();
+        if (g < g1) tile_next_pair<TT>(a, sm.before, &at);
       }
     }
     __syncwarp();
@@ -381,181 +607,179 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
     const int tid = threadIdx.x - (kTileSoftmaxWarps + (keys ? 0 : kTileLoaderWarps)) * 32;  // 0 .. 127
     const uint8_t* codes = keys ? a.c.k_codes : a.c.v_codes;
     unsigned char* tiles = keys ? k_tiles : v_tiles;
-    constexpr int kHalf = 4;                   // 16-byte vectors per thread and half tile
-    constexpr int kPerToken = DP / 16;         // vectors per token
-    constexpr int kStep = 128 / kPerToken;     // tokens per round: 8 or 16
-    const int ch = tid % kPerToken, sub = tid / kPerToken;
-    // The halves of all tiles in order, two on the way while a third is
-    // widened: `ahead` is the place of the next one to load.
-    start();
-    int load_g = g0, load_run = min(at.s.chunks - at.chunk, g1 - g0), load_i = 0, load_half = 0;
-    int pages = -1;  // of this lane's (lane < GROUPS) 16 tokens of the tile to load
-    auto find_pages = [&]() {
-      pages = -1;
-      const int t0 = at.s.low + (at.chunk + load_i) * TT + lane * 16;
-      if (lane < GROUPS && t0 <= at.s.pos_max) {
-        const int column = t0 >> a.c.page_shift;
-        pages = column < a.t.max_pages ? a.t.table[at.b * a.t.table_stride + column] : -1;
-        if (pages < 0 || pages >= a.c.pages) {
-          raise_status(kStatusBadArgument);
-          pages = -1;
-        }
-      }
+    constexpr int kHalf = 4;  // 16-byte vectors per thread and half tile
+    // A warp's vector: 8 tokens x 64 bytes. The 8 lanes of a shared-memory
+    // phase hold one column of 8 tokens: all banks, in the swizzled layout.
+    constexpr int kStep = Shape::kTokens / 8;  // tokens between a thread's vectors: 8 or 16
+    const int w4 = tid >> 5;
+    const int panel = w4 % PANELS, sub = (w4 / PANELS) * 8 + (lane & 7);  // panel of 64 dimensions, token of a vector
+    const int column = panel * 64 + (lane >> 3) * 16;
+    const int dim = a.c.dim;
+    const bool wanted = column < dim;
+    const uint8_t* source = codes + column;
+    const int place = panel * Shape::kPanelBytes + sub * 128;
+    const int place0 = place + ((((lane >> 3) * 2) ^ (lane & 7)) << 4), place1 = place + ((((lane >> 3) * 2 + 1) ^ (lane & 7)) << 4);
+
+    // Lane g < GROUPS keeps, for the tile to load, the row (of all the
+    // cache's rows of `dim` codes) where its 16 tokens begin, -1 if none; its
+    // page for the tile after that is on its way too.
+    tile_start<TT>(a, sm.before, g0, &at);
+    int walk_t0 = at.s.low + at.chunk * TT, walk_left = min(at.s.chunks - at.chunk, g1 - g0), walk_g = g0 + walk_left;
+    int walk_head = at.head, walk_end = at.s.pos_max + 1;
+    const int32_t* walk_table = a.t.table + at.b * a.t.table_stride;
+    int page_next = 0;
+    auto fetch_pages = [&]() {
+      const int t = walk_t0 + lane * 16;
+      page_next = -2;  // none due
+      if (lane < GROUPS && t < walk_end)
+        page_next = (t >> a.c.page_shift) < a.t.max_pages ? walk_table[t >> a.c.page_shift] : -1;
     };
-    float ks = 0.f, vs = 0.f;  // this lane's block scales of the tile loaded last (first warp of the keys)
-    unsigned ok = 0;
-    auto load = [&](uint4 (&r)[kHalf]) {
-      if (load_g >= g1) return;
-      const int t0 = at.s.low + (at.chunk + load_i) * TT;
+    bool missing = false;  // a page that is due is not there
+    int rows_at = -1, limit = 0;  // limit: of a vector's first token, for this lane's token to count
+    float ks = 0.f, vs = 0.f;  // this lane's block scales of that tile (first warp of the keys)
+    auto take_tile = [&]() {   // the fetched pages become the tile to load; fetch the next one's
+      rows_at = -1;
+      missing = page_next != -2 && (page_next < 0 || page_next >= a.c.pages);
+      if (missing)
+        raise_status(kStatusBadArgument);
+      else if (page_next != -2)
+        rows_at = (page_next * heads + walk_head) * a.c.page_size + ((walk_t0 + lane * 16) & (a.c.page_size - 1));
+      limit = wanted ? walk_end - walk_t0 - sub : 0;
+      walk_t0 += TT;
+      if (--walk_left == 0) {
+        if (walk_g >= g1) return;
+        tile_next_pair<TT>(a, sm.before, &at);  // (a pair cut at the run's end is its last)
+        walk_t0 = at.s.low;
+        walk_left = min(at.s.chunks, g1 - walk_g);
+        walk_g += walk_left;
+        walk_head = at.head;
+        walk_end = at.s.pos_max + 1;
+        walk_table = a.t.table + at.b * a.t.table_stride;
+      }
+      fetch_pages();
+    };
+    auto load = [&](uint4 (&r)[kHalf], int first) {
+      int row[kHalf];
+#pragma unroll
+      for (int v = 0; v < kHalf; ++v) row[v] = __shfl_sync(0xFFFFFFFFu, rows_at, ((first + v) * kStep) >> 4);
 #pragma unroll
       for (int v = 0; v < kHalf; ++v) {
-        const int token = (load_half * kHalf + v) * kStep + sub;
-        const int page = __shfl_sync(0xFFFFFFFFu, pages, token >> 4);
-        r[v] = make_uint4(0, 0, 0, 0);
-        if (page >= 0 && t0 + token <= at.s.pos_max && ch * 16 < a.c.dim) {
-          const long long row =
-              (static_cast<long long>(page) * heads + at.head) * a.c.page_size + ((t0 + token) & (a.c.page_size - 1));
-          r[v] = __ldg(reinterpret_cast<const uint4*>(codes + row * a.c.dim + ch * 16));
-        }
+        const int in_group = ((first + v) * kStep & 15) + sub;
+        const bool use = row[v] >= 0 && (first + v) * kStep < limit;
+        r[v] = load_or_zero(source + static_cast<long long>(row[v] + in_group) * dim, use);
       }
-      load_half ^= 1;
-      if (load_half) {  // a new tile begins
-        if (keys && tid < 32) {
-          const long long block = static_cast<long long>(pages) * heads + at.head;
-          ks = pages >= 0 ? a.c.k_scales[block] : 0.f;
-          vs = pages >= 0 ? a.c.v_scales[block] : 1.f;
-          ok = __ballot_sync(0xFFFFFFFFu, pages >= 0);
-        }
-        return;
-      }
-      if (++load_i == load_run) {
-        load_g += load_run;
-        load_i = 0;
-        if (load_g >= g1) return;
-        if (at.chunk + load_run == at.s.chunks) next_pair();
-        else at.chunk += load_run;
-        load_run = min(at.s.chunks - at.chunk, g1 - load_g);
-      }
-      find_pages();
     };
-    auto store = [&](const uint4 (&r)[kHalf], int half, unsigned char* tile) {
+    auto store = [&](const uint4 (&r)[kHalf], int first, unsigned char* tile) {
 #pragma unroll
       for (int v = 0; v < kHalf; ++v) {
-        const int token = (half * kHalf + v) * kStep + sub;
-        uint4 h0, h1;
-        widen<KIND>(r[v].x, h0.x, h0.y);
-        widen<KIND>(r[v].y, h0.z, h0.w);
-        widen<KIND>(r[v].z, h1.x, h1.y);
-        widen<KIND>(r[v].w, h1.z, h1.w);
-        // neighbouring panels' lanes write their two vectors in opposite
-        // order, so that a quarter-warp covers all banks
-        const bool flip = (ch >> 2) & 1;
-        unsigned char* row = tile + (ch >> 2) * Shape::kPanelBytes + token * 128;
-        const int c16 = (ch & 3) * 2;
-        *reinterpret_cast<uint4*>(row + (((c16 + flip) ^ (token & 7)) << 4)) = flip ? h1 : h0;
-        *reinterpret_cast<uint4*>(row + (((c16 + !flip) ^ (token & 7)) << 4)) = flip ? h0 : h1;
+        uint4 h;
+        widen<KIND>(r[v].x, h.x, h.y);
+        widen<KIND>(r[v].y, h.z, h.w);
+        *reinterpret_cast<uint4*>(tile + place0 + (first + v) * kStep * 128) = h;
+        widen<KIND>(r[v].z, h.x, h.y);
+        widen<KIND>(r[v].w, h.z, h.w);
+        *reinterpret_cast<uint4*>(tile + place1 + (first + v) * kStep * 128) = h;
       }
     };
-    uint4 r0[kHalf], r1[kHalf], r2[kHalf];
-    find_pages();
-    load(r0);
-    load(r1);
-    const int halves = 2 * (g1 - g0);
-    auto step = [&](int n, uint4 (&cur)[kHalf], uint4 (&later)[kHalf]) {
-      if (n >= halves) return;
-      const int j = n >> 1, half = n & 1, stage = j & 1;  // ring tile
-      if (half == 0) {
-        // the tile two before has been read by its products
-        if (j >= 2) wait(keys ? &sm.s_full[stage] : &sm.pv_done[stage], ((j >> 1) + 1) & 1);
-        if (keys && tid < 32) {  // loaded with this tile's first half; the next tile's are loaded below
-          const int slot = j % kTileMeta;
-          if (lane < GROUPS) {
-            sm.meta[slot][lane][0] = ks;
-            sm.meta[slot][lane][1] = lg2(vs);
-          }
-          if (lane == 0) sm.meta_ok[slot] = static_cast<int>(ok);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.meta_full[slot]);
-        }
+    // Two halves per tile, each loaded a tile ahead: 32 KB per SM on the way.
+    uint4 ra[kHalf], rb[kHalf];
+    fetch_pages();
+    take_tile();
+    load(ra, 0);
+    load(rb, kHalf);
+    const int tiles_all = g1 - g0;
+#pragma unroll 1
+    for (int j = 0; j < tiles_all; ++j) {
+      const int stage = j & 1;
+      unsigned char* tile = tiles + stage * kTileKvBytes;
+      if (keys && tid < 32) {
+        ks = rows_at >= 0 ? a.c.k_scales[rows_at >> a.c.page_shift] : 1.f;
+        vs = rows_at >= 0 ? a.c.v_scales[rows_at >> a.c.page_shift] : 1.f;
       }
-      load(later);
-      store(cur, half, tiles + stage * kTileKvBytes);
-      if (half == 1) {
-        fence_proxy_async_shared();
+      // the tile two before has been read by its products
+      if (j >= 2) wait(keys ? &sm.s_full[stage] : &sm.pv_done[stage], ((j >> 1) + 1) & 1);
+      const bool more = j + 1 < tiles_all;
+      const unsigned missing_groups = __ballot_sync(0xFFFFFFFFu, missing);
+      if (more) take_tile();
+      store(ra, 0, tile);
+      if (more) load(ra, 0);
+      store(rb, kHalf, tile);
+      if (more) load(rb, kHalf);
+      fence_proxy_async_shared();
+      if (keys && tid < 32) {
+        const int slot = j % kTileMeta;
+        if (lane < GROUPS) {
+          sm.meta[slot][lane][0] = ks;
+          sm.meta[slot][lane][1] = lg2(vs);
+        }
+        if (lane == 0) sm.meta_missing[slot] = static_cast<int>(missing_groups);
         __syncwarp();
-        if (lane == 0) mbar_arrive(keys ? &sm.k_full[stage] : &sm.v_full[stage]);
+        if (lane == 0) mbar_arrive(&sm.meta_full[slot]);
       }
-    };
-    for (int n = 0; n < halves; n += 3) {
-      step(n, r0, r2);
-      step(n + 1, r1, r0);
-      step(n + 2, r2, r1);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(keys ? &sm.k_full[stage] : &sm.v_full[stage]);
     }
   } else {
-    // ---- softmax: row 32 (warp % 4) + lane, tokens half * TT / 2 ..
+    // ---- softmax: row 32 warp + lane
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTileSoftmaxRegs));
-    constexpr int HC = TT / 2, HG = HC / 16;
     constexpr int kSoftmaxThreads = kTileSoftmaxWarps * 32;
-    const int quarter = warp & 3, half = warp >> 2;
-    const int row = quarter * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const int row = threadIdx.x;
+    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     const bool capped_logits = a.softcap != 0.f;
     const float cap2 = a.softcap * kLog2e;
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) {  // one answer for the warp
-      wait(bar, parity);
-      dead = __any_sync(0xFFFFFFFFu, dead);
-    };
-    // A pair's queries as FP16 times 2^-e, two threads per row.
+    // A pair's queries as FP16 times 2^-e (and the scale's sign), eight threads per row.
     auto load_queries = [&]() {
-      const int q_row = threadIdx.x >> 1, part = threadIdx.x & 1;
+      constexpr int kVectors = DP / 64;
+      const int part = threadIdx.x & 7;
       const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
-      const int all = at.tile * kTileAttendRows + q_row;
-      const bool live = all < at.w.rows;
-      const int i = live ? all / a.group : 0;
-      const uint16_t* src = a.q + (token0 + i) * a.q_ts + (at.head * a.group + (live ? all - i * a.group : 0)) * a.q_hs;
-      auto vector = [&](int c) {  // 16-byte chunk c of the row
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live && c * 8 < a.c.dim) {
-          if (a.q_vec) {
-            v = *reinterpret_cast<const uint4*>(src + c * 8);
-          } else {
-            const uint16_t* s = src + c * 8;
-            v = make_uint4(s[0] | (static_cast<uint32_t>(s[1]) << 16), s[2] | (static_cast<uint32_t>(s[3]) << 16),
-                           s[4] | (static_cast<uint32_t>(s[5]) << 16), s[6] | (static_cast<uint32_t>(s[7]) << 16));
+      const int rows_left = at.w.rows - at.tile * kTileAttendRows;
+#pragma unroll 4
+      for (int q_row = threadIdx.x >> 3; q_row < kTileAttendRows; q_row += kSoftmaxThreads / 8) {
+        const int all = at.tile * kTileAttendRows + q_row;
+        const bool live = q_row < rows_left;
+        const int i = live ? all / a.group : 0;
+        const uint16_t* src = a.q + (token0 + i) * a.q_ts + (at.head * a.group + (live ? all - i * a.group : 0)) * a.q_hs;
+        uint4 raw[kVectors];
+        unsigned big = 0;
+#pragma unroll
+        for (int j = 0; j < kVectors; ++j) {
+          const int c = j * 8 + part;  // 16-byte chunk of the row
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (live && c * 8 < a.c.dim) {
+            if (a.q_vec) {
+              v = __ldg(reinterpret_cast<const uint4*>(src + c * 8));
+            } else {
+              const uint16_t* s = src + c * 8;
+              v = make_uint4(s[0] | (static_cast<uint32_t>(s[1]) << 16), s[2] | (static_cast<uint32_t>(s[3]) << 16),
+                             s[4] | (static_cast<uint32_t>(s[5]) << 16), s[6] | (static_cast<uint32_t>(s[7]) << 16));
+            }
+          }
+          raw[j] = v;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t w = word_of(v, k);
+            big = max(big, max((w << 16) & 0x7FFFFFFFu, w & 0x7FFF0000u));
           }
         }
-        return v;
-      };
-      unsigned big = 0;
-#pragma unroll 4
-      for (int j = 0; j < DP / 16; ++j) {
-        const uint4 v = vector(j * 2 + part);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t w = word_of(v, k);
-          big = max(big, max((w << 16) & 0x7FFFFFFFu, w & 0x7FFF0000u));
-        }
+        for (int d = 1; d < 8; d <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
+        int e = static_cast<int>(big >> 23) - 127;
+        e = big == 0 ? 0 : max(min(e, 120), -120);
+        const float down = copysignf(__uint_as_float(static_cast<unsigned>(127 - e) << 23), a.scale);
+        auto halves = [&](uint32_t w) {
+          return half2_bits(__floats2half2_rn(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down));
+        };
+#pragma unroll
+        for (int j = 0; j < kVectors; ++j)
+          *reinterpret_cast<uint4*>(q_tile + j * Shape::kQueryPanel + q_row * 128 + ((part ^ (q_row & 7)) << 4)) =
+              make_uint4(halves(raw[j].x), halves(raw[j].y), halves(raw[j].z), halves(raw[j].w));
+        if (part == 0) sm.row_scale[q_row] = __uint_as_float(static_cast<unsigned>(127 + e) << 23) * fabsf(a.scale);
       }
-      big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-      int e = static_cast<int>(big >> 23) - 127;
-      e = max(min(e, 120), -120);
-      const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
-      auto halves = [&](uint32_t w) {
-        return half2_bits(__floats2half2_rn(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down));
-      };
-#pragma unroll 4
-      for (int j = 0; j < DP / 16; ++j) {  // (from the cache again: fewer registers)
-        const int c = j * 2 + part;
-        const uint4 v = vector(c);
-        *reinterpret_cast<uint4*>(q_tile + (c >> 3) * Shape::kQueryPanel + q_row * 128 + (((c & 7) ^ (q_row & 7)) << 4)) =
-            make_uint4(halves(v.x), halves(v.y), halves(v.z), halves(v.w));
-      }
-      if (part == 0) sm.row_scale[q_row] = __uint_as_float(static_cast<unsigned>(127 + e) << 23) * a.scale;
       fence_proxy_async_shared();
-      named_barrier(5, kSoftmaxThreads);
+      named_barrier(1, kSoftmaxThreads);
       if (lane == 0) mbar_arrive(&sm.q_full);
     };
-    start();
+    tile_start<TT>(a, sm.before, g0, &at);
     load_queries();
     int done = 0;  // KV tiles of the pairs before: the rings' phases
     for (int g = g0; g < g1;) {
@@ -563,143 +787,53 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       const int rows = min(kTileAttendRows, at.w.rows - at.tile * kTileAttendRows);
       const int t_first = at.s.low + at.chunk * TT;
       const int pos_min = at.s.pos_min, pos_max = at.s.pos_max;
-      const bool active = quarter * 32 < rows;  // rows past the tile's are left out, warp by warp
+      const bool active = warp * 32 < rows;  // rows past the tile's are left out, warp by warp
       const float row_scale = sm.row_scale[row] * (capped_logits ? 1.f / a.softcap : kLog2e);
       const int pos = at.w.first + min(at.tile * kTileAttendRows + row, at.w.rows - 1) / a.group;
-      float m = kAttendStart, l = 0.f, mp = kAttendStart;
+      RowSoftmax r{kAttendStart, 0.f, kAttendStart};
+#pragma unroll 1
       for (int i = 0; i < run; ++i) {
         const int j = done + i, slot = j % kTileMeta;
-        const int t0 = t_first + i * TT + half * HC;
-        wait_all(&sm.meta_full[slot], (j / kTileMeta) & 1);
-        wait_all(&sm.s_full[j & 1], (j >> 1) & 1);
+        const int t0 = t_first + i * TT;
+        wait(&sm.meta_full[slot], (j / kTileMeta) & 1);
+        // S of this tile is there; the products run in order, so P V of the
+        // tile two before, which was issued earlier, has read its P
+        wait(&sm.s_full[j & 1], (j >> 1) & 1);
         tc_fence_after();
         if (active) {
-          float x[HC];
+          TileLogits z;
+          z.from = tmem + lanes + Shape::kColS + (j & 1) * TT;
+          z.to = tmem + lanes + Shape::kColP + (j & 1) * (TT / 2);
+          z.meta = sm.meta[slot];
+          z.row_scale = row_scale;
+          z.cap2 = cap2;
+          z.low = a.window ? pos - a.window + 1 - t0 : 0;
+          z.high = pos - t0;
+          const int missing = sm.meta_missing[slot];
+          auto scale_sums = [&](float f) {
+            if (i == 0 || !__any_sync(0xFFFFFFFFu, f != 1.f)) return;
+            wait(&sm.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1);
+            tc_fence_after();
+#pragma unroll 1
+            for (int q = 0; q < DP / 32; ++q) {
+              const uint32_t addr = tmem + lanes + Shape::kColO + q * 32;
+              uint32_t o[32];
+              tmem_load_32(o, addr);
+              tmem_wait_load();
 #pragma unroll
-          for (int q = 0; q < HC / 32; ++q) {
-            uint32_t s[32];
-            tmem_load_32(s, tmem + lanes + Shape::kColS + (j & 1) * TT + half * HC + q * 32);
-            tmem_wait_load();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) x[q * 32 + k] = __uint_as_float(s[k]);
-          }
-          float lv[HG];
-#pragma unroll
-          for (int q = 0; q < HG; ++q) {
-            const float f = row_scale * sm.meta[slot][half * HG + q][0];
-            lv[q] = sm.meta[slot][half * HG + q][1];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) x[q * 16 + k] *= f;
-          }
-          if (capped_logits) {
-            // cap tanh(u), u = x / cap: u times a polynomial of u^2 of degree
-            // 4 (Chebyshev fit of tanh(u) / u on |u| <= 0.7, off by 1.9e-7)
-            float wide = 0.f;
-#pragma unroll
-            for (int k = 0; k < HC; ++k) wide = fmaxf(wide, fabsf(x[k]));
-            if (!__any_sync(0xFFFFFFFFu, wide > 0.7f)) {
-#pragma unroll
-              for (int k = 0; k < HC; ++k) {
-                const float u = x[k], t = u * u;
-                float y = fmaf(0.0137912829f, t, -0.0508535559f);
-                y = fmaf(y, t, 0.132816473f);
-                y = fmaf(y, t, -0.33330266f);
-                y = fmaf(y, t, 0.999999706f);
-                x[k] = y * (u * cap2);
-              }
-            } else {
-#pragma unroll
-              for (int k = 0; k < HC; ++k)
-                x[k] = cap2 - __fdividef(2.f * cap2, ex2(x[k] * (2.f * kLog2e)) + 1.f);
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_store_32(addr, o);
             }
+          };
+          const bool masked = t0 + TT - 1 > pos_min || (a.window && pos_max - t0 >= a.window);
+          bool finished = false;
+          if (missing == 0) {
+            if (capped_logits)
+              finished = masked ? usual_tile<TT, true, true>(r, z, scale_sums) : usual_tile<TT, true, false>(r, z, scale_sums);
+            else
+              finished = masked ? usual_tile<TT, false, true>(r, z, scale_sums) : usual_tile<TT, false, false>(r, z, scale_sums);
           }
-          const int ok = sm.meta_ok[slot] >> (half * HG);
-          const bool masked = t0 + HC - 1 > pos_min || (a.window && pos_max - t0 >= a.window) ||
-                              (ok & ((1 << HG) - 1)) != (1 << HG) - 1;
-          if (masked) {
-#pragma unroll
-            for (int k = 0; k < HC; ++k) {
-              const int t = t0 + k;
-              if (t > pos || (a.window && pos - t >= a.window) || !((ok >> (k >> 4)) & 1)) x[k] = kNegInf;
-            }
-          }
-          float top = kNegInf, top_v = kNegInf;
-#pragma unroll
-          for (int q = 0; q < HG; ++q) {
-            float t = x[q * 16];
-#pragma unroll
-            for (int k = 1; k < 16; ++k) t = fmaxf(t, x[q * 16 + k]);
-            top = fmaxf(top, t);
-            top_v = fmaxf(top_v, t + lv[q]);
-          }
-          if (top - m > kAttendRaiseSum) {  // this half's own reference
-            l *= ex2(m - top);
-            m = top;
-          }
-          if (vote_barrier(1 + quarter, 64, top_v - mp > kAttendRaise)) {
-            sm.exchange[half][row][0] = top_v;
-            named_barrier(1 + quarter, 64);
-            const float tv = fmaxf(mp, fmaxf(top_v, sm.exchange[half ^ 1][row][0]));
-            const float f = ex2(mp - tv);
-            mp = tv;
-            if (i > 0) {  // the sums so far, half of the columns each
-              wait_all(&sm.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1);
-              tc_fence_after();
-#pragma unroll
-              for (int q = 0; q < DP / 64; ++q) {
-                const uint32_t addr = tmem + lanes + Shape::kColO + half * (DP / 2) + q * 32;
-                uint32_t o[32];
-                tmem_load_32(o, addr);
-                tmem_wait_load();
-#pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                tmem_store_32(addr, o);
-              }
-              tmem_wait_store();
-            }
-            named_barrier(1 + quarter, 64);  // the exchange has been read
-          }
-          // weights, and the sum from them: 2^(x - m) = w 2^(mp - lv - m)
-          float up[HG];
-          bool far = false;
-#pragma unroll
-          for (int q = 0; q < HG; ++q) {
-            up[q] = mp - lv[q] - m;
-            far |= !(up[q] <= 80.f);
-          }
-          uint32_t p[HC / 2];
-          if (!__any_sync(0xFFFFFFFFu, far)) {
-#pragma unroll
-            for (int q = 0; q < HG; ++q) {
-              const float shift = lv[q] - mp;
-              float sum = 0.f;
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float w0 = ex2(x[q * 16 + 2 * k] + shift), w1 = ex2(x[q * 16 + 2 * k + 1] + shift);
-                sum += w0 + w1;
-                p[q * 8 + k] = half2_bits(__floats2half2_rn(w0, w1));
-              }
-              l = fmaf(sum, ex2(up[q]), l);
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < HG; ++q) {
-              const float shift = lv[q] - mp;
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float x0 = x[q * 16 + 2 * k], x1 = x[q * 16 + 2 * k + 1];
-                l += ex2(x0 - m) + ex2(x1 - m);
-                // a masked token weighs nothing, whatever its block's scale holds
-                const float w0 = x0 == kNegInf ? 0.f : ex2(x0 + shift), w1 = x1 == kNegInf ? 0.f : ex2(x1 + shift);
-                p[q * 8 + k] = half2_bits(__floats2half2_rn(w0, w1));
-              }
-            }
-          }
-          // P of the tile two before has been read
-          if (j >= 2) wait_all(&sm.pv_done[j & 1], ((j >> 1) + 1) & 1);
-          const uint32_t to = tmem + lanes + Shape::kColP + (j & 1) * (TT / 2) + half * (HC / 2);
-#pragma unroll
-          for (int q = 0; q < HC / 32; ++q) tmem_store_16(to + q * 16, p + q * 16);
+          if (!finished) any_tile<TT>(r, z, missing, scale_sums);
           tmem_wait_store();
         }
         tc_fence_before();
@@ -715,32 +849,26 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
       const int row0 = at.tile * kTileAttendRows, head = at.head;
       const bool more = g + run < g1;
-      named_barrier(5, kSoftmaxThreads);  // every warp has read row_scale and seen the last scores
+      named_barrier(1, kSoftmaxThreads);  // every warp has read row_scale and seen the last scores
       if (more) {
-        next_pair();
+        tile_next_pair<TT>(a, sm.before, &at);
         load_queries();
       }
-      wait_all(&sm.pv_done[(done + run - 1) & 1], ((done + run - 1) >> 1) & 1);
+      wait(&sm.pv_done[(done + run - 1) & 1], ((done + run - 1) >> 1) & 1);
       tc_fence_after();
       if (active) {
-        sm.exchange[half][row][0] = m;
-        sm.exchange[half][row][1] = l;
-        named_barrier(1 + quarter, 64);
-        const float m2 = sm.exchange[half ^ 1][row][0], l2 = sm.exchange[half ^ 1][row][1];
-        const float mm = fmaxf(m, m2);
-        const float sum = half ? l2 * ex2(m2 - mm) + l * ex2(m - mm) : l * ex2(m - mm) + l2 * ex2(m2 - mm);
-        const float f = whole ? (sum == 0.f ? 0.f : ex2(mp - mm) / sum) : 1.f;
-        if (!whole && half == 0 && row < rows) {
+        const float f = whole ? (r.l == 0.f ? 0.f : ex2(r.mp - r.m) / r.l) : 1.f;
+        if (!whole && row < rows) {
           float* st = part_out + kTileAttendRows * 256 + row * 4;
-          st[0] = mm;
-          st[1] = sum;
-          st[2] = mp;
+          st[0] = r.m;
+          st[1] = r.l;
+          st[2] = r.mp;
         }
         const int all = row0 + row, i_tok = all / a.group;
         uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (head * a.group + all - i_tok * a.group) * a.o_hs;
-#pragma unroll
-        for (int q = 0; q < DP / 64; ++q) {
-          const int d0 = half * (DP / 2) + q * 32;
+#pragma unroll 1
+        for (int q = 0; q < DP / 32; ++q) {
+          const int d0 = q * 32;
           uint32_t o[32];
           tmem_load_32(o, tmem + lanes + Shape::kColO + d0);
           tmem_wait_load();
@@ -781,13 +909,13 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       if (!whole) {
         // ---- join the CTAs of the tile: the last to arrive adds all in order
         __threadfence();
-        named_barrier(5, kSoftmaxThreads);
+        named_barrier(1, kSoftmaxThreads);
         if (threadIdx.x == 0) {
           const int arrived = atomic_add_acq_rel_gpu(a.counters + cta_first, 1);
           sm.last = arrived == cta_last - cta_first;
           if (sm.last) a.counters[cta_first] = 0;
         }
-        named_barrier(5, kSoftmaxThreads);
+        named_barrier(1, kSoftmaxThreads);
         if (sm.last) {
           __threadfence();
           const int parts = cta_last - cta_first + 1;
@@ -809,27 +937,41 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
             sm.merged_ref[threadIdx.x] = mmp;
             sm.out_scale[threadIdx.x] = sum == 0.f ? 0.f : ex2(mmp - mm) / sum;
           }
-          named_barrier(5, kSoftmaxThreads);
-          const int vectors = a.c.dim / 4;
-          for (int i = threadIdx.x; i < rows * vectors; i += kSoftmaxThreads) {
-            const int r = i / vectors, d = (i - r * vectors) * 4;
-            const float ref = sm.merged_ref[r], f = sm.out_scale[r];
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+          named_barrier(1, kSoftmaxThreads);
+          // eight vectors per thread at a time: their loads overlap
+          const int vectors = a.c.dim / 4, all_vectors = rows * vectors;
+          constexpr int kBatch = 8;
+#pragma unroll 1
+          for (int i0 = threadIdx.x; i0 < all_vectors; i0 += kBatch * kSoftmaxThreads) {
+            float4 v[kBatch];
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
             for (int n = 0; n < parts; ++n) {
               const float* pt = part_of(n);
-              const float4 u = __ldcg(reinterpret_cast<const float4*>(pt + r * 256 + d));
-              const float w = ex2(__ldcg(pt + kTileAttendRows * 256 + r * 4 + 2) - ref);
-              v.x += u.x * w, v.y += u.y * w, v.z += u.z * w, v.w += u.w * w;
+#pragma unroll
+              for (int e = 0; e < kBatch; ++e) {
+                const int i = min(i0 + e * kSoftmaxThreads, all_vectors - 1), r = i / vectors;
+                const float4 u = __ldcg(reinterpret_cast<const float4*>(pt + r * 256 + (i - r * vectors) * 4));
+                const float w = ex2(__ldcg(pt + kTileAttendRows * 256 + r * 4 + 2) - sm.merged_ref[r]);
+                v[e].x += u.x * w, v[e].y += u.y * w, v[e].z += u.z * w, v[e].w += u.w * w;
+              }
             }
-            const int all = row0 + r, i_tok = all / a.group;
-            uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (head * a.group + all - i_tok * a.group) * a.o_hs + d;
-            out[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v.x * f));
-            out[1] = __bfloat16_as_ushort(__float2bfloat16_rn(v.y * f));
-            out[2] = __bfloat16_as_ushort(__float2bfloat16_rn(v.z * f));
-            out[3] = __bfloat16_as_ushort(__float2bfloat16_rn(v.w * f));
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+              const int i = i0 + e * kSoftmaxThreads;
+              if (i >= all_vectors) break;
+              const int r = i / vectors, d = (i - r * vectors) * 4;
+              const float f = sm.out_scale[r];
+              const int all = row0 + r, i_tok = all / a.group;
+              uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (head * a.group + all - i_tok * a.group) * a.o_hs + d;
+              out[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e].x * f));
+              out[1] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e].y * f));
+              out[2] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e].z * f));
+              out[3] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e].w * f));
+            }
           }
-          named_barrier(5, kSoftmaxThreads);  // sm.last and the references are free
+          named_barrier(1, kSoftmaxThreads);  // sm.last and the references are free
         }
       }
       done += run;
@@ -839,7 +981,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kIssuer) tmem_free(tmem, 512);
+  if (warp == kIssuer) tmem_free(sm.tmem, 512);
 }
 
 // ------------------------------------------------------------------ launch
