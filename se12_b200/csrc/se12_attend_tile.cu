@@ -14,10 +14,12 @@
 //   warps 0-3   softmax: a thread per row
 //   warps 4-7   keys, warps 8-11 values: codes to FP16 tiles, two tiles deep
 //   warp 12     issues the products: S of tile j + 1 before P V of tile j, so
-//               that the tensor pipe works during the softmax (13-15 only
-//               complete its warp group)
+//               that the tensor pipe works during the softmax
+//   warps 13-15 the next pair's queries, while the softmax ends this one
 //
 // The roles walk the CTA's run on their own and meet at mbarriers only.
+// Code that runs once per pair is kept small: it is fetched cold (unrolled by
+// four rows, the queries took 20000 cycles a pair, most of it instructions).
 //
 // The softmax goes over S twice, 64 tokens in registers. First the largest
 // product of every 16 tokens, which decides whether the row's references are
@@ -41,7 +43,8 @@ namespace se12 {
 constexpr int kTileAttendRows = 128;  // query rows of a tile
 constexpr int kTileSoftmaxWarps = 4;
 constexpr int kTileLoaderWarps = 4;   // for keys, and as many for values
-constexpr int kTileAttendThreads = (kTileSoftmaxWarps + 2 * kTileLoaderWarps + 4) * 32;
+constexpr int kTileQueryWarps = 3;
+constexpr int kTileAttendThreads = (kTileSoftmaxWarps + 2 * kTileLoaderWarps + 1 + kTileQueryWarps) * 32;
 // Registers per thread by role (setmaxnreg), out of the launch's 128 for each
 // of the four warp groups.
 constexpr int kTileSoftmaxRegs = 208, kTileLoaderRegs = 104, kTileIssuerRegs = 80;
@@ -270,14 +273,19 @@ __device__ __forceinline__ void tile_next_pair(const AttendArgs& a, const int* b
 struct TileSmem {
   float meta[kTileMeta][8][2];        // [16 tokens of the tile][scale of keys, log2 of values' scale]
   int meta_missing[kTileMeta];        // bit g: those tokens' page is not there
-  float row_scale[kTileAttendRows];
+  float row_scale[2][kTileAttendRows];  // of this pair and the next
   float out_scale[kTileAttendRows];
   float merged_ref[kTileAttendRows];
+  // Pairs shared with other CTAs (a run's first and last) that this CTA
+  // completes: where their parts are and where their rows go.
+  struct {
+    int cta_first, parts, first_slot, b, head, row0, rows;
+  } join[2];
+  int joins;
   uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
-  uint64_t q_full, o_free;
+  uint64_t q_full[2], q_free, o_free;
   uint64_t meta_full[kTileMeta];
   uint32_t tmem;
-  int last;
   int before[1];  // [seqs + 1] KV tiles of the sequences before, per KV head
 };
 
@@ -475,6 +483,20 @@ __device__ __forceinline__ void any_tile(RowSoftmax& r, const TileLogits& z, int
   }
 }
 
+// Eight BF16 values of an output row, from dimension d.
+__device__ __forceinline__ void store_8(uint16_t* out, int d, int dim, int vec, const uint32_t (&w)[4]) {
+  if (d >= dim) return;
+  if (vec) {
+    *reinterpret_cast<uint4*>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      out[d + 2 * e] = static_cast<uint16_t>(w[e]);
+      out[d + 2 * e + 1] = static_cast<uint16_t>(w[e] >> 16);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ kernel
 
 template <int KIND, int DP>
@@ -498,7 +520,10 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       mbar_init(&sm.pv_done[i], 1);
     }
     for (int i = 0; i < kTileMeta; ++i) mbar_init(&sm.meta_full[i], 1);
-    mbar_init(&sm.q_full, kTileSoftmaxWarps);
+    mbar_init(&sm.q_free, 1);
+    mbar_init(&sm.q_full[0], kTileQueryWarps);
+    mbar_init(&sm.q_full[1], kTileQueryWarps);
+    sm.joins = 0;
     mbar_init(&sm.o_free, kTileSoftmaxWarps);
     fence_barrier_init();
   }
@@ -563,7 +588,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
         wait(bar, parity);
         dead = __any_sync(0xFFFFFFFFu, dead);
       };
-      auto scores = [&](uint32_t j) {  // S of tile j (of the ring)
+      auto scores = [&](uint32_t j, bool last) {  // S of tile j (of the ring)
         wait_warp(&sm.k_full[j & 1], (j >> 1) & 1);
         if (dead) return;
         tc_fence_after();
@@ -573,15 +598,16 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
           tc_mma_ss(s_at, q_low + (((k >> 2) * Shape::kQueryPanel + (k & 3) * 32) >> 4),
                     k_at + (((k >> 2) * Shape::kPanelBytes + (k & 3) * 32) >> 4), tc_idesc(TT, false), k > 0, elected);
         tc_commit(&sm.s_full[j & 1], elected);
+        if (last) tc_commit(&sm.q_free, elected);
       };
       uint32_t done = 0, pair = 0;  // KV tiles and pairs before: the rings' phases
       for (int g = g0; g < g1; ++pair) {
         const uint32_t run = __reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(min(at.s.chunks - at.chunk, g1 - g)));
-        wait_warp(&sm.q_full, pair & 1);
-        scores(done);
+        wait_warp(&sm.q_full[pair & 1], (pair >> 1) & 1);
+        scores(done, run == 1);
         for (uint32_t i = 0; i < run && !dead; ++i) {
           const uint32_t j = done + i;
-          if (i + 1 < run) scores(j + 1);
+          if (i + 1 < run) scores(j + 1, i + 2 == run);
           wait_warp(&sm.v_full[j & 1], (j >> 1) & 1);
           wait_warp(&sm.p_full[j & 1], (j >> 1) & 1);
           if (i == 0 && pair > 0) wait_warp(&sm.o_free, (pair - 1) & 1);
@@ -600,6 +626,78 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       }
     }
     __syncwarp();
+    if (warp > kIssuer) {
+      // ---- queries as FP16 times 2^-e (and the scale's sign), eight threads per row
+      constexpr int kVectors = DP / 64, kRowsAtOnce = kTileQueryWarps * 4;
+      const int tid = threadIdx.x - (kIssuer + 1) * 32, part = tid & 7;
+      tile_start<TT>(a, sm.before, g0, &at);
+      int pair = 0;
+      for (int g = g0; g < g1; ++pair) {
+        const int run = min(at.s.chunks - at.chunk, g1 - g);
+        // the pair before has been multiplied
+        if (pair > 0) wait(&sm.q_free, (pair - 1) & 1);
+        const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
+        const int rows_left = at.w.rows - at.tile * kTileAttendRows;
+        auto load_row = [&](uint4 (&r)[kVectors], int q_row) {
+          const int all = at.tile * kTileAttendRows + q_row;
+          const bool live = q_row < rows_left && q_row < kTileAttendRows;
+          const int i = live ? all / a.group : 0;
+          const uint16_t* src = a.q + (token0 + i) * a.q_ts + (at.head * a.group + (live ? all - i * a.group : 0)) * a.q_hs;
+#pragma unroll
+          for (int j = 0; j < kVectors; ++j) {
+            const int d = (j * 8 + part) * 8;
+            const bool use = live && d < a.c.dim;
+            if (a.q_vec) {
+              r[j] = load_or_zero(reinterpret_cast<const uint8_t*>(src + d), use);
+            } else {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                w[k] = use ? src[d + 2 * k] | (static_cast<uint32_t>(src[d + 2 * k + 1]) << 16) : 0;
+              r[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        };
+        uint4 next[kVectors];
+        load_row(next, tid >> 3);
+#pragma unroll 1
+        for (int q_row = tid >> 3; q_row - (tid >> 3) < kTileAttendRows; q_row += kRowsAtOnce) {
+          uint4 raw[kVectors];
+#pragma unroll
+          for (int j = 0; j < kVectors; ++j) raw[j] = next[j];
+          load_row(next, q_row + kRowsAtOnce);
+          unsigned big = 0;
+#pragma unroll
+          for (int j = 0; j < kVectors; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t w = word_of(raw[j], k);
+              big = max(big, max((w << 16) & 0x7FFFFFFFu, w & 0x7FFF0000u));
+            }
+#pragma unroll
+          for (int d = 1; d < 8; d <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
+          int e = static_cast<int>(big >> 23) - 127;
+          e = big == 0 ? 0 : max(min(e, 120), -120);
+          const float down = copysignf(__uint_as_float(static_cast<unsigned>(127 - e) << 23), a.scale);
+          auto halves = [&](uint32_t w) {
+            return half2_bits(__floats2half2_rn(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down));
+          };
+          if (q_row < kTileAttendRows) {
+#pragma unroll
+            for (int j = 0; j < kVectors; ++j)
+              *reinterpret_cast<uint4*>(q_tile + j * Shape::kQueryPanel + q_row * 128 + ((part ^ (q_row & 7)) << 4)) =
+                  make_uint4(halves(raw[j].x), halves(raw[j].y), halves(raw[j].z), halves(raw[j].w));
+            if (part == 0)
+              sm.row_scale[pair & 1][q_row] = __uint_as_float(static_cast<unsigned>(127 + e) << 23) * fabsf(a.scale);
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_full[pair & 1]);
+        g += run;
+        if (g < g1) tile_next_pair<TT>(a, sm.before, &at);
+      }
+    }
   } else if (warp >= kTileSoftmaxWarps) {
     // ---- codes to FP16 tiles
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTileLoaderRegs));
@@ -727,68 +825,16 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     const bool capped_logits = a.softcap != 0.f;
     const float cap2 = a.softcap * kLog2e;
-    // A pair's queries as FP16 times 2^-e (and the scale's sign), eight threads per row.
-    auto load_queries = [&]() {
-      constexpr int kVectors = DP / 64;
-      const int part = threadIdx.x & 7;
-      const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
-      const int rows_left = at.w.rows - at.tile * kTileAttendRows;
-#pragma unroll 4
-      for (int q_row = threadIdx.x >> 3; q_row < kTileAttendRows; q_row += kSoftmaxThreads / 8) {
-        const int all = at.tile * kTileAttendRows + q_row;
-        const bool live = q_row < rows_left;
-        const int i = live ? all / a.group : 0;
-        const uint16_t* src = a.q + (token0 + i) * a.q_ts + (at.head * a.group + (live ? all - i * a.group : 0)) * a.q_hs;
-        uint4 raw[kVectors];
-        unsigned big = 0;
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j) {
-          const int c = j * 8 + part;  // 16-byte chunk of the row
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (live && c * 8 < a.c.dim) {
-            if (a.q_vec) {
-              v = __ldg(reinterpret_cast<const uint4*>(src + c * 8));
-            } else {
-              const uint16_t* s = src + c * 8;
-              v = make_uint4(s[0] | (static_cast<uint32_t>(s[1]) << 16), s[2] | (static_cast<uint32_t>(s[3]) << 16),
-                             s[4] | (static_cast<uint32_t>(s[5]) << 16), s[6] | (static_cast<uint32_t>(s[7]) << 16));
-            }
-          }
-          raw[j] = v;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t w = word_of(v, k);
-            big = max(big, max((w << 16) & 0x7FFFFFFFu, w & 0x7FFF0000u));
-          }
-        }
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
-        int e = static_cast<int>(big >> 23) - 127;
-        e = big == 0 ? 0 : max(min(e, 120), -120);
-        const float down = copysignf(__uint_as_float(static_cast<unsigned>(127 - e) << 23), a.scale);
-        auto halves = [&](uint32_t w) {
-          return half2_bits(__floats2half2_rn(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down));
-        };
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j)
-          *reinterpret_cast<uint4*>(q_tile + j * Shape::kQueryPanel + q_row * 128 + ((part ^ (q_row & 7)) << 4)) =
-              make_uint4(halves(raw[j].x), halves(raw[j].y), halves(raw[j].z), halves(raw[j].w));
-        if (part == 0) sm.row_scale[q_row] = __uint_as_float(static_cast<unsigned>(127 + e) << 23) * fabsf(a.scale);
-      }
-      fence_proxy_async_shared();
-      named_barrier(1, kSoftmaxThreads);
-      if (lane == 0) mbar_arrive(&sm.q_full);
-    };
     tile_start<TT>(a, sm.before, g0, &at);
-    load_queries();
-    int done = 0;  // KV tiles of the pairs before: the rings' phases
+    int done = 0, pair = 0;  // KV tiles of the pairs before: the rings' phases
     for (int g = g0; g < g1;) {
       const int run = min(at.s.chunks - at.chunk, g1 - g);
       const int rows = min(kTileAttendRows, at.w.rows - at.tile * kTileAttendRows);
       const int t_first = at.s.low + at.chunk * TT;
       const int pos_min = at.s.pos_min, pos_max = at.s.pos_max;
       const bool active = warp * 32 < rows;  // rows past the tile's are left out, warp by warp
-      const float row_scale = sm.row_scale[row] * (capped_logits ? 1.f / a.softcap : kLog2e);
+      wait(&sm.q_full[pair & 1], (pair >> 1) & 1);
+      const float row_scale = sm.row_scale[pair & 1][row] * (capped_logits ? 1.f / a.softcap : kLog2e);
       const int pos = at.w.first + min(at.tile * kTileAttendRows + row, at.w.rows - 1) / a.group;
       RowSoftmax r{kAttendStart, 0.f, kAttendStart};
 #pragma unroll 1
@@ -840,65 +886,42 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full[j & 1]);
       }
-      // ---- the pair's end: the next pair's queries first (this one's products
-      // with them are done), then the row's sums
+      // ---- the row's sums
       const int pair_start = g - at.chunk, pair_end = pair_start + at.s.chunks;
       const int cta_first = pair_start / per, cta_last = (pair_end - 1) / per;
       const bool whole = cta_first == cta_last;
       float* part_out = a.partials + (static_cast<size_t>(blockIdx.x) * 2 + (pair_start > g0 ? 1 : 0)) * kTileSlotFloats;
       const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
-      const int row0 = at.tile * kTileAttendRows, head = at.head;
-      const bool more = g + run < g1;
-      named_barrier(1, kSoftmaxThreads);  // every warp has read row_scale and seen the last scores
-      if (more) {
-        tile_next_pair<TT>(a, sm.before, &at);
-        load_queries();
-      }
+      const int row0 = at.tile * kTileAttendRows;
       wait(&sm.pv_done[(done + run - 1) & 1], ((done + run - 1) >> 1) & 1);
       tc_fence_after();
       if (active) {
         const float f = whole ? (r.l == 0.f ? 0.f : ex2(r.mp - r.m) / r.l) : 1.f;
-        if (!whole && row < rows) {
-          float* st = part_out + kTileAttendRows * 256 + row * 4;
-          st[0] = r.m;
-          st[1] = r.l;
-          st[2] = r.mp;
+        if (!whole) {  // statistics after the sums, all with the rows side by side
+          part_out[256 * kTileAttendRows + row] = r.m;
+          part_out[257 * kTileAttendRows + row] = r.l;
+          part_out[258 * kTileAttendRows + row] = r.mp;
         }
         const int all = row0 + row, i_tok = all / a.group;
-        uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (head * a.group + all - i_tok * a.group) * a.o_hs;
+        uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (at.head * a.group + all - i_tok * a.group) * a.o_hs;
 #pragma unroll 1
         for (int q = 0; q < DP / 32; ++q) {
           const int d0 = q * 32;
           uint32_t o[32];
           tmem_load_32(o, tmem + lanes + Shape::kColO + d0);
           tmem_wait_load();
-          if (row < rows && d0 < a.c.dim) {
-            if (whole) {
+          if (!whole) {
 #pragma unroll
-              for (int k = 0; k < 32; k += 8) {
-                uint32_t w[4];
+            for (int k = 0; k < 32; ++k) part_out[(d0 + k) * kTileAttendRows + row] = __uint_as_float(o[k]);
+          } else if (row < rows) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  w[e] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[k + 2 * e]) * f)) |
-                         (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[k + 2 * e + 1]) * f))) << 16);
-                if (d0 + k < a.c.dim) {
-                  if (a.o_vec) {
-                    *reinterpret_cast<uint4*>(out + d0 + k) = make_uint4(w[0], w[1], w[2], w[3]);
-                  } else {
+            for (int k = 0; k < 32; k += 8) {
+              uint32_t w[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                      out[d0 + k + 2 * e] = static_cast<uint16_t>(w[e]);
-                      out[d0 + k + 2 * e + 1] = static_cast<uint16_t>(w[e] >> 16);
-                    }
-                  }
-                }
-              }
-            } else {
-              float4* dst = reinterpret_cast<float4*>(part_out + row * 256 + d0);
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                dst[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
-                                     __uint_as_float(o[4 * k + 3]));
+              for (int e = 0; e < 4; ++e)
+                w[e] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[k + 2 * e]) * f)) |
+                       (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[k + 2 * e + 1]) * f))) << 16);
+              store_8(out, d0 + k, a.c.dim, a.o_vec, w);
             }
           }
         }
@@ -907,81 +930,77 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.o_free);
       if (!whole) {
-        // ---- join the CTAs of the tile: the last to arrive adds all in order
+        // the last of the tile's CTAs to arrive joins them, once its run is done
         __threadfence();
         named_barrier(1, kSoftmaxThreads);
-        if (threadIdx.x == 0) {
-          const int arrived = atomic_add_acq_rel_gpu(a.counters + cta_first, 1);
-          sm.last = arrived == cta_last - cta_first;
-          if (sm.last) a.counters[cta_first] = 0;
-        }
-        named_barrier(1, kSoftmaxThreads);
-        if (sm.last) {
-          __threadfence();
-          const int parts = cta_last - cta_first + 1;
-          const float* rest = a.partials + static_cast<size_t>(cta_first) * 2 * kTileSlotFloats;
-          const float* first = rest + (pair_start > cta_first * per ? kTileSlotFloats : 0);
-          auto part_of = [&](int i) { return i == 0 ? first : rest + static_cast<size_t>(i) * 2 * kTileSlotFloats; };
-          if (threadIdx.x < rows) {
-            float mm = kAttendStart, mmp = kAttendStart;
-            for (int i = 0; i < parts; ++i) {
-              const float* st = part_of(i) + kTileAttendRows * 256 + threadIdx.x * 4;
-              mm = fmaxf(mm, __ldcg(st));
-              mmp = fmaxf(mmp, __ldcg(st + 2));
-            }
-            float sum = 0.f;
-            for (int i = 0; i < parts; ++i) {
-              const float* st = part_of(i) + kTileAttendRows * 256 + threadIdx.x * 4;
-              sum += __ldcg(st + 1) * ex2(__ldcg(st) - mm);
-            }
-            sm.merged_ref[threadIdx.x] = mmp;
-            sm.out_scale[threadIdx.x] = sum == 0.f ? 0.f : ex2(mmp - mm) / sum;
-          }
-          named_barrier(1, kSoftmaxThreads);
-          // eight vectors per thread at a time: their loads overlap
-          const int vectors = a.c.dim / 4, all_vectors = rows * vectors;
-          constexpr int kBatch = 8;
-#pragma unroll 1
-          for (int i0 = threadIdx.x; i0 < all_vectors; i0 += kBatch * kSoftmaxThreads) {
-            float4 v[kBatch];
-#pragma unroll
-            for (int e = 0; e < kBatch; ++e) v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-            for (int n = 0; n < parts; ++n) {
-              const float* pt = part_of(n);
-#pragma unroll
-              for (int e = 0; e < kBatch; ++e) {
-                const int i = min(i0 + e * kSoftmaxThreads, all_vectors - 1), r = i / vectors;
-                const float4 u = __ldcg(reinterpret_cast<const float4*>(pt + r * 256 + (i - r * vectors) * 4));
-                const float w = ex2(__ldcg(pt + kTileAttendRows * 256 + r * 4 + 2) - sm.merged_ref[r]);
-                v[e].x += u.x * w, v[e].y += u.y * w, v[e].z += u.z * w, v[e].w += u.w * w;
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < kBatch; ++e) {
-              const int i = i0 + e * kSoftmaxThreads;
-              if (i >= all_vectors) break;
-              const int r = i / vectors, d = (i - r * vectors) * 4;
-              const float f = sm.out_scale[r];
-              const int all = row0 + r, i_tok = all / a.group;
-              uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (head * a.group + all - i_tok * a.group) * a.o_hs + d;
-              out[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e].x * f));
-              out[1] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e].y * f));
-              out[2] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e].z * f));
-              out[3] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e].w * f));
-            }
-          }
-          named_barrier(1, kSoftmaxThreads);  // sm.last and the references are free
+        if (threadIdx.x == 0 && atomic_add_acq_rel_gpu(a.counters + cta_first, 1) == cta_last - cta_first) {
+          a.counters[cta_first] = 0;
+          auto& join = sm.join[sm.joins++];
+          join.cta_first = cta_first;
+          join.parts = cta_last - cta_first + 1;
+          join.first_slot = pair_start > cta_first * per ? 1 : 0;
+          join.b = at.b;
+          join.head = at.head;
+          join.row0 = row0;
+          join.rows = rows;
         }
       }
       done += run;
       g += run;
+      ++pair;
+      if (g < g1) tile_next_pair<TT>(a, sm.before, &at);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == kIssuer) tmem_free(sm.tmem, 512);
+
+  // ---- join: a thread per row and quarter of the dimensions, parts in order
+  const int joins = sm.joins;
+  for (int n = 0; n < joins; ++n) {
+    __threadfence();
+    const auto join = sm.join[n];
+    const int row = threadIdx.x & (kTileAttendRows - 1);
+    const float* rest = a.partials + static_cast<size_t>(join.cta_first) * 2 * kTileSlotFloats + row;
+    auto part_of = [&](int i) { return rest + static_cast<size_t>(i == 0 ? join.first_slot : 2 * i) * kTileSlotFloats; };
+    float m = kAttendStart, mp = kAttendStart, sum = 0.f;
+    for (int i = 0; i < join.parts; ++i) {
+      m = fmaxf(m, __ldcg(part_of(i) + 256 * kTileAttendRows));
+      mp = fmaxf(mp, __ldcg(part_of(i) + 258 * kTileAttendRows));
+    }
+    for (int i = 0; i < join.parts; ++i)
+      sum += __ldcg(part_of(i) + 257 * kTileAttendRows) * ex2(__ldcg(part_of(i) + 256 * kTileAttendRows) - m);
+    const float f = sum == 0.f ? 0.f : ex2(mp - m) / sum;
+    const int token0 = a.t.query_start ? a.t.query_start[join.b] : join.b;
+    const int all = join.row0 + row, i_tok = all / a.group;
+    uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (join.head * a.group + all - i_tok * a.group) * a.o_hs;
+    static_assert(kTileAttendThreads == 4 * kTileAttendRows, "a quarter of the dimensions per thread");
+#pragma unroll 1
+    for (int d0 = (threadIdx.x / kTileAttendRows) * (DP / 4); d0 < (threadIdx.x / kTileAttendRows + 1) * (DP / 4); d0 += 16) {
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < join.parts; ++i) {
+        const float* part = part_of(i);
+        const float w = ex2(__ldcg(part + 258 * kTileAttendRows) - mp);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = fmaf(__ldcg(part + (d0 + k) * kTileAttendRows), w, v[k]);
+      }
+      if (row < join.rows) {
+#pragma unroll
+        for (int k = 0; k < 16; k += 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = __bfloat16_as_ushort(__float2bfloat16_rn(v[k + 2 * e] * f)) |
+                   (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(v[k + 2 * e + 1] * f))) << 16);
+          store_8(out, d0 + k, a.c.dim, a.o_vec, w);
+        }
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------ launch
