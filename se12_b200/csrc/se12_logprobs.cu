@@ -10,12 +10,20 @@
 // above the list's k-th, pushed by whichever thread meets them. The list is
 // rebuilt (each warp sorts 32 candidates at a time and merges them into its
 // own 32, then the warps' lists are merged) only when the buffer fills up,
-// after the first batch and at the end; before the first batch is pushed,
-// the k-th largest of the threads' own maxima already bounds the list from
-// below. Work units of whole batches are cut into equal runs, one per CTA,
-// and a row's CTAs are joined by the last to finish, in CTA order. The bound
-// is HBM for plain logits, the special-function unit (three calls a value)
-// for capped ones.
+// after a row's first, fourth, sixteenth ... batch and at its end. Before the first batch is pushed,
+// the k-th largest of any one warp's lane maxima bounds the list from below;
+// the best of the warps' bounds leaves a few hundred candidates. A warp
+// takes places in the buffer for all its candidates at once (one by one, the
+// atomics on the counter were half of a row's time).
+//
+// Rows come in batches of 8 KB (4 KB when there are few) by bulk copies, four
+// batches ahead, whatever row they belong to: with three CTAs per SM 96 KB are
+// on the way. (Three CTAs of 256 threads, 80 registers: at two of 512 and 64
+// the spilled registers of the inner loop cost four times the loop.) The warps of a CTA meet only after a row's first batch and every
+// fourth one, to look at the buffer. The batches of all rows are cut into equal runs,
+// one per CTA, and a row's CTAs are joined by the last to finish, in CTA
+// order. The bound is HBM for plain logits, the special-function unit (three
+// calls a value) for capped ones.
 #include "se12_device.cuh"
 #include "se12_serve.h"
 
@@ -25,13 +33,13 @@
 
 namespace se12 {
 
-constexpr int kLogprobThreads = 512;
+constexpr int kLogprobThreads = 256;
+constexpr int kLogprobCtas = 3;  // per SM
 constexpr int kLogprobWarps = kLogprobThreads / 32;
-constexpr int kLogprobValues = 16;                               // per thread and batch
-constexpr int kLogprobBatch = kLogprobThreads * kLogprobValues;  // values of a batch
+constexpr int kLogprobStages = 4;
 constexpr int kLogprobTop = 32;
-constexpr int kLogprobSpare = 1024;                              // candidates kept before the list is rebuilt
-constexpr int kLogprobBuffer = kLogprobSpare + kLogprobBatch;
+constexpr int kLogprobSpare = 1024;   // candidates after which the list is rebuilt
+constexpr int kLogprobBuffer = 2048;  // what four batches may find; if more, they are gone through again
 // -inf and masks of the type's lowest value become this: its exponential is
 // zero and its product with log2(e) still finite.
 constexpr float kLogprobFloor = -2.0e38f;
@@ -62,8 +70,15 @@ __device__ __forceinline__ unsigned long long list_key(float x, int index) {
 
 __device__ __forceinline__ float key_value(unsigned long long key) {
   const unsigned u = static_cast<unsigned>(key >> 32);
-  if (u == 0xFFFFFFFFu) return __uint_as_float(0x7FC00000u);
+  if (u == 0xFFFFFFFFu || u == 0) return __uint_as_float(0x7FC00000u);
   return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u);
+}
+
+// The largest fp32 value below x; NaN below -inf.
+__device__ __forceinline__ float next_below(float x) {
+  const unsigned u = __float_as_uint(x);
+  if (x == 0.f) return __uint_as_float(0x80000001u);
+  return __uint_as_float((u & 0x80000000u) ? u + 1 : u - 1);
 }
 
 __device__ __forceinline__ int key_index(unsigned long long key) { return static_cast<int>(~static_cast<unsigned>(key)); }
@@ -101,12 +116,12 @@ __device__ __forceinline__ K merge_lanes(K a, K b, int lane) {
 struct LogprobSmem {
   unsigned long long buffer[kLogprobBuffer];
   unsigned long long lists[kLogprobWarps][32];
-  float maxima[kLogprobWarps][32];
-  float stat[kLogprobWarps][3];
   unsigned long long list[32];
-  float joined[3];
+  float stat[kLogprobWarps][3];
+  float bounds[kLogprobWarps];
   int count;
   int last;
+  uint64_t full[kLogprobStages], empty[kLogprobStages];
 };
 
 // The largest 32 of every warp's sorted list (`v` of this warp), in all
@@ -153,39 +168,48 @@ __device__ __forceinline__ float load_logit(const void* row, long long i) {
   return static_cast<const float*>(row)[i];
 }
 
-// This thread's kLogprobValues values of the batch at `base`: vector j of
-// thread t holds values base + (j * threads + t) * per vector ... Values at
-// or past `end` are -inf and never candidates.
+// The candidates of a row's batches [first, last), which were too many for the
+// buffer, from memory again: one value per thread at a time.
 template <bool BF16>
-__device__ __forceinline__ void load_batch(float (&x)[kLogprobValues], const void* row, long long base, long long end,
-                                           bool vec) {
-  constexpr int kPer = BF16 ? 8 : 4;
-#pragma unroll
-  for (int j = 0; j < kLogprobValues / kPer; ++j) {
-    const long long i = base + (j * kLogprobThreads + threadIdx.x) * kPer;
-    if (vec && i + kPer <= end) {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(static_cast<const char*>(row) + i * (BF16 ? 2 : 4)));
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (BF16) {
-          x[j * 8 + 2 * k] = __uint_as_float(w[k] << 16);
-          x[j * 8 + 2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
-        } else {
-          x[j * 4 + k] = __uint_as_float(w[k]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) x[j * kPer + k] = i + k < end ? load_logit<BF16>(row, i + k) : kNegInf;
+__device__ __noinline__ void refill_list(LogprobSmem& sm, const void* row, int first, int last, int batch, int vocab, int top,
+                                         int warp, int lane) {
+  __syncthreads();
+  if (threadIdx.x == 0) sm.count = 0;
+  __syncthreads();
+  const long long end = min(static_cast<long long>(last) * batch, static_cast<long long>(vocab));
+  for (long long base = static_cast<long long>(first) * batch; base < end; base += kLogprobThreads) {
+    const long long i = base + threadIdx.x;
+    if (i < end) {
+      const unsigned long long key = list_key(load_logit<BF16>(row, i), static_cast<int>(i));
+      if (key > sm.list[top - 1]) sm.buffer[atomicAdd(&sm.count, 1)] = key;
     }
+    __syncthreads();
+    // (a candidate per thread fits below the limit four times)
+    if (sm.count > kLogprobBuffer - kLogprobThreads) rebuild_list(sm, sm.count, warp, lane);
+    __syncthreads();
   }
+  if (sm.count) rebuild_list(sm, sm.count, warp, lane);
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Values of a 16-byte vector.
 template <bool BF16>
-__device__ __forceinline__ int batch_index(int value) {
-  constexpr int kPer = BF16 ? 8 : 4;
-  return ((value / kPer) * kLogprobThreads + static_cast<int>(threadIdx.x)) * kPer + value % kPer;
+__device__ __forceinline__ void unpack(float* x, const uint4& v) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t w = word_of(v, k);
+    if constexpr (BF16) {
+      x[2 * k] = __uint_as_float(w << 16);
+      x[2 * k + 1] = __uint_as_float(w & 0xFFFF0000u);
+    } else {
+      x[k] = __uint_as_float(w);
+    }
+  }
 }
 
 __device__ __forceinline__ void join_sums(float& max, float& sum, float& weighted, float m2, float s2, float w2) {
@@ -199,90 +223,227 @@ __device__ __forceinline__ void join_sums(float& max, float& sum, float& weighte
   max = m;
 }
 
-template <bool BF16, bool CAP>
-__global__ void __launch_bounds__(kLogprobThreads, 2) token_logprobs_kernel(const LogprobArgs a) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  LogprobSmem& sm = *reinterpret_cast<LogprobSmem*>(smem_raw);
+// VECS: 16-byte vectors a thread takes of a batch.
+template <bool BF16, bool CAP, int VECS>
+__global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_kernel(const LogprobArgs a) {
+  constexpr int kPer = BF16 ? 8 : 4;                 // values per vector
+  constexpr int kValues = kPer * VECS;               // per thread and batch
+  constexpr int kBatch = kLogprobThreads * kValues;
+  constexpr int kBatchBytes = kLogprobThreads * 16 * VECS;
+  constexpr int kSize = BF16 ? 2 : 4;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  LogprobSmem& sm = *reinterpret_cast<LogprobSmem*>(smem_raw + kLogprobStages * kBatchBytes);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kLogprobStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], kLogprobWarps);
+    }
+    fence_barrier_init();
+  }
   grid_launch_dependents();
   grid_dependency_wait();
+  __syncthreads();
 
-  const long long units = static_cast<long long>(a.rows) * a.chunks_per_row;
-  const long long u0 = blockIdx.x * a.units_per_cta, u1 = min(u0 + a.units_per_cta, units);
-  for (long long u = u0; u < u1;) {
-    const int row_id = static_cast<int>(u / a.chunks_per_row);
-    const long long row_u0 = static_cast<long long>(row_id) * a.chunks_per_row, row_u1 = row_u0 + a.chunks_per_row;
-    const long long stop = min(row_u1, u1);
-    const void* row = static_cast<const char*>(a.logits) + row_id * a.ld * (BF16 ? 2 : 4);
-    const long long begin = (u - row_u0) * a.chunk;
-    const long long end = min(static_cast<long long>(a.vocab), (stop - row_u0) * a.chunk);
+  const int units = a.rows * a.chunks_per_row;  // (the host sees to it that they fit)
+  const int u0 = blockIdx.x * a.units_per_cta, u1 = min(u0 + a.units_per_cta, units), batches = u1 - u0;
+  const uint64_t policy = policy_evict_first();
+  // batch n of this CTA's run on its way into its stage: whole vectors only
+  int copy_row = u0 / a.chunks_per_row, copy_chunk = u0 - copy_row * a.chunks_per_row;
+  bool dead = false;  // a wait ran out (status raised)
+  auto copy = [&](int n) {  // in order, by thread 0
+    if (n >= batches) return;
+    const int stage = n % kLogprobStages;
+    if (n >= kLogprobStages && !dead) dead = !mbar_wait(&sm.empty[stage], (n / kLogprobStages + 1) & 1);
+    const int base = copy_chunk * kBatch;
+    const int bytes = min(kBatch, a.vocab - base) * kSize / 16 * 16;
+    mbar_arrive_expect_tx(&sm.full[stage], bytes);
+    if (bytes)
+      bulk_load(smem_raw + stage * kBatchBytes, static_cast<const char*>(a.logits) + (copy_row * a.ld + base) * kSize, bytes,
+                &sm.full[stage], policy);
+    if (++copy_chunk == a.chunks_per_row) {
+      copy_chunk = 0;
+      ++copy_row;
+    }
+  };
+  if (a.vec && threadIdx.x == 0)
+    for (int n = 0; n < kLogprobStages; ++n) copy(n);
+  int batch = 0;  // of the run
+
+  for (int u = u0; u < u1;) {
+    const int row_id = u / a.chunks_per_row;
+    const int row_u0 = row_id * a.chunks_per_row, row_u1 = row_u0 + a.chunks_per_row;
+    const int stop = min(row_u1, u1);
+    const void* row = static_cast<const char*>(a.logits) + row_id * a.ld * kSize;
+    const int first = u - row_u0, chunks = stop - u;
+    // the given token's logit, on its way while the row streams
+    long long token = -1;
+    float token_logit = 0.f;
+    if (threadIdx.x == 0) {
+      token = a.tokens[row_id];
+      if (token >= 0 && token < a.vocab) token_logit = load_logit<BF16>(row, token);
+    }
 
     float max = kLogprobStart, sum = 0.f, weighted = 0.f;
-    float bound = kNegInf;  // candidates: values not below it (first batch) or above it
+    float bound = kNegInf;  // candidates: values above it, and NaN; a NaN bound takes all
+    bool full = false;
+    int seen = 0;  // batches of this row whose candidates are in the list
+    int next = 1;  // and after how many the list is rebuilt
     if (threadIdx.x < 32) sm.list[threadIdx.x] = 0ull;
     if (threadIdx.x == 0) sm.count = 0;
     __syncthreads();
-    bool strict = false;
-    for (long long base = begin; base < end; base += kLogprobBatch) {
-      float x[kLogprobValues];
-      load_batch<BF16>(x, row, base, end, a.vec);
-      float top = x[0];
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c, ++batch) {
+      const int base = (first + c) * kBatch;
+      const int left = a.vocab - base;  // values from here to the row's end
+      const int stage_id = batch % kLogprobStages;
+      const unsigned char* stage = smem_raw + stage_id * kBatchBytes;
+      const int whole = a.vec ? (left < kBatch ? left * kSize / 16 * kPer : kBatch) : 0;  // values the copy brings
+      // place of this thread's value j in the batch; the batch's value i
+      auto index_of = [](int j) { return (j / kPer * kLogprobThreads + static_cast<int>(threadIdx.x)) * kPer + j % kPer; };
+      auto value_of = [&](int i) {
+        return i < whole ? load_logit<BF16>(stage, i) : load_logit<BF16>(row, static_cast<long long>(base) + i);
+      };
+      float x[kValues];
+      if (a.vec) {
+        if (!dead) dead = !mbar_wait(&sm.full[stage_id], (batch / kLogprobStages) & 1);
 #pragma unroll
-      for (int j = 1; j < kLogprobValues; ++j) top = max_nan(top, x[j]);
-      if (a.top) {
-        if (!strict) {
-          // the k-th largest of the threads' maxima
-          float v = sort_lanes(top != top ? INFINITY : top, lane);
-          v = merge_warps(v, sm.maxima, warp, lane);
-          if (warp == 0 && lane == a.top - 1) sm.joined[0] = v;
-          __syncthreads();
-          bound = sm.joined[0];
+        for (int j = 0; j < VECS; ++j)
+          unpack<BF16>(x + j * kPer, *reinterpret_cast<const uint4*>(stage + (j * kLogprobThreads + threadIdx.x) * 16));
+      }
+      if (whole < kBatch) {
+        // past the copy: one by one; past the row: -inf, never a candidate
+#pragma unroll
+        for (int j = 0; j < kValues; ++j) {
+          const int i = index_of(j);
+          if (i >= left) x[j] = kNegInf;
+          else if (i >= whole) x[j] = value_of(i);
         }
-        bool full = false;
-        if (strict ? !(top <= bound) : !(top < bound)) {
+      }
+      float top = max_nan(x[0], x[1]);
 #pragma unroll
-          for (int j = 0; j < kLogprobValues; ++j) {
-            const long long i = base + batch_index<BF16>(j);
-            if ((strict ? !(x[j] <= bound) : !(x[j] < bound)) && i < end) {
-              const int at = atomicAdd(&sm.count, 1);
-              sm.buffer[at] = list_key(x[j], static_cast<int>(i));
-              full |= at >= kLogprobSpare;
-            }
+      for (int j = 2; j < kValues; j += 2) top = max3_nan(top, x[j], x[j + 1]);
+
+      if (a.top) {
+        if (c == 0) {
+          // the k-th largest of each warp's lane maxima bounds the k-th value
+          // from below (values equal to it count)
+          const float v = sort_lanes(top != top ? INFINITY : top, lane);
+          if (lane == a.top - 1) sm.bounds[warp] = v;
+          __syncthreads();
+          float b = sm.bounds[lane & (kLogprobWarps - 1)];
+#pragma unroll
+          for (int d = 1; d < kLogprobWarps; d <<= 1) b = fmaxf(b, __shfl_xor_sync(0xFFFFFFFFu, b, d));
+          bound = next_below(b);
+        }
+        if (__any_sync(0xFFFFFFFFu, !(top <= bound))) {
+          // which of the values, places for all of the warp's at once, then
+          // one by one (few: read again from where they came)
+          unsigned found = 0;
+#pragma unroll
+          for (int j = 0; j < kValues; ++j) found |= static_cast<unsigned>(!(x[j] <= bound)) << j;
+          if (whole < kBatch) {
+#pragma unroll
+            for (int j = 0; j < kValues; ++j)
+              if (index_of(j) >= left) found &= ~(1u << j);
+          }
+          int at = __popc(found);
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xFFFFFFFFu, at, d);
+            if (lane >= d) at += o;
+          }
+          const int all = __shfl_sync(0xFFFFFFFFu, at, 31);
+          int start = 0;
+          if (lane == 0) start = atomicAdd(&sm.count, all);
+          at += __shfl_sync(0xFFFFFFFFu, start, 0) - __popc(found);
+          full |= at + __popc(found) > kLogprobSpare;
+          for (; found; found &= found - 1, ++at) {
+            const int i = index_of(__ffs(found) - 1);
+            if (at < kLogprobBuffer) sm.buffer[at] = list_key(value_of(i), base + i);
           }
         }
-        // (the first batch may hold fewer than k values: -inf stays inclusive)
-        if (__syncthreads_or(full || !strict)) {
-          rebuild_list(sm, sm.count, warp, lane);
-          const unsigned long long kth = sm.list[a.top - 1];
-          strict = kth != 0ull;
-          bound = strict ? key_value(kth) : kNegInf;
-          if (bound != bound) bound = INFINITY;  // a list of NaN takes no more
-        }
       }
+      if (a.vec) {
+        __syncwarp();  // every lane has read its values
+        if (lane == 0) mbar_arrive(&sm.empty[stage_id]);
+        if (threadIdx.x == 0 && batch > 0) copy(batch - 1 + kLogprobStages);
+      }
+
       // sums relative to the running maximum, in units of log 2 (z log2(e)
       // - max is one rounding everywhere: the maximum's own cancels)
-      float high = kLogprobFloor;
+      float high = top;
+      if constexpr (CAP) {
+        float low = fminf(x[0], x[1]);
 #pragma unroll
-      for (int j = 0; j < kLogprobValues; ++j) {
-        x[j] = max_nan(CAP ? capped(x[j], a.softcap) : x[j], kLogprobFloor);
-        high = max_nan(high, x[j]);
+        for (int j = 2; j < kValues; ++j) low = fminf(low, x[j]);
+        const float range = 0.7f * a.softcap;
+        if (__all_sync(0xFFFFFFFFu, top <= range && low >= -range)) {
+          // cap tanh(u): u times a polynomial of u^2 of degree 5 (Chebyshev fit
+          // of tanh(u) / u on |u| <= 0.7, off by 8.5e-9), two at a time
+          const unsigned long long inverse = pair_of(1.f / a.softcap, 1.f / a.softcap);
+          const float c0 = a.softcap;
+#pragma unroll
+          for (int j = 0; j < kValues; j += 2) {
+            const unsigned long long u = mul_pair(pair_of(x[j], x[j + 1]), inverse), t = mul_pair(u, u);
+            unsigned long long y = fma_pair(pair_of(-0.00509482797f * c0, -0.00509482797f * c0), t, pair_of(0.0200324471f * c0, 0.0200324471f * c0));
+            y = fma_pair(y, t, pair_of(-0.0535294551f * c0, -0.0535294551f * c0));
+            y = fma_pair(y, t, pair_of(0.133284756f * c0, 0.133284756f * c0));
+            y = fma_pair(y, t, pair_of(-0.333331342f * c0, -0.333331342f * c0));
+            y = fma_pair(y, t, pair_of(0.999999987f * c0, 0.999999987f * c0));
+            unpair(mul_pair(y, u), x[j], x[j + 1]);
+          }
+          high = capped(top, a.softcap);
+        } else {
+          high = kNegInf;
+#pragma unroll
+          for (int j = 0; j < kValues; ++j) {
+            x[j] = capped(x[j], a.softcap);
+            high = max_nan(high, x[j]);
+          }
+        }
       }
-      high *= kLog2e;
+      high = max_nan(high, kLogprobFloor) * kLog2e;
       if (!(high <= max)) {
         const float d = max_nan(max - high, -1000.f), f = ex2(d);
         weighted = (weighted + sum * d) * f;
         sum *= f;
         max = high;
       }
-      float s = 0.f, w = 0.f;
+      unsigned long long s = 0, w = 0;  // pairs of zeros
+      const unsigned long long scale = pair_of(kLog2e, kLog2e), shift = pair_of(-max, -max);
 #pragma unroll
-      for (int j = 0; j < kLogprobValues; ++j) {
-        const float d = fmaf(x[j], kLog2e, -max), e = ex2(d);
-        s += e;
-        w = fmaf(e, d, w);
+      for (int j = 0; j < kValues; j += 2) {
+        const unsigned long long d =
+            fma_pair(pair_of(max_nan(x[j], kLogprobFloor), max_nan(x[j + 1], kLogprobFloor)), scale, shift);
+        float d0, d1;
+        unpair(d, d0, d1);
+        const unsigned long long e = pair_of(ex2(d0), ex2(d1));
+        s = add_pair(s, e);
+        w = fma_pair(e, d, w);
       }
-      sum += s;
-      weighted += w;
+      float lo, hi;
+      unpair(s, lo, hi);
+      sum += lo + hi;
+      unpair(w, lo, hi);
+      weighted += lo + hi;
+
+      // Look at the buffer every fourth batch; rebuild the list after the
+      // first, the fourth, the sixteenth ...: each time the candidates per
+      // batch get four times fewer.
+      if (a.top && c + 1 < chunks && (c + 1 == next || (c & 3) == 3) && __syncthreads_or(full || c + 1 == next)) {
+        const int count = sm.count;
+        if (count <= kLogprobBuffer) rebuild_list(sm, count, warp, lane);
+        else refill_list<BF16>(sm, row, first + seen, first + c + 1, kBatch, a.vocab, a.top, warp, lane);
+        seen = c + 1;
+        if (seen == next) next *= 4;
+        full = false;
+        // later values equal to the k-th have higher ids; a list that is not
+        // full takes everything, one of NaN nothing but what comes before NaN
+        const unsigned long long kth = sm.list[a.top - 1];
+        bound = key_value(kth);
+        if (bound != bound) bound = kth ? INFINITY : bound;
+      }
     }
 
     // ---- join the threads, then the CTAs of the row
@@ -299,7 +460,11 @@ __global__ void __launch_bounds__(kLogprobThreads, 2) token_logprobs_kernel(cons
     }
     if (a.top) {
       __syncthreads();
-      if (sm.count) rebuild_list(sm, sm.count, warp, lane);
+      const int count = sm.count;
+      if (count > kLogprobBuffer)
+        refill_list<BF16>(sm, row, first + seen, first + chunks, kBatch, a.vocab, a.top, warp, lane);
+      else if (count)
+        rebuild_list(sm, count, warp, lane);
     }
     __syncthreads();
     if (warp == 0) {
@@ -313,7 +478,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 2) token_logprobs_kernel(cons
         join_sums(max, sum, weighted, m2, s2, w2);
       }
     }
-    const long long cta_first = row_u0 / a.units_per_cta, cta_last = (row_u1 - 1) / a.units_per_cta;
+    const int cta_first = row_u0 / a.units_per_cta, cta_last = (row_u1 - 1) / a.units_per_cta;
     unsigned long long mine = warp == 0 ? sm.list[lane] : 0ull;
     bool finish = true;
     if (cta_first != cta_last) {
@@ -334,15 +499,28 @@ __global__ void __launch_bounds__(kLogprobThreads, 2) token_logprobs_kernel(cons
       finish = sm.last;
       if (finish) {
         __threadfence();
-        // a warp takes every 16th part, then the warps' results are merged
-        const LogprobPart* first = parts + cta_first * 2 + (row_u0 > cta_first * a.units_per_cta ? 1 : 0);
-        const int count = static_cast<int>(cta_last - cta_first) + 1;
+        // a warp takes every eighth part, then the warps' results are merged
+        const LogprobPart* first_part = parts + cta_first * 2 + (row_u0 > cta_first * a.units_per_cta ? 1 : 0);
+        const int count = cta_last - cta_first + 1;
         unsigned long long v = 0ull;
         float pm = kLogprobStart, ps = 0.f, pw = 0.f;
-        for (int i = warp; i < count; i += kLogprobWarps) {
-          const LogprobPart* p = i == 0 ? first : parts + (cta_first + i) * 2;
-          join_sums(pm, ps, pw, __ldcg(&p->max), __ldcg(&p->sum), __ldcg(&p->weighted));
-          if (a.top) v = merge_lanes(v, __ldcg(&p->list[lane]), lane);
+        constexpr int kAhead = 4;  // parts whose lists are on the way together
+        for (int i0 = warp; i0 < count; i0 += kAhead * kLogprobWarps) {
+          unsigned long long list[kAhead];
+          float3 stat[kAhead];
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kLogprobWarps;
+            const LogprobPart* p = i == 0 ? first_part : parts + (cta_first + min(i, count - 1)) * 2;
+            list[k] = a.top && i < count ? __ldcg(&p->list[lane]) : 0ull;
+            stat[k] = i < count ? make_float3(__ldcg(&p->max), __ldcg(&p->sum), __ldcg(&p->weighted))
+                                : make_float3(kLogprobStart, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            join_sums(pm, ps, pw, stat[k].x, stat[k].y, stat[k].z);
+            if (a.top && i0 + k * kLogprobWarps < count) v = merge_lanes(v, list[k], lane);
+          }
         }
         if (lane == 0) {
           sm.stat[warp][0] = pm;
@@ -398,10 +576,9 @@ __global__ void __launch_bounds__(kLogprobThreads, 2) token_logprobs_kernel(cons
         return fmaf(z, kLog2e, -max) * kLn2 - log_sum;
       };
       if (lane == 0) {
-        const long long t = a.tokens[row_id];
         float lp = __uint_as_float(0x7FC00000u);
-        if (t >= a.vocab) raise_status(kStatusBadArgument);
-        else if (t >= 0) lp = log_prob(load_logit<BF16>(row, t));
+        if (token >= a.vocab) raise_status(kStatusBadArgument);
+        else if (token >= 0) lp = log_prob(token_logit);
         a.logprob[row_id] = lp;
         a.entropy[row_id] = log_sum - (weighted / sum) * kLn2;
       }
@@ -417,24 +594,32 @@ __global__ void __launch_bounds__(kLogprobThreads, 2) token_logprobs_kernel(cons
 
 // ------------------------------------------------------------------ launch
 
-// Two CTAs per SM at most (their candidate buffers fill the shared memory).
-size_t logprob_partial_bytes(int sm_count) { return static_cast<size_t>(sm_count) * 2 * 2 * sizeof(LogprobPart); }
+size_t logprob_partial_bytes(int sm_count) { return static_cast<size_t>(sm_count) * kLogprobCtas * 2 * sizeof(LogprobPart); }
 
-cudaError_t launch_token_logprobs(bool bf16, LogprobArgs a, int sm_count, cudaStream_t stream) {
-  // units of one batch, or of less when the rows alone do not fill the GPU
-  a.chunk = kLogprobBatch;
-  a.chunks_per_row = (a.vocab + a.chunk - 1) / a.chunk;
+template <bool BF16, int VECS>
+cudaError_t launch_logprobs_as(LogprobArgs a, int sm_count, cudaStream_t stream) {
+  const int batch = kLogprobThreads * VECS * (BF16 ? 8 : 4);
+  a.chunks_per_row = (a.vocab + batch - 1) / batch;
   const long long units = static_cast<long long>(a.rows) * a.chunks_per_row;
-  const long long ctas = std::min<long long>(units, 2ll * sm_count);
-  a.units_per_cta = (units + ctas - 1) / ctas;
+  if (units > INT32_MAX - kLogprobCtas * sm_count) return cudaErrorInvalidValue;  // 2^31 batches: more than a GPU's memory of rows
+  // at most 64 CTAs to a row: joining more takes longer than they save (one
+  // row of 256000 fp32 logits: 19.4 us with 250 CTAs, 15.1 with 63)
+  const long long ctas =
+      std::min({units, static_cast<long long>(kLogprobCtas) * sm_count, static_cast<long long>(a.rows) * 64});
+  a.units_per_cta = static_cast<int>((units + ctas - 1) / ctas);
   const unsigned grid = static_cast<unsigned>((units + a.units_per_cta - 1) / a.units_per_cta);
-  const size_t smem = sizeof(LogprobSmem);
-  const bool cap = a.softcap != 0.f;
-  if (bf16)
-    return launch_overlapped(cap ? token_logprobs_kernel<true, true> : token_logprobs_kernel<true, false>, dim3(grid),
-                             kLogprobThreads, smem, stream, a);
-  return launch_overlapped(cap ? token_logprobs_kernel<false, true> : token_logprobs_kernel<false, false>, dim3(grid),
-                           kLogprobThreads, smem, stream, a);
+  const size_t smem = kLogprobStages * kLogprobThreads * 16 * VECS + sizeof(LogprobSmem);
+  return launch_overlapped(a.softcap != 0.f ? token_logprobs_kernel<BF16, true, VECS> : token_logprobs_kernel<BF16, false, VECS>,
+                           dim3(grid), kLogprobThreads, smem, stream, a);
+}
+
+// Two vectors per thread where that leaves every CTA several batches: half
+// the barriers per value; one where the rows are few: more CTAs to each row.
+cudaError_t launch_token_logprobs(bool bf16, LogprobArgs a, int sm_count, cudaStream_t stream) {
+  const long long bytes = static_cast<long long>(a.rows) * a.vocab * (bf16 ? 2 : 4);
+  const bool two = bytes >= 12ll * sm_count * kLogprobThreads * 32;
+  if (bf16) return two ? launch_logprobs_as<true, 2>(a, sm_count, stream) : launch_logprobs_as<true, 1>(a, sm_count, stream);
+  return two ? launch_logprobs_as<false, 2>(a, sm_count, stream) : launch_logprobs_as<false, 1>(a, sm_count, stream);
 }
 
 }  // namespace se12

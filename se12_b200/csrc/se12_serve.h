@@ -81,9 +81,8 @@ struct LogprobArgs {
   long long* top_ids;
   float* top_logprobs;
   int vec;             // every row is 16-byte aligned
-  int chunk;           // elements a work unit covers
-  int chunks_per_row;
-  long long units_per_cta;
+  int chunks_per_row;  // batches of a row
+  int units_per_cta;
   unsigned char* partials;
   int* counters;
 };
