@@ -133,6 +133,24 @@ __device__ __forceinline__ void for_row(const T* row, const PairMap& map, const 
   }
 }
 
+// A row in registers, for vector lanes (one step covers the row): what
+// lane `lane` has of its first and second halves.
+template <int VP>
+struct RowPart {
+  float a[VP], b[VP];
+
+  template <typename T>
+  __device__ __forceinline__ void load(const T* row, int lane) {
+    load_vector<VP>(a, row + lane * VP);
+    load_vector<VP>(b, row + 32 * VP + lane * VP);
+  }
+
+  __device__ __forceinline__ void rotate(const float (&c)[VP], const float (&s)[VP]) {
+#pragma unroll
+    for (int j = 0; j < VP; ++j) turn(a[j], b[j], c[j], s[j]);
+  }
+};
+
 template <int VP>
 __device__ __forceinline__ unsigned magnitude_bits(const float (&x)[VP], unsigned m) {
 #pragma unroll
@@ -315,43 +333,158 @@ __device__ __forceinline__ int sequence_of(const TokenBatch& t, int token, int l
   return n;
 }
 
+// A block's new tokens (rows first .. first + count - 1 of src, slots slot ..)
+// joined to it by one CTA of 8 warps.
+template <typename T, int KIND, int VP>
+__device__ __forceinline__ void append_block(const AppendArgs& a, bool keys, const T* src, long long ts, int pos, int slot,
+                                             int count, uint8_t* codes, float* scale, unsigned* s_amax) {
+  constexpr int kHeld = 4;  // rows a warp keeps in registers from one pass to the next
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.c.dim;
+  const PairMap map = pair_map(a, keys, VP);
+  const bool turned = keys && a.cos;
+  const bool held = VP > 1 && count <= 8 * kHeld;
+  RowPart<VP> row[kHeld];
+  unsigned amax = 0;
+  auto row_of = [&](RowPart<VP>& r, int i) {
+    r.load(src + i * ts, lane);
+    if (turned) {
+      float c[VP], s[VP];
+      load_vector<VP>(c, a.cos + (pos + i) * a.rope_stride + lane * VP);
+      load_vector<VP>(s, a.sin + (pos + i) * a.rope_stride + lane * VP);
+      r.rotate(c, s);
+    }
+  };
+  if constexpr (VP > 1) {
+    for (int i0 = warp; i0 < count; i0 += 8 * kHeld) {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k)
+        if (i0 + 8 * k < count) row_of(row[k], i0 + 8 * k);
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k)
+        if (i0 + 8 * k < count) amax = magnitude_bits<VP>(row[k].b, magnitude_bits<VP>(row[k].a, amax));
+    }
+  } else {
+    for (int i = warp; i < count; i += 8)
+      for_row<VP>(src + i * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
+                  [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
+                    amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
+                  });
+  }
+  amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+  if (lane == 0) s_amax[warp] = amax;
+  __syncthreads();
+  amax = s_amax[lane & 7];
+  amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+  float ratio;
+  const float now = joined_scale<KIND>(scale, slot > 0, amax, ratio);
+  __syncthreads();  // every thread has read the old scale and the maxima
+  const bool finite = now == now;
+  if (ratio != 1.f) shrink_codes<KIND>(codes, slot * dim, ratio, threadIdx.x, 256);
+  const float inv = finite ? __frcp_rn(now) : 0.f;  // exact for the powers of two stored here
+  auto put = [&](uint8_t* to, const float(&x)[VP]) {
+    if (finite) {
+      store_codes<KIND, VP>(to, x, inv);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VP; ++j) to[j] = 0;
+    }
+  };
+  uint8_t* to = codes + slot * dim;
+  if constexpr (VP > 1) {
+    for (int i0 = warp; i0 < count; i0 += 8 * kHeld) {
+      if (!held) {
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+          if (i0 + 8 * k < count) row_of(row[k], i0 + 8 * k);
+      }
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k)
+        if (i0 + 8 * k < count) {
+          put(to + (i0 + 8 * k) * dim + lane * VP, row[k].a);
+          put(to + (i0 + 8 * k) * dim + 32 * VP + lane * VP, row[k].b);
+        }
+    }
+  } else {
+    for (int i = warp; i < count; i += 8)
+      for_row<VP>(src + i * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
+                  [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
+                    put(to + i * dim + ia, x);
+                    put(to + i * dim + ib, y);
+                  });
+  }
+  if (threadIdx.x == 0) *scale = now;
+}
+
+// One token's queries, a warp: the angle's cosines and sines are loaded once
+// for all heads.
+template <typename T, int VP>
+__device__ __forceinline__ void rotate_queries(const AppendArgs& a, int token, int pos, int lane) {
+  if (VP == 1 || pos < 0 || (a.cos && pos >= a.rope_rows)) {
+    for (int h = 0; h < a.q_heads; ++h) rotate_query<T, VP>(a, token, h, pos, lane);
+    return;
+  }
+  float c[VP], s[VP];
+  if (a.cos) {
+    load_vector<VP>(c, a.cos + pos * a.rope_stride + lane * VP);
+    load_vector<VP>(s, a.sin + pos * a.rope_stride + lane * VP);
+  }
+  const T* src = static_cast<const T*>(a.q) + token * a.q_ts;
+  uint16_t* out = a.q_out + token * a.o_ts;
+  constexpr int kHeads = 4;  // on their way together
+  for (int h0 = 0; h0 < a.q_heads; h0 += kHeads) {
+    RowPart<VP> row[kHeads];
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k)
+      if (h0 + k < a.q_heads) row[k].load(src + (h0 + k) * a.q_hs, lane);
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k)
+      if (h0 + k < a.q_heads) {
+        if (a.cos) row[k].rotate(c, s);
+        store_bf16<VP>(out + (h0 + k) * a.o_hs + lane * VP, row[k].a);
+        store_bf16<VP>(out + (h0 + k) * a.o_hs + 32 * VP + lane * VP, row[k].b);
+      }
+  }
+}
+
 // Any number of tokens per sequence. CTAs with blockIdx.y < 2 * heads: each
 // looks through `span` consecutive tokens for the first new token of a block
-// (of its sequence, or of a page) and stores that block's new tokens, a warp
-// per token: one pass for the largest magnitude, one for the codes. The
-// other CTAs rotate queries, a warp per row.
+// (of its sequence, or of a page) and stores that block's new tokens, four
+// rows per warp on their way at a time; up to 32 stay in registers while the
+// scale is found, more are read again from L2. The last blockIdx.y rotates the
+// queries, a warp per token. (One row per warp at a time, and the queries of a
+// token by a warp per head, 14900 tokens of 16 + 2 x 8 heads of 256 took twice
+// the time.)
 template <typename T, int KIND, int VP>
-__global__ void __launch_bounds__(256) kv_append_prompt_kernel(const AppendArgs a, const int span) {
+__global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendArgs a, const int span) {
   __shared__ unsigned s_amax[8];
   grid_launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int first = blockIdx.x * span, end = min(first + span, a.t.tokens);
-  int b = sequence_of(a.t, first, lane);
   const int what = blockIdx.y;
-  if (what >= 2 * a.c.heads) {
-    // span tokens x 8 heads per CTA
-    const int head = (what - 2 * a.c.heads) * 8 + warp;
-    if (head >= a.q_heads) return;
-    for (int t = first; t < end; ++t) {
-      while (b + 1 < a.t.seqs && a.t.query_start[b + 1] <= t) ++b;
+  const int first = blockIdx.x * span, end = min(first + span, a.t.tokens);
+  if (what == 2 * a.c.heads) {
+    for (int t = first + warp; t < end; t += 8) {
+      const int b = sequence_of(a.t, t, lane);
       const bool owned = t >= a.t.query_start[b] && t < a.t.query_start[b + 1];
-      rotate_query<T, VP>(a, t, head, owned ? a.t.lens[b] - (a.t.query_start[b + 1] - t) : -1, lane);
+      rotate_queries<T, VP>(a, t, owned ? a.t.lens[b] - (a.t.query_start[b + 1] - t) : -1, lane);
     }
     return;
   }
+  int b = sequence_of(a.t, first, lane);
   const bool keys = what < a.c.heads;
   const int head = keys ? what : what - a.c.heads;
   const T* src = static_cast<const T*>(keys ? a.k : a.v) + head * (keys ? a.k_hs : a.v_hs);
   const long long ts = keys ? a.k_ts : a.v_ts;
-  const PairMap map = pair_map(a, keys, VP);
   for (int t = first; t < end; ++t) {
     while (b + 1 < a.t.seqs && a.t.query_start[b + 1] <= t) ++b;
     const int start = a.t.query_start[b], stop = min(a.t.query_start[b + 1], a.t.tokens);
     const int pos = a.t.lens[b] - (a.t.query_start[b + 1] - t);
     if (t < start || t >= stop || pos < 0) continue;  // not a sequence's token, or an inactive one
     const int slot = pos & (a.c.page_size - 1);
-    if (t != start && slot != 0) continue;
+    if (t != start && slot != 0) {  // a token inside a block: on to the next block
+      t += min(min(a.c.page_size - slot, stop - t), end - t) - 1;
+      continue;
+    }
     const int page = page_of(a.t, a.c, b, pos);
     if (page < 0) continue;
     const int count = min(a.c.page_size - slot, stop - t);
@@ -360,61 +493,40 @@ __global__ void __launch_bounds__(256) kv_append_prompt_kernel(const AppendArgs 
       continue;
     }
     const long long block = static_cast<long long>(page) * a.c.heads + head;
-    uint8_t* codes = (keys ? a.c.k_codes : a.c.v_codes) + block * a.c.page_size * a.c.dim;
-    float* scale = (keys ? a.c.k_scales : a.c.v_scales) + block;
-    unsigned amax = 0;
-    for (int i = warp; i < count; i += 8)
-      for_row<VP>(src + (t + i) * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
-                  [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
-                    amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
-                  });
-    amax = __reduce_max_sync(0xFFFFFFFFu, amax);
-    if (lane == 0) s_amax[warp] = amax;
-    __syncthreads();
-    amax = s_amax[lane & 7];
-    amax = __reduce_max_sync(0xFFFFFFFFu, amax);
-    float ratio;
-    const float now = joined_scale<KIND>(scale, slot > 0, amax, ratio);
-    __syncthreads();  // every thread has read the old scale and the maxima
-    const bool finite = now == now;
-    if (ratio != 1.f) shrink_codes<KIND>(codes, slot * a.c.dim, ratio, threadIdx.x, 256);
-    const float inv = finite ? __frcp_rn(now) : 0.f;  // exact for the powers of two stored here
-    for (int i = warp; i < count; i += 8) {
-      uint8_t* to = codes + (slot + i) * a.c.dim;
-      for_row<VP>(src + (t + i) * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
-                  [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
-                    if (finite) {
-                      store_codes<KIND, VP>(to + ia, x, inv);
-                      store_codes<KIND, VP>(to + ib, y, inv);
-                    } else {
-#pragma unroll
-                      for (int j = 0; j < VP; ++j) to[ia + j] = to[ib + j] = 0;
-                    }
-                  });
-    }
-    if (threadIdx.x == 0) *scale = now;
+    append_block<T, KIND, VP>(a, keys, src + t * ts, ts, pos, slot, count,
+                              (keys ? a.c.k_codes : a.c.v_codes) + block * a.c.page_size * a.c.dim,
+                              (keys ? a.c.k_scales : a.c.v_scales) + block, s_amax);
   }
 }
 
-// Pages read back as BF16 (exact: a code has at most 8 significant bits).
+// Pages read back as BF16 (exact: a code has at most 8 significant bits), a
+// CTA per block (page of a head), keys and values by blockIdx.y.
 template <int KIND>
 __global__ void __launch_bounds__(256) kv_decode_kernel(const KvView c, const int32_t* pages, int count, uint16_t* k_out,
                                                         uint16_t* v_out) {
   grid_launch_dependents();
   grid_dependency_wait();
   const int block_codes = c.page_size * c.dim;  // a multiple of 256
-  const long long per_page = static_cast<long long>(c.heads) * block_codes;
-  const long long total = count * per_page;
   const uint8_t* codes = blockIdx.y ? c.v_codes : c.k_codes;
   const float* scales = blockIdx.y ? c.v_scales : c.k_scales;
-  uint16_t* out = blockIdx.y ? v_out : k_out;
-  for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 8; i < total; i += gridDim.x * 2048ll) {
-    const long long n = i / per_page, rest = i - n * per_page;
-    const int page = pages ? pages[n] : static_cast<int>(n);
-    uint32_t w[4] = {};
-    if (page >= 0 && page < c.pages) {
-      const uint2 v = *reinterpret_cast<const uint2*>(codes + page * per_page + rest);
-      const float s = scales[static_cast<long long>(page) * c.heads + rest / block_codes];
+  uint16_t* outs = blockIdx.y ? v_out : k_out;
+  const long long blocks = static_cast<long long>(count) * c.heads;
+  for (long long n = blockIdx.x; n < blocks; n += gridDim.x) {
+    const int nth = static_cast<int>(n / c.heads), head = static_cast<int>(n - static_cast<long long>(nth) * c.heads);
+    const int page = pages ? pages[nth] : nth;
+    uint16_t* out = outs + n * block_codes;
+    if (page < 0 || page >= c.pages) {
+      raise_status(kStatusBadArgument);
+      for (int i = threadIdx.x * 8; i < block_codes; i += 2048) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const long long block = static_cast<long long>(page) * c.heads + head;
+    const uint8_t* in = codes + block * block_codes;
+    const float s = scales[block];
+#pragma unroll 4
+    for (int i = threadIdx.x * 8; i < block_codes; i += 2048) {
+      const uint2 v = *reinterpret_cast<const uint2*>(in + i);
+      uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t pair = (j < 2 ? v.x : v.y) >> (16 * (j & 1));
@@ -422,10 +534,8 @@ __global__ void __launch_bounds__(256) kv_decode_kernel(const KvView c, const in
         w[j] = __bfloat16_as_ushort(__float2bfloat16_rn(lo)) |
                (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(hi))) << 16);
       }
-    } else {
-      raise_status(kStatusBadArgument);
+      *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -440,7 +550,7 @@ cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t stream) {
   }
   // few tokens: one per CTA, so that short sequences' blocks run side by side
   const int span = a.t.tokens <= 256 ? 1 : 16;
-  const dim3 grid((a.t.tokens + span - 1) / span, 2 * a.c.heads + (a.q ? (a.q_heads + 7) / 8 : 0));
+  const dim3 grid((a.t.tokens + span - 1) / span, 2 * a.c.heads + (a.q ? 1 : 0));
   return launch_overlapped(kv_append_prompt_kernel<T, KIND, VP>, grid, 256, 0, stream, a, span);
 }
 
@@ -471,9 +581,8 @@ cudaError_t launch_kv_append(bool bf16, const AppendArgs& a, cudaStream_t stream
 
 cudaError_t launch_kv_decode(const KvView& c, const int32_t* pages, int count, uint16_t* k_out, uint16_t* v_out,
                              cudaStream_t stream) {
-  const long long vectors = static_cast<long long>(count) * c.heads * c.page_size * c.dim / 8;
-  const long long blocks = (vectors + 255) / 256;
-  const dim3 grid(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), 2);
+  const long long blocks = static_cast<long long>(count) * c.heads;
+  const dim3 grid(static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20)), 2);
   return launch_overlapped(c.kind == kKvInt8 ? kv_decode_kernel<kKvInt8> : kv_decode_kernel<kKvE4m3>, grid, 256, 0, stream, c,
                            pages, count, k_out, v_out);
 }

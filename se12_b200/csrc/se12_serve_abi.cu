@@ -3,6 +3,8 @@
 // checks, TMA descriptors, launches). See include/se12.h.
 #include "se12_serve.h"
 
+#include <atomic>
+
 struct se12_kv_cache {
   se12::KvView view;
   alignas(64) CUtensorMap k_map;
@@ -25,6 +27,21 @@ int encode_kv_map(CUtensorMap* map, const void* codes, const se12::KvView& v) {
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(v.dim)};
   const cuuint32_t box[2] = {128, 16};
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box);
+}
+
+// SMs of the current device, at most kMaxSms; asked once per device.
+int device_sm_count(int* sm_count) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices];
+  int device = 0;
+  const cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return cuda_fail(err, "cudaGetDevice");
+  if (device < kDevices && (*sm_count = known[device].load(std::memory_order_relaxed)) > 0) return SE12_OK;
+  const int st = current_device_info(&device, sm_count);
+  if (st != SE12_OK) return st;
+  *sm_count = std::min(*sm_count, kMaxSms);
+  if (device < kDevices) known[device].store(*sm_count, std::memory_order_relaxed);
+  return SE12_OK;
 }
 
 int check_batch(const se12_kv_cache* cache, const se12_kv_batch* b, se12::TokenBatch* out) {
@@ -219,10 +236,9 @@ int se12_token_logprobs(const void* logits, int bf16, int rows, int vocab, int64
   if (!workspace || workspace_bytes < need)
     return fail(SE12_ERR_WORKSPACE_TOO_SMALL, "workspace needs " + std::to_string(need) + " bytes");
   if (!aligned16(workspace)) return fail(SE12_ERR_MISALIGNED, "the workspace must be 16-byte aligned");
-  int device = 0, sm_count = 0;
-  const int st = current_device_info(&device, &sm_count);
+  int sm_count = 0;
+  const int st = device_sm_count(&sm_count);
   if (st != SE12_OK) return st;
-  sm_count = std::min(sm_count, kMaxSms);
   se12::LogprobArgs a{};
   a.logits = logits;
   a.ld = ld;

@@ -34,6 +34,9 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_SEQS = 2048
 COUNTER_BYTES = 4096  # SE12_COUNTER_BYTES: the part of a workspace that must be zero before a call
 
+_FLOATS = (torch.float32, torch.bfloat16)
+_BF16 = (torch.bfloat16,)
+
 _WORKSPACES = _WorkspacePool()
 
 
@@ -50,7 +53,7 @@ def _workspace(pool: _WorkspacePool, device: torch.device, stream: int, nbytes: 
 
 def _launch(index: int, function, name: str, *args) -> None:
     """function(*args, current stream) on GPU ``index``."""
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         status = function(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -151,24 +154,45 @@ class PagedKvCache:
     def handle(self) -> ctypes.c_void_p:
         return self._handle
 
+    # The checks of a call that is right cost as little as they can (a decode
+    # step makes one such call per layer and operator); the functions that say
+    # what is wrong are only called where something is.
     def _batch(self, tokens: int, block_table, lens, query_start) -> bytes:
+        shape, stride, device = block_table.shape, block_table.stride(), self.device
+        seqs = lens.numel()
+        if not (block_table.dtype is torch.int32 and lens.dtype is torch.int32 and len(shape) == 2 and lens.dim() == 1
+                and shape[0] == seqs and shape[1] >= 1 and (stride[1] == 1 or shape[1] == 1)
+                and (seqs == 1 or lens.stride(0) == 1) and block_table.device == device and lens.device == device
+                and 1 <= seqs <= MAX_SEQS):
+            self._refuse_batch(block_table, lens)
+        start = 0
+        if query_start is None:
+            if tokens != seqs:
+                raise ValueError(f"without query_start there is one token per sequence: {tokens} tokens, {seqs} sequences")
+        else:
+            _index(query_start, "query_start", 1, device)
+            if query_start.shape[0] != seqs + 1:
+                raise ValueError(f"query_start must have {seqs + 1} entries, got {query_start.shape[0]}")
+            start = query_start.data_ptr()
+        return _lib.KV_BATCH.pack(seqs, tokens, lens.data_ptr(), start, block_table.data_ptr(), max(stride[0], shape[1]),
+                                  shape[1])
+
+    def _refuse_batch(self, block_table, lens) -> None:
         _index(block_table, "block_table", 2, self.device)
         _index(lens, "lens", 1, self.device)
         seqs = lens.shape[0]
         if block_table.shape[0] != seqs or block_table.shape[1] < 1:
             raise ValueError(f"block_table must have a row per sequence ({seqs}) and a column or more, got {tuple(block_table.shape)}")
-        if seqs < 1 or seqs > MAX_SEQS:
-            raise ValueError(f"1..{MAX_SEQS} sequences, got {seqs}")
-        if query_start is None:
-            if tokens != seqs:
-                raise ValueError(f"without query_start there is one token per sequence: {tokens} tokens, {seqs} sequences")
-        else:
-            _index(query_start, "query_start", 1, self.device)
-            if query_start.shape[0] != seqs + 1:
-                raise ValueError(f"query_start must have {seqs + 1} entries, got {query_start.shape[0]}")
-        columns = block_table.shape[1]
-        return _lib.KV_BATCH.pack(seqs, tokens, lens.data_ptr(), 0 if query_start is None else query_start.data_ptr(),
-                                  block_table.data_ptr(), max(block_table.stride(0), columns), columns)
+        raise ValueError(f"1..{MAX_SEQS} sequences, got {seqs}")
+
+    def _row_strides(self, x: torch.Tensor, name: str, heads: int | None, tokens: int | None, dtypes) -> tuple:
+        """Token and head stride of [tokens, heads, head_dim] rows."""
+        shape, stride = x.shape, x.stride()
+        if (len(shape) == 3 and shape[2] == self.head_dim and (heads is None or shape[1] == heads)
+                and (tokens is None or shape[0] == tokens) and x.dtype in dtypes and stride[2] == 1 and x.device == self.device):
+            return stride[0], stride[1]
+        _rows(x, name, heads, self.head_dim, tokens, dtypes, self.device)
+        return stride[0], stride[1]
 
     # ------------------------------------------------------------------ operators
     def append(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
@@ -186,43 +210,40 @@ class PagedKvCache:
         row: nothing is stored, its queries are zeros. ``cos`` and ``sin``
         (fp32 [positions, rotary / 2]) rotate keys and queries by position,
         pairs (i, i + rotary / 2), or (2i, 2i + 1) when ``interleaved``."""
-        floats = (torch.float32, torch.bfloat16)
+        dtype = k.dtype
+        k_strides = self._row_strides(k, "k", self.kv_heads, None, _FLOATS)
         tokens = k.shape[0]
-        _rows(k, "k", self.kv_heads, self.head_dim, None, floats, self.device)
-        _rows(v, "v", self.kv_heads, self.head_dim, tokens, (k.dtype,), self.device)
-        if tokens == 0:
-            return None if q is None else (q_out if q_out is not None else q.new_empty(q.shape, dtype=torch.bfloat16))
-        batch = self._batch(tokens, block_table, lens, query_start)
-        queries, query_out, q_heads = (0, 0, 0), (0, 0, 0), 0
+        v_strides = self._row_strides(v, "v", self.kv_heads, tokens, (dtype,))
+        q_ptr, q_heads, q_strides, out_ptr, out_strides = 0, 0, (0, 0), 0, (0, 0)
         if q is not None:
-            _rows(q, "q", None, self.head_dim, tokens, (k.dtype,), self.device)
+            q_strides = self._row_strides(q, "q", None, tokens, (dtype,))
             q_heads = q.shape[1]
             if q_heads < 1:
                 raise ValueError("q has no heads")
             if q_out is None:
                 q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+                out_strides = (q_heads * self.head_dim, self.head_dim)
             else:
-                _rows(q_out, "q_out", q_heads, self.head_dim, tokens, (torch.bfloat16,), self.device)
-            queries = (q.data_ptr(), q.stride(0), q.stride(1))
-            query_out = (q_out.data_ptr(), q_out.stride(0), q_out.stride(1))
+                out_strides = self._row_strides(q_out, "q_out", q_heads, tokens, _BF16)
+            q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
-        if (cos is None) != (sin is None):
-            raise ValueError("cos and sin go together")
+        if tokens == 0:
+            return q_out
+        batch = self._batch(tokens, block_table, lens, query_start)
         turn = (0, 0, 0, 0, 0)
-        if cos is not None:
-            for t, name in ((cos, "cos"), (sin, "sin")):
-                if t.dtype != torch.float32 or t.dim() != 2 or t.stride(1) != 1 or t.device != self.device:
-                    raise ValueError(f"{name} must be an fp32 [positions, rotary / 2] tensor on {self.device}")
-            rows, half = cos.shape
-            if sin.shape != cos.shape or cos.stride(0) != sin.stride(0):
-                raise ValueError("cos and sin must have the same shape and strides")
-            if not 1 <= half <= self.head_dim // 2 or rows < 1:
-                raise ValueError(f"cos and sin must have 1..{self.head_dim // 2} columns and a row or more")
-            turn = (cos.data_ptr(), sin.data_ptr(), max(cos.stride(0), half), rows, 2 * half)
-        args = _lib.KV_APPEND.pack(k.dtype == torch.bfloat16, q_heads, queries[0], k.data_ptr(), v.data_ptr(), queries[1],
-                                   queries[2], k.stride(0), k.stride(1), v.stride(0), v.stride(1), *turn, bool(interleaved),
-                                   *query_out)
+        if cos is not None and sin is not None:
+            shape, stride = cos.shape, cos.stride()
+            if not (cos.dtype is torch.float32 and sin.dtype is torch.float32 and len(shape) == 2 and sin.shape == shape
+                    and stride[1] == 1 and sin.stride() == stride and cos.device == self.device and sin.device == self.device
+                    and 1 <= shape[1] <= self.head_dim // 2 and shape[0] >= 1):
+                raise ValueError(f"cos and sin must be fp32 [positions, 1..{self.head_dim // 2}] tensors on {self.device} with the "
+                                 "same shape and strides and unit column stride")
+            turn = (cos.data_ptr(), sin.data_ptr(), max(stride[0], shape[1]), shape[0], 2 * shape[1])
+        elif cos is not None or sin is not None:
+            raise ValueError("cos and sin go together")
+        args = _lib.KV_APPEND.pack(dtype is torch.bfloat16, q_heads, q_ptr, k.data_ptr(), v.data_ptr(), *q_strides, *k_strides,
+                                   *v_strides, *turn, bool(interleaved), out_ptr, *out_strides)
         _launch(self._index, self._lib.se12_kv_append, "se12_kv_append", self._handle, batch, args)
         return q_out
 
@@ -237,23 +258,24 @@ class PagedKvCache:
         see nothing are zero. ``max_query``: the most rows of one sequence
         (default: all tokens; tells the launch how many rows share a page).
         Returns BF16 like q."""
-        tokens = q.shape[0]
-        _rows(q, "q", None, self.head_dim, None, (torch.bfloat16,), self.device)
-        if q.shape[1] < 1 or q.shape[1] % self.kv_heads:
-            raise ValueError(f"q has {q.shape[1]} heads, not a multiple of the cache's {self.kv_heads}")
+        q_strides = self._row_strides(q, "q", None, None, _BF16)
+        tokens, q_heads, _ = q.shape
+        if q_heads < 1 or q_heads % self.kv_heads:
+            raise ValueError(f"q has {q_heads} heads, not a multiple of the cache's {self.kv_heads}")
         if out is None:
             out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+            out_strides = (q_heads * self.head_dim, self.head_dim)
         else:
-            _rows(out, "out", q.shape[1], self.head_dim, tokens, (torch.bfloat16,), self.device)
+            out_strides = self._row_strides(out, "out", q_heads, tokens, _BF16)
         if tokens == 0:
             return out
         batch = self._batch(tokens, block_table, lens, query_start)
         if max_query is None:
             max_query = 1 if query_start is None else tokens
         max_query = int(max_query)
-        args = _lib.KV_ATTEND.pack(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                                   q.shape[1], max_query, int(window), self.head_dim ** -0.5 if scale is None else scale, softcap)
-        need = self._lib.se12_kv_attend_call_bytes(self._handle, q.shape[1], max_query)
+        args = _lib.KV_ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *out_strides, q_heads, max_query, int(window),
+                                   self.head_dim ** -0.5 if scale is None else scale, softcap)
+        need = self._lib.se12_kv_attend_call_bytes(self._handle, q_heads, max_query)
         ws = _workspace(_WORKSPACES, self.device, torch._C._cuda_getCurrentRawStream(self._index), need)
         _launch(self._index, self._lib.se12_kv_attend, "se12_kv_attend", self._handle, batch, args, ws, need)
         return out
