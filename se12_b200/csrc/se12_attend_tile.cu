@@ -333,45 +333,49 @@ __device__ __forceinline__ void group_maxima(float* t, const uint32_t (&s)[2][32
   }
 }
 
-// Weights of the 64 tokens in s into P, and their sum.
+__device__ __forceinline__ unsigned long long twice(float x) { return pair_of(x, x); }
+
+// Weights of the 64 tokens in s into P, and their sum, two tokens at a time.
 template <bool CAP, bool MASK>
 __device__ __forceinline__ void group_weights(RowSoftmax& r, const TileLogits& z, const uint32_t (&s)[2][32], int k0) {
   // cap tanh(u) in units of log 2: u times a polynomial of u^2 of degree 4
   // (Chebyshev fit of tanh(u) / u on |u| <= 0.7, off by 1.9e-7)
-  const float c0 = 0.999999706f * z.cap2, c1 = -0.33330266f * z.cap2, c2 = 0.132816473f * z.cap2,
-              c3 = -0.0508535559f * z.cap2, c4 = 0.0137912829f * z.cap2;
+  const unsigned long long c0 = twice(0.999999706f * z.cap2), c1 = twice(-0.33330266f * z.cap2), c2 = twice(0.132816473f * z.cap2),
+                           c3 = twice(-0.0508535559f * z.cap2), c4 = twice(0.0137912829f * z.cap2);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t p[8];
       const int q = (k0 >> 4) + c * 2 + h;
-      const float f = z.row_scale * z.meta[q][0], shift = z.meta[q][1] - r.mp;
-      float sum0 = 0.f, sum1 = 0.f;
+      const float shift = z.meta[q][1] - r.mp;
+      const unsigned long long f = twice(z.row_scale * z.meta[q][0]), shift2 = twice(shift);
+      unsigned long long sum = 0;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        float w[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = h * 16 + 2 * k + e;
-          const float v = __uint_as_float(s[c][i]);
-          if (CAP) {
-            const float u = v * f, t = u * u;
-            float y = fmaf(c4, t, c3);
-            y = fmaf(y, t, c2);
-            y = fmaf(y, t, c1);
-            y = fmaf(y, t, c0);
-            w[e] = fmaf(y, u, shift);
-          } else {
-            w[e] = fmaf(v, f, shift);
-          }
-          w[e] = ex2(w[e]);
-          if (MASK && (k0 + c * 32 + i < z.low || k0 + c * 32 + i > z.high)) w[e] = 0.f;
+        const int i = h * 16 + 2 * k;
+        const unsigned long long v = pair_of(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+        unsigned long long x;
+        if (CAP) {
+          const unsigned long long u = mul_pair(v, f), t = mul_pair(u, u);
+          x = fma_pair(fma_pair(fma_pair(fma_pair(fma_pair(c4, t, c3), t, c2), t, c1), t, c0), u, shift2);
+        } else {
+          x = fma_pair(v, f, shift2);
         }
-        sum0 += w[0];
-        sum1 += w[1];
-        p[k] = half2_bits(__floats2half2_rn(w[0], w[1]));
+        float w0, w1;
+        unpair(x, w0, w1);
+        w0 = ex2(w0);
+        w1 = ex2(w1);
+        if (MASK) {
+          const int at = k0 + c * 32 + i;
+          if (at < z.low || at > z.high) w0 = 0.f;
+          if (at + 1 < z.low || at + 1 > z.high) w1 = 0.f;
+        }
+        sum = add_pair(sum, pair_of(w0, w1));
+        p[k] = half2_bits(__floats2half2_rn(w0, w1));
       }
+      float sum0, sum1;
+      unpair(sum, sum0, sum1);
       r.l = fmaf(sum0 + sum1, ex2(-shift - r.m), r.l);  // 2^(logit - m) = w 2^(mp - lv - m)
       tmem_store_8(z.to + k0 / 2 + c * 16 + h * 8, p);
     }

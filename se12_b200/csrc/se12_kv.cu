@@ -213,14 +213,14 @@ __device__ __forceinline__ int page_of(const TokenBatch& t, const KvView& c, int
   return -1;
 }
 
-// Scale of a block once tokens with largest magnitude `amax` have joined it;
-// `ratio` = what the older codes shrink by.
+// Scale of a block with older tokens at scale `before` (`older`) once tokens
+// with largest magnitude `amax` have joined it; `ratio` = what the older codes
+// shrink by.
 template <int KIND>
-__device__ __forceinline__ float joined_scale(const float* scale, bool older, unsigned amax, float& ratio) {
+__device__ __forceinline__ float joined_scale(float before, bool older, unsigned amax, float& ratio) {
   const float need = fit_scale<KIND>(amax);
   ratio = 1.f;
   if (!older) return need;
-  const float before = *scale;
   if (!(before >= need)) {  // grows, or one of the two is not finite
     if (before < need) {
       ratio = before * __frcp_rn(need);
@@ -297,13 +297,14 @@ __global__ void __launch_bounds__(128) kv_append_step_kernel(const AppendArgs a)
   const long long block = static_cast<long long>(page) * a.c.heads + head;
   uint8_t* codes = (keys ? a.c.k_codes : a.c.v_codes) + block * a.c.page_size * a.c.dim;
   float* scale = (keys ? a.c.k_scales : a.c.v_scales) + block;
+  const float before = *scale;
   unsigned amax = 0;
   for_row<VP>(row, map, cos, sin, lane, [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
     amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
   });
   amax = __reduce_max_sync(0xFFFFFFFFu, amax);
   float ratio;
-  const float now = joined_scale<KIND>(scale, slot > 0, amax, ratio);
+  const float now = joined_scale<KIND>(before, slot > 0, amax, ratio);
   const bool finite = now == now;
   if (ratio != 1.f) shrink_codes<KIND>(codes, slot * a.c.dim, ratio, lane, 32);
   const float inv = finite ? __frcp_rn(now) : 0.f;  // exact for the powers of two stored here
@@ -333,20 +334,19 @@ __device__ __forceinline__ int sequence_of(const TokenBatch& t, int token, int l
   return n;
 }
 
-// A block's new tokens (rows first .. first + count - 1 of src, slots slot ..)
-// joined to it by one CTA of 8 warps.
+// New tokens of one page (rows 0 .. count - 1 at src, slots slot ..) joined to
+// it by a CTA of 8 warps, for the heads head .. head + heads - 1 one after the
+// other: the next head's rows are on their way while this one's scale is found.
 template <typename T, int KIND, int VP>
-__device__ __forceinline__ void append_block(const AppendArgs& a, bool keys, const T* src, long long ts, int pos, int slot,
-                                             int count, uint8_t* codes, float* scale, unsigned* s_amax) {
+__device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, const T* src, long long ts, long long hs, int head,
+                                            int heads, int pos, int slot, int count, int page, unsigned (*s_amax)[8]) {
   constexpr int kHeld = 4;  // rows a warp keeps in registers from one pass to the next
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.c.dim;
   const PairMap map = pair_map(a, keys, VP);
   const bool turned = keys && a.cos;
   const bool held = VP > 1 && count <= 8 * kHeld;
   RowPart<VP> row[kHeld];
-  unsigned amax = 0;
-  auto row_of = [&](RowPart<VP>& r, int i) {
-    r.load(src + i * ts, lane);
+  auto rotate = [&](RowPart<VP>& r, int i) {
     if (turned) {
       float c[VP], s[VP];
       load_vector<VP>(c, a.cos + (pos + i) * a.rope_stride + lane * VP);
@@ -354,65 +354,83 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, bool keys, con
       r.rotate(c, s);
     }
   };
-  if constexpr (VP > 1) {
-    for (int i0 = warp; i0 < count; i0 += 8 * kHeld) {
+  auto load = [&](int h, int i0) {
 #pragma unroll
-      for (int k = 0; k < kHeld; ++k)
-        if (i0 + 8 * k < count) row_of(row[k], i0 + 8 * k);
-#pragma unroll
-      for (int k = 0; k < kHeld; ++k)
-        if (i0 + 8 * k < count) amax = magnitude_bits<VP>(row[k].b, magnitude_bits<VP>(row[k].a, amax));
-    }
-  } else {
-    for (int i = warp; i < count; i += 8)
-      for_row<VP>(src + i * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
-                  [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
-                    amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
-                  });
-  }
-  amax = __reduce_max_sync(0xFFFFFFFFu, amax);
-  if (lane == 0) s_amax[warp] = amax;
-  __syncthreads();
-  amax = s_amax[lane & 7];
-  amax = __reduce_max_sync(0xFFFFFFFFu, amax);
-  float ratio;
-  const float now = joined_scale<KIND>(scale, slot > 0, amax, ratio);
-  __syncthreads();  // every thread has read the old scale and the maxima
-  const bool finite = now == now;
-  if (ratio != 1.f) shrink_codes<KIND>(codes, slot * dim, ratio, threadIdx.x, 256);
-  const float inv = finite ? __frcp_rn(now) : 0.f;  // exact for the powers of two stored here
-  auto put = [&](uint8_t* to, const float(&x)[VP]) {
-    if (finite) {
-      store_codes<KIND, VP>(to, x, inv);
-    } else {
-#pragma unroll
-      for (int j = 0; j < VP; ++j) to[j] = 0;
-    }
+    for (int k = 0; k < kHeld; ++k)
+      if (i0 + 8 * k < count) row[k].load(src + h * hs + (i0 + 8 * k) * ts, lane);
   };
-  uint8_t* to = codes + slot * dim;
-  if constexpr (VP > 1) {
-    for (int i0 = warp; i0 < count; i0 += 8 * kHeld) {
-      if (!held) {
+  if (VP > 1 && held) load(head, warp);
+  for (int n = 0; n < heads; ++n) {
+    const int h = head + n;
+    const T* rows = src + h * hs;
+    const long long block = static_cast<long long>(page) * a.c.heads + h;
+    float* scale = (keys ? a.c.k_scales : a.c.v_scales) + block;
+    uint8_t* codes = (keys ? a.c.k_codes : a.c.v_codes) + block * a.c.page_size * dim;
+    const float before = slot > 0 ? *scale : 0.f;
+    unsigned amax = 0;
+    if constexpr (VP > 1) {
+      for (int i0 = warp; i0 < count; i0 += 8 * kHeld) {
+        if (!held) load(h, i0);
 #pragma unroll
         for (int k = 0; k < kHeld; ++k)
-          if (i0 + 8 * k < count) row_of(row[k], i0 + 8 * k);
+          if (i0 + 8 * k < count) {
+            rotate(row[k], i0 + 8 * k);
+            amax = magnitude_bits<VP>(row[k].b, magnitude_bits<VP>(row[k].a, amax));
+          }
       }
-#pragma unroll
-      for (int k = 0; k < kHeld; ++k)
-        if (i0 + 8 * k < count) {
-          put(to + (i0 + 8 * k) * dim + lane * VP, row[k].a);
-          put(to + (i0 + 8 * k) * dim + 32 * VP + lane * VP, row[k].b);
-        }
+    } else {
+      for (int i = warp; i < count; i += 8)
+        for_row<VP>(rows + i * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
+                    [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
+                      amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
+                    });
     }
-  } else {
-    for (int i = warp; i < count; i += 8)
-      for_row<VP>(src + i * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
-                  [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
-                    put(to + i * dim + ia, x);
-                    put(to + i * dim + ib, y);
-                  });
+    amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+    if (lane == 0) s_amax[n & 1][warp] = amax;
+    __syncthreads();  // the maxima are there, and every thread has read the old scale
+    amax = s_amax[n & 1][lane & 7];
+    amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+    float ratio;
+    const float now = joined_scale<KIND>(before, slot > 0, amax, ratio);
+    const bool finite = now == now;
+    if (ratio != 1.f) shrink_codes<KIND>(codes, slot * dim, ratio, threadIdx.x, 256);
+    const float inv = finite ? __frcp_rn(now) : 0.f;  // exact for the powers of two stored here
+    auto put = [&](uint8_t* to, const float(&x)[VP]) {
+      if (finite) {
+        store_codes<KIND, VP>(to, x, inv);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VP; ++j) to[j] = 0;
+      }
+    };
+    uint8_t* to = codes + slot * dim;
+    if constexpr (VP > 1) {
+      for (int i0 = warp; i0 < count; i0 += 8 * kHeld) {
+        if (!held) {
+          load(h, i0);
+#pragma unroll
+          for (int k = 0; k < kHeld; ++k)
+            if (i0 + 8 * k < count) rotate(row[k], i0 + 8 * k);
+        }
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+          if (i0 + 8 * k < count) {
+            put(to + (i0 + 8 * k) * dim + lane * VP, row[k].a);
+            put(to + (i0 + 8 * k) * dim + 32 * VP + lane * VP, row[k].b);
+          }
+      }
+      if (held && n + 1 < heads) load(h + 1, warp);
+    } else {
+      for (int i = warp; i < count; i += 8)
+        for_row<VP>(rows + i * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
+                    [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
+                      put(to + i * dim + ia, x);
+                      put(to + i * dim + ib, y);
+                    });
+    }
+    if (threadIdx.x == 0) *scale = now;
   }
-  if (threadIdx.x == 0) *scale = now;
+  __syncthreads();  // the maxima are free
 }
 
 // One token's queries, a warp: the angle's cosines and sines are loaded once
@@ -446,23 +464,22 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int token, i
   }
 }
 
-// Any number of tokens per sequence. CTAs with blockIdx.y < 2 * heads: each
-// looks through `span` consecutive tokens for the first new token of a block
-// (of its sequence, or of a page) and stores that block's new tokens, four
-// rows per warp on their way at a time; up to 32 stay in registers while the
-// scale is found, more are read again from L2. The last blockIdx.y rotates the
-// queries, a warp per token. (One row per warp at a time, and the queries of a
-// token by a warp per head, 14900 tokens of 16 + 2 x 8 heads of 256 took twice
-// the time.)
+// Any number of tokens per sequence. All blockIdx.y but the last, each for
+// `heads_each` heads of the keys or of the values: a CTA looks through `span`
+// consecutive tokens for the first new token of a block (of its sequence, or
+// of a page) and stores that block's new tokens, four rows per warp on their
+// way at a time; up to 32 stay in registers while the scale is found, more are
+// read again from L2. The last blockIdx.y rotates the queries, a warp per
+// token.
 template <typename T, int KIND, int VP>
-__global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendArgs a, const int span) {
-  __shared__ unsigned s_amax[8];
+__global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendArgs a, const int span, const int heads_each) {
+  __shared__ unsigned s_amax[2][8];
   grid_launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int what = blockIdx.y;
+  const int groups = (a.c.heads + heads_each - 1) / heads_each, what = blockIdx.y;
   const int first = blockIdx.x * span, end = min(first + span, a.t.tokens);
-  if (what == 2 * a.c.heads) {
+  if (what == 2 * groups) {
     for (int t = first + warp; t < end; t += 8) {
       const int b = sequence_of(a.t, t, lane);
       const bool owned = t >= a.t.query_start[b] && t < a.t.query_start[b + 1];
@@ -471,9 +488,9 @@ __global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendAr
     return;
   }
   int b = sequence_of(a.t, first, lane);
-  const bool keys = what < a.c.heads;
-  const int head = keys ? what : what - a.c.heads;
-  const T* src = static_cast<const T*>(keys ? a.k : a.v) + head * (keys ? a.k_hs : a.v_hs);
+  const bool keys = what < groups;
+  const int head = (keys ? what : what - groups) * heads_each;
+  const T* src = static_cast<const T*>(keys ? a.k : a.v);
   const long long ts = keys ? a.k_ts : a.v_ts;
   for (int t = first; t < end; ++t) {
     while (b + 1 < a.t.seqs && a.t.query_start[b + 1] <= t) ++b;
@@ -492,10 +509,8 @@ __global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendAr
       raise_status(kStatusBadArgument);
       continue;
     }
-    const long long block = static_cast<long long>(page) * a.c.heads + head;
-    append_block<T, KIND, VP>(a, keys, src + t * ts, ts, pos, slot, count,
-                              (keys ? a.c.k_codes : a.c.v_codes) + block * a.c.page_size * a.c.dim,
-                              (keys ? a.c.k_scales : a.c.v_scales) + block, s_amax);
+    append_page<T, KIND, VP>(a, keys, src + t * ts, ts, keys ? a.k_hs : a.v_hs, head, min(heads_each, a.c.heads - head), pos,
+                             slot, count, page, s_amax);
   }
 }
 
@@ -548,10 +563,15 @@ cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t stream) {
     return launch_overlapped(kv_append_step_kernel<T, KIND, VP>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0,
                              stream, a);
   }
-  // few tokens: one per CTA, so that short sequences' blocks run side by side
-  const int span = a.t.tokens <= 256 ? 1 : 16;
-  const dim3 grid((a.t.tokens + span - 1) / span, 2 * a.c.heads + (a.q ? 1 : 0));
-  return launch_overlapped(kv_append_prompt_kernel<T, KIND, VP>, grid, 256, 0, stream, a, span);
+  // few tokens: one per CTA, so that short sequences' blocks run side by side;
+  // many: a page's, and several heads per CTA, which finds its pages once for
+  // them (14900 tokens of 8 heads, with the queries: 139 us with 16 tokens and
+  // one head per CTA, 100 us with 32 and four)
+  const bool many = a.t.tokens > 2048;
+  const int span = a.t.tokens <= 256 ? 1 : many ? a.c.page_size : 16;
+  const int heads_each = many ? 4 : 1;
+  const dim3 grid((a.t.tokens + span - 1) / span, 2 * ((a.c.heads + heads_each - 1) / heads_each) + (a.q ? 1 : 0));
+  return launch_overlapped(kv_append_prompt_kernel<T, KIND, VP>, grid, 256, 0, stream, a, span, heads_each);
 }
 
 template <typename T, int KIND>
