@@ -420,7 +420,7 @@ def filled(g, pool, page, heads, dim, kind, spread=1.0):
     for _ in range(2):
         x = torch.randn(pool, heads, page, dim, generator=g)
         x *= 2.0 ** ((torch.rand(pool, heads, 1, 1, generator=g) * 2 - 1) * spread)
-        s = torch.tensor([[least_scale(float(x[p, h].abs().max()), kind) for h in range(heads)] for p in range(pool)])
+        s = torch.tensor([[least_scale(m, kind) for m in page] for page in x.abs().amax(dim=(2, 3)).tolist()])
         tensors.append((code_of(x / s[:, :, None, None], kind), s))
     (k, ks), (v, vs) = tensors
     cache = PagedKvCache.from_tensors(k.cuda(), v.cuda(), ks.cuda(), vs.cuda(), kind)
@@ -520,6 +520,68 @@ def test_attend_weights_of_zero_values_count():
     cache.append(k, v, table, lens, query_start=torch.tensor([0, 32], dtype=torch.int32, device="cuda"))
     out = cache.attend(torch.ones(1, 2, 128, dtype=torch.bfloat16, device="cuda"), table, lens)
     assert bool((out == 4.0).all())
+
+
+def check_on_gpu(cache, q, table, lens, counts, got, softcap, window):
+    """Against 64-bit sums on the GPU over the cache's values (BF16 holds them
+    exactly), with the tolerance above; for batches too large for the CPU."""
+    keys, values = cache.decode()
+    page, dim, group = cache.page_size, cache.head_dim, q.shape[1] // cache.kv_heads
+    starts = starts_of(counts)
+    for b, ln in enumerate(lens):
+        if counts[b] == 0 or ln == 0:
+            continue
+        ids = table[b, : (ln + page - 1) // page].long()
+        rows = slice(starts[b], starts[b + 1])
+        i, j = torch.arange(ln - counts[b], ln, device="cuda"), torch.arange(ln, device="cuda")
+        hidden = j[None, :] > i[:, None]
+        if window:
+            hidden |= i[:, None] - j[None, :] >= window
+        for h in range(cache.kv_heads):
+            k, v = (t[ids, h].reshape(-1, dim)[:ln].double() for t in (keys, values))
+            for g in range(h * group, (h + 1) * group):
+                s = q[rows, g].double() @ k.T * dim**-0.5
+                s = softcap * torch.tanh(s / softcap) if softcap else s
+                p = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
+                want, size = p @ v, p @ v.abs()
+                half_unit = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=1e-300))) - 8)
+                tol = half_unit + 2.0**-10 * size + 2.0**-24 * ln * v.abs().max()
+                assert bool(((got[rows, g].double() - want).abs() <= tol).all()), (b, g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,q_heads,dim,page", [("int8", 4, 32, 128, 16), ("e4m3", 8, 16, 256, 64), ("int8", 2, 24, 192, 32)])
+@pytest.mark.parametrize("softcap,window", [(0.0, 0), (30.0, 700)])
+def test_attend_many_tiles_per_cta(kind, heads, q_heads, dim, page, softcap, window):
+    """Runs of many tiles of many pairs: drafted tokens and prompt chunks, also
+    sequences whose chunk is all they have."""
+    g = torch.Generator().manual_seed(heads)
+    counts = [2 + i % 5 for i in range(20)] + [300, 0, 70, 513]
+    lens = [n + (i * 397) % 2500 for i, n in enumerate(counts)]
+    lens[-2] = 70
+    table, pool = random_tables(g, lens, page)
+    cache, _, _ = filled(g, pool, page, heads, dim, kind, 2.0)
+    q = (torch.randn(sum(counts), q_heads, dim, generator=g) * 2).to(torch.bfloat16).cuda()
+    start = torch.tensor(starts_of(counts), dtype=torch.int32).cuda()
+    for _ in range(2):
+        got = cache.attend(q, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), query_start=start,
+                           max_query=max(counts), softcap=softcap, window=window)
+        check_on_gpu(cache, q, table.cuda(), lens, counts, got, softcap, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,kind", [(128, "e4m3"), (256, "int8")])
+def test_attend_long_ragged_batch(dim, kind):
+    """Next tokens of a ragged batch over long sequences: runs of many pairs,
+    pairs of many runs."""
+    g = torch.Generator().manual_seed(dim)
+    lens = [1 + (i * 2999) % 9001 for i in range(30)] + [0, 30000]
+    table, pool = random_tables(g, lens, 64)
+    cache, _, _ = filled(g, pool, 64, 2, dim, kind, 2.0)
+    q = torch.randn(32, 16, dim, generator=g).to(torch.bfloat16).cuda()
+    got = cache.attend(q, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), softcap=40.0)
+    check_on_gpu(cache, q, table.cuda(), lens, [1] * 32, got, 40.0, 0)
+    assert bool((got[30] == 0).all())
 
 
 @pytest.mark.gpu
