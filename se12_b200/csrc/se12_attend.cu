@@ -17,9 +17,9 @@
 // a TMA pipeline of its own (no CTA-wide barrier inside a pair's chunks) and
 // its own references and sums; a pair's warps are joined in shared memory,
 // its CTAs through global memory by the CTA that finishes last, in CTA order.
-// Small CTAs, 2 to 4 per SM: 12 or 16 warps hide each other's latencies (8
-// warps in one CTA ran at half of the issue rate: 142 us against 107 for
-// 131071 tokens of 16 KV heads of 128), and short sequences' pairs run side by side.
+// Small CTAs, 2 or 3 per SM: 8 or 12 warps hide each other's latencies (8
+// warps in one CTA per SM took 142 us against 107 for 131071 tokens of 16 KV
+// heads of 128: 5.0 TB/s), and short sequences' pairs run side by side.
 //
 // Layout of the products (mma.sync m16n8k16, tokens or dimensions as M,
 // query rows as N = 8): with a group of up to 8 query rows per KV head the
@@ -27,8 +27,10 @@
 // 16-byte vectors of codes: S^T = K Q^T takes the contraction in the order
 // the bytes lie in, O^T = V^T P^T interleaves two tokens' bytes with one
 // byte permute per pair. P^T is S^T's accumulator transposed by movmatrix.
-// The bound is HBM; tcgen05 would need the codes widened into shared memory
-// first and pads the rows to 64 or more.
+// The floor is HBM's; what bounds the kernel is the issue of its instructions
+// and their latencies (2.2 of 4 a cycle with 12 warps per SM, DRAM 58 % busy,
+// the tensor pipe 16 %). tcgen05 would need the codes widened into shared
+// memory first and pads the rows to 64 or more.
 //
 // Two references instead of one running maximum: m for the sum l of 2^(s - m),
 // and mp for the weights 2^(s + log2 vs - mp) that multiply the codes, so that
@@ -49,7 +51,6 @@ constexpr int kAttendStages = 2;
 constexpr int kAttendBox = 2048;         // 16 tokens x 128 bytes
 constexpr int kAttendStageBytes = 8192;  // keys and values of a chunk
 constexpr int kAttendDeposit = 8192;     // joining the warps' sums
-constexpr int kAttendMaxSeqs = 2048;
 constexpr int kAttendSlotRows = 16;
 constexpr int kAttendSlotFloats = kAttendSlotRows * (256 + 4);  // sums, then (m, l, mp) per row
 constexpr int kAttendMaxCtas = 3;        // per SM

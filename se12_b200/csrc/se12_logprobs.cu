@@ -6,24 +6,26 @@
 //   top: the k largest x, ties to the lowest index (the cap keeps the order)
 //
 // The pass keeps, per thread, the running maximum with S and the weighted
-// sum below it, and per CTA a buffer of candidates for the top list: values
-// above the list's k-th, pushed by whichever thread meets them. The list is
-// rebuilt (each warp sorts 32 candidates at a time and merges them into its
-// own 32, then the warps' lists are merged) only when the buffer fills up,
-// after a row's first, fourth, sixteenth ... batch and at its end. Before the first batch is pushed,
-// the k-th largest of any one warp's lane maxima bounds the list from below;
-// the best of the warps' bounds leaves a few hundred candidates. A warp
-// takes places in the buffer for all its candidates at once (one by one, the
-// atomics on the counter were half of a row's time).
+// sum below it, and the largest value the thread has met. The top list is found
+// afterwards: the k-th largest of the 256 threads' own largest is no larger
+// than the k-th value, so that only the threads whose largest reaches it, k of
+// them but for equal values, hold anything of the list; their values are read
+// again from L2, a warp per thread, and the few that reach the bound are sorted
+// (32 at a time over a warp's lanes, the warps' lists then merged). Rows with
+// too many equal values for that (nearly all tokens banned) go through memory
+// once more. 1023 x 128256 BF16 logits, top 20, against a list kept during the
+// pass with the candidates pushed into a buffer: 118 us and 137 us, rows in
+// ascending order 129 us and 2604 us; but all rows with ten tokens left 285 us
+// and 201 us (16 such rows 32 us and 30 us).
 //
 // Rows come in batches of 8 KB (4 KB when there are few) by bulk copies, four
 // batches ahead, whatever row they belong to: with three CTAs per SM 96 KB are
 // on the way. (Three CTAs of 256 threads, 80 registers: at two of 512 and 64
-// the spilled registers of the inner loop cost four times the loop.) The warps of a CTA meet only after a row's first batch and every
-// fourth one, to look at the buffer. The batches of all rows are cut into equal runs,
-// one per CTA, and a row's CTAs are joined by the last to finish, in CTA
-// order. The bound is HBM for plain logits, the special-function unit (three
-// calls a value) for capped ones.
+// the spilled registers of the inner loop cost four times the loop.) The warps
+// of a CTA meet at a row's end only. The batches of all rows are cut into
+// equal runs, one per CTA, and a row's CTAs are joined by the last to finish,
+// in CTA order. Streaming alone takes 83 us of the 118, twice what HBM needs
+// for the bytes: the instructions of a value bound it, not the bytes.
 #include "se12_device.cuh"
 #include "se12_serve.h"
 
@@ -38,8 +40,8 @@ constexpr int kLogprobCtas = 3;  // per SM
 constexpr int kLogprobWarps = kLogprobThreads / 32;
 constexpr int kLogprobStages = 4;
 constexpr int kLogprobTop = 32;
-constexpr int kLogprobSpare = 1024;   // candidates after which the list is rebuilt
-constexpr int kLogprobBuffer = 2048;  // what four batches may find; if more, they are gone through again
+constexpr int kLogprobBuffer = 2048;  // candidates
+constexpr int kLogprobHolders = 128;  // threads whose values are looked through for them
 // -inf and masks of the type's lowest value become this: its exponential is
 // zero and its product with log2(e) still finite.
 constexpr float kLogprobFloor = -2.0e38f;
@@ -74,17 +76,7 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
   return __uint_as_float((u & 0x80000000u) ? u & 0x7FFFFFFFu : ~u);
 }
 
-// The largest fp32 value below x; NaN below -inf.
-__device__ __forceinline__ float next_below(float x) {
-  const unsigned u = __float_as_uint(x);
-  if (x == 0.f) return __uint_as_float(0x80000001u);
-  return __uint_as_float((u & 0x80000000u) ? u + 1 : u - 1);
-}
-
 __device__ __forceinline__ int key_index(unsigned long long key) { return static_cast<int>(~static_cast<unsigned>(key)); }
-
-__device__ __forceinline__ unsigned long long larger(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
-__device__ __forceinline__ unsigned long long smaller(unsigned long long a, unsigned long long b) { return a < b ? a : b; }
 
 // One compare-exchange step of a descending bitonic network over the lanes.
 template <typename K>
@@ -118,7 +110,10 @@ struct LogprobSmem {
   unsigned long long lists[kLogprobWarps][32];
   unsigned long long list[32];
   float stat[kLogprobWarps][3];
-  float bounds[kLogprobWarps];
+  float maxima[kLogprobWarps][32];
+  float bound;
+  int holders[kLogprobThreads];  // threads that hold something of the list
+  int held;
   int count;
   int last;
   uint64_t full[kLogprobStages], empty[kLogprobStages];
@@ -168,29 +163,6 @@ __device__ __forceinline__ float load_logit(const void* row, long long i) {
   return static_cast<const float*>(row)[i];
 }
 
-// The candidates of a row's batches [first, last), which were too many for the
-// buffer, from memory again: one value per thread at a time.
-template <bool BF16>
-__device__ __noinline__ void refill_list(LogprobSmem& sm, const void* row, int first, int last, int batch, int vocab, int top,
-                                         int warp, int lane) {
-  __syncthreads();
-  if (threadIdx.x == 0) sm.count = 0;
-  __syncthreads();
-  const long long end = min(static_cast<long long>(last) * batch, static_cast<long long>(vocab));
-  for (long long base = static_cast<long long>(first) * batch; base < end; base += kLogprobThreads) {
-    const long long i = base + threadIdx.x;
-    if (i < end) {
-      const unsigned long long key = list_key(load_logit<BF16>(row, i), static_cast<int>(i));
-      if (key > sm.list[top - 1]) sm.buffer[atomicAdd(&sm.count, 1)] = key;
-    }
-    __syncthreads();
-    // (a candidate per thread fits below the limit four times)
-    if (sm.count > kLogprobBuffer - kLogprobThreads) rebuild_list(sm, sm.count, warp, lane);
-    __syncthreads();
-  }
-  if (sm.count) rebuild_list(sm, sm.count, warp, lane);
-}
-
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -208,6 +180,53 @@ __device__ __forceinline__ void unpack(float* x, const uint4& v) {
       x[2 * k + 1] = __uint_as_float(w & 0xFFFF0000u);
     } else {
       x[k] = __uint_as_float(w);
+    }
+  }
+}
+
+// The list of a row's values [begin, end), from memory, whatever they are: a
+// buffer of them at a time, the next one on its way. The warps meet once a
+// buffer, and sort only when it holds something.
+template <bool BF16>
+__device__ __noinline__ void list_all(LogprobSmem& sm, const void* row, int begin, int end, int top, bool vec, int warp, int lane) {
+  constexpr int kPer = BF16 ? 8 : 4, kVecs = kLogprobBuffer / (kLogprobThreads * kPer);
+  const int tid = static_cast<int>(threadIdx.x);
+  auto at = [&](int base, int n) { return base + (n * kLogprobThreads + tid) * kPer; };  // first value of vector n
+  uint4 next[kVecs];
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int n = 0; n < kVecs; ++n)
+      if (vec && at(base, n) + kPer <= end)
+        next[n] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const char*>(row) + static_cast<long long>(at(base, n)) * (BF16 ? 2 : 4)));
+  };
+  fetch(begin);
+  __syncthreads();  // (the list is there, the counter zero)
+  unsigned long long kth = sm.list[top - 1];
+  for (int base = begin; base < end; base += kLogprobBuffer) {
+    float x[kVecs * kPer];
+#pragma unroll
+    for (int n = 0; n < kVecs; ++n) {
+      if (vec && at(base, n) + kPer <= end) {
+        unpack<BF16>(x + n * kPer, next[n]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) x[n * kPer + j] = at(base, n) + j < end ? load_logit<BF16>(row, at(base, n) + j) : 0.f;
+      }
+    }
+    fetch(base + kLogprobBuffer);
+    bool found = false;
+#pragma unroll
+    for (int k = 0; k < kVecs * kPer; ++k) {
+      const int i = at(base, k / kPer) + k % kPer;
+      const unsigned long long key = list_key(x[k], i);
+      if (i < end && key > kth) {
+        sm.buffer[atomicAdd(&sm.count, 1)] = key;
+        found = true;
+      }
+    }
+    if (__syncthreads_or(found)) {
+      rebuild_list(sm, sm.count, warp, lane);
+      kth = sm.list[top - 1];
     }
   }
 }
@@ -285,13 +304,7 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
     }
 
     float max = kLogprobStart, sum = 0.f, weighted = 0.f;
-    float bound = kNegInf;  // candidates: values above it, and NaN; a NaN bound takes all
-    bool full = false;
-    int seen = 0;  // batches of this row whose candidates are in the list
-    int next = 1;  // and after how many the list is rebuilt
-    if (threadIdx.x < 32) sm.list[threadIdx.x] = 0ull;
-    if (threadIdx.x == 0) sm.count = 0;
-    __syncthreads();
+    float largest = kNegInf;  // of this thread's values; NaN counts as +inf
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c, ++batch) {
       const int base = (first + c) * kBatch;
@@ -324,46 +337,7 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
 #pragma unroll
       for (int j = 2; j < kValues; j += 2) top = max3_nan(top, x[j], x[j + 1]);
 
-      if (a.top) {
-        if (c == 0) {
-          // the k-th largest of each warp's lane maxima bounds the k-th value
-          // from below (values equal to it count)
-          const float v = sort_lanes(top != top ? INFINITY : top, lane);
-          if (lane == a.top - 1) sm.bounds[warp] = v;
-          __syncthreads();
-          float b = sm.bounds[lane & (kLogprobWarps - 1)];
-#pragma unroll
-          for (int d = 1; d < kLogprobWarps; d <<= 1) b = fmaxf(b, __shfl_xor_sync(0xFFFFFFFFu, b, d));
-          bound = next_below(b);
-        }
-        if (__any_sync(0xFFFFFFFFu, !(top <= bound))) {
-          // which of the values, places for all of the warp's at once, then
-          // one by one (few: read again from where they came)
-          unsigned found = 0;
-#pragma unroll
-          for (int j = 0; j < kValues; ++j) found |= static_cast<unsigned>(!(x[j] <= bound)) << j;
-          if (whole < kBatch) {
-#pragma unroll
-            for (int j = 0; j < kValues; ++j)
-              if (index_of(j) >= left) found &= ~(1u << j);
-          }
-          int at = __popc(found);
-#pragma unroll
-          for (int d = 1; d < 32; d <<= 1) {
-            const int o = __shfl_up_sync(0xFFFFFFFFu, at, d);
-            if (lane >= d) at += o;
-          }
-          const int all = __shfl_sync(0xFFFFFFFFu, at, 31);
-          int start = 0;
-          if (lane == 0) start = atomicAdd(&sm.count, all);
-          at += __shfl_sync(0xFFFFFFFFu, start, 0) - __popc(found);
-          full |= at + __popc(found) > kLogprobSpare;
-          for (; found; found &= found - 1, ++at) {
-            const int i = index_of(__ffs(found) - 1);
-            if (at < kLogprobBuffer) sm.buffer[at] = list_key(value_of(i), base + i);
-          }
-        }
-      }
+      largest = fmaxf(largest, top != top ? INFINITY : top);
       if (a.vec) {
         __syncwarp();  // every lane has read its values
         if (lane == 0) mbar_arrive(&sm.empty[stage_id]);
@@ -427,23 +401,6 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
       sum += lo + hi;
       unpair(w, lo, hi);
       weighted += lo + hi;
-
-      // Look at the buffer every fourth batch; rebuild the list after the
-      // first, the fourth, the sixteenth ...: each time the candidates per
-      // batch get four times fewer.
-      if (a.top && c + 1 < chunks && (c + 1 == next || (c & 3) == 3) && __syncthreads_or(full || c + 1 == next)) {
-        const int count = sm.count;
-        if (count <= kLogprobBuffer) rebuild_list(sm, count, warp, lane);
-        else refill_list<BF16>(sm, row, first + seen, first + c + 1, kBatch, a.vocab, a.top, warp, lane);
-        seen = c + 1;
-        if (seen == next) next *= 4;
-        full = false;
-        // later values equal to the k-th have higher ids; a list that is not
-        // full takes everything, one of NaN nothing but what comes before NaN
-        const unsigned long long kth = sm.list[a.top - 1];
-        bound = key_value(kth);
-        if (bound != bound) bound = kth ? INFINITY : bound;
-      }
     }
 
     // ---- join the threads, then the CTAs of the row
@@ -459,12 +416,48 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
       sm.stat[warp][2] = weighted;
     }
     if (a.top) {
+      // ---- the segment's list
+      float v = sort_lanes(largest, lane);
+      v = merge_warps(v, sm.maxima, warp, lane);
+      if (threadIdx.x < 32) sm.list[threadIdx.x] = 0ull;
+      if (threadIdx.x == a.top - 1) sm.bound = v;
+      if (threadIdx.x == 0) sm.count = sm.held = 0;
       __syncthreads();
+      const float bound = sm.bound;
+      const int begin = first * kBatch, end = min(a.vocab, (first + chunks) * kBatch);
+      if (bound > kNegInf) {
+        if (largest >= bound) sm.holders[atomicAdd(&sm.held, 1)] = threadIdx.x;
+        __syncthreads();
+        const int held = sm.held <= kLogprobHolders ? sm.held : 0;  // more: equal values, nearly everywhere
+        for (int n = warp; n < held; n += kLogprobWarps) {
+          const int of = sm.holders[n];
+          for (int k = lane; k < chunks * VECS; k += 32) {
+            const int i0 = begin + (k * kLogprobThreads + of) * kPer;  // (vectors of a thread: every 256th)
+            float y[kPer];
+            if (a.vec && i0 + kPer <= end) {
+              unpack<BF16>(y, __ldcg(reinterpret_cast<const uint4*>(static_cast<const char*>(row) + static_cast<long long>(i0) * kSize)));
+            } else {
+#pragma unroll
+              for (int j = 0; j < kPer; ++j) y[j] = i0 + j < end ? load_logit<BF16>(row, i0 + j) : kNegInf;
+            }
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+              if (!(y[j] < bound)) {
+                const int at = atomicAdd(&sm.count, 1);
+                if (at < kLogprobBuffer) sm.buffer[at] = list_key(y[j], i0 + j);
+              }
+          }
+        }
+        __syncthreads();
+      }
       const int count = sm.count;
-      if (count > kLogprobBuffer)
-        refill_list<BF16>(sm, row, first + seen, first + chunks, kBatch, a.vocab, a.top, warp, lane);
-      else if (count)
+      if (count && count <= kLogprobBuffer) {
         rebuild_list(sm, count, warp, lane);
+      } else {
+        __syncthreads();
+        if (threadIdx.x == 0) sm.count = 0;
+        list_all<BF16>(sm, row, begin, end, a.top, a.vec, warp, lane);
+      }
     }
     __syncthreads();
     if (warp == 0) {

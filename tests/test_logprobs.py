@@ -129,6 +129,26 @@ def test_sorted_rows(vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("period,equal", [(2048, 300), (1024, 100), (4096, 40), (2048, 2000)])
+def test_equal_values_of_a_stripe_of_columns(dtype, period, equal):
+    """Thousands of equal values at the top, all of them in a few (or most) of
+    the threads that share a row; rows with NaN and +inf among them."""
+    rows, vocab = 600, 40007
+    x, t = logits(period + equal, rows, vocab, dtype)
+    stripe = torch.arange(vocab) % period < equal
+    x[:, stripe] = 64.0
+    x[1, 30000] = math.inf
+    x[2, ::5000] = math.inf
+    x[3, 5000:5010] = math.nan
+    x[4, ~stripe] = -math.inf
+    x[5, stripe] = -math.inf
+    check(x, t, 20)
+    wide = torch.zeros(rows, vocab + 4, dtype=dtype, device="cuda")[:, 1 : vocab + 1]  # not on 16 bytes
+    check(x, t, 32, device_logits=wide.copy_(x))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("softcap", [0.0, 30.0])
 @pytest.mark.parametrize("vocab", [40, 20000, 200000])
 def test_banned_tokens(vocab, softcap):
