@@ -450,7 +450,8 @@ int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const
  *   out_i = sum_j softmax_j(s_ij) v_j, s_ij = scale q_i . k_j, then, with
  *   softcap > 0, softcap * tanh(s_ij / softcap);
  * a row at position p sees the positions j <= p, with window > 0 only those
- * with p - j < window. A row that sees nothing is zero. q and out: BF16
+ * with p - j < window. A row that sees nothing is zero; rows that belong to no
+ * sequence (query_start skips them) are left as they are. q and out: BF16
  * [tokens][q_heads][head_dim] with token and head strides; query head h uses
  * KV head h / (q_heads / kv_heads). max_query: the largest number of rows of a
  * sequence. The first SE12_COUNTER_BYTES of the workspace (16-byte aligned)
@@ -467,7 +468,7 @@ typedef struct se12_kv_attend_args {
 } se12_kv_attend_args;
 
 /* Enough for any call on the cache; enough for calls of these sizes (a third
- * for up to 16 query rows per KV head). */
+ * for up to 16 query rows per KV head, 32 for head dimensions up to 128). */
 size_t se12_kv_attend_workspace_bytes(const se12_kv_cache* cache);
 size_t se12_kv_attend_call_bytes(const se12_kv_cache* cache, int q_heads, int max_query);
 int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_attend_args* args,

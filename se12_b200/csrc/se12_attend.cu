@@ -748,9 +748,16 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
 
 // ------------------------------------------------------------------ launch
 
-// More than 16 query rows per KV head go to attend_tile_kernel.
-bool kv_attend_takes_tiles(int max_query, int group) {
-  return static_cast<long long>(max_query) * group > kAttendSlotRows;
+// This file's kernel reads the codes again for every 16 query rows of a
+// sequence, attend_tile_kernel for every 128, at a cost that hardly depends on
+// how many of them there are. Of 24 sequences of 2040 tokens, 8 KV heads of 128
+// (e4m3), this kernel and that one took 66 and 76 us at 24 rows per KV head, 69
+// and 76 at 32, 96 and 78 at 48, 119 and 78 at 64 (int8, capped: 74 and 98, 76
+// and 98, 106 and 100, 133 and 101); of heads of 256 (int8, capped) 135 and 121
+// at 24, 141 and 120 at 32. (Pages of 16 and 64 tokens alike. Heads of 64 at 32
+// rows: 70 and 73, but 84 and 76 for 4 sequences of 16000.)
+bool kv_attend_takes_tiles(int max_query, int group, int dim) {
+  return static_cast<long long>(max_query) * group > (dim <= 128 ? 32 : 16);
 }
 
 size_t kv_attend_partial_bytes(int sm_count, bool tile) {
@@ -780,7 +787,7 @@ cudaError_t launch_attend_kind(const CUtensorMap& kmap, const CUtensorMap& vmap,
 
 cudaError_t launch_kv_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int max_query,
                              int sm_count, cudaStream_t stream) {
-  if (kv_attend_takes_tiles(max_query, a.group)) return launch_attend_tile(a, sm_count, stream);
+  if (kv_attend_takes_tiles(max_query, a.group, a.c.dim)) return launch_attend_tile(a, sm_count, stream);
   return a.c.kind == kKvInt8 ? launch_attend_kind<kKvInt8>(kmap, vmap, a, max_query, sm_count, stream)
                              : launch_attend_kind<kKvE4m3>(kmap, vmap, a, max_query, sm_count, stream);
 }

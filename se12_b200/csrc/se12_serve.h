@@ -93,7 +93,7 @@ cudaError_t launch_kv_decode(const KvView& c, const int32_t* pages, int count, u
 cudaError_t launch_kv_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int max_query,
                              int sm_count, cudaStream_t stream);
 size_t kv_attend_partial_bytes(int sm_count, bool tile);
-bool kv_attend_takes_tiles(int max_query, int group);
+bool kv_attend_takes_tiles(int max_query, int group, int dim);
 cudaError_t launch_attend_tile(const AttendArgs& a, int sm_count, cudaStream_t stream);
 size_t kv_attend_tile_partial_bytes(int sm_count);
 cudaError_t launch_token_logprobs(bool bf16, LogprobArgs a, int sm_count, cudaStream_t stream);

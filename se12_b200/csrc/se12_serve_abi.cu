@@ -157,7 +157,7 @@ size_t se12_kv_attend_workspace_bytes(const se12_kv_cache* c) {
 
 size_t se12_kv_attend_call_bytes(const se12_kv_cache* c, int q_heads, int max_query) {
   if (!c || q_heads < 1 || max_query < 1) return 0;
-  const bool tiles = se12::kv_attend_takes_tiles(max_query, std::max(q_heads / c->view.heads, 1));
+  const bool tiles = se12::kv_attend_takes_tiles(max_query, std::max(q_heads / c->view.heads, 1), c->view.dim);
   return SE12_COUNTER_BYTES + se12::kv_attend_partial_bytes(c->sm_count, tiles);
 }
 

@@ -255,7 +255,8 @@ class PagedKvCache:
         position p sees positions up to p, with ``window`` only the last
         ``window`` of them. Logits are ``scale`` (default head_dim ** -0.5) q . k,
         with ``softcap`` > 0 then softcap * tanh(logit / softcap). Rows that
-        see nothing are zero. ``max_query``: the most rows of one sequence
+        see nothing are zero; rows of ``out`` that ``query_start`` gives to no
+        sequence are left as they are. ``max_query``: the most rows of one sequence
         (default: all tokens; tells the launch how many rows share a page).
         Returns BF16 like q."""
         q_strides = self._row_strides(q, "q", None, None, _BF16)
