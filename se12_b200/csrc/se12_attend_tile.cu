@@ -31,8 +31,8 @@
 // of instructions per logit; the sum l comes from the weights, by a factor per
 // 16 tokens. Other tiles take the slow way, eight tokens at a time.
 //
-// The work list (sequences, KV heads, row tiles, KV tiles) is cut into equal
-// runs, one per CTA, and a tile's CTAs are joined as in attend_rows_kernel.
+// The work list (sequences, KV heads, row tiles, KV tiles) is cut into runs of
+// equal cost, one per CTA, and a tile's CTAs are joined as in attend_rows_kernel.
 #include "se12_device.cuh"
 #include "se12_serve.h"
 
@@ -51,6 +51,11 @@ constexpr int kTileSoftmaxRegs = 208, kTileLoaderRegs = 104, kTileIssuerRegs = 8
 static_assert(kTileSoftmaxRegs + 2 * kTileLoaderRegs + kTileIssuerRegs <= 4 * 128, "more registers than the launch has");
 constexpr int kTileKvBytes = 32768;   // an FP16 tile of keys or values
 constexpr int kTileMeta = 4;          // tiles whose block scales are kept
+// What a pair's queries, first loads and output cost, in KV tiles. (24 sequences
+// of 77 to 4093 tokens, 2 to 6 new ones of 8 rows: uncounted 105 us, the SMs
+// active 63 % of the time; 2, 3, 4 and 6: 76, 78, 78 and 79 us. 3 sequences of
+// 2014 to 8655 tokens, 78 new ones, 256 dimensions: 70 us; 68, 63, 63 and 63.)
+constexpr int kTilePairCost = 3;
 constexpr int kTileSlotFloats = kTileAttendRows * (256 + 4);
 
 // ------------------------------------------------------------------ tensor memory and tcgen05
@@ -270,6 +275,34 @@ __device__ __forceinline__ void tile_next_pair(const AttendArgs& a, const int* b
   at->s = tile_span<TT>(a, at->w, at->tile);
 }
 
+// Where the run begins whose first unit is t, when every pair counts `cost`
+// units before its KV tiles: the first entry at or past it.
+template <int TT>
+__device__ __forceinline__ int tile_boundary(const AttendArgs& a, const int* before, const int* pairs, long long t, int cost) {
+  const int heads = a.c.heads;
+  auto units = [&](int b) { return (before[b] + static_cast<long long>(cost) * pairs[b]) * heads; };
+  if (t >= units(a.t.seqs)) return before[a.t.seqs] * heads;
+  int lo = 0, hi = a.t.seqs - 1;  // last b with units(b) <= t
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (units(mid) <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  const TileSeq w = tile_sequence(a, lo);
+  const int each = before[lo + 1] - before[lo];
+  const long long each_units = each + static_cast<long long>(cost) * w.tiles;
+  long long x = t - units(lo);
+  const int head = static_cast<int>(x / each_units);
+  x -= head * each_units;
+  int g = before[lo] * heads + head * each;
+  for (int tile = 0;; ++tile) {
+    const int chunks = tile_span<TT>(a, w, tile).chunks;
+    if (x < cost + chunks || tile + 1 == w.tiles) return g + static_cast<int>(max(x - cost, 0ll));
+    x -= cost + chunks;
+    g += chunks;
+  }
+}
+
 struct TileSmem {
   float meta[kTileMeta][8][2];        // [16 tokens of the tile][scale of keys, log2 of values' scale]
   int meta_missing[kTileMeta];        // bit g: those tokens' page is not there
@@ -286,7 +319,8 @@ struct TileSmem {
   uint64_t q_full[2], q_free, o_free;
   uint64_t meta_full[kTileMeta];
   uint32_t tmem;
-  int before[1];  // [seqs + 1] KV tiles of the sequences before, per KV head
+  int bounds[2];  // of this CTA's run
+  int before[1];  // [seqs + 1] KV tiles of the sequences before, per KV head; then as many counts of row tiles
 };
 
 template <int KIND, int DP>
@@ -537,36 +571,44 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
 
   // ---- the work list
   const int heads = a.c.heads;
+  int* pairs = sm.before + a.t.seqs + 1;
   for (int b = threadIdx.x; b < a.t.seqs; b += kTileAttendThreads) {
     const TileSeq w = tile_sequence(a, b);
     int n = 0;
     for (int t = 0; t < w.tiles; ++t) n += tile_span<TT>(a, w, t).chunks;
     sm.before[b + 1] = n;
+    pairs[b + 1] = w.tiles;
   }
-  if (threadIdx.x == 0) sm.before[0] = 0;
+  if (threadIdx.x == 0) sm.before[0] = pairs[0] = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 0) {
+  if (warp < 2) {
+    int* sums = warp == 0 ? sm.before : pairs;
     int carry = 0;
     for (int i = 1; i <= a.t.seqs; i += 32) {
-      int v = i + lane <= a.t.seqs ? sm.before[i + lane] : 0;
+      int v = i + lane <= a.t.seqs ? sums[i + lane] : 0;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
         if (lane >= d) v += u;
       }
       v += carry;
-      if (i + lane <= a.t.seqs) sm.before[i + lane] = v;
+      if (i + lane <= a.t.seqs) sums[i + lane] = v;
       carry = __shfl_sync(0xFFFFFFFFu, v, 31);
     }
   }
   __syncthreads();
   constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: they begin at 0
   const int total = sm.before[a.t.seqs] * heads;
-  const int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-  const int g0 = static_cast<int>(min(static_cast<long long>(blockIdx.x) * per, static_cast<long long>(total)));
-  const int g1 = min(g0 + per, total);
+  // Runs are equal in units, a pair's beginning counting as `cost` KV tiles
+  // (fewer when a run is short: they would leave CTAs without work).
+  const int cost = min(kTilePairCost, total / (4 * static_cast<int>(gridDim.x)));
+  const long long units = total + static_cast<long long>(cost) * pairs[a.t.seqs] * heads;
+  const long long per = (units + gridDim.x - 1) / gridDim.x;
+  if (lane == 0 && warp < 2) sm.bounds[warp] = tile_boundary<TT>(a, sm.before, pairs, (blockIdx.x + warp) * per, cost);
+  __syncthreads();
+  const int g0 = sm.bounds[0], g1 = sm.bounds[1];
 
   // ---- each role walks the CTA's run pair by pair
   TilePlace at;
@@ -892,7 +934,9 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       }
       // ---- the row's sums
       const int pair_start = g - at.chunk, pair_end = pair_start + at.s.chunks;
-      const int cta_first = pair_start / per, cta_last = (pair_end - 1) / per;
+      const long long cost_before = static_cast<long long>(cost) * (pairs[at.b] * heads + at.head * at.w.tiles + at.tile);
+      const int cta_first = static_cast<int>((pair_start + cost_before + cost) / per),
+                cta_last = static_cast<int>((pair_end - 1 + cost_before + cost) / per);
       const bool whole = cta_first == cta_last;
       float* part_out = a.partials + (static_cast<size_t>(blockIdx.x) * 2 + (pair_start > g0 ? 1 : 0)) * kTileSlotFloats;
       const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
@@ -942,7 +986,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
           auto& join = sm.join[sm.joins++];
           join.cta_first = cta_first;
           join.parts = cta_last - cta_first + 1;
-          join.first_slot = pair_start > cta_first * per ? 1 : 0;
+          join.first_slot = pair_start + cost_before > cta_first * per ? 1 : 0;
           join.b = at.b;
           join.head = at.head;
           join.row0 = row0;
@@ -1013,7 +1057,7 @@ size_t kv_attend_tile_partial_bytes(int sm_count) { return static_cast<size_t>(s
 
 template <int KIND, int DP>
 cudaError_t launch_attend_tile_as(const AttendArgs& a, int sm_count, cudaStream_t stream) {
-  const size_t smem = TileShape<KIND, DP>::kSmem + a.t.seqs * sizeof(int);
+  const size_t smem = TileShape<KIND, DP>::kSmem + (2 * a.t.seqs + 1) * sizeof(int);
   return launch_overlapped(attend_tile_kernel<KIND, DP>, dim3(sm_count), kTileAttendThreads, smem, stream, a);
 }
 
