@@ -10,7 +10,7 @@
 // 2^-16 of its largest).
 //
 // Work is the list of all (sequence, KV head, row tile, chunk of tokens), a
-// chunk being 8 KB of keys and values, cut into equal runs, one per CTA; the
+// chunk being 8 KB of keys and values, cut into runs of equal cost, one per CTA; the
 // list comes from the lengths in device memory, so that the launch does not
 // depend on them (a captured graph follows the lengths) and a ragged batch
 // is balanced to a chunk. A CTA's 4 warps take its chunks in turn, each with
@@ -54,6 +54,11 @@ constexpr int kAttendDeposit = 8192;     // joining the warps' sums
 constexpr int kAttendSlotRows = 16;
 constexpr int kAttendSlotFloats = kAttendSlotRows * (256 + 4);  // sums, then (m, l, mp) per row
 constexpr int kAttendMaxCtas = 3;        // per SM
+// What a pair's queries, joins and output cost, in chunks. (64 sequences of 1000
+// to 16384 tokens, 8 KV heads of 128, e4m3: uncounted 196 us; 4, 8 and 16: 188,
+// 183 and 185. 16 of 301 to 8191, window 4096, 8 heads of 256: 57 us; 52, 51 and
+// 50. 7 of 86 to 702 tokens: 24 us; 17, 16 and 16. Equal lengths gain little.)
+constexpr int kAttendPairCost = 8;
 constexpr float kAttendStart = -1.0e30f; // both references before the first token
 constexpr float kAttendRaise = 8.f;      // weights up to 2^8 of the reference
 constexpr float kAttendRaiseSum = 30.f;
@@ -134,11 +139,13 @@ __device__ __forceinline__ SeqWork sequence_work(const AttendArgs& a, int b) {
 }
 
 // A place in the work list: chunk `chunk` of pair `pair` (KV head x row
-// tile) of sequence b, whose pairs start at `base`.
+// tile) of sequence b. The list counts units: a pair's are kAttendPairCost for
+// its beginning and end, from `start` on, and one per chunk.
 struct Place {
   int b, pair, chunk;
-  int base;
+  int start;
   SeqWork w;
+  __device__ __forceinline__ int unit() const { return start + kAttendPairCost + chunk; }
 };
 
 template <int KIND, int DP, int NT>
@@ -164,7 +171,7 @@ struct AttendSmem {
   uint64_t full[kAttendWarps][kAttendStages];
   int last;
   int most;                               // chunks of the longest pair
-  int before[1];  // [seqs + 1] chunks x tiles of the sequences before (per KV head)
+  int before[1];  // [seqs + 1] units of the sequences before (per KV head)
 };
 
 template <int KIND, int DP, int NT, int CTAS>
@@ -197,7 +204,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
   int most = 0;
   for (int b = threadIdx.x; b < a.t.seqs; b += kAttendThreads) {
     const SeqWork w = sequence_work<CHUNK, ROWS>(a, b);
-    sm.before[b + 1] = w.chunks * w.tiles;
+    sm.before[b + 1] = (w.chunks + kAttendPairCost) * w.tiles;
     most = max(most, w.chunks);
   }
   atomicMax(&sm.most, most);
@@ -220,47 +227,53 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
   const int total = sm.before[a.t.seqs] * heads;
   // short pairs are not cut below a chunk per warp
   const int per = max(min(kAttendWarps, sm.most), (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-  const int g0 = static_cast<int>(min(static_cast<long long>(blockIdx.x) * per, static_cast<long long>(total)));
-  const int g1 = min(g0 + per, total);
-  if (g0 >= g1) return;
+  const int u0 = static_cast<int>(min(static_cast<long long>(blockIdx.x) * per, static_cast<long long>(total)));
+  const int u1 = min(u0 + per, total);
+  if (u0 >= u1) return;
 
-  auto locate = [&](int g) {
-    int lo = 0, hi = a.t.seqs - 1;  // last b with before[b] * heads <= g
+  // The first chunk at or past a unit of the list.
+  auto locate = [&](int u) {
+    int lo = 0, hi = a.t.seqs - 1;  // last b with before[b] * heads <= u
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (static_cast<long long>(sm.before[mid]) * heads <= g) lo = mid;
+      if (static_cast<long long>(sm.before[mid]) * heads <= u) lo = mid;
       else hi = mid - 1;
     }
     Place p;
     p.b = lo;
-    p.base = sm.before[lo] * heads;
     p.w = sequence_work<CHUNK, ROWS>(a, lo);
-    p.pair = (g - p.base) / p.w.chunks;
-    p.chunk = (g - p.base) - p.pair * p.w.chunks;
+    const int x = u - sm.before[lo] * heads, each = p.w.chunks + kAttendPairCost;
+    p.pair = x / each;
+    const int at = x - p.pair * each;
+    p.start = u - at;
+    p.chunk = max(at - kAttendPairCost, 0);
     return p;
   };
-  auto advance = [&](Place& p, int by) {  // to the place `by` chunks on (before total)
+  // To the place `by` chunks on; false where that is past this CTA's run.
+  auto advance = [&](Place& p, int by) {
     p.chunk += by;
     while (p.chunk >= p.w.chunks) {
       p.chunk -= p.w.chunks;
+      p.start += p.w.chunks + kAttendPairCost;
+      if (p.start + kAttendPairCost >= u1) return false;
       if (++p.pair == p.w.tiles * heads) {
         p.pair = 0;
         do {
           ++p.b;
         } while (sm.before[p.b + 1] == sm.before[p.b]);
-        p.base = sm.before[p.b] * heads;
         // (chunks left over continue in the next sequence)
         p.w = sequence_work<CHUNK, ROWS>(a, p.b);
       }
     }
+    return p.unit() < u1;
   };
 
-  // ---- this warp's pipeline: chunks g0 + warp, + 8, ...
+  // ---- this warp's pipeline: every fourth chunk of the run
   unsigned char* pipe = pipes + warp * (kAttendStages * kAttendStageBytes);
   const uint32_t pipe_addr = smem_addr(pipe);
   const uint64_t policy = policy_evict_first();
-  Place next{};
-  int next_g = g0 + warp;
+  Place next = locate(u0);
+  bool more = advance(next, warp);  // `next` is a chunk of the run
   int next_page = -1;  // this lane's (lane < SUBS) page for the next chunk to issue
   auto fetch_page = [&]() {
     next_page = -1;
@@ -303,28 +316,23 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
         tma_load_2d(dst + kAttendStageBytes / 2 + hb * kAttendBox, &vmap, hb * 128, row, bar, policy);
       }
     }
-    next_g += kAttendWarps;
-    if (next_g < g1) {
-      advance(next, kAttendWarps);
-      fetch_page();
-    }
+    more = advance(next, kAttendWarps);
+    if (more) fetch_page();
   };
-  if (next_g < g1) {
-    next = locate(next_g);
-    fetch_page();
-  }
+  if (more) fetch_page();
 #pragma unroll
   for (int s = 0; s < kAttendStages; ++s)
-    if (next_g < g1) issue(s);
+    if (more) issue(s);
 
   int stage = 0;
   uint32_t phase = 0;
   bool dead = false;  // a wait ran out: skip the rest (status raised)
 
   // ---- the pairs of this CTA's run
-  Place at = locate(g0);
-  for (int g = g0; g < g1;) {
-    const int run = min(at.w.chunks - at.chunk, g1 - g);  // chunks of this pair here
+  Place at = locate(u0);
+  int done = 0;  // chunks of the run before this pair
+  for (bool here = advance(at, 0); here;) {
+    const int run = min(at.w.chunks - at.chunk, u1 - at.unit());  // chunks of this pair here
     const int head = at.pair / at.w.tiles, tile = at.pair % at.w.tiles;
     const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
     const int rows_all = at.w.tokens * a.group;
@@ -414,8 +422,8 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
 #pragma unroll
             for (int k = 0; k < 4; ++k) acc[hb][w][h][n][k] = 0.f;
 
-    // this warp's first chunk of the pair: the run's chunks are g .. g + run - 1
-    int mine = (warp - (g - g0)) & (kAttendWarps - 1);
+    // this warp's first chunk of the pair
+    int mine = (warp - done) & (kAttendWarps - 1);
     for (; mine < run; mine += kAttendWarps) {
       if (!dead) dead = !__all_sync(0xFFFFFFFFu, mbar_wait(&sm.full[warp][stage], phase));
       if (dead) break;
@@ -582,7 +590,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
         }
       }
       __syncwarp();  // every lane has read the stage
-      if (next_g < g1) issue(stage);
+      if (more) issue(stage);
       if (++stage == kAttendStages) {
         stage = 0;
         phase ^= 1;
@@ -607,11 +615,10 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
         }
       }
     __syncthreads();
-    const int pair_start = g - at.chunk;  // work-list places of this pair
-    const int pair_end = pair_start + at.w.chunks;
-    const int cta_first = pair_start / per, cta_last = (pair_end - 1) / per;
+    const int first_unit = at.start + kAttendPairCost;  // of the pair's chunks
+    const int cta_first = first_unit / per, cta_last = (first_unit + at.w.chunks - 1) / per;
     const bool whole = cta_first == cta_last;
-    const int slot = pair_start > g0 ? 1 : 0;
+    const int slot = at.start > u0 ? 1 : 0;
     float* part = a.partials + (static_cast<size_t>(blockIdx.x) * 2 + slot) * kAttendSlotFloats;
     if (threadIdx.x < rows) {
       const int row = threadIdx.x;
@@ -700,7 +707,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
       if (sm.last) {
         __threadfence();
         const int parts = cta_last - cta_first + 1;
-        const float* first = a.partials + (static_cast<size_t>(cta_first) * 2 + (pair_start > cta_first * per ? 1 : 0)) * kAttendSlotFloats;
+        const float* first = a.partials + (static_cast<size_t>(cta_first) * 2 + (at.start > cta_first * per ? 1 : 0)) * kAttendSlotFloats;
         const float* rest = a.partials + static_cast<size_t>(cta_first) * 2 * kAttendSlotFloats;  // + 2 slots per CTA
         auto part_of = [&](int i) { return i == 0 ? first : rest + static_cast<size_t>(i) * 2 * kAttendSlotFloats; };
         if (threadIdx.x < rows) {
@@ -741,8 +748,8 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
       }
       __syncthreads();
     }
-    g += run;
-    if (g < g1) advance(at, run);
+    done += run;
+    here = advance(at, run);
   }
 }
 
@@ -750,12 +757,12 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
 
 // This file's kernel reads the codes again for every 16 query rows of a
 // sequence, attend_tile_kernel for every 128, at a cost that hardly depends on
-// how many of them there are. Of 24 sequences of 2040 tokens, 8 KV heads of 128
-// (e4m3), this kernel and that one took 66 and 76 us at 24 rows per KV head, 69
-// and 76 at 32, 96 and 78 at 48, 119 and 78 at 64 (int8, capped: 74 and 98, 76
-// and 98, 106 and 100, 133 and 101); of heads of 256 (int8, capped) 135 and 121
-// at 24, 141 and 120 at 32. (Pages of 16 and 64 tokens alike. Heads of 64 at 32
-// rows: 70 and 73, but 84 and 76 for 4 sequences of 16000.)
+// how many of them there are. This kernel and that one, 8 KV heads of 128, 32
+// rows per KV head (e4m3; int8 with capped logits): one sequence of 1000 tokens
+// 18 and 25 us (18 and 28), 24 of 2040 70 and 72 (78 and 93), 24 of 77 to 4093
+// 72 and 75 (79 and 94), 64 of 100 to 8000 256 and 277 (292 and 334); at worst 16
+// of 1000 to 2000 48 and 47. At 48 rows 24 of 2040 took 96 and 78 us (106 and
+// 100). Heads of 256 (int8, capped), 24 of 2040: 135 and 121 at 24 rows.
 bool kv_attend_takes_tiles(int max_query, int group, int dim) {
   return static_cast<long long>(max_query) * group > (dim <= 128 ? 32 : 16);
 }

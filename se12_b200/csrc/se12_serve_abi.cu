@@ -177,9 +177,9 @@ int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const
     return fail(SE12_ERR_INVALID_ARGUMENT, "scale and softcap must be finite, softcap not negative");
   const int group = p->q_heads / v.heads;
   // the kernel counts its work in 31 bits: chunks of 16 tokens or more, row
-  // tiles of 8 rows or more
+  // tiles of 8 rows or more, and what a pair of both costs besides its chunks
   const double work = static_cast<double>(v.heads) * batch->seqs *
-                      (static_cast<double>(batch->max_pages) * v.page_size / 16 + 2) *
+                      (static_cast<double>(batch->max_pages) * v.page_size / 16 + 32) *
                       (static_cast<double>(p->max_query) * group / 8 + 1);
   if (work > 2.0e9) return fail(SE12_ERR_INVALID_ARGUMENT, "the batch is too large for one call: split it by sequences");
   const size_t need = se12_kv_attend_call_bytes(cache, p->q_heads, p->max_query);
