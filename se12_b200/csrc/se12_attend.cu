@@ -10,10 +10,10 @@
 // 2^-16 of its largest).
 //
 // Work is the list of all (sequence, KV head, row tile, chunk of tokens), a
-// chunk being 8 KB of keys and values, cut into runs of equal cost, one per CTA; the
-// list comes from the lengths in device memory, so that the launch does not
-// depend on them (a captured graph follows the lengths) and a ragged batch
-// is balanced to a chunk. A CTA's 4 warps take its chunks in turn, each with
+// chunk being 8 KB of keys and values, cut into runs of equal cost, one per
+// CTA; the list comes from the lengths in device memory, so that the launch
+// does not depend on them (a captured graph follows the lengths) and a ragged
+// batch is balanced. A CTA's 4 warps take its chunks in turn, each with
 // a TMA pipeline of its own (no CTA-wide barrier inside a pair's chunks) and
 // its own references and sums; a pair's warps are joined in shared memory,
 // its CTAs through global memory by the CTA that finishes last, in CTA order.
