@@ -550,6 +550,30 @@ def check_on_gpu(cache, q, table, lens, counts, got, softcap, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("group,n", [(1, 1), (8, 1), (8, 2), (8, 3), (8, 4), (11, 3), (8, 6)])
+@pytest.mark.parametrize("long", [0, 3000])
+def test_attend_many_short_pairs(dim, group, n, long):
+    """Sequences of no token to a few tiles, alone and around a long one: runs
+    that begin and end anywhere in a pair, or hold no token of it."""
+    g = torch.Generator().manual_seed(dim + group * n)
+    lens = [(i * 37) % 90 for i in range(150)] + [0, n, 700]
+    if long:
+        lens[70] = long
+    counts = [min(1 + i % n, ln) if ln else 1 for i, ln in enumerate(lens)]
+    table, pool = random_tables(g, lens, 16)
+    cache, _, _ = filled(g, pool, 16, 2, dim, "int8", 2.0)
+    q = (torch.randn(sum(counts), 2 * group, dim, generator=g) * 2).to(torch.bfloat16).cuda()
+    start = torch.tensor(starts_of(counts), dtype=torch.int32).cuda()
+    for _ in range(2):
+        got = cache.attend(q, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), query_start=start, max_query=n)
+        check_on_gpu(cache, q, table.cuda(), lens, counts, got, 0.0, 0)
+        for b, ln in enumerate(lens):
+            if ln == 0:
+                assert not got[starts_of(counts)[b] : starts_of(counts)[b + 1]].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind,heads,q_heads,dim,page", [("int8", 4, 32, 128, 16), ("e4m3", 8, 16, 256, 64), ("int8", 2, 24, 192, 32)])
 @pytest.mark.parametrize("softcap,window", [(0.0, 0), (30.0, 700)])
 def test_attend_many_tiles_per_cta(kind, heads, q_heads, dim, page, softcap, window):
