@@ -480,7 +480,8 @@ int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const
 int se12_kv_decode(const se12_kv_cache* cache, const int32_t* pages_dev, int count, uint16_t* k_out, uint16_t* v_out,
                    void* stream);
 
-/* Log probabilities over rows of logits (fp32 or BF16, `ld` elements apart):
+/* Log probabilities over rows of logits (fp32 or BF16, `ld` elements apart; 0:
+ * the same row every time, for several tokens):
  * logprob[i] of token tokens[i] (a negative id: none, NaN), the entropy of the
  * row's distribution, and the `top` (0 .. SE12_LOGPROBS_MAX_TOP) largest
  * logits' ids and log probabilities, ties to the lowest id. With softcap > 0

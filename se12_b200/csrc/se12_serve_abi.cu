@@ -227,7 +227,8 @@ int se12_token_logprobs(const void* logits, int bf16, int rows, int vocab, int64
                         float softcap, float* logprob, float* entropy, int64_t* top_ids, float* top_logprobs,
                         void* workspace, size_t workspace_bytes, void* stream) {
   if (!logits || !tokens || !logprob || !entropy) return fail(SE12_ERR_INVALID_ARGUMENT, "null argument");
-  if (rows < 1 || vocab < 1 || ld < vocab) return fail(SE12_ERR_INVALID_ARGUMENT, "rows and vocab must be positive, ld >= vocab");
+  if (rows < 1 || vocab < 1 || (ld < vocab && ld != 0))
+    return fail(SE12_ERR_INVALID_ARGUMENT, "rows and vocab must be positive, ld 0 or at least vocab");
   if (top < 0 || top > SE12_LOGPROBS_MAX_TOP || top > vocab)
     return fail(SE12_ERR_INVALID_ARGUMENT, "top must be in 0.." + std::to_string(SE12_LOGPROBS_MAX_TOP) + " and at most vocab");
   if (top && (!top_ids || !top_logprobs)) return fail(SE12_ERR_INVALID_ARGUMENT, "null top outputs");

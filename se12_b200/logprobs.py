@@ -31,8 +31,8 @@ class TokenLogprobs(typing.NamedTuple):
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, softcap: float = 0.0) -> TokenLogprobs:
-    """``logits``: fp32 or BF16 [rows, vocab] (any row stride), ``tokens``:
-    int64 [rows] ids; a negative id asks for none (its log probability is
+    """``logits``: fp32 or BF16 [rows, vocab] (any row stride: an expanded row
+    is read as it is, rows that overlap are copied), ``tokens``: int64 [rows] ids; a negative id asks for none (its log probability is
     NaN), one past the vocabulary is NaN too and sets the device status.
     ``top``: alternatives per row, up to 32. ``softcap`` > 0 caps the logits
     (softcap * tanh(x / softcap)) first, -inf (a banned token) staying -inf."""
@@ -52,6 +52,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
         raise ValueError("logits and tokens must be on one GPU")
     if tokens.stride(0) != 1 and rows > 1:
         tokens = tokens.contiguous()
+    if rows > 1 and 0 < logits.stride(0) < vocab:
+        logits = logits.contiguous()
+    ld = logits.stride(0) if rows > 1 else vocab
     index = device.index
     logprob = torch.empty(rows, dtype=torch.float32, device=device)
     entropy = torch.empty(rows, dtype=torch.float32, device=device)
@@ -62,7 +65,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
         need = lib.se12_token_logprobs_workspace_bytes()
         ws = _workspace(_WORKSPACES, device, torch._C._cuda_getCurrentRawStream(index), need)
         _launch(index, lib.se12_token_logprobs, "se12_token_logprobs", logits.data_ptr(), logits.dtype == torch.bfloat16, rows,
-                vocab, max(logits.stride(0), vocab), tokens.data_ptr(), top, softcap, logprob.data_ptr(), entropy.data_ptr(),
+                vocab, ld, tokens.data_ptr(), top, softcap, logprob.data_ptr(), entropy.data_ptr(),
                 ids.data_ptr(), top_logprobs.data_ptr(), ws, need)
     return TokenLogprobs(logprob, entropy, ids, top_logprobs)
 

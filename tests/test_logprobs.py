@@ -273,3 +273,33 @@ def test_rows_past_31_bits_of_values():
 def test_no_rows():
     got = token_logprobs(torch.zeros(0, 10, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda"), top=3)
     assert got.logprob.shape == (0,) and got.top_ids.shape == (0, 3)
+
+
+def test_abi_takes_one_row_for_several_tokens():
+    """A row stride of zero passes the checks (the next one is the workspace's)."""
+    from se12_b200 import _build, _lib
+
+    _build.build()
+
+    def call(ld):
+        return _lib.load().se12_token_logprobs(256, 0, 2, 10, ld, 256, 2, 0.0, 256, 256, 256, 256, None, 0, None)
+
+    assert call(0) == 4 and call(-10) == 1 and call(9) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [1, 33, 5000, 70000])
+def test_expanded_and_overlapping_rows(dtype, vocab):
+    """Several candidates against one expanded row, rows that overlap, one row
+    of any stride: as for a copy of them."""
+    x, t = logits(16, 5, vocab + 8, dtype)
+    t = t % vocab
+    row = x[1:2, :vocab]
+    check(row.expand(5, -1), t, min(4, vocab), device_logits=x.cuda()[1:2, :vocab].expand(5, -1))
+    flat = x.reshape(-1)[: vocab + 8]
+    for step in (1, 2):
+        view = flat.cuda().as_strided((5, vocab), (step, 1))
+        check(flat.as_strided((5, vocab), (step, 1)), t, min(4, vocab), device_logits=view)
+    check(row, t[:1], min(4, vocab), device_logits=x.cuda()[1:2, :vocab].as_strided((1, vocab), (0, 1), x.shape[1]))
+    check(x[:, :vocab], t, min(4, vocab), device_logits=x.cuda()[:, :vocab])
