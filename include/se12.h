@@ -411,16 +411,16 @@ typedef struct se12_kv_batch {
   int32_t seqs, tokens;
   const int32_t* lens;         /* device [seqs] */
   const int32_t* query_start;  /* device [seqs + 1], or null */
-  const int32_t* block_table;  /* device [seqs][table_stride] */
-  int64_t table_stride;
+  const int32_t* block_table;  /* device: row b at block_table + b * table_stride */
+  int64_t table_stride;        /* rows may overlap; 0: one row for all */
   int32_t max_pages;           /* columns of block_table */
 } se12_kv_batch;
 
 /* Appends the batch's keys and values (fp32 or BF16, rows of head_dim values
  * at k + token * k_token_stride + head * k_head_stride) and, with q, writes
  * the queries, rotated, as BF16. Keys and queries are rotated by their
- * positions: cos and sin are fp32 [rope_rows][rope_stride], rotary_dim / 2
- * columns used; the pair (x1, x2) becomes (x1 cos - x2 sin, x2 cos + x1 sin),
+ * positions: row p of cos and sin is the rotary_dim / 2 fp32 values at
+ * p * rope_stride (rows may overlap); the pair (x1, x2) becomes (x1 cos - x2 sin, x2 cos + x1 sin),
  * pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved. cos null:
  * no rotation. A block's scale is the least power of two, 2^-100 at least,
  * that holds its tokens; when a token raises it, the block's older codes are

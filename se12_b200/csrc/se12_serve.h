@@ -32,7 +32,7 @@ struct KvView {
 struct TokenBatch {
   const int32_t* query_start;  // [seqs + 1], or null: one token per sequence
   const int32_t* lens;         // [seqs] tokens in the cache, the new ones included
-  const int32_t* table;        // [seqs][table_stride] page ids
+  const int32_t* table;        // page ids, row b at table + b * table_stride
   long long table_stride;
   int max_pages;
   int seqs, tokens;
@@ -44,7 +44,7 @@ struct AppendArgs {
   const void *q, *k, *v;  // fp32 or BF16; q may be null
   long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // token and head strides, elements
   int q_heads;
-  const float *cos, *sin;  // [rope_rows][rope_stride], or null: no rotation
+  const float *cos, *sin;  // row p at p * rope_stride, or null: no rotation
   long long rope_stride;
   int rope_rows, rotary;   // rotated dimensions (even, <= dim)
   int interleaved;

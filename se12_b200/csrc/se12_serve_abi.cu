@@ -52,8 +52,8 @@ int check_batch(const se12_kv_cache* cache, const se12_kv_batch* b, se12::TokenB
   if (!b->query_start && b->tokens != b->seqs)
     return fail(SE12_ERR_INVALID_ARGUMENT, "without query_start there is one token per sequence");
   if (!b->lens || !b->block_table) return fail(SE12_ERR_INVALID_ARGUMENT, "null lens or block_table");
-  if (b->max_pages < 1 || b->table_stride < b->max_pages)
-    return fail(SE12_ERR_INVALID_ARGUMENT, "block_table needs a column, and table_stride >= max_pages");
+  if (b->max_pages < 1 || b->table_stride < 0)
+    return fail(SE12_ERR_INVALID_ARGUMENT, "block_table needs a column, and a table_stride that is not negative");
   if (static_cast<long long>(b->max_pages) * cache->view.page_size > INT32_MAX)
     return fail(SE12_ERR_INVALID_ARGUMENT, "positions must fit 31 bits");
   out->query_start = b->query_start;
@@ -125,8 +125,8 @@ int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const
   if (!p->cos != !p->sin) return fail(SE12_ERR_INVALID_ARGUMENT, "cos and sin go together");
   if (p->cos && (p->rotary_dim < 2 || p->rotary_dim % 2 || p->rotary_dim > cache->view.dim))
     return fail(SE12_ERR_INVALID_ARGUMENT, "rotary_dim must be even, in 2..head_dim");
-  if (p->cos && (p->rope_rows < 1 || p->rope_stride < p->rotary_dim / 2))
-    return fail(SE12_ERR_INVALID_ARGUMENT, "the rotation table needs rows of rotary_dim / 2 values");
+  if (p->cos && (p->rope_rows < 1 || p->rope_stride < 0))
+    return fail(SE12_ERR_INVALID_ARGUMENT, "the rotation table needs a row, and a rope_stride that is not negative");
   a.c = cache->view;
   a.q = p->q;
   a.k = p->k;

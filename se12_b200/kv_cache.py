@@ -174,8 +174,7 @@ class PagedKvCache:
             if query_start.shape[0] != seqs + 1:
                 raise ValueError(f"query_start must have {seqs + 1} entries, got {query_start.shape[0]}")
             start = query_start.data_ptr()
-        return _lib.KV_BATCH.pack(seqs, tokens, lens.data_ptr(), start, block_table.data_ptr(), max(stride[0], shape[1]),
-                                  shape[1])
+        return _lib.KV_BATCH.pack(seqs, tokens, lens.data_ptr(), start, block_table.data_ptr(), stride[0], shape[1])
 
     def _refuse_batch(self, block_table, lens) -> None:
         _index(block_table, "block_table", 2, self.device)
@@ -206,7 +205,7 @@ class PagedKvCache:
         ``lens`` [seqs] counts the tokens of each sequence with the new ones,
         which are its last; ``query_start`` [seqs + 1] says where each
         sequence's rows begin (None: one row per sequence). ``block_table``
-        [seqs, columns] holds page ids. A sequence with ``lens`` 0 is a padding
+        [seqs, columns] (any row stride) holds page ids. A sequence with ``lens`` 0 is a padding
         row: nothing is stored, its queries are zeros. ``cos`` and ``sin``
         (fp32 [positions, rotary / 2]) rotate keys and queries by position,
         pairs (i, i + rotary / 2), or (2i, 2i + 1) when ``interleaved``."""
@@ -239,7 +238,7 @@ class PagedKvCache:
                     and 1 <= shape[1] <= self.head_dim // 2 and shape[0] >= 1):
                 raise ValueError(f"cos and sin must be fp32 [positions, 1..{self.head_dim // 2}] tensors on {self.device} with the "
                                  "same shape and strides and unit column stride")
-            turn = (cos.data_ptr(), sin.data_ptr(), max(stride[0], shape[1]), shape[0], 2 * shape[1])
+            turn = (cos.data_ptr(), sin.data_ptr(), stride[0], shape[0], 2 * shape[1])
         elif cos is not None or sin is not None:
             raise ValueError("cos and sin go together")
         args = _lib.KV_APPEND.pack(dtype is torch.bfloat16, q_heads, q_ptr, k.data_ptr(), v.data_ptr(), *q_strides, *k_strides,

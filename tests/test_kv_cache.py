@@ -770,3 +770,51 @@ def test_refusals_on_the_device():
             cache.attend(q, table, lens, **args)
     assert cache.append(x[:0], x[:0], table, lens, q=x[:0]).shape == (0, 2, 64)
     assert cache.attend(q[:0], table, lens).shape == (0, 2, 64)
+
+
+# ------------------------------------------------------------------ expanded and overlapping views
+
+
+@pytest.mark.parametrize("rows,columns,stride", [(3, 5, 0), (3, 5, 2), (1, 5, 0), (3, 1, 0), (4, 2, 7)])
+def test_page_table_strides_reach_the_call(rows, columns, stride):
+    """What a call is told of the table's rows is where they lie."""
+    from se12_b200 import _lib
+    from se12_b200.kv_cache import PagedKvCache
+
+    cache = PagedKvCache.__new__(PagedKvCache)
+    cache.device = torch.device("cpu")
+    table = torch.zeros(64, dtype=torch.int32).as_strided((rows, columns), (stride, 1))
+    packed = _lib.KV_BATCH.unpack(cache._batch(rows, table, torch.ones(rows, dtype=torch.int32), None))
+    assert packed[4:] == (table.data_ptr(), stride, columns)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 3, 40])
+@pytest.mark.parametrize("step", [0, 1])
+def test_expanded_and_overlapping_tables(n, step):
+    """One table row for several sequences (candidates behind one prefix),
+    rows that overlap, a rotation by the same angle everywhere: as copies."""
+    g = torch.Generator().manual_seed(n)
+    page, heads, q_heads, dim, seqs = 16, 2, 8, 128, 3
+    length = 90
+    order = torch.randperm(12, generator=g).to(torch.int32)
+    view = order.cuda().as_strided((seqs, 6), (step, 1))
+    table = order.as_strided((seqs, 6), (step, 1)).contiguous()
+    cache, keys, values = filled(g, 12, page, heads, dim, "int8")
+    lens = torch.tensor([length, length - 5, length - 9], dtype=torch.int32)
+    starts = starts_of([n] * seqs)
+    q = torch.randn(n * seqs, q_heads, dim, generator=g).to(torch.bfloat16)
+    start = torch.tensor(starts, dtype=torch.int32).cuda()
+    got = cache.attend(q.cuda(), view, lens.cuda(), query_start=start, max_query=n)
+    check_attend(got, *plain_attend(q, keys, values, table, lens.tolist(), starts, dim**-0.5, 0.0, 0), length)
+    # append: one sequence, a rotation table whose rows are the same
+    one, plain = make_pair(12, page, heads, dim, "int8")
+    cos, sin = rope(g, 1, dim // 2)
+    y = torch.randn(20, q_heads + 2 * heads, dim, generator=g)
+    k, v, q = y[:, :heads], y[:, heads : 2 * heads], y[:, 2 * heads :]
+    want = plain.append(k, v, table[:1], [20], [0, 20], cos.expand(20, -1), sin.expand(20, -1), False, q)
+    out = one.append(k.cuda(), v.cuda(), view[:1], torch.tensor([20], dtype=torch.int32).cuda(), q=q.cuda(),
+                     query_start=torch.tensor([0, 20], dtype=torch.int32).cuda(), cos=cos.cuda().expand(20, -1),
+                     sin=sin.cuda().expand(20, -1))
+    assert torch.equal(out.cpu().view(torch.int16), want.view(torch.int16))
+    same_cache(one, plain)
