@@ -41,9 +41,10 @@ _WORKSPACES = _WorkspacePool()
 
 
 def _workspace(pool: _WorkspacePool, device: torch.device, stream: int, nbytes: int) -> int:
-    """Address of a workspace for this call, its counters zero. While a graph
-    is captured it belongs to the graph (the clearing is captured with it);
-    otherwise it is the stream's, which every call leaves zeroed."""
+    """Address of a workspace for this call, its counters zero; ``device`` is
+    the current one. While a graph is captured it belongs to the graph (the
+    clearing is captured with it); otherwise it is the stream's, which every
+    call leaves zeroed."""
     if torch.cuda.is_current_stream_capturing():
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         buf[:COUNTER_BYTES].zero_()
@@ -51,13 +52,19 @@ def _workspace(pool: _WorkspacePool, device: torch.device, stream: int, nbytes: 
     return pool.get(device, stream, nbytes).data_ptr()
 
 
-def _launch(index: int, function, name: str, *args) -> None:
-    """function(*args, current stream) on GPU ``index``."""
-    if torch._C._cuda_getDevice() == index:
-        status = function(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
+def _launch(device: torch.device, function, name: str, *args, workspace: tuple | None = None) -> None:
+    """function(*args, current stream) on the GPU ``device``; with ``workspace``
+    (pool, bytes) function(*args, workspace, bytes, current stream), the
+    workspace prepared on that GPU too."""
+    index = device.index
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
-            status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+            return _launch(device, function, name, *args, workspace=workspace)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if workspace is not None:
+        pool, nbytes = workspace
+        args += (_workspace(pool, device, stream, nbytes), nbytes)
+    status = function(*args, stream)
     if status:
         _lib.check(status, name)
 
@@ -140,7 +147,6 @@ class PagedKvCache:
         self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.kind = k_codes, v_codes, k_scales, v_scales, kind
         self.pages, self.kv_heads, self.page_size, self.head_dim = k_codes.shape
         self.device = k_codes.device
-        self._index = self.device.index
         s = _lib.Se12KvPagesStruct(self.pages, self.page_size, self.kv_heads, self.head_dim, KINDS[kind], k_codes.data_ptr(),
                                    v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
         handle = ctypes.c_void_p()
@@ -243,7 +249,7 @@ class PagedKvCache:
             raise ValueError("cos and sin go together")
         args = _lib.KV_APPEND.pack(dtype is torch.bfloat16, q_heads, q_ptr, k.data_ptr(), v.data_ptr(), *q_strides, *k_strides,
                                    *v_strides, *turn, bool(interleaved), out_ptr, *out_strides)
-        _launch(self._index, self._lib.se12_kv_append, "se12_kv_append", self._handle, batch, args)
+        _launch(self.device, self._lib.se12_kv_append, "se12_kv_append", self._handle, batch, args)
         return q_out
 
     def attend(self, q: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, query_start: torch.Tensor | None = None,
@@ -276,8 +282,7 @@ class PagedKvCache:
         args = _lib.KV_ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *out_strides, q_heads, max_query, int(window),
                                    self.head_dim ** -0.5 if scale is None else scale, softcap)
         need = self._lib.se12_kv_attend_call_bytes(self._handle, q_heads, max_query)
-        ws = _workspace(_WORKSPACES, self.device, torch._C._cuda_getCurrentRawStream(self._index), need)
-        _launch(self._index, self._lib.se12_kv_attend, "se12_kv_attend", self._handle, batch, args, ws, need)
+        _launch(self.device, self._lib.se12_kv_attend, "se12_kv_attend", self._handle, batch, args, workspace=(_WORKSPACES, need))
         return out
 
     def decode(self, pages: torch.Tensor | None = None) -> tuple:
@@ -288,7 +293,7 @@ class PagedKvCache:
         k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         if count:
-            _launch(self._index, self._lib.se12_kv_decode, "se12_kv_decode", self._handle,
+            _launch(self.device, self._lib.se12_kv_decode, "se12_kv_decode", self._handle,
                     None if pages is None else pages.data_ptr(), count, k.data_ptr(), v.data_ptr())
         return k, v
 

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .device import _WorkspacePool
-from .kv_cache import _launch, _workspace
+from .kv_cache import _launch
 
 MAX_TOP = 32
 
@@ -55,7 +55,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
     if rows > 1 and 0 < logits.stride(0) < vocab:
         logits = logits.contiguous()
     ld = logits.stride(0) if rows > 1 else vocab
-    index = device.index
     logprob = torch.empty(rows, dtype=torch.float32, device=device)
     entropy = torch.empty(rows, dtype=torch.float32, device=device)
     ids = torch.empty(rows, top, dtype=torch.int64, device=device)
@@ -63,10 +62,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
     if rows:
         lib = _lib.load()
         need = lib.se12_token_logprobs_workspace_bytes()
-        ws = _workspace(_WORKSPACES, device, torch._C._cuda_getCurrentRawStream(index), need)
-        _launch(index, lib.se12_token_logprobs, "se12_token_logprobs", logits.data_ptr(), logits.dtype == torch.bfloat16, rows,
+        _launch(device, lib.se12_token_logprobs, "se12_token_logprobs", logits.data_ptr(), logits.dtype == torch.bfloat16, rows,
                 vocab, ld, tokens.data_ptr(), top, softcap, logprob.data_ptr(), entropy.data_ptr(),
-                ids.data_ptr(), top_logprobs.data_ptr(), ws, need)
+                ids.data_ptr(), top_logprobs.data_ptr(), workspace=(_WORKSPACES, need))
     return TokenLogprobs(logprob, entropy, ids, top_logprobs)
 
 

@@ -818,3 +818,59 @@ def test_expanded_and_overlapping_tables(n, step):
                      sin=sin.cuda().expand(20, -1))
     assert torch.equal(out.cpu().view(torch.int16), want.view(torch.int16))
     same_cache(one, plain)
+
+
+# ------------------------------------------------------------------ devices
+
+
+class OtherDevice:
+    """Stands in for torch.cuda.device while another GPU is the current one."""
+
+    inside = False
+
+    def __init__(self, index):
+        pass
+
+    def __enter__(self):
+        OtherDevice.inside = True
+
+    def __exit__(self, *_):
+        OtherDevice.inside = False
+
+
+def test_workspace_is_prepared_on_the_cache_device(monkeypatch):
+    """With another GPU current, everything a call does there (asking whether
+    a graph is captured, clearing the workspace, the launch) is done with the
+    cache's GPU current."""
+    from se12_b200 import kv_cache
+
+    seen = []
+
+    class Library:
+        def se12_kv_attend_call_bytes(self, *_):
+            return 8192
+
+        def se12_kv_attend(self, *_):
+            seen.append(("launch", OtherDevice.inside))
+            return 0
+
+    class Pool:
+        def get(self, device, stream, nbytes):
+            seen.append(("workspace", OtherDevice.inside))
+            return torch.zeros(nbytes, dtype=torch.uint8)
+
+    def capturing():
+        seen.append(("capturing", OtherDevice.inside))
+        return False
+
+    cache = kv_cache.PagedKvCache.__new__(kv_cache.PagedKvCache)
+    cache.device, cache._handle, cache._lib = torch.device("cpu"), None, Library()
+    cache.pages, cache.kv_heads, cache.page_size, cache.head_dim = 2, 1, 16, 64
+    monkeypatch.setattr(kv_cache, "_WORKSPACES", Pool())
+    monkeypatch.setattr(torch.cuda, "device", OtherDevice)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", capturing)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: None if OtherDevice.inside else 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    cache.attend(torch.zeros(1, 2, 64, dtype=torch.bfloat16), ints([[0]]), ints([3]))
+    assert sorted(seen) == [("capturing", True), ("launch", True), ("workspace", True)]

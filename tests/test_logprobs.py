@@ -303,3 +303,38 @@ def test_expanded_and_overlapping_rows(dtype, vocab):
         check(flat.as_strided((5, vocab), (step, 1)), t, min(4, vocab), device_logits=view)
     check(row, t[:1], min(4, vocab), device_logits=x.cuda()[1:2, :vocab].as_strided((1, vocab), (0, 1), x.shape[1]))
     check(x[:, :vocab], t, min(4, vocab), device_logits=x.cuda()[:, :vocab])
+
+
+@pytest.mark.gpu
+def test_workspace_is_prepared_on_the_logits_device(monkeypatch):
+    """With another GPU current (here by what the library is told), the
+    workspace is cleared and the kernel launched with the logits' GPU current."""
+    from se12_b200 import _lib, logprobs
+
+    x, t = logits(17, 2, 5000)
+    dx, dt = x.cuda(), t.cuda()
+    want = token_logprobs(dx, dt, top=3)
+    inside, seen = [], []
+    real_device, real_pool = torch.cuda.device, logprobs._WORKSPACES
+
+    class Device(real_device):
+        def __enter__(self):
+            inside.append(1)
+            return super().__enter__()
+
+        def __exit__(self, *args):
+            inside.pop()
+            return super().__exit__(*args)
+
+    class Pool:
+        def get(self, device, stream, nbytes):
+            seen.append(len(inside))
+            return real_pool.get(device, stream, nbytes)
+
+    monkeypatch.setattr(logprobs, "_WORKSPACES", Pool())
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0 if inside else 1)
+    got = token_logprobs(dx, dt, top=3)
+    assert seen == [1] and _lib.is_loaded()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
