@@ -405,8 +405,10 @@ void se12_kv_cache_destroy(se12_kv_cache* cache);
  * one token per sequence (tokens == seqs). A row at a negative position is
  * inactive (a padding row: lens[b] == 0): nothing is stored for it and its
  * outputs are zero. Position p is slot p % page_size of page
- * block_table[b][p / page_size]; entries past the length are not read.
- * seqs <= SE12_KV_MAX_SEQS. */
+ * block_table[b][p / page_size]; entries past the length are not read. A
+ * length past the table's last column sets the status: attention then goes over
+ * the positions the table has. query_start does not decrease, and what it says
+ * past the batch's rows is cut to them. seqs <= SE12_KV_MAX_SEQS. */
 typedef struct se12_kv_batch {
   int32_t seqs, tokens;
   const int32_t* lens;         /* device [seqs] */

@@ -109,33 +109,35 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// A sequence's part of the work list.
-struct SeqWork {
-  int tokens;   // new tokens
-  int first;    // position of the first one (may be negative: inactive tokens)
-  int length;   // tokens in the cache
-  int low;      // first chunk's first token: a multiple of the chunk, at or below the first visible token
-  int chunks;   // per pair
-  int tiles;    // row tiles
-};
+__device__ __forceinline__ ListSizes list_sizes(const AttendArgs& a) {
+  return {a.t.tokens, a.t.max_pages << a.c.page_shift, a.group, a.window};
+}
+
+// A sequence longer than its page table row: the tokens past it are skipped.
+__device__ __forceinline__ void check_length(const AttendArgs& a, int b) {
+  if (blockIdx.x == 0 && a.t.lens[b] > a.t.max_pages << a.c.page_shift) raise_status(kStatusBadArgument);
+}
 
 template <int CHUNK, int ROWS>
 __device__ __forceinline__ SeqWork sequence_work(const AttendArgs& a, int b) {
-  SeqWork w;
-  if (a.t.query_start) {
-    const int q0 = max(a.t.query_start[b], 0), q1 = min(a.t.query_start[b + 1], a.t.tokens);
-    w.tokens = max(q1 - q0, 0);
-  } else {
-    w.tokens = 1;
+  return sequence_work(a.t.rows_of(b, list_sizes(a)), list_sizes(a), CHUNK, ROWS);
+}
+
+// Sums over the sequences, in place, by one warp: sums[i] of entries 1 .. i,
+// at most `limit`.
+__device__ __forceinline__ void sum_up_to(int* sums, int seqs, int limit, int lane) {
+  int carry = 0;
+  for (int i = 1; i <= seqs; i += 32) {
+    int v = i + lane <= seqs ? sums[i + lane] : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+      if (lane >= d) v = add_work(v, u, limit);
+    }
+    v = add_work(v, carry, limit);
+    if (i + lane <= seqs) sums[i + lane] = v;
+    carry = __shfl_sync(0xFFFFFFFFu, v, 31);
   }
-  w.length = max(a.t.lens[b], 0);
-  w.first = w.length - w.tokens;
-  const int visible = a.window ? max(w.first - a.window + 1, 0) : 0;
-  w.low = visible / CHUNK * CHUNK;
-  // an empty sequence keeps one chunk, whose CTA writes its rows' zeros
-  w.chunks = max((w.length - w.low + CHUNK - 1) / CHUNK, 1);
-  w.tiles = (w.tokens * a.group + ROWS - 1) / ROWS;
-  return w;
 }
 
 // A place in the work list: chunk `chunk` of pair `pair` (KV head x row
@@ -201,29 +203,22 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
   const int heads = a.c.heads;
   if (threadIdx.x == 0) sm.before[0] = sm.most = 0;
   __syncthreads();
+  const int limit = static_cast<int>(kWorkLimit / heads);
   int most = 0;
   for (int b = threadIdx.x; b < a.t.seqs; b += kAttendThreads) {
     const SeqWork w = sequence_work<CHUNK, ROWS>(a, b);
-    sm.before[b + 1] = (w.chunks + kAttendPairCost) * w.tiles;
+    check_length(a, b);
+    sm.before[b + 1] = times_work(w.chunks + kAttendPairCost, w.tiles, limit);
     most = max(most, w.chunks);
   }
   atomicMax(&sm.most, most);
   __syncthreads();
-  if (warp == 0) {
-    int carry = 0;
-    for (int i = 1; i <= a.t.seqs; i += 32) {
-      int v = i + lane <= a.t.seqs ? sm.before[i + lane] : 0;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
-        if (lane >= d) v += u;
-      }
-      v += carry;
-      if (i + lane <= a.t.seqs) sm.before[i + lane] = v;
-      carry = __shfl_sync(0xFFFFFFFFu, v, 31);
-    }
-  }
+  if (warp == 0) sum_up_to(sm.before, a.t.seqs, limit, lane);
   __syncthreads();
+  if (sm.before[a.t.seqs] == limit) {
+    if (threadIdx.x == 0) raise_status(kStatusBadArgument);
+    return;
+  }
   const int total = sm.before[a.t.seqs] * heads;
   // short pairs are not cut below a chunk per warp
   const int per = max(min(kAttendWarps, sm.most), (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
@@ -279,8 +274,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
     next_page = -1;
     if (lane < SUBS) {
       const int t0 = next.w.low + next.chunk * CHUNK + lane * 16;
-      const int visible = a.window ? next.w.first - a.window + 1 : 0;
-      if (t0 < next.w.length && t0 + 16 > visible) {
+      if (t0 < next.w.s.length && t0 + 16 > visible_from(next.w.s.first, a.window)) {
         const int i = t0 >> a.c.page_shift;
         next_page = i < a.t.max_pages ? a.t.table[next.b * a.t.table_stride + i] : -1;
         if (next_page < 0 || next_page >= a.c.pages) {
@@ -334,8 +328,8 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
   for (bool here = advance(at, 0); here;) {
     const int run = min(at.w.chunks - at.chunk, u1 - at.unit());  // chunks of this pair here
     const int head = at.pair / at.w.tiles, tile = at.pair % at.w.tiles;
-    const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
-    const int rows_all = at.w.tokens * a.group;
+    const int token0 = a.t.begin_of(at.b, list_sizes(a));
+    const int rows_all = at.w.s.tokens * a.group;
 
     // queries as the second operand's fragments: lane (r, c) of an n-tile
     // needs, of row r, the dimensions 128 hb + 32 c .. + 31 in byte order. A
@@ -397,10 +391,10 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
       for (int k = 0; k < 2; ++k) {
         const int row = n * 8 + 2 * c + k;
         row_scale[n][k] = sm.row_scale[row] * (a.softcap != 0.f ? 2.f * kLog2e / a.softcap : kLog2e);
-        row_pos[n][k] = at.w.first + min(tile * ROWS + row, rows_all - 1) / a.group;
+        row_pos[n][k] = at.w.s.first + min(tile * ROWS + row, rows_all - 1) / a.group;
       }
-    const int pos_min = at.w.first + min(tile * ROWS, rows_all - 1) / a.group;
-    const int pos_max = at.w.first + min(tile * ROWS + ROWS - 1, rows_all - 1) / a.group;
+    const int pos_min = at.w.s.first + min(tile * ROWS, rows_all - 1) / a.group;
+    const int pos_max = at.w.s.first + min(tile * ROWS + ROWS - 1, rows_all - 1) / a.group;
 
     float m[NT][2], l[NT][2], mp[NT][2];
     float acc[HB][4][2][NT][4];
@@ -562,7 +556,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
         // of tokens 2c, 2c + 1, 2c + 8, 2c + 9
         const uint32_t vbase = base + kAttendStageBytes / 2 + sub * HB * kAttendBox + 2 * c * 128;
         const int ts = t0 + sub * 16;
-        const bool clip = ts + 16 > at.w.length;  // codes past the sequence may be anything
+        const bool clip = ts + 16 > at.w.s.length;  // codes past the sequence may be anything
 #pragma unroll
         for (int hb = 0; hb < HB; ++hb) {
           uint4 v[4];
@@ -572,7 +566,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
           if (clip) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (ts + 2 * c + (i & 1) + (i >> 1) * 8 >= at.w.length) v[i] = make_uint4(0, 0, 0, 0);
+              if (ts + 2 * c + (i & 1) + (i >> 1) * 8 >= at.w.s.length) v[i] = make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
           for (int w = 0; w < 4; ++w) {

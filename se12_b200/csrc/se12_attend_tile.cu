@@ -195,39 +195,22 @@ __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool transposed_b)
 
 // ------------------------------------------------------------------ work list
 
-// A row tile's part of the work list.
-struct TileSpan {
-  int low;      // first token, a multiple of the KV tile
-  int chunks;   // KV tiles (at least one: its CTA writes the rows)
-  int pos_min, pos_max;
-};
-
 struct TileSeq {
-  int tokens, first, length;
+  SeqRows s;
   int rows, tiles;
 };
 
 __device__ __forceinline__ TileSeq tile_sequence(const AttendArgs& a, int b) {
   TileSeq w;
-  const int q0 = a.t.query_start ? max(a.t.query_start[b], 0) : b;
-  const int q1 = a.t.query_start ? min(a.t.query_start[b + 1], a.t.tokens) : b + 1;
-  w.tokens = max(q1 - q0, 0);
-  w.length = max(a.t.lens[b], 0);
-  w.first = w.length - w.tokens;
-  w.rows = w.tokens * a.group;
+  w.s = a.t.rows_of(b, list_sizes(a));
+  w.rows = w.s.tokens * a.group;
   w.tiles = (w.rows + kTileAttendRows - 1) / kTileAttendRows;
   return w;
 }
 
 template <int TT>
 __device__ __forceinline__ TileSpan tile_span(const AttendArgs& a, const TileSeq& w, int tile) {
-  TileSpan s;
-  s.pos_min = w.first + tile * kTileAttendRows / a.group;
-  s.pos_max = w.first + min(tile * kTileAttendRows + kTileAttendRows - 1, w.rows - 1) / a.group;
-  const int visible = a.window ? max(s.pos_min - a.window + 1, 0) : 0;
-  s.low = visible / TT * TT;
-  s.chunks = max((s.pos_max + 1 - s.low + TT - 1) / TT, 1);
-  return s;
+  return tile_span(w.s, tile, kTileAttendRows, list_sizes(a), TT);
 }
 
 struct TilePlace {
@@ -572,10 +555,12 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
   // ---- the work list
   const int heads = a.c.heads;
   int* pairs = sm.before + a.t.seqs + 1;
+  const int limit = static_cast<int>(kWorkLimit / heads);
   for (int b = threadIdx.x; b < a.t.seqs; b += kTileAttendThreads) {
     const TileSeq w = tile_sequence(a, b);
+    check_length(a, b);
     int n = 0;
-    for (int t = 0; t < w.tiles; ++t) n += tile_span<TT>(a, w, t).chunks;
+    for (int t = 0; t < w.tiles; ++t) n = add_work(n, tile_span<TT>(a, w, t).chunks, limit);
     sm.before[b + 1] = n;
     pairs[b + 1] = w.tiles;
   }
@@ -583,21 +568,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp < 2) {
-    int* sums = warp == 0 ? sm.before : pairs;
-    int carry = 0;
-    for (int i = 1; i <= a.t.seqs; i += 32) {
-      int v = i + lane <= a.t.seqs ? sums[i + lane] : 0;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
-        if (lane >= d) v += u;
-      }
-      v += carry;
-      if (i + lane <= a.t.seqs) sums[i + lane] = v;
-      carry = __shfl_sync(0xFFFFFFFFu, v, 31);
-    }
-  }
+  if (warp < 2) sum_up_to(warp == 0 ? sm.before : pairs, a.t.seqs, limit, lane);
   __syncthreads();
   constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: they begin at 0
   const int total = sm.before[a.t.seqs] * heads;
@@ -606,7 +577,10 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
   const int cost = min(kTilePairCost, total / (4 * static_cast<int>(gridDim.x)));
   const long long units = total + static_cast<long long>(cost) * pairs[a.t.seqs] * heads;
   const long long per = (units + gridDim.x - 1) / gridDim.x;
-  if (lane == 0 && warp < 2) sm.bounds[warp] = tile_boundary<TT>(a, sm.before, pairs, (blockIdx.x + warp) * per, cost);
+  const bool fits = sm.before[a.t.seqs] < limit;
+  if (!fits && threadIdx.x == 0) raise_status(kStatusBadArgument);
+  if (lane == 0 && warp < 2)
+    sm.bounds[warp] = fits ? tile_boundary<TT>(a, sm.before, pairs, (blockIdx.x + warp) * per, cost) : 0;
   __syncthreads();
   const int g0 = sm.bounds[0], g1 = sm.bounds[1];
 
@@ -682,7 +656,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
         const int run = min(at.s.chunks - at.chunk, g1 - g);
         // the pair before has been multiplied
         if (pair > 0) wait(&sm.q_free, (pair - 1) & 1);
-        const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
+        const int token0 = a.t.begin_of(at.b, list_sizes(a));
         const int rows_left = at.w.rows - at.tile * kTileAttendRows;
         auto load_row = [&](uint4 (&r)[kVectors], int q_row) {
           const int all = at.tile * kTileAttendRows + q_row;
@@ -769,7 +743,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
     // page for the tile after that is on its way too.
     tile_start<TT>(a, sm.before, g0, &at);
     int walk_t0 = at.s.low + at.chunk * TT, walk_left = min(at.s.chunks - at.chunk, g1 - g0), walk_g = g0 + walk_left;
-    int walk_head = at.head, walk_end = at.s.pos_max + 1;
+    int walk_head = at.head, walk_end = span_end(at.w.s, at.s.pos_max);
     const int32_t* walk_table = a.t.table + at.b * a.t.table_stride;
     int page_next = 0;
     auto fetch_pages = [&]() {
@@ -797,7 +771,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
         walk_left = min(at.s.chunks, g1 - walk_g);
         walk_g += walk_left;
         walk_head = at.head;
-        walk_end = at.s.pos_max + 1;
+        walk_end = span_end(at.w.s, at.s.pos_max);
         walk_table = a.t.table + at.b * a.t.table_stride;
       }
       fetch_pages();
@@ -877,11 +851,12 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       const int run = min(at.s.chunks - at.chunk, g1 - g);
       const int rows = min(kTileAttendRows, at.w.rows - at.tile * kTileAttendRows);
       const int t_first = at.s.low + at.chunk * TT;
-      const int pos_min = at.s.pos_min, pos_max = at.s.pos_max;
+      const int last = at.w.s.length - 1;  // the last token there is: rows past the page table see up to it
+      const int pos_min = min(at.s.pos_min, last), pos_max = at.s.pos_max;
       const bool active = warp * 32 < rows;  // rows past the tile's are left out, warp by warp
       wait(&sm.q_full[pair & 1], (pair >> 1) & 1);
       const float row_scale = sm.row_scale[pair & 1][row] * (capped_logits ? 1.f / a.softcap : kLog2e);
-      const int pos = at.w.first + min(at.tile * kTileAttendRows + row, at.w.rows - 1) / a.group;
+      const int pos = at.w.s.first + min(at.tile * kTileAttendRows + row, at.w.rows - 1) / a.group;
       RowSoftmax r{kAttendStart, 0.f, kAttendStart};
 #pragma unroll 1
       for (int i = 0; i < run; ++i) {
@@ -899,8 +874,8 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
           z.meta = sm.meta[slot];
           z.row_scale = row_scale;
           z.cap2 = cap2;
-          z.low = a.window ? pos - a.window + 1 - t0 : 0;
-          z.high = pos - t0;
+          z.low = a.window ? pos - t0 - (a.window - 1) : 0;
+          z.high = min(pos, last) - t0;
           const int missing = sm.meta_missing[slot];
           auto scale_sums = [&](float f) {
             if (i == 0 || !__any_sync(0xFFFFFFFFu, f != 1.f)) return;
@@ -939,7 +914,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
                 cta_last = static_cast<int>((pair_end - 1 + cost_before + cost) / per);
       const bool whole = cta_first == cta_last;
       float* part_out = a.partials + (static_cast<size_t>(blockIdx.x) * 2 + (pair_start > g0 ? 1 : 0)) * kTileSlotFloats;
-      const int token0 = a.t.query_start ? a.t.query_start[at.b] : at.b;
+      const int token0 = a.t.begin_of(at.b, list_sizes(a));
       const int row0 = at.tile * kTileAttendRows;
       wait(&sm.pv_done[(done + run - 1) & 1], ((done + run - 1) >> 1) & 1);
       tc_fence_after();
@@ -1020,7 +995,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
     for (int i = 0; i < join.parts; ++i)
       sum += __ldcg(part_of(i) + 257 * kTileAttendRows) * ex2(__ldcg(part_of(i) + 256 * kTileAttendRows) - m);
     const float f = sum == 0.f ? 0.f : ex2(mp - m) / sum;
-    const int token0 = a.t.query_start ? a.t.query_start[join.b] : join.b;
+    const int token0 = a.t.begin_of(join.b, list_sizes(a));
     const int all = join.row0 + row, i_tok = all / a.group;
     uint16_t* out = a.out + (token0 + i_tok) * a.o_ts + (join.head * a.group + all - i_tok * a.group) * a.o_hs;
     static_assert(kTileAttendThreads == 4 * kTileAttendRows, "a quarter of the dimensions per thread");

@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(128) kv_append_step_kernel(const AppendArgs a)
   const int what = static_cast<int>(item % per_seq);
   grid_dependency_wait();
   if (b >= a.t.seqs) return;
-  const int pos = a.t.lens[b] - 1;
+  const int pos = max(a.t.lens[b], 0) - 1;
   if (what >= 2 * a.c.heads) {
     rotate_query<T, VP>(a, b, what - 2 * a.c.heads, pos, lane);
     return;
@@ -479,11 +479,13 @@ __global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendAr
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int groups = (a.c.heads + heads_each - 1) / heads_each, what = blockIdx.y;
   const int first = blockIdx.x * span, end = min(first + span, a.t.tokens);
+  const ListSizes sizes{a.t.tokens, a.t.max_pages << a.c.page_shift, 1, 0};
   if (what == 2 * groups) {
     for (int t = first + warp; t < end; t += 8) {
       const int b = sequence_of(a.t, t, lane);
-      const bool owned = t >= a.t.query_start[b] && t < a.t.query_start[b + 1];
-      rotate_queries<T, VP>(a, t, owned ? a.t.lens[b] - (a.t.query_start[b + 1] - t) : -1, lane);
+      const SeqRows s = a.t.rows_of(b, sizes);
+      const int row = t - a.t.begin_of(b, sizes);
+      rotate_queries<T, VP>(a, t, row >= 0 && row < s.tokens ? s.first + row : -1, lane);
     }
     return;
   }
@@ -494,8 +496,9 @@ __global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendAr
   const long long ts = keys ? a.k_ts : a.v_ts;
   for (int t = first; t < end; ++t) {
     while (b + 1 < a.t.seqs && a.t.query_start[b + 1] <= t) ++b;
-    const int start = a.t.query_start[b], stop = min(a.t.query_start[b + 1], a.t.tokens);
-    const int pos = a.t.lens[b] - (a.t.query_start[b + 1] - t);
+    const SeqRows s = a.t.rows_of(b, sizes);
+    const int start = a.t.begin_of(b, sizes), stop = start + s.tokens;
+    const int pos = s.first + (t - start);
     if (t < start || t >= stop || pos < 0) continue;  // not a sequence's token, or an inactive one
     const int slot = pos & (a.c.page_size - 1);
     if (t != start && slot != 0) {  // a token inside a block: on to the next block

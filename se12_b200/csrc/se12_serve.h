@@ -9,6 +9,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "se12_worklist.h"
+
 namespace se12 {
 
 // Cache element kinds (SE12_KV_INT8, SE12_KV_E4M3).
@@ -36,6 +38,16 @@ struct TokenBatch {
   long long table_stride;
   int max_pages;
   int seqs, tokens;
+
+#if defined(__CUDACC__)
+  // Sequence b's first row, and its rows and tokens; z.capacity is max_pages pages.
+  __device__ __forceinline__ int begin_of(int b, const ListSizes& z) const {
+    return first_row(query_start ? query_start[b] : b, z);
+  }
+  __device__ __forceinline__ SeqRows rows_of(int b, const ListSizes& z) const {
+    return sequence_rows(query_start ? query_start[b] : b, query_start ? query_start[b + 1] : b + 1, lens[b], z);
+  }
+#endif
 };
 
 struct AppendArgs {

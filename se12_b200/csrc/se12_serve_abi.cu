@@ -54,7 +54,7 @@ int check_batch(const se12_kv_cache* cache, const se12_kv_batch* b, se12::TokenB
   if (!b->lens || !b->block_table) return fail(SE12_ERR_INVALID_ARGUMENT, "null lens or block_table");
   if (b->max_pages < 1 || b->table_stride < 0)
     return fail(SE12_ERR_INVALID_ARGUMENT, "block_table needs a column, and a table_stride that is not negative");
-  if (static_cast<long long>(b->max_pages) * cache->view.page_size > INT32_MAX)
+  if (static_cast<long long>(b->max_pages) * cache->view.page_size > se12::kMaxPositions)
     return fail(SE12_ERR_INVALID_ARGUMENT, "positions must fit 31 bits");
   out->query_start = b->query_start;
   out->lens = b->lens;
@@ -181,7 +181,7 @@ int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const
   const double work = static_cast<double>(v.heads) * batch->seqs *
                       (static_cast<double>(batch->max_pages) * v.page_size / 16 + 32) *
                       (static_cast<double>(p->max_query) * group / 8 + 1);
-  if (work > 2.0e9) return fail(SE12_ERR_INVALID_ARGUMENT, "the batch is too large for one call: split it by sequences");
+  if (work > 2.0e9 || static_cast<long long>(batch->tokens) * group > (1 << 30)) return fail(SE12_ERR_INVALID_ARGUMENT, "the batch is too large for one call: split it by sequences");
   const size_t need = se12_kv_attend_call_bytes(cache, p->q_heads, p->max_query);
   if (!workspace || workspace_bytes < need)
     return fail(SE12_ERR_WORKSPACE_TOO_SMALL, "workspace needs " + std::to_string(need) + " bytes");
@@ -197,7 +197,8 @@ int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const
   a.group = group;
   a.scale = p->scale;
   a.softcap = p->softcap;
-  a.window = p->window;
+  // (a window as long as the page table hides nothing)
+  a.window = p->window < batch->max_pages * v.page_size ? p->window : 0;
   a.counters = static_cast<int*>(workspace);
   a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + SE12_COUNTER_BYTES);
   const cudaError_t err = se12::launch_kv_attend(cache->k_map, cache->v_map, a, p->max_query, cache->sm_count,

@@ -874,3 +874,85 @@ def test_workspace_is_prepared_on_the_cache_device(monkeypatch):
     ints = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
     cache.attend(torch.zeros(1, 2, 64, dtype=torch.bfloat16), ints([[0]]), ints([3]))
     assert sorted(seen) == [("capturing", True), ("launch", True), ("workspace", True)]
+
+
+# ------------------------------------------------------------------ lengths and row starts that may be anything
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("n", [1, 3, 70])
+@pytest.mark.parametrize("length", [321, 1 << 30, 2**31 - 1, -5, -(2**31)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attend_lengths_past_the_page_table(dim, n, length, window):
+    """Rows past the page table see what it has (nothing, behind a window) and
+    set the status; negative lengths are empty; the others' rows are right."""
+    from se12_b200.device import device_status
+
+    g = torch.Generator().manual_seed(n)
+    page, heads, q_heads, capacity = 16, 2, 8, 320
+    cache, keys, values = filled(g, 60, page, heads, dim, "int8")
+    table = torch.randperm(60, generator=g).to(torch.int32).view(3, 20)
+    q = torch.randn(3 * n, q_heads, dim, generator=g).to(torch.bfloat16)
+    starts = starts_of([n] * 3)
+    lens = [300, length, 91]
+    got = cache.attend(q.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+                       query_start=torch.tensor(starts, dtype=torch.int32).cuda(), max_query=n, window=window)
+    assert device_status() == (2 if length > capacity else 0)
+    for b in (0, 2):
+        rows = slice(starts[b], starts[b + 1])
+        check_attend(got[rows], *plain_attend(q[rows], keys, values, table[b : b + 1], lens[b : b + 1], [0, n], dim**-0.5, 0.0, window), 300)
+    for i in range(n, 2 * n):
+        pos = max(length, 0) - n + (i - n)
+        if pos < 0 or (window and pos - window + 1 >= capacity):
+            assert not bool(got[i].any())
+            continue
+        seen, back = min(pos + 1, capacity), max(pos + 1 - capacity, 0)  # the window's tokens past the table are missing
+        check_attend(got[i : i + 1], *plain_attend(q[i : i + 1], keys, values, table[1:2], [seen], [0, 1], dim**-0.5, 0.0,
+                                                   window - back if window else 0), seen)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [2, 70])
+@pytest.mark.parametrize("starts", [[-9, 1, 2, 3], [0, 1, 2, 2**31 - 1], [-(2**31), 1, 2, 30], [0, 1, 0, 1], [3, 2, 1, 0], [9, 10, 11, 12],
+                                    [2**31 - 1, -(2**31), 5, -5]])
+def test_row_starts_outside_the_batch_reach_no_other_memory(n, starts):
+    """Starts in units of n rows: those within the batch (3 n rows) give the
+    sequences their rows, the others end at its first and last row."""
+    g = torch.Generator().manual_seed(n)
+    cache, _, _ = filled(g, 60, 16, 2, 128, "int8")
+    table = torch.randperm(60, generator=g).to(torch.int32).view(3, 20).cuda()
+    lens = torch.tensor([300, 260, 91], dtype=torch.int32).cuda()
+    q = torch.randn(3 * n, 8, 128, generator=g).to(torch.bfloat16).cuda()
+    ints = [s * n if abs(s) < 1000 else s for s in starts]
+    out = torch.full_like(q, 7.0)
+    got = cache.attend(q, table, lens, query_start=torch.tensor(ints, dtype=torch.int32).cuda(), max_query=n, out=out)
+    assert bool(torch.isfinite(got).all())
+    held = [min(max(s, 0), 3 * n) for s in ints]
+    if held == [0, n, 2 * n, 3 * n]:
+        want = cache.attend(q, table, lens, query_start=torch.tensor(held, dtype=torch.int32).cuda(), max_query=n)
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+    if all(a >= b for a, b in zip(held, held[1:])):
+        assert bool((got == 7.0).all())
+    k = torch.randn(3 * n, 2, 128, generator=g).cuda()
+    held = cache.append(k, k, table, lens, q=k, query_start=torch.tensor(ints, dtype=torch.int32).cuda())
+    assert bool(torch.isfinite(held).all())
+    from se12_b200.device import device_status
+
+    device_status()  # positions past the page table may have been met
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 2, 2**20])
+@pytest.mark.parametrize("n", [1, 5, 70])
+def test_attend_windows_longer_than_any_sequence(window, n):
+    """Such a window hides nothing, also where rows lie before the sequence."""
+    g = torch.Generator().manual_seed(n)
+    lens = [300, max(n - 4, 1), 2]
+    table, pool = random_tables(g, lens, 16)
+    cache, _, _ = filled(g, pool, 16, 2, 128, "int8")
+    q = torch.randn(3 * n, 8, 128, generator=g).to(torch.bfloat16).cuda()
+    args = (table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    start = torch.tensor([0, n, 2 * n, 3 * n], dtype=torch.int32).cuda()
+    want = cache.attend(q, *args, query_start=start, max_query=n)
+    assert torch.equal(cache.attend(q, *args, query_start=start, max_query=n, window=window), want)
