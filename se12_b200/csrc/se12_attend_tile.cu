@@ -167,14 +167,17 @@ __device__ __forceinline__ void tmem_store_4(uint32_t addr, const uint32_t (&r)[
                : "memory");
 }
 
-// 16 bytes, or zeros where `use` is false (without a branch).
+// 16 bytes, or zeros where `use` is false (without a branch). A coherent load:
+// the kernel may have begun while the one before it, which writes the codes
+// and queries, was still running, and .nc asks that nothing writes them meanwhile.
 __device__ __forceinline__ uint4 load_or_zero(const uint8_t* p, bool use) {
   uint4 v;
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-      "@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
       : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
-      : "l"(p), "r"(static_cast<uint32_t>(use)));
+      : "l"(p), "r"(static_cast<uint32_t>(use))
+      : "memory");
   return v;
 }
 

@@ -956,3 +956,13 @@ def test_attend_windows_longer_than_any_sequence(window, n):
     start = torch.tensor([0, n, 2 * n, 3 * n], dtype=torch.int32).cuda()
     want = cache.attend(q, *args, query_start=start, max_query=n)
     assert torch.equal(cache.attend(q, *args, query_start=start, max_query=n, window=window), want)
+
+
+def test_overlapped_kernels_load_coherently():
+    """These kernels begin while the kernel before them may still write what
+    they read: none of their loads is a non-coherent one."""
+    from se12_b200 import _build
+
+    for name in ("se12_kv.cu", "se12_attend.cu", "se12_attend_tile.cu", "se12_logprobs.cu", "se12_device.cuh"):
+        code = [line.split("//")[0] for line in (_build.PACKAGE_DIR / "csrc" / name).read_text().splitlines()]
+        assert not any("global.nc" in line or "__ldg" in line for line in code), name
