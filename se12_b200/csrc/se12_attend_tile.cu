@@ -355,13 +355,18 @@ __device__ __forceinline__ void group_maxima(float* t, const uint32_t (&s)[2][32
 
 __device__ __forceinline__ unsigned long long twice(float x) { return pair_of(x, x); }
 
+// cap tanh(u) in units of log 2, and `add`: u times a polynomial of u^2 of
+// degree 4 (Chebyshev fit of tanh(u) / u on |u| <= 0.7, off by 1.9e-7), two at a time.
+__device__ __forceinline__ unsigned long long capped_pair(unsigned long long u, float cap2, unsigned long long add) {
+  const unsigned long long c0 = twice(0.999999706f * cap2), c1 = twice(-0.33330266f * cap2), c2 = twice(0.132816473f * cap2),
+                           c3 = twice(-0.0508535559f * cap2), c4 = twice(0.0137912829f * cap2);
+  const unsigned long long t = mul_pair(u, u);
+  return fma_pair(fma_pair(fma_pair(fma_pair(fma_pair(c4, t, c3), t, c2), t, c1), t, c0), u, add);
+}
+
 // Weights of the 64 tokens in s into P, and their sum, two tokens at a time.
 template <bool CAP, bool MASK>
 __device__ __forceinline__ void group_weights(RowSoftmax& r, const TileLogits& z, const uint32_t (&s)[2][32], int k0) {
-  // cap tanh(u) in units of log 2: u times a polynomial of u^2 of degree 4
-  // (Chebyshev fit of tanh(u) / u on |u| <= 0.7, off by 1.9e-7)
-  const unsigned long long c0 = twice(0.999999706f * z.cap2), c1 = twice(-0.33330266f * z.cap2), c2 = twice(0.132816473f * z.cap2),
-                           c3 = twice(-0.0508535559f * z.cap2), c4 = twice(0.0137912829f * z.cap2);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
 #pragma unroll
@@ -375,13 +380,7 @@ __device__ __forceinline__ void group_weights(RowSoftmax& r, const TileLogits& z
       for (int k = 0; k < 8; ++k) {
         const int i = h * 16 + 2 * k;
         const unsigned long long v = pair_of(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-        unsigned long long x;
-        if (CAP) {
-          const unsigned long long u = mul_pair(v, f), t = mul_pair(u, u);
-          x = fma_pair(fma_pair(fma_pair(fma_pair(fma_pair(c4, t, c3), t, c2), t, c1), t, c0), u, shift2);
-        } else {
-          x = fma_pair(v, f, shift2);
-        }
+        const unsigned long long x = CAP ? capped_pair(mul_pair(v, f), z.cap2, shift2) : fma_pair(v, f, shift2);
         float w0, w1;
         unpair(x, w0, w1);
         w0 = ex2(w0);
@@ -422,16 +421,25 @@ __device__ __forceinline__ bool usual_tile(RowSoftmax& r, const TileLogits& z, S
     load_64(s, z.from + h * 64);
     group_maxima<MASK>(t + h * 4, s, h * 64, z.low, z.high);
 #pragma unroll
-    for (int q = h * 4; q < h * 4 + 4; ++q) {
-      const float f = z.row_scale * z.meta[q][0], lv = z.meta[q][1];
-      const float u = t[q] * f;
-      const bool none = MASK && t[q] == kNegInf;
-      unusual |= !(f > 0.f) || (CAP && !none && !(fabsf(u) <= 0.7f));
-      // (capped: u bounds tanh(u) above for u >= 0, and is near it below)
-      const float v = none ? kNegInf : (CAP ? u * z.cap2 : u) + lv;
-      if (v > top) {
-        top = v;
-        top_lv = lv;
+    for (int q = h * 4; q < h * 4 + 4; q += 2) {
+      // the groups' largest logits, capped as the weights will be (the cap
+      // bends them by up to 0.1 of it: more than a weight has room for)
+      float u[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float f = z.row_scale * z.meta[q + e][0];
+        u[e] = t[q + e] * f;
+        unusual |= !(f > 0.f) || (CAP && !(MASK && t[q + e] == kNegInf) && !(fabsf(u[e]) <= 0.7f));
+      }
+      if (CAP) unpair(capped_pair(pair_of(u[0], u[1]), z.cap2, twice(0.f)), u[0], u[1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float lv = z.meta[q + e][1];
+        const float v = MASK && t[q + e] == kNegInf ? kNegInf : u[e] + lv;
+        if (v > top) {
+          top = v;
+          top_lv = lv;
+        }
       }
     }
   }

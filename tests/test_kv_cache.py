@@ -966,3 +966,62 @@ def test_overlapped_kernels_load_coherently():
     for name in ("se12_kv.cu", "se12_attend.cu", "se12_attend_tile.cu", "se12_logprobs.cu", "se12_device.cuh"):
         code = [line.split("//")[0] for line in (_build.PACKAGE_DIR / "csrc" / name).read_text().splitlines()]
         assert not any("global.nc" in line or "__ldg" in line for line in code), name
+
+
+# ------------------------------------------------------------------ caps of any size
+
+
+def capped_case(seed, kind, page, dim, group, cap, reach, counts, lens, sign):
+    """Keys along one direction, so that the raw logits of every row are
+    sign * cap * reach(position) with a little noise. Tolerance as above, plus
+    2^-20 |s| of sum_j p_j |v_j| for the fp32 roundings of logits past 100
+    (eight of 2^-24 each, for two logits)."""
+    from se12_b200.kv_cache import PagedKvCache
+
+    g = torch.Generator().manual_seed(seed)
+    heads = 2
+    table, pool = random_tables(g, lens, page)
+    k = torch.zeros(pool, heads, page, dim)
+    for b, ln in enumerate(lens):
+        for j in range(ln):
+            k[table[b, j // page], :, j % page] = reach(j / max(ln - 1, 1))
+    k += 0.004 * torch.randn(k.shape, generator=g)
+    v = torch.randn(pool, heads, page, dim, generator=g)
+    tensors = []
+    for x in (k, v):
+        s = torch.tensor([[least_scale(m, kind) for m in row] for row in x.abs().amax(dim=(2, 3)).tolist()])
+        tensors.append((code_of(x / s[:, :, None, None], kind), s))
+    (kc, ks), (vc, vs) = tensors
+    cache = PagedKvCache.from_tensors(kc.cuda(), vc.cuda(), ks.cuda(), vs.cuda(), kind)
+    keys, values = (value_of(c, kind).double() * s.double()[:, :, None, None] for c, s in tensors)
+    starts = starts_of(counts)
+    q = torch.full((starts[-1], heads * group, dim), sign * cap * dim**-0.5) * (1 + 0.01 * torch.randn(starts[-1], heads * group, 1, generator=g))
+    q = q.to(torch.bfloat16)
+    got = cache.attend(q.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+                       query_start=torch.tensor(starts, dtype=torch.int32).cuda(), max_query=max(counts), softcap=cap)
+    want, size, biggest = plain_attend(q, keys, values, table, lens, starts, dim**-0.5, cap, 0)
+    tol = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=1e-300))) - 8) + (2.0**-10 + 2.0**-20 * cap) * size + (
+        2.0**-24 * max(lens) * biggest)
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= tol).all()), f"worst {float((err / tol).nan_to_num(nan=math.inf).max()):.2f} of the tolerance"
+
+
+# Where the logits lie, as a share of the cap, from the first position to the last.
+REACH = {
+    "rising": lambda t: 0.5 + 0.2 * t,
+    "falling": lambda t: 0.7 - 0.2 * t,
+    "level": lambda t: 0.6 + 0.001 * (t * 7919 % 1),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [5.0, 30.0, 80.0, 120.0, 200.0, 1000.0])
+@pytest.mark.parametrize("reach", sorted(REACH))
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("dim,kind", [(128, "int8"), (256, "e4m3")])
+@pytest.mark.parametrize("rows", ["few", "many"])
+def test_attend_caps_of_any_size(cap, reach, sign, dim, kind, rows):
+    """All of a row's logits near the cap's bend, on either side of zero; rows
+    that see one token, a few, and many."""
+    counts = [1, 1, 2] if rows == "few" else [40, 70, 1]
+    capped_case(int(cap * 10), kind, 16, dim, 4, cap, REACH[reach], counts, [40, 333, 129], sign)
