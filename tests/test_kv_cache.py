@@ -1025,3 +1025,16 @@ def test_attend_caps_of_any_size(cap, reach, sign, dim, kind, rows):
     that see one token, a few, and many."""
     counts = [1, 1, 2] if rows == "few" else [40, 70, 1]
     capped_case(int(cap * 10), kind, 16, dim, 4, cap, REACH[reach], counts, [40, 333, 129], sign)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [0.5, 1.0, 2.0, 5.0, 20.0, 50.0, 100.0])
+@pytest.mark.parametrize("deep", [1.0, 1.3, 1.6, 3.0])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("dim,kind", [(128, "int8"), (256, "e4m3")])
+@pytest.mark.parametrize("rows", ["few", "many"])
+def test_attend_logits_on_both_sides_of_a_cap(cap, deep, sign, dim, kind, rows):
+    """Raw logits from 0.4 of the cap down to `deep` times it below zero (and
+    the other way round): with a small cap the deep ones still weigh."""
+    counts = [1, 1, 2] if rows == "few" else [40, 70, 1]
+    capped_case(int(cap * 10), kind, 16, dim, 4, cap, lambda t: 0.4 - (0.4 + deep) * (t * 104729 % 1), counts, [40, 333, 129], sign)
