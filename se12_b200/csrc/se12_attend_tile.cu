@@ -934,6 +934,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
               for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
               tmem_store_32(addr, o);
             }
+            tmem_wait_store();  // (the slow way may scale them again)
           };
           const bool masked = t0 + TT - 1 > pos_min || (a.window && pos_max - t0 >= a.window);
           bool finished = false;

@@ -1038,3 +1038,14 @@ def test_attend_logits_on_both_sides_of_a_cap(cap, deep, sign, dim, kind, rows):
     the other way round): with a small cap the deep ones still weigh."""
     counts = [1, 1, 2] if rows == "few" else [40, 70, 1]
     capped_case(int(cap * 10), kind, 16, dim, 4, cap, lambda t: 0.4 - (0.4 + deep) * (t * 104729 % 1), counts, [40, 333, 129], sign)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+@pytest.mark.parametrize("spread,q_scale", [(40.0, 2.0**-41), (18.0, 2.0**-15), (6.0, 0.1)])
+def test_attend_tiles_of_very_different_scales(kind, dim, softcap, spread, q_scale):
+    """Rows of many queries over blocks whose scales are 2^(+-spread): tiles
+    where rows raise their references and then turn out to be unusual."""
+    attend_case(int(spread), kind, 16, 2, 8, dim, [700, 60], [40, 50], softcap=softcap, spread=spread, q_scale=q_scale)
