@@ -395,7 +395,8 @@ __device__ __forceinline__ void group_weights(RowSoftmax& r, const TileLogits& z
       }
       float sum0, sum1;
       unpair(sum, sum0, sum1);
-      r.l = fmaf(sum0 + sum1, ex2(-shift - r.m), r.l);  // 2^(logit - m) = w 2^(mp - lv - m)
+      // 2^(logit - m) = w 2^(mp - lv - m); where the row sees none of the 16, lv may be anything
+      if (!MASK || sum0 + sum1 != 0.f) r.l = fmaf(sum0 + sum1, ex2(-shift - r.m), r.l);
       tmem_store_8(z.to + k0 / 2 + c * 16 + h * 8, p);
     }
   }

@@ -1049,3 +1049,35 @@ def test_attend_tiles_of_very_different_scales(kind, dim, softcap, spread, q_sca
     """Rows of many queries over blocks whose scales are 2^(+-spread): tiles
     where rows raise their references and then turn out to be unusual."""
     attend_case(int(spread), kind, 16, 2, 8, dim, [700, 60], [40, 50], softcap=softcap, spread=spread, q_scale=q_scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("n,q_heads", [(1, 8), (3, 8), (70, 8), (140, 2)])
+@pytest.mark.parametrize("what,bad", [("k_scales", math.nan), ("k_scales", 0.0), ("v_scales", math.nan), ("v_scales", math.inf),
+                                      ("v_scales", 0.0)])
+def test_attend_blocks_outside_the_window_may_hold_anything(dim, n, q_heads, what, bad):
+    """A block that is not finite reaches the rows that see it, and no row
+    whose window ends above it; a scale of zero makes no row NaN."""
+    g = torch.Generator().manual_seed(dim + n)
+    length, window, page = 400, 100, 16
+    table, pool = random_tables(g, [length], page)
+    cache, _, _ = filled(g, pool, page, 2, dim, "int8")
+    q = torch.randn(n, q_heads, dim, generator=g).to(torch.bfloat16).cuda()
+    args = (table.cuda(), torch.tensor([length], dtype=torch.int32).cuda())
+    start = torch.tensor([0, n], dtype=torch.int32).cuda()
+    want = cache.attend(q, *args, query_start=start, window=window)
+    for block in ((length - n - window + 1) // page, (length - n - window + 1) // page + 2):
+        scales = getattr(cache, what)
+        kept = scales.clone()
+        scales[int(table[0, block])] = bad
+        got = cache.attend(q, *args, query_start=start, window=window)
+        scales.copy_(kept)
+        last = block * page + page - 1  # the block's last position
+        for i in range(n):
+            pos = length - n + i
+            if pos - last >= window:  # the block lies below this row's window
+                # (only the order of the sums may differ: the unusual tile's weights are summed apart)
+                assert torch.allclose(got[i].float(), want[i].float(), rtol=2.0**-6, atol=2.0**-8), (block, i)
+            else:
+                assert bool((torch.isfinite(got[i]) == (bad == 0.0)).all()), (block, i)
