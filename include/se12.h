@@ -452,7 +452,8 @@ int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const
  *   out_i = sum_j softmax_j(s_ij) v_j, s_ij = scale q_i . k_j, then, with
  *   softcap > 0, softcap * tanh(s_ij / softcap);
  * a row at position p sees the positions j <= p, with window > 0 only those
- * with p - j < window. A row that sees nothing is zero; rows that belong to no
+ * with p - j < window; table entries of pages below the first position that
+ * a sequence's rows see are not read. A row that sees nothing is zero; rows that belong to no
  * sequence (query_start skips them) are left as they are. q and out: BF16
  * [tokens][q_heads][head_dim] with token and head strides; query head h uses
  * KV head h / (q_heads / kv_heads). max_query: the largest number of rows of a

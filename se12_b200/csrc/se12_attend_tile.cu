@@ -787,13 +787,13 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
     // page for the tile after that is on its way too.
     tile_start<TT>(a, sm.before, g0, &at);
     int walk_t0 = at.s.low + at.chunk * TT, walk_left = min(at.s.chunks - at.chunk, g1 - g0), walk_g = g0 + walk_left;
-    int walk_head = at.head, walk_end = span_end(at.w.s, at.s.pos_max);
+    int walk_head = at.head, walk_end = span_end(at.w.s, at.s.pos_max), walk_from = visible_from(at.s.pos_min, a.window);
     const int32_t* walk_table = a.t.table + at.b * a.t.table_stride;
     int page_next = 0;
     auto fetch_pages = [&]() {
       const int t = walk_t0 + lane * 16;
-      page_next = -2;  // none due
-      if (lane < GROUPS && t < walk_end)
+      page_next = -2;  // none due: past the last row's position, or below the first row's window
+      if (lane < GROUPS && t < walk_end && t + 16 > walk_from)
         page_next = (t >> a.c.page_shift) < a.t.max_pages ? walk_table[t >> a.c.page_shift] : -1;
     };
     bool missing = false;  // a page that is due is not there
@@ -816,6 +816,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
         walk_g += walk_left;
         walk_head = at.head;
         walk_end = span_end(at.w.s, at.s.pos_max);
+        walk_from = visible_from(at.s.pos_min, a.window);
         walk_table = a.t.table + at.b * a.t.table_stride;
       }
       fetch_pages();

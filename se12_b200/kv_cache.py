@@ -258,11 +258,13 @@ class PagedKvCache:
         """Attention of the rows q (BF16 [tokens, q_heads, head_dim]) over
         their sequences; batch arguments as for ``append``. Causal: a row at
         position p sees positions up to p, with ``window`` only the last
-        ``window`` of them. Logits are ``scale`` (default head_dim ** -0.5) q . k,
-        with ``softcap`` > 0 then softcap * tanh(logit / softcap). Rows that
-        see nothing are zero; rows of ``out`` that ``query_start`` gives to no
-        sequence are left as they are. ``max_query``: the most rows of one sequence
-        (default: all tokens; tells the launch how many rows share a page).
+        ``window`` of them; page table entries below the first position that a
+        sequence's rows see are not read (those pages may have been given
+        back). Logits are ``scale`` (default head_dim ** -0.5) q . k, with
+        ``softcap`` > 0 then softcap * tanh(logit / softcap). Rows that see
+        nothing are zero; rows of ``out`` that ``query_start`` gives to no
+        sequence are left as they are. ``max_query``: the most rows of one
+        sequence (default: all tokens; tells the launch how many rows share a page).
         Returns BF16 like q."""
         q_strides = self._row_strides(q, "q", None, None, _BF16)
         tokens, q_heads, _ = q.shape

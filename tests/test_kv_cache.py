@@ -1081,3 +1081,29 @@ def test_attend_blocks_outside_the_window_may_hold_anything(dim, n, q_heads, wha
                 assert torch.allclose(got[i].float(), want[i].float(), rtol=2.0**-6, atol=2.0**-8), (block, i)
             else:
                 assert bool((torch.isfinite(got[i]) == (bad == 0.0)).all()), (block, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("n", [1, 3, 8, 70])
+@pytest.mark.parametrize("length,window", [(400, 100), (777, 513), (130, 1), (97, 97)])
+def test_attend_pages_given_back_below_the_window(dim, n, length, window):
+    """Page table entries below the first position a batch's rows see are
+    not read: no status, the same output."""
+    from se12_b200.device import device_status
+
+    g = torch.Generator().manual_seed(length)
+    page = 16
+    lens, counts = [length, 45, length - 7], [n, 1, n]
+    table, pool = random_tables(g, lens, page)
+    cache, _, _ = filled(g, pool, page, 2, dim, "e4m3")
+    q = torch.randn(sum(counts), 8, dim, generator=g).to(torch.bfloat16).cuda()
+    start = torch.tensor(starts_of(counts), dtype=torch.int32).cuda()
+    dev_lens = torch.tensor(lens, dtype=torch.int32).cuda()
+    want = cache.attend(q, table.cuda(), dev_lens, query_start=start, max_query=n, window=window, softcap=20.0)
+    for b in range(3):
+        first = max(lens[b] - counts[b] - window + 1, 0)
+        table[b, : first // page] = -1
+    got = cache.attend(q, table.cuda(), dev_lens, query_start=start, max_query=n, window=window, softcap=20.0)
+    assert device_status() == 0
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
