@@ -59,6 +59,7 @@ constexpr int kAttendMaxCtas = 3;        // per SM
 // 183 and 185. 16 of 301 to 8191, window 4096, 8 heads of 256: 57 us; 52, 51 and
 // 50. 7 of 86 to 702 tokens: 24 us; 17, 16 and 16. Equal lengths gain little.)
 constexpr int kAttendPairCost = 8;
+constexpr float kAttendWideCap = 128.f;  // a logit off by 2^-15 there, an eighth of a weight's FP16 rounding
 constexpr float kAttendStart = -1.0e30f; // both references before the first token
 constexpr float kAttendRaise = 8.f;      // weights up to 2^8 of the reference
 constexpr float kAttendRaiseSum = 30.f;
@@ -318,6 +319,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
   for (int s = 0; s < kAttendStages; ++s)
     if (more) issue(s);
 
+  const bool wide = a.softcap > kAttendWideCap;
   int stage = 0;
   uint32_t phase = 0;
   bool dead = false;  // a wait ran out: skip the rest (status raised)
@@ -474,10 +476,17 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
           for (int k = 0; k < 4; ++k) {
             float x = (s[n][0][k] + s[n][1][k]) * (row_scale[n][k & 1] * ks);
             // cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1); the
-            // factor 2 log2(e) / cap is in row_scale
-            if (a.softcap != 0.f) x = a.softcap * kLog2e - __fdividef(2.f * kLog2e * a.softcap, ex2(x) + 1.f);
+            // factor 2 log2(e) / cap is in row_scale. The difference is off by
+            // some 2^-23 of the cap: above kAttendWideCap not taken.
+            if (a.softcap != 0.f && !wide) x = a.softcap * kLog2e - __fdividef(2.f * kLog2e * a.softcap, ex2(x) + 1.f);
             p[sub][n][k] = x;
           }
+        if (wide) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) p[sub][n][k] = capped_by(p[sub][n][k] * (0.5f / kLog2e), a.softcap * kLog2e);
+        }
       }
       const bool masked = t0 + CHUNK - 1 > pos_min || (a.window && pos_max - t0 >= a.window);
       if (masked) {

@@ -511,7 +511,7 @@ __device__ __forceinline__ void any_tile(RowSoftmax& r, const TileLogits& z, int
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       float v = __uint_as_float(s[k]) * f;
-      if (z.cap2 != 0.f) v = z.cap2 - __fdividef(2.f * z.cap2, ex2(v * (2.f * kLog2e)) + 1.f);
+      if (z.cap2 != 0.f) v = capped_by(v, z.cap2);
       y[k] = k0 + k < z.low || k0 + k > z.high || !there ? kNegInf : v;
     }
   };

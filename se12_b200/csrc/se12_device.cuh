@@ -355,6 +355,21 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
+// cap * tanh(u) for any u, off by a few roundings of its own size whatever the
+// cap: u times a polynomial of u^2 of degree 5 (Chebyshev fit of tanh(u) / u on
+// |u| <= 0.7, off by 8.5e-9), beyond it cap - 2 cap / (exp(2 u) + 1), whose
+// difference would cost a small u its digits.
+__device__ __forceinline__ float capped_by(float u, float cap) {
+  const float t = __fmul_rn(u, u);
+  float y = fmaf(-0.00509482797f * cap, t, 0.0200324471f * cap);
+  y = fmaf(y, t, -0.0535294551f * cap);
+  y = fmaf(y, t, 0.133284756f * cap);
+  y = fmaf(y, t, -0.333331342f * cap);
+  y = fmaf(y, t, 0.999999987f * cap);
+  const float far = cap - __fdividef(2.f * cap, ex2(u * (2.f * kLog2e)) + 1.f);
+  return fabsf(u) <= 0.7f ? __fmul_rn(y, u) : far;
+}
+
 // ------------------------------------------------------------------ pairs of fp32
 
 // Two fp32 operations per instruction, each rounded as the scalar one.

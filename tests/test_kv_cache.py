@@ -1107,3 +1107,12 @@ def test_attend_pages_given_back_below_the_window(dim, n, length, window):
     got = cache.attend(q, table.cuda(), dev_lens, query_start=start, max_query=n, window=window, softcap=20.0)
     assert device_status() == 0
     assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e3, 1e4, 1e6, 1e9])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attend_caps_far_above_the_logits(cap, dim, n):
+    """A cap that hardly bends the logits costs them no precision."""
+    attend_case(dim + n, "int8", 16, 2, 8, dim, [300, 41], [n, n], softcap=cap, q_scale=2.0, max_query=n)
