@@ -355,21 +355,6 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
-// cap * tanh(u) for any u, off by a few roundings of its own size whatever the
-// cap: u times a polynomial of u^2 of degree 5 (Chebyshev fit of tanh(u) / u on
-// |u| <= 0.7, off by 8.5e-9), beyond it cap - 2 cap / (exp(2 u) + 1), whose
-// difference would cost a small u its digits.
-__device__ __forceinline__ float capped_by(float u, float cap) {
-  const float t = __fmul_rn(u, u);
-  float y = fmaf(-0.00509482797f * cap, t, 0.0200324471f * cap);
-  y = fmaf(y, t, -0.0535294551f * cap);
-  y = fmaf(y, t, 0.133284756f * cap);
-  y = fmaf(y, t, -0.333331342f * cap);
-  y = fmaf(y, t, 0.999999987f * cap);
-  const float far = cap - __fdividef(2.f * cap, ex2(u * (2.f * kLog2e)) + 1.f);
-  return fabsf(u) <= 0.7f ? __fmul_rn(y, u) : far;
-}
-
 // ------------------------------------------------------------------ pairs of fp32
 
 // Two fp32 operations per instruction, each rounded as the scalar one.
@@ -399,6 +384,35 @@ __device__ __forceinline__ unsigned long long mul_pair(unsigned long long a, uns
   unsigned long long d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+
+// ------------------------------------------------------------------ capped logits
+
+// tanh(u) / u as a polynomial of u^2 (Chebyshev fit on |u| <= 0.7, off by
+// 7.6e-9 as rounded here), constant term first. The last one is positive:
+// u = -inf gives -inf.
+__device__ constexpr float kTanhFit[7] = {1.f,           -0.333333224f,  0.133329257f, -0.053916972f,
+                                          0.0215576552f, -0.00786164403f, 0.00188218791f};
+
+// cap * tanh(u), two at a time, |u| <= 0.7 or u = -inf.
+__device__ __forceinline__ unsigned long long capped_pair_near(unsigned long long u, float cap) {
+  const unsigned long long t = mul_pair(u, u);
+  unsigned long long y = pair_of(kTanhFit[6] * cap, kTanhFit[6] * cap);
+#pragma unroll
+  for (int i = 5; i >= 0; --i) y = fma_pair(y, t, pair_of(kTanhFit[i] * cap, kTanhFit[i] * cap));
+  return mul_pair(y, u);
+}
+
+// cap * tanh(u) for any u, off by a few roundings of its own size whatever the
+// cap: the polynomial (the bits of capped_pair_near), beyond it
+// cap - 2 cap / (exp(2 u) + 1), whose difference would cost a small u its digits.
+__device__ __forceinline__ float capped_by(float u, float cap) {
+  const float t = __fmul_rn(u, u);
+  float y = kTanhFit[6] * cap;
+#pragma unroll
+  for (int i = 5; i >= 0; --i) y = fmaf(y, t, kTanhFit[i] * cap);
+  const float far = cap - __fdividef(2.f * cap, ex2(u * (2.f * kLog2e)) + 1.f);
+  return fabsf(u) <= 0.7f ? __fmul_rn(y, u) : far;
 }
 
 // ------------------------------------------------------------------ SE12 decode pieces

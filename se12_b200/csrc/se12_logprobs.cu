@@ -150,11 +150,10 @@ __device__ __forceinline__ void rebuild_list(LogprobSmem& sm, int count, int war
   __syncthreads();
 }
 
-// cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1); -inf stays.
-__device__ __forceinline__ float capped(float x, float cap) {
-  const float e = ex2(x * (2.f * kLog2e / cap));
-  const float z = cap - __fdividef(2.f * cap, e + 1.f);
-  return x == kNegInf ? kNegInf : z;
+// The capped logit; -inf stays. The sums, their reference and the logits that
+// are reported all take this value, so that the largest one's term is 1.
+__device__ __forceinline__ float capped(float x, float cap, float inverse) {
+  return x == kNegInf ? kNegInf : capped_by(__fmul_rn(x, inverse), cap);
 }
 
 template <bool BF16>
@@ -266,6 +265,7 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
 
   const int units = a.rows * a.chunks_per_row;  // (the host sees to it that they fit)
   const int u0 = blockIdx.x * a.units_per_cta, u1 = min(u0 + a.units_per_cta, units), batches = u1 - u0;
+  const float inverse = CAP ? 1.f / a.softcap : 0.f;
   const uint64_t policy = policy_evict_first();
   // batch n of this CTA's run on its way into its stage: whole vectors only
   int copy_row = u0 / a.chunks_per_row, copy_chunk = u0 - copy_row * a.chunks_per_row;
@@ -348,31 +348,27 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
       // - max is one rounding everywhere: the maximum's own cancels)
       float high = top;
       if constexpr (CAP) {
-        float low = fminf(x[0], x[1]);
+        // |x / cap| below 0.7 but for banned tokens, usually: the polynomial
+        // alone, two values at a time. The lowest value that is not -inf: as
+        // unsigned numbers, negative ones are the larger the lower they are, and
+        // an exponent step more turns -inf into 0.
+        constexpr unsigned kStep = 0x00800000u;
+        const float range = 0.6999f * a.softcap;
+        unsigned low = 0;
 #pragma unroll
-        for (int j = 2; j < kValues; ++j) low = fminf(low, x[j]);
-        const float range = 0.7f * a.softcap;
-        if (__all_sync(0xFFFFFFFFu, top <= range && low >= -range)) {
-          // cap tanh(u): u times a polynomial of u^2 of degree 5 (Chebyshev fit
-          // of tanh(u) / u on |u| <= 0.7, off by 8.5e-9), two at a time
-          const unsigned long long inverse = pair_of(1.f / a.softcap, 1.f / a.softcap);
-          const float c0 = a.softcap;
+        for (int j = 0; j < kValues; ++j) low = umax(low, __float_as_uint(x[j]) + kStep);
+        if (__all_sync(0xFFFFFFFFu, top <= range && low <= __float_as_uint(-range) + kStep)) {
 #pragma unroll
-          for (int j = 0; j < kValues; j += 2) {
-            const unsigned long long u = mul_pair(pair_of(x[j], x[j + 1]), inverse), t = mul_pair(u, u);
-            unsigned long long y = fma_pair(pair_of(-0.00509482797f * c0, -0.00509482797f * c0), t, pair_of(0.0200324471f * c0, 0.0200324471f * c0));
-            y = fma_pair(y, t, pair_of(-0.0535294551f * c0, -0.0535294551f * c0));
-            y = fma_pair(y, t, pair_of(0.133284756f * c0, 0.133284756f * c0));
-            y = fma_pair(y, t, pair_of(-0.333331342f * c0, -0.333331342f * c0));
-            y = fma_pair(y, t, pair_of(0.999999987f * c0, 0.999999987f * c0));
-            unpair(mul_pair(y, u), x[j], x[j + 1]);
-          }
-          high = capped(top, a.softcap);
+          for (int j = 0; j < kValues; j += 2)
+            unpair(capped_pair_near(mul_pair(pair_of(x[j], x[j + 1]), pair_of(inverse, inverse)), a.softcap), x[j], x[j + 1]);
+          high = fmaxf(x[0], x[1]);
+#pragma unroll
+          for (int j = 2; j < kValues; j += 2) high = max3_nan(high, x[j], x[j + 1]);
         } else {
           high = kNegInf;
 #pragma unroll
           for (int j = 0; j < kValues; ++j) {
-            x[j] = capped(x[j], a.softcap);
+            x[j] = capped(x[j], a.softcap, inverse);
             high = max_nan(high, x[j]);
           }
         }
@@ -537,13 +533,13 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
         double s = 0.0, w = 0.0;
         for (long long i = lane; i < a.vocab; i += 32) {
           const float x = load_logit<BF16>(row, i);
-          low_max = fmaxf(low_max, CAP ? capped(x, a.softcap) : x);
+          low_max = fmaxf(low_max, CAP ? capped(x, a.softcap, inverse) : x);
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) low_max = fmaxf(low_max, __shfl_xor_sync(0xFFFFFFFFu, low_max, d));
         for (long long i = lane; i < a.vocab; i += 32) {
           const float x = load_logit<BF16>(row, i);
-          const double below = static_cast<double>(CAP ? capped(x, a.softcap) : x) - low_max;  // -inf - -inf: NaN, as it must be
+          const double below = static_cast<double>(CAP ? capped(x, a.softcap, inverse) : x) - low_max;  // -inf - -inf: NaN, as it must be
           const double e = exp(below);
           s += e;
           if (e > 0.0) w += e * below;
@@ -561,19 +557,21 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
       // that large logits lose nothing
       constexpr float kLn2 = 0.6931471805599453f;
       const float log_sum = logf(sum);
+      // (a probability is at most 1: what rounding leaves above that goes)
+      auto at_most_zero = [](float v) { return v > 0.f ? 0.f : v; };
       auto log_prob = [&](float x) {
-        const float z = CAP ? capped(x, a.softcap) : x;
+        const float z = CAP ? capped(x, a.softcap, inverse) : x;
         if (sum != sum) return sum;
-        if (again) return (z - low_max) - log_sum;
+        if (again) return at_most_zero((z - low_max) - log_sum);
         if (z < kLogprobStart) return z - (max * kLn2 + log_sum);  // would leave fp32's range in units of log 2
-        return fmaf(z, kLog2e, -max) * kLn2 - log_sum;
+        return at_most_zero(fmaf(z, kLog2e, -max) * kLn2 - log_sum);
       };
       if (lane == 0) {
         float lp = __uint_as_float(0x7FC00000u);
         if (token >= a.vocab) raise_status(kStatusBadArgument);
         else if (token >= 0) lp = log_prob(token_logit);
         a.logprob[row_id] = lp;
-        a.entropy[row_id] = log_sum - (weighted / sum) * kLn2;
+        a.entropy[row_id] = 0.f - at_most_zero((weighted / sum) * kLn2 - log_sum);
       }
       if (lane < a.top) {
         a.top_ids[static_cast<long long>(row_id) * a.top + lane] = key_index(mine);

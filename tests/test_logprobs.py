@@ -338,3 +338,42 @@ def test_workspace_is_prepared_on_the_logits_device(monkeypatch):
     assert seen == [1] and _lib.is_loaded()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("others", [-20.0, -60.0])
+def test_certain_rows_have_no_positive_log_probability(softcap, dtype, others):
+    """Rows with one token of probability 1 but for 1e-9 or less: a log
+    probability is never above zero, an entropy never below."""
+    g = torch.Generator().manual_seed(13)
+    rows, vocab = 2000, 1000
+    x = others + torch.randn(rows, vocab, generator=g) * 0.3
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    x.scatter_(1, t[:, None], 5.0 + 40.0 * torch.rand(rows, 1, generator=g))
+    got = check(x.to(dtype), t, 3, softcap)
+    assert bool((got.logprob <= 0).all()), float(got.logprob.max())
+    assert bool((got.top_logprobs <= 0).all()) and bool((got.entropy >= 0).all()), float(got.entropy.min())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("softcap", [0.5, 30.0, 1e3, 1e5, 1e8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("banned", [0.0, 0.3])
+def test_caps_of_any_size(softcap, dtype, banned):
+    """Caps far below and far above the logits, with and without banned
+    tokens: a capped logit is off by a few roundings of its own size (six of
+    2^-23), not of the cap's."""
+    x, t = logits(14, 6, 30011, dtype)
+    g = torch.Generator().manual_seed(15)
+    ban = torch.rand(x.shape, generator=g) < banned
+    ban.scatter_(1, t[:, None], False)
+    x[ban] = -math.inf
+    got = token_logprobs(x.cuda(), t.cuda(), top=8, softcap=softcap)
+    want = plain(x, t, 8, softcap)
+    assert torch.equal(got.top_ids.cpu(), want[2])
+    largest = min(softcap, 20.0)
+    for a, b in ((got.logprob, want[0]), (got.entropy, want[1]), (got.top_logprobs, want[3])):
+        tol = 1e-5 + 6 * 2.0**-23 * largest + 2.0**-21 * b.abs()
+        assert bool(((a.double().cpu() - b).abs() <= tol).all()), float(((a.double().cpu() - b).abs() / tol).max())
