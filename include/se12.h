@@ -370,7 +370,8 @@ int se12_encode_raw(const uint16_t* w_dev, int rows, int cols, int ldw, const in
  * tables and token ids are read on the device, so a captured call follows
  * their contents. What a kernel finds out of range there (a page id, a
  * position beyond the page table or the rotation table, a token id beyond the
- * vocabulary) is skipped and sets bit 1 of se12_device_status.
+ * vocabulary) is skipped (of an appended token both halves, key and value) and
+ * sets bit 1 of se12_device_status.
  *
  * A cache holds one layer's keys and values. A block is one page of one KV
  * head: page_size codes rows of head_dim bytes and one fp32 scale; a value is

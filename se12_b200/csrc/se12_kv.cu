@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(128) kv_append_step_kernel(const AppendArgs a)
   if (pos < 0) return;
   const bool keys = what < a.c.heads;
   const int head = keys ? what : what - a.c.heads;
-  if (keys && a.cos && pos >= a.rope_rows) {
+  if (a.cos && pos >= a.rope_rows) {  // neither half of the token is stored
     raise_status(kStatusBadArgument);
     return;
   }
@@ -507,10 +507,11 @@ __global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendAr
     }
     const int page = page_of(a.t, a.c, b, pos);
     if (page < 0) continue;
-    const int count = min(a.c.page_size - slot, stop - t);
-    if (keys && a.cos && pos + count > a.rope_rows) {
+    int count = min(a.c.page_size - slot, stop - t);
+    if (a.cos && pos + count > a.rope_rows) {  // tokens past the rotation table: neither half is stored
       raise_status(kStatusBadArgument);
-      continue;
+      count = a.rope_rows - pos;
+      if (count <= 0) continue;
     }
     append_page<T, KIND, VP>(a, keys, src + t * ts, ts, keys ? a.k_hs : a.v_hs, head, min(heads_each, a.c.heads - head), pos,
                              slot, count, page, s_amax);

@@ -1116,3 +1116,40 @@ def test_attend_pages_given_back_below_the_window(dim, n, length, window):
 def test_attend_caps_far_above_the_logits(cap, dim, n):
     """A cap that hardly bends the logits costs them no precision."""
     attend_case(dim + n, "int8", 16, 2, 8, dim, [300, 41], [n, n], softcap=cap, q_scale=2.0, max_query=n)
+
+
+# ------------------------------------------------------------------ rotation tables
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,rotary,interleaved", [(128, 128, False), (64, 32, True)])
+@pytest.mark.parametrize("rope_rows", [1, 12, 16, 17])
+def test_append_past_the_rotation_table_stores_neither_half(dim, rotary, interleaved, rope_rows):
+    """Tokens the table reaches are stored, keys and values; the others are
+    not, neither half, and set the status."""
+    from se12_b200.device import device_status
+
+    g = torch.Generator().manual_seed(dim)
+    n, page, heads, q_heads = 20, 16, 2, 4
+    table = torch.tensor([[2, 0]], dtype=torch.int32)
+    cos, sin = rope(g, rope_rows, rotary // 2)
+    y = torch.randn(n, q_heads + 2 * heads, dim, generator=g)
+    q, k, v = y[:, :q_heads], y[:, q_heads : q_heads + heads], y[:, q_heads + heads :]
+    reached = min(n, rope_rows)
+    prompt, plain = make_pair(3, page, heads, dim, "int8")
+    want = torch.zeros(n, q_heads, dim, dtype=torch.bfloat16)
+    want[:reached] = plain.append(k[:reached], v[:reached], table, [reached], [0, reached], cos, sin, interleaved, q[:reached])
+    got = prompt.append(k.cuda(), v.cuda(), table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), q=q.cuda(), cos=cos.cuda(),
+                        sin=sin.cuda(), query_start=torch.tensor([0, n], dtype=torch.int32).cuda(), interleaved=interleaved)
+    assert device_status() == 2
+    assert torch.equal(got.cpu().view(torch.int16), want.view(torch.int16))
+    same_cache(prompt, plain)
+    step, plain = make_pair(3, page, heads, dim, "int8")  # one token at a time
+    for i in range(n):
+        got = step.append(k[i : i + 1].cuda(), v[i : i + 1].cuda(), table.cuda(), torch.tensor([i + 1], dtype=torch.int32).cuda(),
+                          q=q[i : i + 1].cuda(), cos=cos.cuda(), sin=sin.cuda(), interleaved=interleaved)
+        assert device_status() == (2 if i >= rope_rows else 0)
+        if i < rope_rows:
+            plain.append(k[i : i + 1], v[i : i + 1], table, [i + 1], [0, 1], cos, sin, interleaved)
+        assert torch.equal(got.cpu()[0].view(torch.int16), want[i].view(torch.int16))
+    same_cache(step, plain)
