@@ -1153,3 +1153,38 @@ def test_append_past_the_rotation_table_stores_neither_half(dim, rotary, interle
             plain.append(k[i : i + 1], v[i : i + 1], table, [i + 1], [0, 1], cos, sin, interleaved)
         assert torch.equal(got.cpu()[0].view(torch.int16), want[i].view(torch.int16))
     same_cache(step, plain)
+
+
+# ------------------------------------------------------------------ long prompts
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype,page,heads,q_heads,dim,rotary,interleaved", [
+    ("int8", torch.float32, 32, 6, 6, 128, 128, False),    # heads that do not divide by the heads of a CTA
+    ("e4m3", torch.bfloat16, 256, 5, 5, 256, 256, False),  # more tokens per page than stay in registers
+    ("int8", torch.bfloat16, 16, 5, 10, 96, 32, False),    # scalar lanes
+    ("e4m3", torch.float32, 128, 1, 2, 80, 80, True),
+    ("int8", torch.float32, 64, 9, 9, 128, 0, False),
+])
+def test_append_thousands_of_tokens(kind, dtype, page, heads, q_heads, dim, rotary, interleaved):
+    """Calls of more than 2048 tokens, on empty sequences and behind prefixes."""
+    g = torch.Generator().manual_seed(page)
+    steps = [[1900, 1, 0, 180], [700, 1200, 300, 7]]
+    counts = [sum(s[b] for s in steps) for b in range(4)]
+    table, pool = random_tables(g, counts, page)
+    cache, plain = make_pair(pool, page, heads, dim, kind)
+    cos, sin = rope(g, max(counts), rotary // 2) if rotary else (None, None)
+    lens = [0] * 4
+    for step, new in enumerate(steps):
+        lens = [a + b for a, b in zip(lens, new)]
+        starts = starts_of(new)
+        y = (torch.randn(starts[-1], q_heads + 2 * heads, dim, generator=g) * 3.0**step).to(dtype)
+        q, k, v = y[:, :q_heads], y[:, q_heads : q_heads + heads], y[:, q_heads + heads :]
+        want = plain.append(k, v, table, lens, starts, cos, sin, interleaved, q)
+        d = y.cuda()
+        got = cache.append(d[:, q_heads : q_heads + heads], d[:, q_heads + heads :], table.cuda(),
+                           torch.tensor(lens, dtype=torch.int32).cuda(), q=d[:, :q_heads],
+                           query_start=torch.tensor(starts, dtype=torch.int32).cuda(), cos=None if cos is None else cos.cuda(),
+                           sin=None if sin is None else sin.cuda(), interleaved=interleaved)
+        assert torch.equal(got.cpu().view(torch.int16), want.view(torch.int16))
+        same_cache(cache, plain)
