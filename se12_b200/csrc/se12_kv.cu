@@ -567,13 +567,18 @@ cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t stream) {
     return launch_overlapped(kv_append_step_kernel<T, KIND, VP>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0,
                              stream, a);
   }
-  // few tokens: one per CTA, so that short sequences' blocks run side by side;
-  // many: a page's, and several heads per CTA, which finds its pages once for
-  // them (14900 tokens of 8 heads, with the queries: 139 us with 16 tokens and
-  // one head per CTA, 100 us with 32 and four)
-  const bool many = a.t.tokens > 2048;
-  const int span = a.t.tokens <= 256 ? 1 : many ? a.c.page_size : 16;
-  const int heads_each = many ? 4 : 1;
+  // Few tokens: one per CTA, so that short sequences' blocks run side by side;
+  // more: 16, among them one CTA's queries. A CTA takes four heads of short
+  // pages, which it finds once for them, one of long ones, two where there are
+  // many. us for one, two and four heads per CTA, BF16 with the queries: pages
+  // of 32, 16 query and 8 KV heads of 256, 500 tokens 11, 12, 13; 2100 tokens 26,
+  // 24, 17; 16000 tokens 141, 122, 111. Pages of 128, 2100 tokens 26, 45, 84;
+  // 8000 (992 blocks) 81, 75, 104. Pages of 256, 8000 tokens (496 blocks) 94,
+  // 113, 184; 16000 (992) 164, 161, 222. 32 tokens per CTA instead of 16: pages
+  // of 128, 64 query heads of 128, 2100 tokens 41 -> 62; 16000 170 -> 183 (four heads).
+  const int span = a.t.tokens <= 256 ? 1 : 16;
+  const long long blocks = static_cast<long long>(a.t.tokens) / a.c.page_size * 2 * a.c.heads;
+  const int heads_each = a.t.tokens <= 256 ? 1 : a.c.page_size <= 32 ? 4 : blocks >= 900 ? 2 : 1;
   const dim3 grid((a.t.tokens + span - 1) / span, 2 * ((a.c.heads + heads_each - 1) / heads_each) + (a.q ? 1 : 0));
   return launch_overlapped(kv_append_prompt_kernel<T, KIND, VP>, grid, 256, 0, stream, a, span, heads_each);
 }

@@ -1188,3 +1188,22 @@ def test_append_thousands_of_tokens(kind, dtype, page, heads, q_heads, dim, rota
                            sin=None if sin is None else sin.cuda(), interleaved=interleaved)
         assert torch.equal(got.cpu().view(torch.int16), want.view(torch.int16))
         same_cache(cache, plain)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [256, 257, 4100])
+@pytest.mark.parametrize("kind,page,heads,dim", [("int8", 64, 9, 128), ("e4m3", 16, 3, 256), ("int8", 128, 5, 64)])
+def test_append_heads_per_block_of_threads(tokens, kind, page, heads, dim):
+    """One, two or four heads per CTA, by the tokens and the page; heads that
+    do not divide by them."""
+    g = torch.Generator().manual_seed(tokens)
+    table, pool = random_tables(g, [tokens + 5], page)
+    cache, plain = make_pair(pool, page, heads, dim, kind)
+    cos, sin = rope(g, tokens + 5, dim // 2)
+    for new, length in ((5, 5), (tokens, tokens + 5)):
+        y = torch.randn(new, 2 * heads, dim, generator=g)
+        plain.append(y[:, :heads], y[:, heads:], table, [length], [0, new], cos, sin)
+        d = y.cuda()
+        cache.append(d[:, :heads], d[:, heads:], table.cuda(), torch.tensor([length], dtype=torch.int32).cuda(),
+                     query_start=torch.tensor([0, new], dtype=torch.int32).cuda(), cos=cos.cuda(), sin=sin.cuda())
+        same_cache(cache, plain)
