@@ -135,9 +135,9 @@ def generate(model: Decoder, prompts: list, new: int, top: int = 5, graph: bool 
     out.append(ids)
     captured = None
     if graph:
+        held = ids.clone()
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
-        held = ids.clone()
         with torch.cuda.stream(side):
             scratch = torch.zeros_like(lens)
             step(held, scratch)  # padding rows: nothing is stored

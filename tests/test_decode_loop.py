@@ -59,3 +59,76 @@ def test_the_first_layer_sees_what_plain_attention_sees():
             want, size = p @ v, p @ v.abs()
             half_unit = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=1e-300))) - 8)
             assert bool(((got[b, h].double() - want).abs() <= half_unit + 2.0**-10 * size + 2.0**-24 * n * v.abs().max()).all())
+
+
+def test_the_captured_step_waits_for_its_inputs(monkeypatch):
+    """generate(graph=True) with a model that records what runs on which
+    stream: the side stream waits after the ids it reads have been written."""
+    import contextlib
+
+    import decode_loop
+
+    log, current = [], ["main"]
+
+    class Stream:
+        def __init__(self, name="side"):
+            self.name = name
+
+        def wait_stream(self, other):
+            log.append(("wait", self.name, other.name))
+
+    class Ids(torch.Tensor):
+        def clone(self):
+            log.append(("clone", current[0]))
+            return torch.Tensor.clone(self).as_subclass(torch.Tensor)
+
+    @contextlib.contextmanager
+    def on(stream):
+        before, current[0] = current[0], stream.name
+        yield
+        current[0] = before
+
+    class Graph:
+        def replay(self):
+            pass
+
+    class Cuda:
+        CUDAGraph = Graph
+
+        def __init__(self):
+            self.Stream, self.stream = Stream, on
+
+        def current_stream(self):
+            return Stream(current[0])
+
+        def graph(self, captured, stream=None):
+            return on(stream)
+
+    class Torch:  # torch, on the CPU, with the streams above
+        cuda = Cuda()
+
+        def __getattr__(self, name):
+            return getattr(torch, name)
+
+        def zeros(self, *shape, device=None, **rest):
+            return torch.zeros(*shape, **rest)
+
+    class Model:
+        shape = decode_loop.Shape()
+
+        def prefill(self, prompts, lens):
+            return torch.zeros(len(prompts), 4)
+
+        def forward(self, ids, lens):
+            log.append(("forward", current[0]))
+            return torch.zeros(len(ids), 4)
+
+        def logits(self, x):
+            return x.as_subclass(Ids)
+
+    monkeypatch.setattr(decode_loop, "torch", Torch())
+    monkeypatch.setattr(decode_loop, "token_logprobs",
+                        lambda logits, ids, **_: decode_loop.TokenLogprobs(*(torch.zeros(len(logits)) for _ in range(4))))
+    decode_loop.generate(Model(), [[1], [2]], 2, graph=True)
+    assert ("clone", "main") in log and ("forward", "side") in log
+    assert log.index(("clone", "main")) < log.index(("wait", "side", "main")) < log.index(("forward", "side"))
