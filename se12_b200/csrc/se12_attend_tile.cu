@@ -33,10 +33,9 @@
 //
 // The work list (sequences, KV heads, row tiles, KV tiles) is cut into runs of
 // equal cost, one per CTA, and a tile's CTAs are joined as in attend_rows_kernel.
-#include "se12_device.cuh"
-#include "se12_serve.h"
+#include "se12_attend.cuh"
 
-#include <cuda_fp16.h>
+#include <cuda_bf16.h>
 
 namespace se12 {
 
@@ -293,8 +292,6 @@ struct TileSmem {
   float meta[kTileMeta][8][2];        // [16 tokens of the tile][scale of keys, log2 of values' scale]
   int meta_missing[kTileMeta];        // bit g: those tokens' page is not there
   float row_scale[2][kTileAttendRows];  // of this pair and the next
-  float out_scale[kTileAttendRows];
-  float merged_ref[kTileAttendRows];
   // Pairs shared with other CTAs (a run's first and last) that this CTA
   // completes: where their parts are and where their rows go.
   struct {

@@ -60,12 +60,6 @@ __device__ __forceinline__ int tile_owner(int i, int units, int grid, int stage)
   return static_cast<int>(((u + 1) * grid - 1) / units);
 }
 
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t selector) {
-  uint32_t d;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(selector));
-  return d;
-}
-
 // (a & m) | (b & ~m)
 __device__ __forceinline__ uint32_t select_bits(uint32_t a, uint32_t b, uint32_t m) {
   uint32_t d;

@@ -121,7 +121,8 @@ int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const
   if (st != SE12_OK) return st;
   if (!p || !p->k || !p->v) return fail(SE12_ERR_INVALID_ARGUMENT, "null keys or values");
   if (p->q && (!p->q_out || p->q_heads < 1)) return fail(SE12_ERR_INVALID_ARGUMENT, "queries need q_out and q_heads");
-  if (p->q && p->q_heads > 65535 * 4) return fail(SE12_ERR_INVALID_ARGUMENT, "too many query heads");
+  if (static_cast<long long>(batch->seqs) * (p->q ? p->q_heads : 0) > INT32_MAX)
+    return fail(SE12_ERR_INVALID_ARGUMENT, "too many query heads");
   if (!p->cos != !p->sin) return fail(SE12_ERR_INVALID_ARGUMENT, "cos and sin go together");
   if (p->cos && (p->rotary_dim < 2 || p->rotary_dim % 2 || p->rotary_dim > cache->view.dim))
     return fail(SE12_ERR_INVALID_ARGUMENT, "rotary_dim must be even, in 2..head_dim");
