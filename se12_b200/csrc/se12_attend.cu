@@ -702,6 +702,9 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
     done += run;
     here = advance(at, run);
   }
+  if (dead) {  // copies may still be on their way into this warp's stages
+    for (int i = 0; i < kAttendStages; ++i) mbar_wait(&sm.full[warp][i], i >= stage ? phase : phase ^ 1);
+  }
 }
 
 // ------------------------------------------------------------------ launch

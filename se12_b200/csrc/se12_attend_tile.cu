@@ -299,7 +299,7 @@ struct TileSmem {
   } join[2];
   int joins;
   uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
-  uint64_t q_full[2], q_free, o_free;
+  uint64_t q_full[2], q_free, o_free, drained;
   uint64_t meta_full[kTileMeta];
   uint32_t tmem;
   int bounds[2];  // of this CTA's run
@@ -587,6 +587,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
     mbar_init(&sm.q_full[1], kTileQueryWarps);
     sm.joins = 0;
     mbar_init(&sm.o_free, kTileSoftmaxWarps);
+    mbar_init(&sm.drained, 1);
     fence_barrier_init();
   }
   if (warp == kIssuer) tmem_alloc(&sm.tmem, 512);
@@ -684,6 +685,10 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
         done += run;
         g += run;
         if (g < g1) tile_next_pair<TT>(a, sm.before, &at);
+      }
+      if (dead) {  // products may still be reading the tiles and tensor memory
+        tc_commit(&sm.drained, elected);
+        mbar_wait(&sm.drained, 0);
       }
     }
     __syncwarp();

@@ -269,11 +269,14 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
   const uint64_t policy = policy_evict_first();
   // batch n of this CTA's run on its way into its stage: whole vectors only
   int copy_row = u0 / a.chunks_per_row, copy_chunk = u0 - copy_row * a.chunks_per_row;
-  bool dead = false;  // a wait ran out (status raised)
+  int dead = 0;  // a wait ran out (status raised); in thread 0: after so many copies, its last
   auto copy = [&](int n) {  // in order, by thread 0
-    if (n >= batches) return;
+    if (n >= batches || dead) return;
     const int stage = n % kLogprobStages;
-    if (n >= kLogprobStages && !dead) dead = !mbar_wait(&sm.empty[stage], (n / kLogprobStages + 1) & 1);
+    if (n >= kLogprobStages && !mbar_wait(&sm.empty[stage], (n / kLogprobStages + 1) & 1)) {
+      dead = n;
+      return;
+    }
     const int base = copy_chunk * kBatch;
     const int bytes = min(kBatch, a.vocab - base) * kSize / 16 * 16;
     mbar_arrive_expect_tx(&sm.full[stage], bytes);
@@ -319,7 +322,8 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
       };
       float x[kValues];
       if (a.vec) {
-        if (!dead) dead = !mbar_wait(&sm.full[stage_id], (batch / kLogprobStages) & 1);
+        if (!dead && !mbar_wait(&sm.full[stage_id], (batch / kLogprobStages) & 1))
+          dead = int_min(int_max(batch - 1, 0) + kLogprobStages, batches);
 #pragma unroll
         for (int j = 0; j < VECS; ++j)
           unpack<BF16>(x + j * kPer, *reinterpret_cast<const uint4*>(stage + (j * kLogprobThreads + threadIdx.x) * 16));
@@ -580,6 +584,9 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
     }
     __syncthreads();
     u = stop;
+  }
+  if (dead && threadIdx.x == 0) {  // copies may still be on their way into the stages
+    for (int n = int_max(dead - kLogprobStages, 0); n < dead; ++n) mbar_wait(&sm.full[n % kLogprobStages], (n / kLogprobStages) & 1);
   }
 }
 
