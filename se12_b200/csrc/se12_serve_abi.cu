@@ -66,6 +66,10 @@ int check_batch(const se12_kv_cache* cache, const se12_kv_batch* b, se12::TokenB
   return SE12_OK;
 }
 
+// A cap below 1e-30 as 1e-30: its reciprocal stays finite, and either way the
+// logits differ by nothing that an exponential shows.
+float usable_cap(float softcap) { return softcap > 0.f && softcap < 1e-30f ? 1e-30f : softcap; }
+
 }  // namespace
 
 extern "C" {
@@ -197,7 +201,7 @@ int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const
   a.q_heads = p->q_heads;
   a.group = group;
   a.scale = p->scale;
-  a.softcap = p->softcap;
+  a.softcap = usable_cap(p->softcap);
   // (a window as long as the page table hides nothing)
   a.window = p->window < batch->max_pages * v.page_size ? p->window : 0;
   a.counters = static_cast<int*>(workspace);
@@ -249,7 +253,7 @@ int se12_token_logprobs(const void* logits, int bf16, int rows, int vocab, int64
   a.vocab = vocab;
   a.tokens = reinterpret_cast<const long long*>(tokens);
   a.top = top;
-  a.softcap = softcap;
+  a.softcap = usable_cap(softcap);
   a.logprob = logprob;
   a.entropy = entropy;
   a.top_ids = reinterpret_cast<long long*>(top_ids);

@@ -1207,3 +1207,17 @@ def test_append_heads_per_block_of_threads(tokens, kind, page, heads, dim):
         cache.append(d[:, :heads], d[:, heads:], table.cuda(), torch.tensor([length], dtype=torch.int32).cuda(),
                      query_start=torch.tensor([0, new], dtype=torch.int32).cuda(), cos=cos.cuda(), sin=sin.cuda())
         same_cache(cache, plain)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 40])
+def test_attend_under_a_vanishing_cap_is_the_mean(n):
+    """All weights are equal, a zero query's among them."""
+    g = torch.Generator().manual_seed(n)
+    table, pool = random_tables(g, [60], 16)
+    cache, keys, values = filled(g, pool, 16, 2, 128, "int8")
+    q = torch.randn(n, 8, 128, generator=g).to(torch.bfloat16)
+    q[0, 1] = 0.0
+    start = torch.tensor([0, n], dtype=torch.int32).cuda()
+    got = cache.attend(q.cuda(), table.cuda(), torch.tensor([60], dtype=torch.int32).cuda(), query_start=start, softcap=1e-40)
+    check_attend(got, *plain_attend(q, keys, values, table, [60], [0, n], 0.0, 0.0, 0), 60)

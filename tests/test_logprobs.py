@@ -377,3 +377,26 @@ def test_caps_of_any_size(softcap, dtype, banned):
     for a, b in ((got.logprob, want[0]), (got.entropy, want[1]), (got.top_logprobs, want[3])):
         tol = 1e-5 + 6 * 2.0**-23 * largest + 2.0**-21 * b.abs()
         assert bool(((a.double().cpu() - b).abs() <= tol).all()), float(((a.double().cpu() - b).abs() / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [100, 20000])
+def test_infinite_logits_under_a_cap(vocab):
+    """+inf is a logit of the cap there, NaN stays NaN."""
+    x, t = logits(18, 4, vocab)
+    x[1, vocab - 1] = math.inf
+    x[2, 0] = math.nan
+    x[3] = -math.inf
+    x[3, 7] = math.inf
+    got = check(x, t, 8, softcap=30.0)
+    assert bool(torch.isfinite(got.entropy[1])) and bool(got.entropy[2].isnan())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("softcap", [1e-20, 1e-38, 1e-40])
+def test_a_vanishing_cap_makes_all_tokens_equal(softcap):
+    x, t = logits(19, 2, 500)
+    x[0, 3] = 0.0
+    got = token_logprobs(x.cuda(), t.cuda(), top=2, softcap=softcap)
+    for v in (got.logprob, got.top_logprobs):
+        assert bool(((v.double() + math.log(500)).abs() < 1e-5).all())
