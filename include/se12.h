@@ -489,8 +489,9 @@ int se12_kv_decode(const se12_kv_cache* cache, const int32_t* pages_dev, int cou
  * logprob[i] of token tokens[i] (a negative id: none, NaN), the entropy of the
  * row's distribution, and the `top` (0 .. SE12_LOGPROBS_MAX_TOP) largest
  * logits' ids and log probabilities, ties to the lowest id. With softcap > 0
- * the logits are softcap * tanh(x / softcap), -inf staying -inf. A NaN or +inf
- * in a row, or nothing but -inf, makes its log probabilities and entropy NaN.
+ * the logits are softcap * tanh(x / softcap), -inf staying -inf. A NaN in a
+ * row, +inf without a cap, or nothing but -inf makes its log probabilities and
+ * entropy NaN; with a cap +inf is a logit of softcap.
  * Workspace as for se12_kv_attend. */
 #define SE12_LOGPROBS_MAX_TOP 32
 size_t se12_token_logprobs_workspace_bytes(void);

@@ -125,7 +125,9 @@ class PagedKvCache:
     @classmethod
     def from_tensors(cls, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
                      kind: str = "int8") -> "PagedKvCache":
-        """A cache over existing contiguous tensors (used in place, not copied)."""
+        """A cache over existing contiguous tensors (used in place, not copied).
+        e4m3 codes are finite ones (append writes no others): attention multiplies
+        a hidden token's values by a weight of zero."""
         if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
             raise ValueError("codes must be [pages, kv_heads, page_size, head_dim], the same for keys and values")
         pages, heads, page_size, dim = k_codes.shape
