@@ -1221,3 +1221,20 @@ def test_attend_under_a_vanishing_cap_is_the_mean(n):
     start = torch.tensor([0, n], dtype=torch.int32).cuda()
     got = cache.attend(q.cuda(), table.cuda(), torch.tensor([60], dtype=torch.int32).cuda(), query_start=start, softcap=1e-40)
     check_attend(got, *plain_attend(q, keys, values, table, [60], [0, n], 0.0, 0.0, 0), 60)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 20])
+def test_attend_as_many_sequences_as_there_may_be(n):
+    from se12_b200.kv_cache import MAX_SEQS
+
+    g = torch.Generator().manual_seed(n)
+    lens = [n + (i * 37) % 50 for i in range(MAX_SEQS)]
+    table, pool = random_tables(g, lens, 16)
+    cache, _, _ = filled(g, pool, 16, 1, 64, "int8")
+    q = torch.randn(n * MAX_SEQS, 2, 64, generator=g).to(torch.bfloat16).cuda()
+    got = cache.attend(q, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), max_query=n,
+                       query_start=torch.tensor(starts_of([n] * MAX_SEQS), dtype=torch.int32).cuda())
+    some = list(range(0, MAX_SEQS, 97)) + [MAX_SEQS - 1]
+    rows = torch.cat([torch.arange(b * n, b * n + n) for b in some]).cuda()
+    check_on_gpu(cache, q[rows], table[some].cuda(), [lens[b] for b in some], [n] * len(some), got[rows], 0.0, 0)
