@@ -46,13 +46,20 @@ constexpr int kLogprobHolders = 128;  // threads whose values are looked through
 // zero and its product with log2(e) still finite.
 constexpr float kLogprobFloor = -2.0e38f;
 // Where every running maximum starts: far enough above the floor that floor
-// values add nothing to a sum, below every logit that counts. A row that
-// ends there is summed again in 64 bits.
+// values add nothing to a sum, below every logit that counts.
 constexpr float kLogprobStart = -1.0e38f;
+
+// Whether a maximum (in units of log 2) is one the sums below it can be told
+// from. Elsewhere the row's largest value itself decides: with infinities the
+// row is NaN; with finite values that large (masks of the type's lowest value
+// alone, forced tokens near its largest) any two that differ do so by more than
+// 2^100, so that the sum is the number of values equal to the largest.
+__device__ __forceinline__ bool usual_maximum(float max) { return max > kLogprobStart && max < 1e38f; }
 
 // A CTA's part of a row, for the CTA that joins them.
 struct LogprobPart {
-  float max, sum, weighted, pad;  // of z * log2(e): max; sum 2^(z - max); sum 2^(z - max) (z - max)
+  float max, sum, weighted;  // of z * log2(e): max; sum 2^(z - max); sum 2^(z - max) (z - max)
+  float largest;             // value of the part, where the maximum is not a usual one (0 otherwise)
   unsigned long long list[kLogprobTop];  // sorted, largest first
 };
 
@@ -109,13 +116,15 @@ struct LogprobSmem {
   unsigned long long buffer[kLogprobBuffer];
   unsigned long long lists[kLogprobWarps][32];
   unsigned long long list[32];
-  float stat[kLogprobWarps][3];
+  float stat[kLogprobWarps][4];
   float maxima[kLogprobWarps][32];
   float bound;
   int holders[kLogprobThreads];  // threads that hold something of the list
   int held;
   int count;
   int last;
+  int equal;      // 1: the row's sum is the number of values equal to `extreme`
+  float extreme;
   uint64_t full[kLogprobStages], empty[kLogprobStages];
 };
 
@@ -410,10 +419,17 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
                   w2 = __shfl_xor_sync(0xFFFFFFFFu, weighted, d);
       join_sums(max, sum, weighted, m2, s2, w2);
     }
+    float extreme = 0.f;  // the largest value, where the maximum is not a usual one
+    if (!usual_maximum(max)) {
+      extreme = largest;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) extreme = fmaxf(extreme, __shfl_xor_sync(0xFFFFFFFFu, extreme, d));
+    }
     if (lane == 0) {
       sm.stat[warp][0] = max;
       sm.stat[warp][1] = sum;
       sm.stat[warp][2] = weighted;
+      sm.stat[warp][3] = extreme;
     }
     if (a.top) {
       // ---- the segment's list
@@ -470,6 +486,11 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
                     w2 = __shfl_xor_sync(0xFFFFFFFFu, weighted, d);
         join_sums(max, sum, weighted, m2, s2, w2);
       }
+      extreme = 0.f;
+      if (!usual_maximum(max)) {
+        extreme = kNegInf;
+        for (int i = 0; i < kLogprobWarps; ++i) extreme = fmaxf(extreme, sm.stat[i][3]);
+      }
     }
     const int cta_first = row_u0 / a.units_per_cta, cta_last = (row_u1 - 1) / a.units_per_cta;
     unsigned long long mine = warp == 0 ? sm.list[lane] : 0ull;
@@ -479,7 +500,7 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
       LogprobPart* part = parts + blockIdx.x * 2 + (row_u0 > u0 ? 1 : 0);
       if (warp == 0) {
         part->list[lane] = mine;
-        if (lane == 0) part->max = max, part->sum = sum, part->weighted = weighted;
+        if (lane == 0) part->max = max, part->sum = sum, part->weighted = weighted, part->largest = extreme;
         __threadfence();
         __syncwarp();
         if (lane == 0) {
@@ -525,38 +546,20 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
         if (warp == 0) {
           max = sm.stat[0][0], sum = sm.stat[0][1], weighted = sm.stat[0][2];
           for (int i = 1; i < kLogprobWarps; ++i) join_sums(max, sum, weighted, sm.stat[i][0], sm.stat[i][1], sm.stat[i][2]);
+          if (!usual_maximum(max)) {
+            extreme = kNegInf;
+            for (int i = 0; i < count; ++i) extreme = fmaxf(extreme, __ldcg(&(i == 0 ? first_part : parts + (cta_first + i) * 2)->largest));
+          }
         }
       }
     }
     if (finish && warp == 0) {
-      // a row with nothing above the start, values past fp32's range in units
-      // of log 2, infinities or NaN: again in 64 bits from its true maximum
-      float low_max = kNegInf;
-      const bool again = !(max > kLogprobStart && max < 1e38f);
-      if (again) {
-        double s = 0.0, w = 0.0;
-        for (long long i = lane; i < a.vocab; i += 32) {
-          const float x = load_logit<BF16>(row, i);
-          low_max = fmaxf(low_max, CAP ? capped(x, a.softcap, inverse) : x);
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) low_max = fmaxf(low_max, __shfl_xor_sync(0xFFFFFFFFu, low_max, d));
-        for (long long i = lane; i < a.vocab; i += 32) {
-          const float x = load_logit<BF16>(row, i);
-          const double below = static_cast<double>(CAP ? capped(x, a.softcap, inverse) : x) - low_max;  // -inf - -inf: NaN, as it must be
-          const double e = exp(below);
-          s += e;
-          if (e > 0.0) w += e * below;
-          else if (e != e) w = e;
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-          s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-          w += __shfl_xor_sync(0xFFFFFFFFu, w, d);
-        }
-        sum = static_cast<float>(s);
-        weighted = static_cast<float>(w * 1.4426950408889634);
+      bool equal = false;
+      if (!usual_maximum(max)) {
+        equal = !CAP && fabsf(extreme) < INFINITY;
+        if (!equal) sum = __uint_as_float(0x7FC00000u);
       }
+      if (lane == 0) sm.equal = equal, sm.extreme = extreme, sm.count = 0;
       // lse = (max + log2 sum) ln 2; differences to the maximum first, so
       // that large logits lose nothing
       constexpr float kLn2 = 0.6931471805599453f;
@@ -566,7 +569,6 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
       auto log_prob = [&](float x) {
         const float z = CAP ? capped(x, a.softcap, inverse) : x;
         if (sum != sum) return sum;
-        if (again) return at_most_zero((z - low_max) - log_sum);
         if (z < kLogprobStart) return z - (max * kLn2 + log_sum);  // would leave fp32's range in units of log 2
         return at_most_zero(fmaf(z, kLog2e, -max) * kLn2 - log_sum);
       };
@@ -583,6 +585,36 @@ __global__ void __launch_bounds__(kLogprobThreads, kLogprobCtas) token_logprobs_
       }
     }
     __syncthreads();
+    if (!CAP && finish && sm.equal) {
+      // ---- the values equal to the largest, counted by all threads
+      const float value = sm.extreme;
+      int count = 0;
+      const int whole = a.vec ? a.vocab / kPer : 0;  // vectors
+#pragma unroll 4
+      for (int i = threadIdx.x; i < whole; i += kLogprobThreads) {
+        float x[kPer];
+        unpack<BF16>(x, __ldcg(static_cast<const uint4*>(row) + i));
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) count += x[j] == value;
+      }
+      for (long long i = static_cast<long long>(whole) * kPer + threadIdx.x; i < a.vocab; i += kLogprobThreads)
+        count += load_logit<BF16>(row, i) == value;
+      count = __reduce_add_sync(0xFFFFFFFFu, count);
+      if (lane == 0) atomicAdd(&sm.count, count);
+      __syncthreads();
+      if (warp == 0) {
+        const float log_count = logf(static_cast<float>(sm.count));
+        if (lane == 0) {
+          if (token >= 0 && token < a.vocab) a.logprob[row_id] = (token_logit - value) - log_count;
+          a.entropy[row_id] = log_count;
+        }
+        if (lane < a.top) {
+          const long long at = static_cast<long long>(row_id) * a.top + lane;
+          a.top_logprobs[at] = (load_logit<BF16>(row, a.top_ids[at]) - value) - log_count;
+        }
+      }
+      __syncthreads();
+    }
     u = stop;
   }
   if (dead && threadIdx.x == 0) {  // copies may still be on their way into the stages

@@ -400,3 +400,53 @@ def test_a_vanishing_cap_makes_all_tokens_equal(softcap):
     got = token_logprobs(x.cuda(), t.cuda(), top=2, softcap=softcap)
     for v in (got.logprob, got.top_logprobs):
         assert bool(((v.double() + math.log(500)).abs() < 1e-5).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [40, 9001, 70000])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("top", [0, 9])
+def test_rows_that_are_summed_again(dtype, vocab, softcap, top):
+    """Empty rows, masks of the lowest value alone, values near the largest
+    and infinities, among ordinary rows, aligned and not."""
+    x, t = logits(20, 9, vocab, dtype)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x[1] = -math.inf
+    x[2] = low
+    x[3] = low
+    x[3, 5:30] = -math.inf
+    x[4, 7] = high
+    x[5, 3] = x[5, 30] = high
+    x[6, 11] = math.inf
+    x[7] = low / 2
+    x[7, 20:] = low / 2 * (1 + 2.0**-6)
+    check(x, t, top, softcap)
+    wide = torch.zeros(9, vocab + 3, dtype=dtype, device="cuda")[:, 1 : vocab + 1]
+    check(x, t, top, softcap, device_logits=wide.copy_(x))
+
+
+@pytest.mark.gpu
+def test_an_empty_row_does_not_hold_up_the_others():
+    """One row with nothing left among 16 takes no more than a few times the
+    others' time (it was seventy times: one warp went over the row twice)."""
+    x, t = logits(21, 16, 256000)
+    plain_rows, with_empty = x.cuda(), x.cuda()
+    with_empty[3] = -math.inf
+    t = t.cuda()
+
+    def time(logits_):
+        for _ in range(3):
+            token_logprobs(logits_, t, top=5)
+        best = math.inf
+        for _ in range(5):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            for _ in range(10):
+                token_logprobs(logits_, t, top=5)
+            end.record()
+            end.synchronize()
+            best = min(best, begin.elapsed_time(end))
+        return best
+
+    assert time(with_empty) < 10 * time(plain_rows)
