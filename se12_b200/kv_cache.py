@@ -34,6 +34,7 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_SEQS = 2048
 COUNTER_BYTES = 4096  # SE12_COUNTER_BYTES: the part of a workspace that must be zero before a call
 
+_INT_MAX = 2**31 - 1
 _FLOATS = (torch.float32, torch.bfloat16)
 _BF16 = (torch.bfloat16,)
 
@@ -282,8 +283,8 @@ class PagedKvCache:
         batch = self._batch(tokens, block_table, lens, query_start)
         if max_query is None:
             max_query = 1 if query_start is None else tokens
-        max_query = int(max_query)
-        args = _lib.KV_ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *out_strides, q_heads, max_query, int(window),
+        max_query = min(int(max_query), _INT_MAX)
+        args = _lib.KV_ATTEND.pack(q.data_ptr(), *q_strides, out.data_ptr(), *out_strides, q_heads, max_query, min(int(window), _INT_MAX),
                                    self.head_dim ** -0.5 if scale is None else scale, softcap)
         need = self._lib.se12_kv_attend_call_bytes(self._handle, q_heads, max_query)
         _launch(self.device, self._lib.se12_kv_attend, "se12_kv_attend", self._handle, batch, args, workspace=(_WORKSPACES, need))

@@ -1238,3 +1238,22 @@ def test_attend_as_many_sequences_as_there_may_be(n):
     some = list(range(0, MAX_SEQS, 97)) + [MAX_SEQS - 1]
     rows = torch.cat([torch.arange(b * n, b * n + n) for b in some]).cuda()
     check_on_gpu(cache, q[rows], table[some].cuda(), [lens[b] for b in some], [n] * len(some), got[rows], 0.0, 0)
+
+
+@pytest.mark.gpu
+def test_windows_and_row_counts_past_32_bits():
+    """A window of any length is a window; a row count past the batch's is
+    refused as any other is."""
+    from se12_b200.kv_cache import PagedKvCache
+
+    cache = PagedKvCache(4, 16, 2, 64)
+    x = torch.randn(2, 2, 64, device="cuda")
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    lens = torch.ones(2, dtype=torch.int32, device="cuda")
+    q = cache.append(x, x, table, lens, q=x)
+    want = cache.attend(q, table, lens)
+    for window in (2**31 - 1, 2**31, 2**63):
+        assert torch.equal(cache.attend(q, table, lens, window=window), want)
+    start = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError):
+        cache.attend(q, table, lens, query_start=start, max_query=2**40)
