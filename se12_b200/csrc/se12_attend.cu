@@ -17,9 +17,10 @@
 // a TMA pipeline of its own (no CTA-wide barrier inside a pair's chunks) and
 // its own references and sums; a pair's warps are joined in shared memory,
 // its CTAs through global memory by the CTA that finishes last, in CTA order.
-// Small CTAs, 2 or 3 per SM: 8 or 12 warps hide each other's latencies (8
-// warps in one CTA per SM took 142 us against 107 for 131071 tokens of 16 KV
-// heads of 128: 5.0 TB/s), and short sequences' pairs run side by side.
+// Small CTAs, 2 or 3 per SM: 8 or 12 warps hide each other's latencies (131071
+// tokens of 16 KV heads of 128, capped, calls repeated in a graph: 109 us, 4.9
+// TB/s; 8 warps in one CTA per SM took a third longer), and short sequences'
+// pairs run side by side.
 //
 // Layout of the products (mma.sync m16n8k16, tokens or dimensions as M,
 // query rows as N = 8): with a group of up to 8 query rows per KV head the
@@ -53,7 +54,8 @@ constexpr int kAttendDeposit = 8192;     // joining the warps' sums
 constexpr int kAttendSlotRows = 16;
 constexpr int kAttendSlotFloats = kAttendSlotRows * (256 + 4);  // sums, then (m, l, mp) per row
 constexpr int kAttendMaxCtas = 3;        // per SM
-// What a pair's queries, joins and output cost, in chunks. (64 sequences of 1000
+// What a pair's queries, joins and output cost, in chunks. (Calls repeated in a
+// graph; calls among others take more, 64 sequences 210 us. 64 of 1000
 // to 16384 tokens, 8 KV heads of 128, e4m3: uncounted 196 us; 4, 8 and 16: 188,
 // 183 and 185. 16 of 301 to 8191, window 4096, 8 heads of 256: 57 us; 52, 51 and
 // 50. 7 of 86 to 702 tokens: 24 us; 17, 16 and 16. Equal lengths gain little.)
@@ -717,6 +719,9 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
 // 72 and 75 (79 and 94), 64 of 100 to 8000 256 and 277 (292 and 334); at worst 16
 // of 1000 to 2000 48 and 47. At 48 rows 24 of 2040 took 96 and 78 us (106 and
 // 100). Heads of 256 (int8, capped), 24 of 2040: 135 and 121 at 24 rows.
+// The batch's largest sequence decides for all: 63 sequences with one new token
+// (2000 to 16000 tokens, 8 rows) and one with 512 (6000 tokens) take 765 us in
+// one call and 189 and 223 in two; batches like that are better split.
 bool kv_attend_takes_tiles(int max_query, int group, int dim) {
   return static_cast<long long>(max_query) * group > (dim <= 128 ? 32 : 16);
 }

@@ -27,9 +27,10 @@
 // scaled by the row's own thread, after P V of the tile before) and whether
 // the tile is usual: block scales within 2^60 of each other, capped logits
 // within |x / cap| <= 0.7, or below by so much that they weigh nothing, where
-// a polynomial of tanh serves (two special-function calls less per logit). A usual tile's second pass takes a handful
-// of instructions per logit; the sum l comes from the weights, by a factor per
-// 16 tokens. Other tiles take the slow way, eight tokens at a time.
+// a polynomial of tanh serves (two special-function calls less per logit). A
+// usual tile's second pass takes a handful of instructions per logit; the sum l
+// comes from the weights, by a factor per 16 tokens. Other tiles take the slow
+// way, eight tokens at a time.
 //
 // The work list (sequences, KV heads, row tiles, KV tiles) is cut into runs of
 // equal cost, one per CTA, and a tile's CTAs are joined as in attend_rows_kernel.
@@ -50,7 +51,8 @@ constexpr int kTileSoftmaxRegs = 208, kTileLoaderRegs = 104, kTileIssuerRegs = 8
 static_assert(kTileSoftmaxRegs + 2 * kTileLoaderRegs + kTileIssuerRegs <= 4 * 128, "more registers than the launch has");
 constexpr int kTileKvBytes = 32768;   // an FP16 tile of keys or values
 constexpr int kTileMeta = 4;          // tiles whose block scales are kept
-// What a pair's queries, first loads and output cost, in KV tiles. (24 sequences
+// What a pair's queries, first loads and output cost, in KV tiles. (Calls
+// repeated in a graph, before later checks added a few per cent: 24 sequences
 // of 77 to 4093 tokens, 2 to 6 new ones of 8 rows: uncounted 105 us, the SMs
 // active 63 % of the time; 2, 3, 4 and 6: 76, 78, 78 and 79 us. 3 sequences of
 // 2014 to 8655 tokens, 78 new ones, 256 dimensions: 70 us; 68, 63, 63 and 63.)

@@ -14,9 +14,9 @@
 // (32 at a time over a warp's lanes, the warps' lists then merged). Rows with
 // too many equal values for that (nearly all tokens banned) go through memory
 // once more. 1023 x 128256 BF16 logits, top 20, against a list kept during the
-// pass with the candidates pushed into a buffer: 118 us and 137 us, rows in
-// ascending order 129 us and 2604 us; but all rows with ten tokens left 285 us
-// and 201 us (16 such rows 32 us and 30 us).
+// pass with the candidates pushed into a buffer: 117 us and 137 us, rows in
+// ascending order 126 us and 2604 us; but all rows with ten tokens or none left
+// 245 us and 201 us (16 rows of 256000 34 us and 30 us).
 //
 // Rows come in batches of 8 KB (4 KB when there are few) by bulk copies, four
 // batches ahead, whatever row they belong to: with three CTAs per SM 96 KB are
@@ -24,8 +24,11 @@
 // the spilled registers of the inner loop cost four times the loop.) The warps
 // of a CTA meet at a row's end only. The batches of all rows are cut into
 // equal runs, one per CTA, and a row's CTAs are joined by the last to finish,
-// in CTA order. Streaming alone takes 83 us of the 118, twice what HBM needs
-// for the bytes: the instructions of a value bound it, not the bytes.
+// in CTA order. Streaming alone takes 85 us of the 117, twice what HBM needs
+// for the bytes. Neither fills its pipes: 2.2 of 4 instructions a cycle, special
+// functions 31 %, DRAM 36 %; the warps wait for copies (2.2 warps per issue) and,
+// at the rows' ends, for each other (1.6). Rows that are not on 16 bytes come by
+// scalar loads (1023 x 50257 BF16, top 20: 103 us, the bytes alone 16).
 #include "se12_device.cuh"
 #include "se12_serve.h"
 
