@@ -25,8 +25,8 @@
 // of a CTA meet at a row's end only. The batches of all rows are cut into
 // equal runs, one per CTA, and a row's CTAs are joined by the last to finish,
 // in CTA order. Streaming alone takes 85 us of the 117, twice what HBM needs
-// for the bytes. Neither fills its pipes: 2.2 of 4 instructions a cycle, special
-// functions 31 %, DRAM 36 %; the warps wait for copies (2.2 warps per issue) and,
+// for the bytes. Neither fills its pipes: 2.1 of 4 instructions a cycle, special
+// functions 32 %, DRAM 36 %; the warps wait for memory (2.4 warps per issue) and,
 // at the rows' ends, for each other (1.6). Rows that are not on 16 bytes come by
 // scalar loads (1023 x 50257 BF16, top 20: 103 us, the bytes alone 16).
 #include "se12_device.cuh"
