@@ -363,7 +363,7 @@ int se12_encode_raw(const uint16_t* w_dev, int rows, int cols, int ldw, const in
                     int16_t* raw_dev, void* stream);
 
 /*
- * The decode step around the GEMVs: a paged 8-bit key/value cache, attention
+ * The decode step around the GEMVs: a paged 8-bit or 4-bit key/value cache, attention
  * over it, and log probabilities of the LM head's logits. No counterpart in
  * the reference, which has the GEMV only. All of them are asynchronous on
  * `stream`, allocate nothing and can be captured in a graph; lengths, page
@@ -380,9 +380,21 @@ int se12_encode_raw(const uint16_t* w_dev, int rows, int cols, int ldw, const in
  *   codes:  [pages][kv_heads][page_size][head_dim] u8, 16-byte aligned
  *   scales: [pages][kv_heads] fp32
  * The handle keeps the pointers and TMA descriptors; it holds no device memory.
+ *
+ * kind int4 (head_dim 64, 128 or 256): every token of a head by itself, in
+ * groups of 64 dimensions, a value being (u - 8) * scale + offset, u a code
+ * 0..15; of a token's values all scales and offsets are relative to 2^E.
+ *   codes:    [pages][kv_heads][page_size][head_dim / 2] u8, 16-byte aligned; a
+ *             row's words of 8 codes (the first in the lowest bits), word 8 g + r
+ *             at place r * groups + g
+ *   k_scales: [pages][kv_heads][page_size][groups][scale, offset] fp16
+ *   v_scales: [pages][kv_heads][page_size / 16] cells of 32 * groups + 16 fp16:
+ *             [8 pairs of tokens][groups scales, groups offsets][2 tokens], [16] E
+ * both 16-byte aligned, scales and offsets of values finite.
  */
 #define SE12_KV_INT8 0
 #define SE12_KV_E4M3 1
+#define SE12_KV_INT4 4
 #define SE12_KV_MAX_SEQS 2048
 #define SE12_COUNTER_BYTES 4096
 
@@ -391,8 +403,8 @@ typedef struct se12_kv_pages {
   int32_t kind;
   void* k_codes;
   void* v_codes;
-  float* k_scales;
-  float* v_scales;
+  void* k_scales;
+  void* v_scales;
 } se12_kv_pages;
 
 typedef struct se12_kv_cache se12_kv_cache;
@@ -429,7 +441,11 @@ typedef struct se12_kv_batch {
  * that holds its tokens; when a token raises it, the block's older codes are
  * rounded again at the new scale. A block that receives a value that is not
  * finite gets the scale NaN, which attention over it returns, until the page
- * starts anew. Two sequences of a call must not append to one page. */
+ * starts anew. int4: scale = fp16((hi - lo) / 15) and offset = fp16(lo + 8 scale)
+ * of a group's largest and smallest value, for values of x 2^-E with E =
+ * floor(log2 max |x|) - 3, -30 at least; a key group that is not finite or passes
+ * 65000, and a token whose values are not finite or reach 2^34, are NaN. Two
+ * sequences of a call must not append to one page. */
 typedef struct se12_kv_append_args {
   int32_t bf16;                /* 0: q, k, v are fp32; 1: BF16 */
   int32_t q_heads;
@@ -448,6 +464,19 @@ typedef struct se12_kv_append_args {
 } se12_kv_append_args;
 
 int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_append_args* args, void* stream);
+
+/* The same with norms of the queries and keys of each head before the
+ * rotation: a row x becomes x / sqrt(mean(x^2) + eps) * weight, its squares
+ * summed in 64 bits. A null weight, or norms null: none for those rows. */
+typedef struct se12_kv_norms {
+  const void* q_weight;        /* device [head_dim], fp32 or BF16 */
+  const void* k_weight;
+  int32_t q_bf16, k_bf16;      /* 0: fp32; 1: BF16 */
+  double eps;                  /* finite, not negative */
+} se12_kv_norms;
+
+int se12_kv_append_normed(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_append_args* args,
+                          const se12_kv_norms* norms, void* stream);
 
 /* Attention of the batch's rows over their sequences:
  *   out_i = sum_j softmax_j(s_ij) v_j, s_ij = scale q_i . k_j, then, with
@@ -478,7 +507,7 @@ size_t se12_kv_attend_call_bytes(const se12_kv_cache* cache, int q_heads, int ma
 int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_attend_args* args,
                    void* workspace_dev, size_t workspace_bytes, void* stream);
 
-/* Pages read back as BF16 (exact): page ids pages_dev[0 .. count - 1], or the
+/* Pages read back as BF16 (exact; int4: rounded): page ids pages_dev[0 .. count - 1], or the
  * first `count` pages where it is null, into k_out and v_out
  * [count][kv_heads][page_size][head_dim], 16-byte aligned. */
 int se12_kv_decode(const se12_kv_cache* cache, const int32_t* pages_dev, int count, uint16_t* k_out, uint16_t* v_out,

@@ -72,9 +72,10 @@ class Se12KvPagesStruct(ctypes.Structure):
 
 # The argument blocks of the calls a decode step makes many of, as packed
 # bytes (a quarter of the time ctypes fields take): se12_kv_batch,
-# se12_kv_append_args and se12_kv_attend_args in include/se12.h, in order.
+# se12_kv_append_args, se12_kv_norms and se12_kv_attend_args in include/se12.h.
 KV_BATCH = struct.Struct("=2i3Qqi4x")
 KV_APPEND = struct.Struct("=2i3Q6q2Qq3i4xQ2q")
+KV_NORMS = struct.Struct("=2Q2id")
 KV_ATTEND = struct.Struct("=Q2qQ2q3i2f4x")
 
 
@@ -131,6 +132,7 @@ SIGNATURES = {
     "se12_kv_cache_create": (c_int, [ctypes.POINTER(Se12KvPagesStruct), ctypes.POINTER(c_void_p)]),
     "se12_kv_cache_destroy": (None, [c_void_p]),
     "se12_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),  # KV_BATCH, KV_APPEND bytes
+    "se12_kv_append_normed": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),  # and KV_NORMS bytes
     "se12_kv_attend_workspace_bytes": (c_size_t, [c_void_p]),
     "se12_kv_attend_call_bytes": (c_size_t, [c_void_p, c_int, c_int]),
     "se12_kv_attend": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),  # KV_BATCH, KV_ATTEND bytes

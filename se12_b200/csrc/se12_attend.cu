@@ -243,8 +243,8 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
     if (lane < SUBS) {
       sm.usable[warp][stage][lane] = use;
       if (use) {
-        cp_async_4(&sm.scales[warp][stage][lane][0], a.c.k_scales + block);
-        cp_async_4(&sm.scales[warp][stage][lane][1], a.c.v_scales + block);
+        cp_async_4(&sm.scales[warp][stage][lane][0], static_cast<const float*>(a.c.k_scales) + block);
+        cp_async_4(&sm.scales[warp][stage][lane][1], static_cast<const float*>(a.c.v_scales) + block);
         cp_async_mbar_arrive(bar);
       }
     }

@@ -860,8 +860,8 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       const int stage = j & 1;
       unsigned char* tile = tiles + stage * kTileKvBytes;
       if (keys && tid < 32) {
-        ks = rows_at >= 0 ? a.c.k_scales[rows_at >> a.c.page_shift] : 1.f;
-        vs = rows_at >= 0 ? a.c.v_scales[rows_at >> a.c.page_shift] : 1.f;
+        ks = rows_at >= 0 ? static_cast<const float*>(a.c.k_scales)[rows_at >> a.c.page_shift] : 1.f;
+        vs = rows_at >= 0 ? static_cast<const float*>(a.c.v_scales)[rows_at >> a.c.page_shift] : 1.f;
       }
       // the tile two before has been read by its products
       if (j >= 2) wait(keys ? &sm.s_full[stage] : &sm.pv_done[stage], ((j >> 1) + 1) & 1);

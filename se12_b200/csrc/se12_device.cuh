@@ -365,6 +365,21 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
+// ------------------------------------------------------------------ extremes
+
+// NaN where one of the two is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // ------------------------------------------------------------------ pairs of fp32
 
 // Two fp32 operations per instruction, each rounded as the scalar one.

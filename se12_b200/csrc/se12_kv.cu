@@ -14,10 +14,8 @@
 //
 // Both kernels are bound by memory: the new tokens are read once from HBM
 // (the second pass of a prompt block hits L2) and the codes written once.
-#include "se12_device.cuh"
-#include "se12_serve.h"
+#include "se12_kv.cuh"
 
-#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -53,37 +51,6 @@ __device__ __forceinline__ float code_value(uint32_t c) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(c), __NV_E4M3)));
 }
 
-__device__ __forceinline__ float load_value(const float* p) { return *p; }
-__device__ __forceinline__ float load_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-
-// VP consecutive elements (VP > 1: the address is a multiple of their size).
-template <int VP>
-__device__ __forceinline__ void load_vector(float (&x)[VP], const float* p) {
-  if constexpr (VP == 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-  } else if constexpr (VP == 2) {
-    const float2 v = *reinterpret_cast<const float2*>(p);
-    x[0] = v.x, x[1] = v.y;
-  } else {
-    x[0] = *p;
-  }
-}
-
-template <int VP>
-__device__ __forceinline__ void load_vector(float (&x)[VP], const __nv_bfloat16* p) {
-  if constexpr (VP == 4) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xFFFF0000u);
-    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xFFFF0000u);
-  } else if constexpr (VP == 2) {
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
-    x[0] = __uint_as_float(v << 16), x[1] = __uint_as_float(v & 0xFFFF0000u);
-  } else {
-    x[0] = load_value(p);
-  }
-}
-
 // A row of `dim` values as dim / 2 pairs (a, b): the pairs the rotation turns
 // together first, then neighbours. A lane takes VP consecutive pairs at a
 // time, so that both members stay in one lane.
@@ -104,24 +71,48 @@ struct PairMap {
   }
 };
 
-// (a, b) turned by the angle whose cosine and sine are c and s; each product
-// and each sum is rounded by itself, as elementary tensor operations do.
-__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
-  const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-  b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
-  a = x;
-}
+// A row's norm with the factor found for it.
+struct RowScale {
+  RowNorm norm;  // weight null: none
+  float factor;
+};
 
-// Calls f(a index, b index, values a, values b) for this lane's pairs of one row.
-template <int VP, typename T, typename F>
-__device__ __forceinline__ void for_row(const T* row, const PairMap& map, const float* cos, const float* sin, int lane,
-                                        F&& f) {
+template <int VP, typename T>
+__device__ __forceinline__ RowScale row_scale(const T* row, const PairMap& map, const RowNorm& norm, int dim, double eps,
+                                              int lane) {
+  RowScale r{norm, 1.f};
+  if (!norm.weight) return r;
+  double sum = 0.0;
   for (int p = lane * VP; p < map.pairs; p += 32 * VP) {
     float a[VP], b[VP];
     int ia, ib;
     map.at(p, ia, ib);
     load_vector<VP>(a, row + ia);
     load_vector<VP>(b, row + ib);
+    sum = add_squares<VP>(b, add_squares<VP>(a, sum));
+  }
+  r.factor = norm_factor(team_sum(sum, 32), dim, eps);
+  return r;
+}
+
+// Calls f(a index, b index, values a, values b) for this lane's pairs of one
+// row, normalised (NORM) and rotated.
+template <int VP, bool NORM, typename T, typename F>
+__device__ __forceinline__ void for_row(const T* row, const PairMap& map, const RowScale& scale, const float* cos,
+                                        const float* sin, int lane, F&& f) {
+  for (int p = lane * VP; p < map.pairs; p += 32 * VP) {
+    float a[VP], b[VP];
+    int ia, ib;
+    map.at(p, ia, ib);
+    load_vector<VP>(a, row + ia);
+    load_vector<VP>(b, row + ib);
+    if (NORM && scale.norm.weight) {
+      float w[VP];
+      load_weights<VP>(w, scale.norm, ia);
+      apply_norm<VP>(a, scale.factor, w);
+      load_weights<VP>(w, scale.norm, ib);
+      apply_norm<VP>(b, scale.factor, w);
+    }
     if (p < map.turned) {
       float c[VP], s[VP];
       load_vector<VP>(c, cos + p);
@@ -145,18 +136,20 @@ struct RowPart {
     load_vector<VP>(b, row + 32 * VP + lane * VP);
   }
 
+  __device__ __forceinline__ void normalise(const RowNorm& norm, int dim, double eps, int lane) {
+    const float factor = norm_factor(team_sum(add_squares<VP>(b, add_squares<VP>(a, 0.0)), 32), dim, eps);
+    float w[VP];
+    load_weights<VP>(w, norm, lane * VP);
+    apply_norm<VP>(a, factor, w);
+    load_weights<VP>(w, norm, 32 * VP + lane * VP);
+    apply_norm<VP>(b, factor, w);
+  }
+
   __device__ __forceinline__ void rotate(const float (&c)[VP], const float (&s)[VP]) {
 #pragma unroll
     for (int j = 0; j < VP; ++j) turn(a[j], b[j], c[j], s[j]);
   }
 };
-
-template <int VP>
-__device__ __forceinline__ unsigned magnitude_bits(const float (&x)[VP], unsigned m) {
-#pragma unroll
-  for (int j = 0; j < VP; ++j) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-  return m;
-}
 
 template <int KIND, int VP>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[VP], float inv) {
@@ -169,19 +162,6 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[VP], fl
     *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w);
   else
     *p = static_cast<uint8_t>(w);
-}
-
-template <int VP>
-__device__ __forceinline__ void store_bf16(uint16_t* p, const float (&x)[VP]) {
-  uint16_t h[VP];
-#pragma unroll
-  for (int j = 0; j < VP; ++j) h[j] = __bfloat16_as_ushort(__float2bfloat16_rn(x[j]));
-  if constexpr (VP == 4)
-    *reinterpret_cast<uint2*>(p) = make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
-  else if constexpr (VP == 2)
-    *reinterpret_cast<uint32_t*>(p) = h[0] | (static_cast<uint32_t>(h[1]) << 16);
-  else
-    *p = h[0];
 }
 
 // Rounds `bytes` codes (a multiple of 16) again after the scale grew by 1 / ratio.
@@ -199,18 +179,6 @@ __device__ __forceinline__ void shrink_codes(uint8_t* codes, int bytes, float ra
     }
     *reinterpret_cast<uint4*>(codes + i) = v;
   }
-}
-
-// Page of position `pos` of sequence b, or -1 (and the status word raised)
-// where the table has none for it.
-__device__ __forceinline__ int page_of(const TokenBatch& t, const KvView& c, int b, int pos) {
-  const int i = pos >> c.page_shift;
-  if (i < t.max_pages) {
-    const int page = t.table[b * t.table_stride + i];
-    if (page >= 0 && page < c.pages) return page;
-  }
-  raise_status(kStatusBadArgument);
-  return -1;
 }
 
 // Scale of a block with older tokens at scale `before` (`older`) once tokens
@@ -245,7 +213,7 @@ __device__ __forceinline__ PairMap pair_map(const AppendArgs& a, bool turned, in
 
 // One query row (token t, head h), rotated, as BF16. `pos` < 0: an inactive
 // row, written as zeros.
-template <typename T, int VP>
+template <typename T, int VP, bool NORM>
 __device__ __forceinline__ void rotate_query(const AppendArgs& a, int token, int head, int pos, int lane) {
   uint16_t* out = a.q_out + token * a.o_ts + head * a.o_hs;
   const bool bad = a.cos && pos >= a.rope_rows;
@@ -256,16 +224,18 @@ __device__ __forceinline__ void rotate_query(const AppendArgs& a, int token, int
   }
   const T* row = static_cast<const T*>(a.q) + token * a.q_ts + head * a.q_hs;
   PairMap map = pair_map(a, true, VP);
-  for_row<VP>(row, map, a.cos + pos * a.rope_stride, a.sin + pos * a.rope_stride, lane,
-              [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
-                store_bf16<VP>(out + ia, x);
-                store_bf16<VP>(out + ib, y);
-              });
+  RowScale scale{};
+  if (NORM) scale = row_scale<VP>(row, map, a.q_norm, a.c.dim, a.norm_eps, lane);
+  for_row<VP, NORM>(row, map, scale, a.cos + pos * a.rope_stride, a.sin + pos * a.rope_stride, lane,
+                    [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
+                      store_bf16<VP>(out + ia, x);
+                      store_bf16<VP>(out + ib, y);
+                    });
 }
 
 // One token per sequence: a warp per (sequence, KV head, keys or values) and
 // one per (sequence, query head).
-template <typename T, int KIND, int VP>
+template <typename T, int KIND, int VP, bool NORM>
 __global__ void __launch_bounds__(128) kv_append_step_kernel(const AppendArgs a) {
   grid_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -277,7 +247,7 @@ __global__ void __launch_bounds__(128) kv_append_step_kernel(const AppendArgs a)
   if (b >= a.t.seqs) return;
   const int pos = max(a.t.lens[b], 0) - 1;
   if (what >= 2 * a.c.heads) {
-    rotate_query<T, VP>(a, b, what - 2 * a.c.heads, pos, lane);
+    rotate_query<T, VP, NORM>(a, b, what - 2 * a.c.heads, pos, lane);
     return;
   }
   if (pos < 0) return;
@@ -296,10 +266,12 @@ __global__ void __launch_bounds__(128) kv_append_step_kernel(const AppendArgs a)
   const int slot = pos & (a.c.page_size - 1);
   const long long block = static_cast<long long>(page) * a.c.heads + head;
   uint8_t* codes = (keys ? a.c.k_codes : a.c.v_codes) + block * a.c.page_size * a.c.dim;
-  float* scale = (keys ? a.c.k_scales : a.c.v_scales) + block;
+  float* scale = static_cast<float*>(keys ? a.c.k_scales : a.c.v_scales) + block;
   const float before = *scale;
+  RowScale norm{};
+  if (NORM) norm = row_scale<VP>(row, map, keys ? a.k_norm : RowNorm{}, a.c.dim, a.norm_eps, lane);
   unsigned amax = 0;
-  for_row<VP>(row, map, cos, sin, lane, [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
+  for_row<VP, NORM>(row, map, norm, cos, sin, lane, [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
     amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
   });
   amax = __reduce_max_sync(0xFFFFFFFFu, amax);
@@ -309,7 +281,7 @@ __global__ void __launch_bounds__(128) kv_append_step_kernel(const AppendArgs a)
   if (ratio != 1.f) shrink_codes<KIND>(codes, slot * a.c.dim, ratio, lane, 32);
   const float inv = finite ? __frcp_rn(now) : 0.f;  // exact for the powers of two stored here
   uint8_t* to = codes + slot * a.c.dim;
-  for_row<VP>(row, map, cos, sin, lane, [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
+  for_row<VP, NORM>(row, map, norm, cos, sin, lane, [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
     if (finite) {
       store_codes<KIND, VP>(to + ia, x, inv);
       store_codes<KIND, VP>(to + ib, y, inv);
@@ -337,7 +309,7 @@ __device__ __forceinline__ int sequence_of(const TokenBatch& t, int token, int l
 // New tokens of one page (rows 0 .. count - 1 at src, slots slot ..) joined to
 // it by a CTA of 8 warps, for the heads head .. head + heads - 1 one after the
 // other: the next head's rows are on their way while this one's scale is found.
-template <typename T, int KIND, int VP>
+template <typename T, int KIND, int VP, bool NORM>
 __device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, const T* src, long long ts, long long hs, int head,
                                             int heads, int pos, int slot, int count, int page, unsigned (*s_amax)[8]) {
   constexpr int kHeld = 4;  // rows a warp keeps in registers from one pass to the next
@@ -346,7 +318,9 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, cons
   const bool turned = keys && a.cos;
   const bool held = VP > 1 && count <= 8 * kHeld;
   RowPart<VP> row[kHeld];
+  const RowNorm norm = NORM && keys ? a.k_norm : RowNorm{};
   auto rotate = [&](RowPart<VP>& r, int i) {
+    if (NORM && norm.weight) r.normalise(norm, dim, a.norm_eps, lane);
     if (turned) {
       float c[VP], s[VP];
       load_vector<VP>(c, a.cos + (pos + i) * a.rope_stride + lane * VP);
@@ -364,7 +338,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, cons
     const int h = head + n;
     const T* rows = src + h * hs;
     const long long block = static_cast<long long>(page) * a.c.heads + h;
-    float* scale = (keys ? a.c.k_scales : a.c.v_scales) + block;
+    float* scale = static_cast<float*>(keys ? a.c.k_scales : a.c.v_scales) + block;
     uint8_t* codes = (keys ? a.c.k_codes : a.c.v_codes) + block * a.c.page_size * dim;
     const float before = slot > 0 ? *scale : 0.f;
     unsigned amax = 0;
@@ -379,11 +353,14 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, cons
           }
       }
     } else {
-      for (int i = warp; i < count; i += 8)
-        for_row<VP>(rows + i * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
-                    [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
-                      amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
-                    });
+      for (int i = warp; i < count; i += 8) {
+        RowScale scaled{};
+        if (NORM) scaled = row_scale<VP>(rows + i * ts, map, norm, dim, a.norm_eps, lane);
+        for_row<VP, NORM>(rows + i * ts, map, scaled, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride,
+                          lane, [&](int, int, const float(&x)[VP], const float(&y)[VP]) {
+                            amax = magnitude_bits<VP>(y, magnitude_bits<VP>(x, amax));
+                          });
+      }
     }
     amax = __reduce_max_sync(0xFFFFFFFFu, amax);
     if (lane == 0) s_amax[n & 1][warp] = amax;
@@ -421,12 +398,15 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, cons
       }
       if (held && n + 1 < heads) load(h + 1, warp);
     } else {
-      for (int i = warp; i < count; i += 8)
-        for_row<VP>(rows + i * ts, map, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride, lane,
-                    [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
-                      put(to + i * dim + ia, x);
-                      put(to + i * dim + ib, y);
-                    });
+      for (int i = warp; i < count; i += 8) {
+        RowScale scaled{};
+        if (NORM) scaled = row_scale<VP>(rows + i * ts, map, norm, dim, a.norm_eps, lane);
+        for_row<VP, NORM>(rows + i * ts, map, scaled, a.cos + (pos + i) * a.rope_stride, a.sin + (pos + i) * a.rope_stride,
+                          lane, [&](int ia, int ib, const float(&x)[VP], const float(&y)[VP]) {
+                            put(to + i * dim + ia, x);
+                            put(to + i * dim + ib, y);
+                          });
+      }
     }
     if (threadIdx.x == 0) *scale = now;
   }
@@ -435,10 +415,10 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, cons
 
 // One token's queries, a warp: the angle's cosines and sines are loaded once
 // for all heads.
-template <typename T, int VP>
+template <typename T, int VP, bool NORM>
 __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int token, int pos, int lane) {
   if (VP == 1 || pos < 0 || (a.cos && pos >= a.rope_rows)) {
-    for (int h = 0; h < a.q_heads; ++h) rotate_query<T, VP>(a, token, h, pos, lane);
+    for (int h = 0; h < a.q_heads; ++h) rotate_query<T, VP, NORM>(a, token, h, pos, lane);
     return;
   }
   float c[VP], s[VP];
@@ -457,6 +437,7 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int token, i
 #pragma unroll
     for (int k = 0; k < kHeads; ++k)
       if (h0 + k < a.q_heads) {
+        if (NORM && a.q_norm.weight) row[k].normalise(a.q_norm, a.c.dim, a.norm_eps, lane);
         if (a.cos) row[k].rotate(c, s);
         store_bf16<VP>(out + (h0 + k) * a.o_hs + lane * VP, row[k].a);
         store_bf16<VP>(out + (h0 + k) * a.o_hs + 32 * VP + lane * VP, row[k].b);
@@ -471,7 +452,7 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int token, i
 // way at a time; up to 32 stay in registers while the scale is found, more are
 // read again from L2. The last blockIdx.y rotates the queries, a warp per
 // token.
-template <typename T, int KIND, int VP>
+template <typename T, int KIND, int VP, bool NORM>
 __global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendArgs a, const int span, const int heads_each) {
   __shared__ unsigned s_amax[2][8];
   grid_launch_dependents();
@@ -485,7 +466,7 @@ __global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendAr
       const int b = sequence_of(a.t, t, lane);
       const SeqRows s = a.t.rows_of(b, sizes);
       const int row = t - a.t.begin_of(b, sizes);
-      rotate_queries<T, VP>(a, t, row >= 0 && row < s.tokens ? s.first + row : -1, lane);
+      rotate_queries<T, VP, NORM>(a, t, row >= 0 && row < s.tokens ? s.first + row : -1, lane);
     }
     return;
   }
@@ -513,7 +494,7 @@ __global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendAr
       count = a.rope_rows - pos;
       if (count <= 0) continue;
     }
-    append_page<T, KIND, VP>(a, keys, src + t * ts, ts, keys ? a.k_hs : a.v_hs, head, min(heads_each, a.c.heads - head), pos,
+    append_page<T, KIND, VP, NORM>(a, keys, src + t * ts, ts, keys ? a.k_hs : a.v_hs, head, min(heads_each, a.c.heads - head), pos,
                              slot, count, page, s_amax);
   }
 }
@@ -527,7 +508,7 @@ __global__ void __launch_bounds__(256) kv_decode_kernel(const KvView c, const in
   grid_dependency_wait();
   const int block_codes = c.page_size * c.dim;  // a multiple of 256
   const uint8_t* codes = blockIdx.y ? c.v_codes : c.k_codes;
-  const float* scales = blockIdx.y ? c.v_scales : c.k_scales;
+  const float* scales = static_cast<const float*>(blockIdx.y ? c.v_scales : c.k_scales);
   uint16_t* outs = blockIdx.y ? v_out : k_out;
   const long long blocks = static_cast<long long>(count) * c.heads;
   for (long long n = blockIdx.x; n < blocks; n += gridDim.x) {
@@ -560,11 +541,11 @@ __global__ void __launch_bounds__(256) kv_decode_kernel(const KvView c, const in
 
 // ------------------------------------------------------------------ launches
 
-template <typename T, int KIND, int VP>
+template <typename T, int KIND, int VP, bool NORM>
 cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t stream) {
   if (!a.t.query_start) {
     const long long warps = static_cast<long long>(a.t.seqs) * (2 * a.c.heads + (a.q ? a.q_heads : 0));
-    return launch_overlapped(kv_append_step_kernel<T, KIND, VP>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0,
+    return launch_overlapped(kv_append_step_kernel<T, KIND, VP, NORM>, dim3(static_cast<unsigned>((warps + 3) / 4)), 128, 0,
                              stream, a);
   }
   // Few tokens: one per CTA, so that short sequences' blocks run side by side;
@@ -580,10 +561,10 @@ cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t stream) {
   const long long blocks = static_cast<long long>(a.t.tokens) / a.c.page_size * 2 * a.c.heads;
   const int heads_each = a.t.tokens <= 256 ? 1 : a.c.page_size <= 32 ? 4 : blocks >= 900 ? 2 : 1;
   const dim3 grid((a.t.tokens + span - 1) / span, 2 * ((a.c.heads + heads_each - 1) / heads_each) + (a.q ? 1 : 0));
-  return launch_overlapped(kv_append_prompt_kernel<T, KIND, VP>, grid, 256, 0, stream, a, span, heads_each);
+  return launch_overlapped(kv_append_prompt_kernel<T, KIND, VP, NORM>, grid, 256, 0, stream, a, span, heads_each);
 }
 
-template <typename T, int KIND>
+template <typename T, int KIND, bool NORM>
 cudaError_t launch_append_kind(const AppendArgs& a, cudaStream_t stream) {
   // vector lanes: whole rows turned in halves (or not at all), 32 * VP pairs
   // a step, and every row and table address a multiple of VP elements
@@ -597,19 +578,30 @@ cudaError_t launch_append_kind(const AppendArgs& a, cudaStream_t stream) {
     if (ptr[i] && (reinterpret_cast<uintptr_t>(ptr[i]) % (vp * sizeof(T)) || stride[2 * i] % vp || stride[2 * i + 1] % vp))
       vec = false;
   if (a.q && (reinterpret_cast<uintptr_t>(a.q_out) % (vp * 2) || a.o_ts % vp || a.o_hs % vp)) vec = false;
-  if (!vec) return launch_append_as<T, KIND, 1>(a, stream);
-  return vp == 4 ? launch_append_as<T, KIND, 4>(a, stream) : launch_append_as<T, KIND, 2>(a, stream);
+  for (const RowNorm& n : {a.q_norm, a.k_norm})
+    if (reinterpret_cast<uintptr_t>(n.weight) % (vp * (n.bf16 ? 2 : 4))) vec = false;
+  if (!vec) return launch_append_as<T, KIND, 1, NORM>(a, stream);
+  return vp == 4 ? launch_append_as<T, KIND, 4, NORM>(a, stream) : launch_append_as<T, KIND, 2, NORM>(a, stream);
+}
+
+template <typename T, int KIND>
+cudaError_t launch_append_normed(const AppendArgs& a, cudaStream_t stream) {
+  return a.q_norm.weight || a.k_norm.weight ? launch_append_kind<T, KIND, true>(a, stream)
+                                            : launch_append_kind<T, KIND, false>(a, stream);
 }
 
 cudaError_t launch_kv_append(bool bf16, const AppendArgs& a, cudaStream_t stream) {
+  if (a.c.kind == kKvInt4) return launch_kv4_append(bf16, a, stream);
   if (bf16)
-    return a.c.kind == kKvInt8 ? launch_append_kind<__nv_bfloat16, kKvInt8>(a, stream)
-                               : launch_append_kind<__nv_bfloat16, kKvE4m3>(a, stream);
-  return a.c.kind == kKvInt8 ? launch_append_kind<float, kKvInt8>(a, stream) : launch_append_kind<float, kKvE4m3>(a, stream);
+    return a.c.kind == kKvInt8 ? launch_append_normed<__nv_bfloat16, kKvInt8>(a, stream)
+                               : launch_append_normed<__nv_bfloat16, kKvE4m3>(a, stream);
+  return a.c.kind == kKvInt8 ? launch_append_normed<float, kKvInt8>(a, stream)
+                             : launch_append_normed<float, kKvE4m3>(a, stream);
 }
 
 cudaError_t launch_kv_decode(const KvView& c, const int32_t* pages, int count, uint16_t* k_out, uint16_t* v_out,
                              cudaStream_t stream) {
+  if (c.kind == kKvInt4) return launch_kv4_decode(c, pages, count, k_out, v_out, stream);
   const long long blocks = static_cast<long long>(count) * c.heads;
   const dim3 grid(static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20)), 2);
   return launch_overlapped(c.kind == kKvInt8 ? kv_decode_kernel<kKvInt8> : kv_decode_kernel<kKvE4m3>, grid, 256, 0, stream, c,

@@ -5,6 +5,7 @@
 #include "se12_chain.cu"
 #include "se12_abi.cu"
 #include "se12_kv.cu"
+#include "se12_kv4.cu"
 #include "se12_attend.cu"
 #include "se12_attend_tile.cu"
 #include "se12_logprobs.cu"

@@ -66,12 +66,6 @@ struct LogprobPart {
   unsigned long long list[kLogprobTop];  // sorted, largest first
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // Order of the top list: larger value first (NaN above all, -0 as 0), then
 // the lower index. 0: no entry.
 __device__ __forceinline__ unsigned long long list_key(float x, int index) {

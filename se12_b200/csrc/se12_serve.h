@@ -1,5 +1,5 @@
 // Host/device parameter blocks of the decode-step operators around the GEMVs:
-// the paged 8-bit key/value cache (se12_kv.cu), attention over it
+// the paged key/value cache in 8 and in 4 bits (se12_kv.cu, se12_kv4.cu), attention over it
 // (se12_attend.cu) and token log probabilities (se12_logprobs.cu). Not part
 // of the public interface (include/se12.h is).
 #pragma once
@@ -13,17 +13,19 @@
 
 namespace se12 {
 
-// Cache element kinds (SE12_KV_INT8, SE12_KV_E4M3).
+// Cache element kinds (SE12_KV_INT8, SE12_KV_E4M3, SE12_KV_INT4).
 constexpr int kKvInt8 = 0;
 constexpr int kKvE4m3 = 1;
+constexpr int kKvInt4 = 4;
 
 // One layer's cache on the device. A block is one page of one KV head:
-// codes [pages][heads][page_size][dim], one fp32 scale per block.
+// codes [pages][heads][page_size][dim], one fp32 scale per block; 4 bits: as
+// se12_kv4.cu has them.
 struct KvView {
   uint8_t* k_codes;
   uint8_t* v_codes;
-  float* k_scales;  // [pages][heads]
-  float* v_scales;
+  void* k_scales;
+  void* v_scales;
   int pages, page_size, page_shift;
   int heads, dim;
   int kind;
@@ -50,6 +52,12 @@ struct TokenBatch {
 #endif
 };
 
+// A row x becomes x / sqrt(mean(x^2) + eps), times the weights.
+struct RowNorm {
+  const void* weight;  // [dim], or null: no norm
+  int bf16;            // of the weights: fp32 or BF16
+};
+
 struct AppendArgs {
   KvView c;
   TokenBatch t;
@@ -62,6 +70,8 @@ struct AppendArgs {
   int interleaved;
   uint16_t* q_out;         // BF16
   long long o_ts, o_hs;
+  RowNorm q_norm, k_norm;  // before the rotation
+  double norm_eps;
 };
 
 struct AttendArgs {
@@ -102,6 +112,9 @@ struct LogprobArgs {
 cudaError_t launch_kv_append(bool bf16, const AppendArgs& a, cudaStream_t stream);
 cudaError_t launch_kv_decode(const KvView& c, const int32_t* pages, int count, uint16_t* k_out, uint16_t* v_out,
                              cudaStream_t stream);
+cudaError_t launch_kv4_append(bool bf16, const AppendArgs& a, cudaStream_t stream);
+cudaError_t launch_kv4_decode(const KvView& c, const int32_t* pages, int count, uint16_t* k_out, uint16_t* v_out,
+                              cudaStream_t stream);
 cudaError_t launch_kv_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int max_query,
                              int sm_count, cudaStream_t stream);
 size_t kv_attend_partial_bytes(int sm_count, bool tile);

@@ -4,6 +4,7 @@
 #include "se12_serve.h"
 
 #include <atomic>
+#include <cmath>
 
 struct se12_kv_cache {
   se12::KvView view;
@@ -22,11 +23,15 @@ static_assert(kMaxSms * se12::kAttendMaxCtas * sizeof(int) <= SE12_COUNTER_BYTES
 // 128 bytes (a page is a multiple of 16 tokens, so a box never leaves it;
 // columns past dim read as zero codes, which stand for zero).
 int encode_kv_map(CUtensorMap* map, const void* codes, const se12::KvView& v) {
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(v.dim),
-                              static_cast<cuuint64_t>(v.pages) * v.heads * v.page_size};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(v.dim)};
-  const cuuint32_t box[2] = {128, 16};
-  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box);
+  const bool four = v.kind == se12::kKvInt4;  // a box is 16 whole rows, swizzled as their length allows
+  const cuuint64_t row = four ? v.dim / 2 : v.dim;
+  const cuuint64_t dims[2] = {row, static_cast<cuuint64_t>(v.pages) * v.heads * v.page_size};
+  const cuuint64_t strides[1] = {row};
+  const cuuint32_t box[2] = {four ? static_cast<cuuint32_t>(row) : 128, 16};
+  const CUtensorMapSwizzle swizzle = !four || row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : row == 64         ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                         : CU_TENSOR_MAP_SWIZZLE_NONE;
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box, swizzle);
 }
 
 // SMs of the current device, at most kMaxSms; asked once per device.
@@ -82,14 +87,19 @@ int se12_kv_cache_create(const se12_kv_pages* p, se12_kv_cache** out) {
     return fail(SE12_ERR_INVALID_ARGUMENT, "page_size must be 16, 32, 64, 128 or 256, got " + std::to_string(p->page_size));
   if (p->head_dim < 16 || p->head_dim > 256 || p->head_dim % 16)
     return fail(SE12_ERR_INVALID_ARGUMENT, "head_dim must be a multiple of 16 up to 256, got " + std::to_string(p->head_dim));
-  if (p->kind != SE12_KV_INT8 && p->kind != SE12_KV_E4M3)
-    return fail(SE12_ERR_UNSUPPORTED_FORMAT, "kind must be SE12_KV_INT8 or SE12_KV_E4M3");
+  if (p->kind != SE12_KV_INT8 && p->kind != SE12_KV_E4M3 && p->kind != SE12_KV_INT4)
+    return fail(SE12_ERR_UNSUPPORTED_FORMAT, "kind must be SE12_KV_INT8, SE12_KV_E4M3 or SE12_KV_INT4");
+  const bool four = p->kind == SE12_KV_INT4;
+  if (four && p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+    return fail(SE12_ERR_INVALID_ARGUMENT, "head_dim must be 64, 128 or 256 in 4 bits, got " + std::to_string(p->head_dim));
   if (static_cast<long long>(p->pages) * p->kv_heads * p->page_size > INT32_MAX)
     return fail(SE12_ERR_INVALID_ARGUMENT, "pages * kv_heads * page_size must fit 31 bits");
   if (!p->k_codes || !p->v_codes || !p->k_scales || !p->v_scales)
     return fail(SE12_ERR_INVALID_ARGUMENT, "null cache pointer");
   if (!aligned16(p->k_codes) || !aligned16(p->v_codes))
     return fail(SE12_ERR_MISALIGNED, "cache codes must be 16-byte aligned");
+  if (four && (!aligned16(p->k_scales) || !aligned16(p->v_scales)))
+    return fail(SE12_ERR_MISALIGNED, "the scales of a 4-bit cache must be 16-byte aligned");
   int device = 0, sm_count = 0;
   int st = current_device_info(&device, &sm_count);
   if (st != SE12_OK) return st;
@@ -120,6 +130,11 @@ int se12_kv_cache_create(const se12_kv_pages* p, se12_kv_cache** out) {
 void se12_kv_cache_destroy(se12_kv_cache* c) { delete c; }
 
 int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_append_args* p, void* stream) {
+  return se12_kv_append_normed(cache, batch, p, nullptr, stream);
+}
+
+int se12_kv_append_normed(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_append_args* p,
+                          const se12_kv_norms* norms, void* stream) {
   se12::AppendArgs a{};
   const int st = check_batch(cache, batch, &a.t);
   if (st != SE12_OK) return st;
@@ -132,6 +147,13 @@ int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const
     return fail(SE12_ERR_INVALID_ARGUMENT, "rotary_dim must be even, in 2..head_dim");
   if (p->cos && (p->rope_rows < 1 || p->rope_stride < 0))
     return fail(SE12_ERR_INVALID_ARGUMENT, "the rotation table needs a row, and a rope_stride that is not negative");
+  if (norms) {
+    if (!(norms->eps >= 0.0) || std::isinf(norms->eps))
+      return fail(SE12_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+    a.q_norm = {p->q ? norms->q_weight : nullptr, norms->q_bf16};
+    a.k_norm = {norms->k_weight, norms->k_bf16};
+    a.norm_eps = norms->eps;
+  }
   a.c = cache->view;
   a.q = p->q;
   a.k = p->k;
@@ -173,6 +195,7 @@ int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const
   if (st != SE12_OK) return st;
   if (!p || !p->q || !p->out) return fail(SE12_ERR_INVALID_ARGUMENT, "null queries or output");
   const se12::KvView& v = cache->view;
+  if (v.kind == SE12_KV_INT4) return fail(SE12_ERR_UNSUPPORTED_FORMAT, "attention over 4-bit pages is not built");
   if (p->q_heads < 1 || p->q_heads % v.heads)
     return fail(SE12_ERR_INVALID_ARGUMENT, "q_heads must be a multiple of kv_heads");
   if (p->max_query < 1 || p->max_query > batch->tokens || (!batch->query_start && p->max_query != 1))

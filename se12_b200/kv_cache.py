@@ -22,6 +22,7 @@ stream; nothing here has a CPU path.
 from __future__ import annotations
 
 import ctypes
+import math
 import weakref
 
 import torch
@@ -29,7 +30,9 @@ import torch
 from . import _lib
 from .device import _WorkspacePool
 
-KINDS = {"int8": 0, "e4m3": 1}
+KINDS = {"int8": 0, "e4m3": 1, "int4": 4}
+INT4_GROUP = 64  # dimensions that share a scale and an offset in 4 bits
+INT4_HEAD_DIMS = (64, 128, 256)
 PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_SEQS = 2048
 COUNTER_BYTES = 4096  # SE12_COUNTER_BYTES: the part of a workspace that must be zero before a call
@@ -98,15 +101,35 @@ class PagedKvCache:
     """``pages`` pages of ``page_size`` tokens (16, 32, 64, 128 or 256) of
     ``kv_heads`` heads of ``head_dim`` (a multiple of 16 up to 256) values,
     for keys and for values. ``kind``: "int8" (codes of 7 bits and a sign,
-    for heads whose values spread evenly) or "e4m3" (for wide ranges).
+    for heads whose values spread evenly), "e4m3" (for wide ranges) or "int4"
+    (4.6 bits a value with the scales; head_dim 64, 128 or 256).
 
     ``k_codes`` and ``v_codes`` are [pages, kv_heads, page_size, head_dim]
     int8 tensors (e4m3: the bit patterns), ``k_scales`` and ``v_scales`` [pages,
-    kv_heads] fp32; a value is code * scale."""
+    kv_heads] fp32; a value is code * scale.
+
+    "int4" quantises every token of a head by itself, in groups of 64
+    dimensions: a value is (u - 8) * scale + offset, u its code 0..15.
+    ``k_codes`` and ``v_codes`` are uint8 [pages, kv_heads, page_size,
+    head_dim / 2]: words of 8 codes, the first in the lowest bits, word 8 g + r
+    of a row at place r * groups + g. ``k_scales`` is fp16 [pages, kv_heads,
+    page_size, groups, 2] (scale, offset); ``v_scales`` fp16 [pages, kv_heads,
+    page_size / 16, 32 * groups + 16]: of 16 tokens, for each two neighbours
+    the groups' scales and then their offsets (the two tokens' side by side),
+    then a whole number E per token: its values are 2^E times what scale and
+    offset give. Scales and offsets of values are finite; E is NaN for a token
+    whose values were not."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, kind: str = "int8", device="cuda"):
         self._check(pages, page_size, kv_heads, head_dim, kind)
         device = torch.device(device)
+        if kind == "int4":
+            groups = head_dim // INT4_GROUP
+            codes = (pages, kv_heads, page_size, head_dim // 2)
+            self._adopt(torch.zeros(codes, dtype=torch.uint8, device=device), torch.zeros(codes, dtype=torch.uint8, device=device),
+                        torch.zeros(pages, kv_heads, page_size, groups, 2, dtype=torch.float16, device=device),
+                        torch.zeros(pages, kv_heads, page_size // 16, 32 * groups + 16, dtype=torch.float16, device=device), kind)
+            return
         shape = (pages, kv_heads, page_size, head_dim)
         self._adopt(torch.zeros(shape, dtype=torch.int8, device=device), torch.zeros(shape, dtype=torch.int8, device=device),
                     torch.ones(shape[:2], dtype=torch.float32, device=device),
@@ -120,7 +143,10 @@ class PagedKvCache:
             raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
         if pages < 1 or kv_heads < 1:
             raise ValueError("pages and kv_heads must be positive")
-        if head_dim < 16 or head_dim > 256 or head_dim % 16:
+        if kind == "int4":
+            if head_dim not in INT4_HEAD_DIMS:
+                raise ValueError(f"head_dim must be one of {INT4_HEAD_DIMS} in 4 bits, got {head_dim}")
+        elif head_dim < 16 or head_dim > 256 or head_dim % 16:
             raise ValueError(f"head_dim must be a multiple of 16 up to 256, got {head_dim}")
 
     @classmethod
@@ -132,13 +158,21 @@ class PagedKvCache:
         if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
             raise ValueError("codes must be [pages, kv_heads, page_size, head_dim], the same for keys and values")
         pages, heads, page_size, dim = k_codes.shape
+        dim *= 2 if kind == "int4" else 1
         cls._check(pages, page_size, heads, dim, kind)
         for t in (k_codes, v_codes):
             if t.dtype not in (torch.int8, torch.uint8, torch.float8_e4m3fn) or not t.is_contiguous():
                 raise ValueError("codes must be contiguous 8-bit tensors")
-        for t in (k_scales, v_scales):
-            if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads) or not t.is_contiguous():
-                raise ValueError("scales must be contiguous fp32 [pages, kv_heads] tensors")
+        if kind == "int4":
+            groups = dim // INT4_GROUP
+            for t, name, shape in ((k_scales, "k_scales", (pages, heads, page_size, groups, 2)),
+                                   (v_scales, "v_scales", (pages, heads, page_size // 16, 32 * groups + 16))):
+                if t.dtype != torch.float16 or tuple(t.shape) != shape or not t.is_contiguous():
+                    raise ValueError(f"{name} must be a contiguous fp16 tensor of shape {shape}, got {tuple(t.shape)}")
+        else:
+            for t in (k_scales, v_scales):
+                if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads) or not t.is_contiguous():
+                    raise ValueError("scales must be contiguous fp32 [pages, kv_heads] tensors")
         if any(t.device != k_codes.device for t in (v_codes, k_scales, v_scales)):
             raise ValueError("codes and scales must be on one device")
         self = cls.__new__(cls)
@@ -149,6 +183,8 @@ class PagedKvCache:
         lib = _lib.load()
         self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.kind = k_codes, v_codes, k_scales, v_scales, kind
         self.pages, self.kv_heads, self.page_size, self.head_dim = k_codes.shape
+        if kind == "int4":
+            self.head_dim *= 2
         self.device = k_codes.device
         s = _lib.Se12KvPagesStruct(self.pages, self.page_size, self.kv_heads, self.head_dim, KINDS[kind], k_codes.data_ptr(),
                                    v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
@@ -202,11 +238,19 @@ class PagedKvCache:
         _rows(x, name, heads, self.head_dim, tokens, dtypes, self.device)
         return stride[0], stride[1]
 
+    def _norm_weight(self, w: torch.Tensor | None, name: str) -> tuple:
+        if w is None:
+            return 0, False
+        if w.dim() != 1 or w.shape[0] != self.head_dim or w.dtype not in _FLOATS or w.stride(0) != 1 or w.device != self.device:
+            raise ValueError(f"{name} must be fp32 or BF16 [{self.head_dim}] on {self.device}, with unit stride")
+        return w.data_ptr(), w.dtype is torch.bfloat16
+
     # ------------------------------------------------------------------ operators
     def append(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
                q: torch.Tensor | None = None, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
                query_start: torch.Tensor | None = None, interleaved: bool = False,
-               q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+               q_out: torch.Tensor | None = None, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+               norm_eps: float = 1e-6) -> torch.Tensor | None:
         """Stores new keys and values (fp32 or BF16 [tokens, kv_heads,
         head_dim], any token and head strides) and returns the queries q
         [tokens, q_heads, head_dim] rotated, as BF16 (None without q).
@@ -217,7 +261,11 @@ class PagedKvCache:
         [seqs, columns] (any row stride) holds page ids. A sequence with ``lens`` 0 is a padding
         row: nothing is stored, its queries are zeros. ``cos`` and ``sin``
         (fp32 [positions, rotary / 2]) rotate keys and queries by position,
-        pairs (i, i + rotary / 2), or (2i, 2i + 1) when ``interleaved``."""
+        pairs (i, i + rotary / 2), or (2i, 2i + 1) when ``interleaved``.
+        ``q_norm`` and ``k_norm`` (fp32 or BF16 [head_dim] weights) normalise
+        each head's queries or keys before that: x / sqrt(mean(x^2) +
+        ``norm_eps``) * weight, in fp32 (the mean from 64-bit sums) without a
+        rounding in between."""
         dtype = k.dtype
         k_strides = self._row_strides(k, "k", self.kv_heads, None, _FLOATS)
         tokens = k.shape[0]
@@ -236,6 +284,14 @@ class PagedKvCache:
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
+        norms = None
+        if q_norm is not None or k_norm is not None:
+            if q_norm is not None and q is None:
+                raise ValueError("q_norm without q")
+            if not 0.0 <= norm_eps < math.inf:
+                raise ValueError(f"norm_eps must be finite and not negative, got {norm_eps}")
+            (q_weight, q_bf16), (k_weight, k_bf16) = self._norm_weight(q_norm, "q_norm"), self._norm_weight(k_norm, "k_norm")
+            norms = _lib.KV_NORMS.pack(q_weight, k_weight, q_bf16, k_bf16, norm_eps)
         if tokens == 0:
             return q_out
         batch = self._batch(tokens, block_table, lens, query_start)
@@ -252,7 +308,10 @@ class PagedKvCache:
             raise ValueError("cos and sin go together")
         args = _lib.KV_APPEND.pack(dtype is torch.bfloat16, q_heads, q_ptr, k.data_ptr(), v.data_ptr(), *q_strides, *k_strides,
                                    *v_strides, *turn, bool(interleaved), out_ptr, *out_strides)
-        _launch(self.device, self._lib.se12_kv_append, "se12_kv_append", self._handle, batch, args)
+        if norms is None:
+            _launch(self.device, self._lib.se12_kv_append, "se12_kv_append", self._handle, batch, args)
+        else:
+            _launch(self.device, self._lib.se12_kv_append_normed, "se12_kv_append_normed", self._handle, batch, args, norms)
         return q_out
 
     def attend(self, q: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, query_start: torch.Tensor | None = None,
@@ -291,8 +350,8 @@ class PagedKvCache:
         return out
 
     def decode(self, pages: torch.Tensor | None = None) -> tuple:
-        """Keys and values of the given pages (int32 ids; None: all) as exact
-        BF16 tensors [pages, kv_heads, page_size, head_dim]."""
+        """Keys and values of the given pages (int32 ids; None: all) as BF16
+        tensors [pages, kv_heads, page_size, head_dim], exact (int4: rounded)."""
         count = self.pages if pages is None else _index(pages, "pages", 1, self.device).shape[0]
         shape = (count, self.kv_heads, self.page_size, self.head_dim)
         k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
