@@ -62,44 +62,9 @@ constexpr int kAttendMaxCtas = 3;        // per SM
 constexpr int kAttendPairCost = 8;
 constexpr float kAttendWideCap = 128.f;  // a logit off by 2^-15 there, an eighth of a weight's FP16 rounding
 
-__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                              uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
-  uint32_t y;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-
 __device__ __forceinline__ void cp_async_4(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
 }
-
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-
-template <int CHUNK, int ROWS>
-__device__ __forceinline__ SeqWork sequence_work(const AttendArgs& a, int b) {
-  return sequence_work(a.t.rows_of(b, list_sizes(a)), list_sizes(a), CHUNK, ROWS);
-}
-
-// A place in the work list: chunk `chunk` of pair `pair` (KV head x row
-// tile) of sequence b. The list counts units: a pair's are kAttendPairCost for
-// its beginning and end, from `start` on, and one per chunk.
-struct Place {
-  int b, pair, chunk;
-  int start;
-  SeqWork w;
-  __device__ __forceinline__ int unit() const { return start + kAttendPairCost + chunk; }
-};
 
 template <int KIND, int DP, int NT>
 struct AttendShape {
@@ -185,7 +150,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
       if (static_cast<long long>(sm.before[mid]) * heads <= u) lo = mid;
       else hi = mid - 1;
     }
-    Place p;
+    Place<kAttendPairCost> p;
     p.b = lo;
     p.w = sequence_work<CHUNK, ROWS>(a, lo);
     const int x = u - sm.before[lo] * heads, each = p.w.chunks + kAttendPairCost;
@@ -196,7 +161,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
     return p;
   };
   // To the place `by` chunks on; false where that is past this CTA's run.
-  auto advance = [&](Place& p, int by) {
+  auto advance = [&](Place<kAttendPairCost>& p, int by) {
     p.chunk += by;
     while (p.chunk >= p.w.chunks) {
       p.chunk -= p.w.chunks;
@@ -218,7 +183,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
   unsigned char* pipe = pipes + warp * (kAttendStages * kAttendStageBytes);
   const uint32_t pipe_addr = smem_addr(pipe);
   const uint64_t policy = policy_evict_first();
-  Place next = locate(u0);
+  Place<kAttendPairCost> next = locate(u0);
   bool more = advance(next, warp);  // `next` is a chunk of the run
   int next_page = -1;  // this lane's (lane < SUBS) page for the next chunk to issue
   auto fetch_page = [&]() {
@@ -275,7 +240,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
   bool dead = false;  // a wait ran out: skip the rest (status raised)
 
   // ---- the pairs of this CTA's run
-  Place at = locate(u0);
+  Place<kAttendPairCost> at = locate(u0);
   int done = 0;  // chunks of the run before this pair
   for (bool here = advance(at, 0); here;) {
     const int run = min(at.w.chunks - at.chunk, u1 - at.unit());  // chunks of this pair here
@@ -753,6 +718,7 @@ cudaError_t launch_attend_kind(const CUtensorMap& kmap, const CUtensorMap& vmap,
 
 cudaError_t launch_kv_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, int max_query,
                              int sm_count, cudaStream_t stream) {
+  if (a.c.kind == kKvInt4) return launch_attend4(a, max_query, sm_count, stream);
   if (kv_attend_takes_tiles(max_query, a.group, a.c.dim)) return launch_attend_tile(a, sm_count, stream);
   return a.c.kind == kKvInt8 ? launch_attend_kind<kKvInt8>(kmap, vmap, a, max_query, sm_count, stream)
                              : launch_attend_kind<kKvE4m3>(kmap, vmap, a, max_query, sm_count, stream);

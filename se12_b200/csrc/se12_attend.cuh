@@ -1,4 +1,4 @@
-// What the two attention kernels share: codes as FP16, the softmax's
+// What the attention kernels share: codes as FP16, the softmax's
 // references and the work list's sums on the device.
 #pragma once
 
@@ -33,6 +33,30 @@ __device__ __forceinline__ void widen(uint32_t codes, uint32_t& lo, uint32_t& hi
   }
 }
 
+// ------------------------------------------------------------------ mma.sync of the few-rows kernels
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+// ------------------------------------------------------------------ work list
+
 __device__ __forceinline__ ListSizes list_sizes(const AttendArgs& a) {
   return {a.t.tokens, a.t.max_pages << a.c.page_shift, a.group, a.window};
 }
@@ -58,5 +82,21 @@ __device__ __forceinline__ void sum_up_to(int* sums, int seqs, int limit, int la
     carry = __shfl_sync(0xFFFFFFFFu, v, 31);
   }
 }
+
+template <int CHUNK, int ROWS>
+__device__ __forceinline__ SeqWork sequence_work(const AttendArgs& a, int b) {
+  return sequence_work(a.t.rows_of(b, list_sizes(a)), list_sizes(a), CHUNK, ROWS);
+}
+
+// A place in the work list: chunk `chunk` of pair `pair` (KV head x row
+// tile) of sequence b. The list counts units: a pair's are COST for its beginning
+// and end, from `start` on, and one per chunk.
+template <int COST>
+struct Place {
+  int b, pair, chunk;
+  int start;
+  SeqWork w;
+  __device__ __forceinline__ int unit() const { return start + COST + chunk; }
+};
 
 }  // namespace se12

@@ -7,6 +7,7 @@
 #include "se12_kv.cu"
 #include "se12_kv4.cu"
 #include "se12_attend.cu"
+#include "se12_attend4.cu"
 #include "se12_attend_tile.cu"
 #include "se12_logprobs.cu"
 #include "se12_serve_abi.cu"

@@ -184,6 +184,7 @@ size_t se12_kv_attend_workspace_bytes(const se12_kv_cache* c) {
 
 size_t se12_kv_attend_call_bytes(const se12_kv_cache* c, int q_heads, int max_query) {
   if (!c || q_heads < 1 || max_query < 1) return 0;
+  if (c->view.kind == SE12_KV_INT4) return SE12_COUNTER_BYTES + se12::kv_attend4_partial_bytes(c->sm_count);
   const bool tiles = se12::kv_attend_takes_tiles(max_query, std::max(q_heads / c->view.heads, 1), c->view.dim);
   return SE12_COUNTER_BYTES + se12::kv_attend_partial_bytes(c->sm_count, tiles);
 }
@@ -195,7 +196,6 @@ int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const
   if (st != SE12_OK) return st;
   if (!p || !p->q || !p->out) return fail(SE12_ERR_INVALID_ARGUMENT, "null queries or output");
   const se12::KvView& v = cache->view;
-  if (v.kind == SE12_KV_INT4) return fail(SE12_ERR_UNSUPPORTED_FORMAT, "attention over 4-bit pages is not built");
   if (p->q_heads < 1 || p->q_heads % v.heads)
     return fail(SE12_ERR_INVALID_ARGUMENT, "q_heads must be a multiple of kv_heads");
   if (p->max_query < 1 || p->max_query > batch->tokens || (!batch->query_start && p->max_query != 1))
