@@ -23,6 +23,7 @@
 #include "se12_attend.cuh"
 
 #include <cuda_bf16.h>
+#include <type_traits>
 
 namespace se12 {
 
@@ -56,7 +57,7 @@ struct Rows4Smem {
     uint4 queries[2 * DIM / 32 * 32];     // FP16 fragments: [n-tile][group][word][lane]
     float deposit[2048];                  // the warps' sums while they are joined
   };
-  float query_sums[2][DIM / 64][8];       // 2^-22 sum of a group's, [n-tile][group][row]
+  float query_sums[2 * DIM / 64][8];       // 2^-22 sum of a group's, [n-tile][group][row]
   float row_scale[kRows4SlotRows];
   float stat[kRows4Warps][kRows4SlotRows][2];  // mp, l of each warp
   float factor[kRows4Warps][kRows4SlotRows];
@@ -65,6 +66,11 @@ struct Rows4Smem {
   int most;
   int before[1];  // [seqs + 1] units of the sequences before (per KV head)
 };
+
+// A value that stays in its register: the compiler would rather work out again
+// for every chunk what it knows from the lane (40 of 350 instructions per 16
+// tokens).
+__device__ __forceinline__ void keep(uint32_t& x) { asm volatile("" : "+r"(x)); }
 
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
@@ -101,6 +107,15 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
   }
 }
 
+// The first product of a sum.
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ uint32_t mul_halves(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -115,9 +130,15 @@ __device__ __forceinline__ float2 halves_of(uint32_t w) { return __half22float2(
 // its sum as if a subnormal began at 2^-14: two bits more are worth a shift.)
 constexpr uint32_t kLowCodes = 0x003C003Cu, kHighCodes = 0x03C003C0u;
 
-// 16 bytes, asynchronously.
-__device__ __forceinline__ void copy_16(uint32_t dst, const void* src, uint64_t policy) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
+// 16 bytes, asynchronously (where `use`).
+__device__ __forceinline__ void copy_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_16_if(bool use, uint32_t dst, const void* src) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst), "l"(src),
+      "r"(static_cast<uint32_t>(use))
+      : "memory");
 }
 
 // Where in a box of 16 tokens' codes a sixteenth of token `token`'s row lies:
@@ -144,15 +165,20 @@ __device__ __forceinline__ void store_four(const AttendArgs& a, int token0, int 
   }
 }
 
-template <int DIM, int NT, int CTAS>
+// ONE: pages are as long as a chunk or longer (a chunk lies in one page).
+template <int DIM, int NT, int CTAS, bool ONE>
 __global__ void __launch_bounds__(kRows4Threads, CTAS)
     attend4_rows_kernel(const AttendArgs a) {
   using Shape = Rows4Shape<DIM>;
-  // A place in the list, with its pair's KV head and row tile.
-  struct Spot : Place<kRows4PairCost> {
-    int head, tile;
+  // A place in the work list, as Place: KV head, row tile and chunk; the pair's
+  // chunks in this CTA's run end before `stop`.
+  struct Spot {
+    int b, head, tile, chunk, stop;
+    int start;
+    SeqWork w;
   };
   constexpr int G = Shape::kGroups, SUBS = Shape::kSubs, CHUNK = Shape::kChunk, STAGES = Shape::kStages, ROWS = 8 * NT;
+  constexpr int Z = (G + 1) / 2;
   extern __shared__ unsigned char smem_raw[];
   Rows4Smem<DIM>& sm = *reinterpret_cast<Rows4Smem<DIM>*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -200,117 +226,158 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
     p.b = lo;
     p.w = sequence_work<CHUNK, ROWS>(a, lo);
     const int x = u - sm.before[lo] * heads, each = p.w.chunks + kRows4PairCost;
-    p.pair = x / each;
-    p.head = p.pair / p.w.tiles;
-    p.tile = p.pair - p.head * p.w.tiles;
-    const int at = x - p.pair * each;
+    const int pair = x / each, at = x - pair * each;
+    p.head = pair / p.w.tiles;
+    p.tile = pair - p.head * p.w.tiles;
     p.start = u - at;
     p.chunk = max(at - kRows4PairCost, 0);
+    p.stop = min(p.w.chunks, u1 - p.start - kRows4PairCost);
     return p;
   };
   // To the place `by` chunks on; false where that is past this CTA's run.
   auto advance = [&](Spot& p, int by) {
     p.chunk += by;
+    if (p.chunk < p.stop) return true;
+#pragma unroll 1
     while (p.chunk >= p.w.chunks) {
       p.chunk -= p.w.chunks;
       p.start += p.w.chunks + kRows4PairCost;
       if (p.start + kRows4PairCost >= u1) return false;
-      if (++p.tile < p.w.tiles) continue;
-      p.tile = 0;
-      if (++p.head == heads) {
-        p.head = 0;
-        do {
-          ++p.b;
-        } while (sm.before[p.b + 1] == sm.before[p.b]);
-        // (chunks left over continue in the next sequence)
-        p.w = sequence_work<CHUNK, ROWS>(a, p.b);
+      if (++p.tile == p.w.tiles) {
+        p.tile = 0;
+        if (++p.head == heads) {
+          p.head = 0;
+          do {
+            ++p.b;
+          } while (sm.before[p.b + 1] == sm.before[p.b]);
+          // (chunks left over continue in the next sequence)
+          p.w = sequence_work<CHUNK, ROWS>(a, p.b);
+        }
       }
     }
-    return p.unit() < u1;
+    p.stop = min(p.w.chunks, u1 - p.start - kRows4PairCost);
+    return p.chunk < p.stop;
   };
 
   // ---- this warp's pipeline: every fourth chunk of the run. A lane copies the
   // same 16 bytes of every box; a chunk is one group of its copies.
   const uint32_t pipe = smem_addr(sm.pipes[warp]);
-  const uint64_t policy = policy_evict_first();
   Spot next = locate(u0);
   bool more = advance(next, warp);  // `next` is a chunk of the run
-  int next_row = -1;  // of the next chunk to issue: where 16 tokens of it begin (lane `sub`'s), -1: not to be read
+  // ONE: a chunk is one piece, whose row every lane has; otherwise 16 tokens are,
+  // and lane `sub` has theirs.
+  constexpr int kPiece = ONE ? CHUNK : 16;
+  int next_row = -1;  // of the next chunk to issue: where a piece of it begins, -1: not to be read
   auto fetch_rows = [&]() {
-    next_row = -1;
-    const int t0 = next.w.low + next.chunk * CHUNK + lane * 16;
-    if (lane < SUBS && t0 < next.w.s.length && t0 + 16 > visible_from(next.w.s.first, a.window)) {
-      const int i = t0 >> a.c.page_shift;
-      const int page = i < a.t.max_pages ? a.t.table[next.b * a.t.table_stride + i] : -1;
-      if (page >= 0 && page < a.c.pages)
-        next_row = (page * heads + next.head) * a.c.page_size + (t0 & (a.c.page_size - 1));
-      else
-        raise_status(kStatusBadArgument);
-    }
+    const int t0 = next.w.low + next.chunk * CHUNK + (ONE ? 0 : lane * 16);
+    const bool due = (ONE || lane < SUBS) && t0 < next.w.s.length && t0 + kPiece > visible_from(next.w.s.first, a.window);
+    unsigned page = 0;  // (a sequence's length is one that its table row has pages for)
+    if (due) page = a.t.table[next.b * a.t.table_stride + (t0 >> a.c.page_shift)];
+    const bool there = due && page < static_cast<unsigned>(a.c.pages);
+    next_row = there ? (static_cast<int>(page) * heads + next.head) * a.c.page_size + (t0 & (a.c.page_size - 1)) : -1;
+    if (due && !there) raise_status(kStatusBadArgument);
   };
-  constexpr int kCopies = Shape::kBox / 512 > 0 ? Shape::kBox / 512 : 1;  // of 512 bytes, of a box
+  constexpr int kCopies = Shape::kBox / 512;  // of 512 bytes, of a box
   uint32_t copy_to[kCopies];
 #pragma unroll
   for (int i = 0; i < kCopies; ++i) {
     const int vector = i * 32 + lane;
-    copy_to[i] = row_part<DIM>(vector / (DIM / 32), vector % (DIM / 32));
+    copy_to[i] = pipe + row_part<DIM>(vector / (DIM / 32), vector % (DIM / 32));
+    keep(copy_to[i]);
   }
-  uint32_t usable = 0;  // bits of the chunks on the way, the oldest lowest
-  int fill = 0;         // stage of the next chunk to issue
-  auto issue = [&]() {  // the chunk at `next`, if there is one, then move on
+  uint32_t line_to = pipe + Shape::kCodes + lane * 16;
+  keep(line_to);
+  // N boxes of codes and their lines, from `row` on, to the stage's `sub`-th
+  auto copy_boxes = [&](auto n, int row, int sub, uint32_t stage_at) {
+    constexpr int N = decltype(n)::value;
+    const long long from = static_cast<long long>(row) * (DIM / 2) + lane * 16;
+    const uint8_t* keys = a.c.k_codes + from;
+    const uint8_t* values = a.c.v_codes + from;
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        copy_16(copy_to[i] + stage_at + (sub + b) * Shape::kBox, keys + b * Shape::kBox + i * 512);
+        copy_16(copy_to[i] + stage_at + (SUBS + sub + b) * Shape::kBox, values + b * Shape::kBox + i * 512);
+      }
+    copy_16_if(lane < N * Shape::kKeyLines / 16, line_to + stage_at + sub * Shape::kKeyLines,
+               static_cast<const char*>(a.c.k_scales) + static_cast<long long>(row) * (4 * G) + lane * 16);
+    copy_16_if(lane < N * Shape::kValueLines / 16, line_to + stage_at + SUBS * Shape::kKeyLines + sub * Shape::kValueLines,
+               static_cast<const char*>(a.c.v_scales) + static_cast<long long>(row >> 4) * Shape::kValueLines + lane * 16);
+  };
+  constexpr uint32_t kAll = (1u << SUBS) - 1;
+  uint32_t usable = 0;    // bits of the chunks on the way, the oldest lowest
+  uint32_t fill = 0;      // stage of the next chunk to issue, in bytes
+  auto issue = [&]() {    // the chunk at `next`, if there is one, then move on
     uint32_t bits = 0;
     if (more) {
-      const uint32_t to = pipe + fill * Shape::kStage;
-#pragma unroll
-      for (int sub = 0; sub < SUBS; ++sub) {
-        const int row = __shfl_sync(0xFFFFFFFFu, next_row, sub);
-        if (row < 0) continue;
-        bits |= 1u << sub;
-        const long long from = static_cast<long long>(row) * (DIM / 2) + lane * 16;
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-          copy_16(to + sub * Shape::kBox + copy_to[i], a.c.k_codes + from + i * 512, policy);
-          copy_16(to + (SUBS + sub) * Shape::kBox + copy_to[i], a.c.v_codes + from + i * 512, policy);
+      if constexpr (ONE) {
+        if (next_row >= 0) {
+          copy_boxes(std::integral_constant<int, SUBS>{}, next_row, 0, fill);
+          bits = kAll;
         }
-        if (lane < Shape::kKeyLines / 16)
-          copy_16(to + Shape::kCodes + sub * Shape::kKeyLines + lane * 16,
-                  static_cast<const char*>(a.c.k_scales) + static_cast<long long>(row) * (4 * G) + lane * 16, policy);
-        if (lane < Shape::kValueLines / 16)
-          copy_16(to + Shape::kCodes + SUBS * Shape::kKeyLines + sub * Shape::kValueLines + lane * 16,
-                  static_cast<const char*>(a.c.v_scales) + static_cast<long long>(row >> 4) * Shape::kValueLines + lane * 16, policy);
+      } else {
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub) {
+          const int row = __shfl_sync(0xFFFFFFFFu, next_row, sub);
+          if (row < 0) continue;
+          copy_boxes(std::integral_constant<int, 1>{}, row, sub, fill);
+          bits |= 1u << sub;
+        }
       }
       more = advance(next, kRows4Warps);
       if (more) fetch_rows();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     usable = (usable >> SUBS) | (bits << (SUBS * (STAGES - 2)));
-    fill = fill + 1 == STAGES ? 0 : fill + 1;
+    fill = fill == (STAGES - 1) * Shape::kStage ? 0 : fill + Shape::kStage;
   };
   if (more) fetch_rows();
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) issue();
 
   const bool capped = a.softcap != 0.f, wide = a.softcap > kRows4WideCap;
-  // where this lane's parts of a sub lie
+  const float cap2 = a.softcap * kLog2e;
+  // Where this lane's parts of a stage lie.
   uint32_t key_at[DIM / 128 + (DIM < 128)], value_at[2];
 #pragma unroll
-  for (int i = 0; i < DIM / 128; ++i) key_at[i] = row_part<DIM>(r, c * (DIM / 128) + i);
-  if (DIM == 64) key_at[0] = r * 32 + c * 8;
+  for (int i = 0; i < DIM / 128; ++i) key_at[i] = pipe + row_part<DIM>(r, c * (DIM / 128) + i);
+  if (DIM == 64) key_at[0] = pipe + r * 32 + c * 8;
+#pragma unroll
+  for (int i = 0; i < DIM / 128 + (DIM < 128); ++i) keep(key_at[i]);
   // The tokens 2 c and 2 c + 1 in the order that meets all banks.
   const bool swapped = DIM == 256 ? false : DIM == 128 ? c & 1 : c >> 1;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int token = 2 * c + (i ^ static_cast<int>(swapped));
-    value_at[i] = DIM == 256 ? row_part<DIM>(token, r) : DIM == 128 ? row_part<DIM>(token, r >> 1) + (r & 1) * 8 : token * 32 + r * 4;
+    value_at[i] = pipe + SUBS * Shape::kBox +
+                  (DIM == 256 ? row_part<DIM>(token, r) : DIM == 128 ? row_part<DIM>(token, r >> 1) + (r & 1) * 8 : token * 32 + r * 4);
+    keep(value_at[i]);
   }
-  const uint32_t low_pair = swapped ? 0x1054u : 0x5410u, high_pair = swapped ? 0x3276u : 0x7632u;
-  int stage = 0;
+  uint32_t low_pair = swapped ? 0x1054u : 0x5410u, high_pair = swapped ? 0x3276u : 0x7632u;
+  keep(low_pair);
+  keep(high_pair);
+  uint32_t key_line_at = pipe + Shape::kCodes + r * (4 * G), value_line_at = pipe + Shape::kCodes + SUBS * Shape::kKeyLines + c * (8 * G),
+           power_at = pipe + Shape::kCodes + SUBS * Shape::kKeyLines + 64 * G + 2 * r;
+  keep(key_line_at);
+  keep(value_line_at);
+  keep(power_at);
+  uint32_t queries_at = smem_addr(sm.queries) + lane * 16, sums_at = smem_addr(sm.query_sums) + c * 8;
+  keep(queries_at);
+  keep(sums_at);
+  uint32_t minus8[G > 1 ? 2 : 1][4];  // a first operand of -8 in the upper rows, and one in the lower (kept as they are)
+#pragma unroll
+  for (int i = 0; i < (G > 1 ? 2 : 1); ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      asm volatile("mov.b32 %0, %1;" : "=r"(minus8[i][k]) : "r"((k & 1) == i ? 0xC800C800u : 0u));
+  uint32_t stage = 0;  // in bytes
 
   // ---- the pairs of this CTA's run
   Spot at = locate(u0);
   int done = 0;  // chunks of the run before this pair
   for (bool here = advance(at, 0); here;) {
-    const int run = min(at.w.chunks - at.chunk, u1 - at.unit());  // chunks of this pair here
+    const int run = at.stop - at.chunk;  // chunks of this pair here
     const int head = at.head, tile = at.tile;
     const int token0 = a.t.begin_of(at.b, list_sizes(a));
     const int rows_all = at.w.s.tokens * a.group;
@@ -382,7 +449,7 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
         }
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-        if (c == 0) sm.query_sums[n][g][r] = sum * 0x1p-22f;
+        if (c == 0) sm.query_sums[n * G + g][r] = sum * 0x1p-22f;
       }
       if (c == 0) sm.row_scale[n * 8 + r] = __uint_as_float(static_cast<unsigned>(127 + e + 8) << 23) * a.scale;
     }
@@ -402,7 +469,7 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
 
     float l[NT][2], mp[NT][2];
     float acc[G][4][NT][4];  // sums of codes: rows 2 j and 2 j + 1 of the lane's word of a group
-    float zero[NT][4];       // row g < G: what the zero points and offsets of group g add
+    float zero[NT][Z][4];    // what zero points and offsets add: rows 0 .. 7 of group 2 z, 8 .. 15 of 2 z + 1
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -411,7 +478,9 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
         l[n][k] = 0.f;
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) zero[n][k] = 0.f;
+      for (int z = 0; z < Z; ++z)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) zero[n][z][k] = 0.f;
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -425,97 +494,92 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
     for (; mine < run; mine += kRows4Warps) {
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
       __syncwarp();  // every lane's copies are there, and every lane has read the stage filled next
-      const uint32_t base = pipe + stage * Shape::kStage;
-      const uint32_t key_lines = base + Shape::kCodes, value_lines = key_lines + SUBS * Shape::kKeyLines;
-      const uint32_t there = usable;
+      const uint32_t there = usable & kAll;
       issue();
       const int t0 = at.w.low + (at.chunk + mine) * CHUNK;
-      bool use[SUBS];
       float power[SUBS][2];   // E of tokens r, r + 8
       float p[SUBS][NT][4];   // logits in units of log 2, with E, then weights
+      // S^T: 16 tokens x 8 rows at a time, group by group
+      uint32_t x[SUBS][2][2 * G];  // of tokens r and r + 8: words 2 c of all groups, then 2 c + 1's
+      uint32_t line[SUBS][2][G];   // (scale, offset) of tokens r and r + 8
 #pragma unroll
-      for (int sub = 0; sub < SUBS; ++sub) {
-        use[sub] = (there >> sub) & 1;
-        power[sub][0] = power[sub][1] = 0.f;
+      for (int sub = 0; sub < SUBS; ++sub)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) p[sub][n][k] = kNegInf;
-        if (!use[sub]) continue;
-        // S^T: 16 tokens x 8 rows, group by group
-        const uint32_t keys = base + sub * Shape::kBox;
-        uint32_t x[2][2 * G];  // of tokens r and r + 8: words 2 c of all groups, then 2 c + 1's
-        if constexpr (DIM == 64) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) lds_words<2>(x[h], keys + key_at[0] + h * 256);
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t keys = stage + sub * Shape::kBox + h * (4 * DIM);
+          if constexpr (DIM == 64) {
+            lds_words<2>(x[sub][h], keys + key_at[0]);
+          } else {
 #pragma unroll
             for (int i = 0; i < DIM / 128; ++i) {
-              const uint4 v = lds128(keys + key_at[i] + h * (4 * DIM));
-              x[h][4 * i] = v.x, x[h][4 * i + 1] = v.y, x[h][4 * i + 2] = v.z, x[h][4 * i + 3] = v.w;
+              const uint4 v = lds128(keys + key_at[i]);
+              x[sub][h][4 * i] = v.x, x[sub][h][4 * i + 1] = v.y, x[sub][h][4 * i + 2] = v.z, x[sub][h][4 * i + 3] = v.w;
             }
+          }
+          lds_words<G>(line[sub][h], key_line_at + stage + sub * Shape::kKeyLines + h * (32 * G));
+          power[sub][h] = lds_half(power_at + stage + sub * Shape::kValueLines + 16 * h);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) p[sub][n][2 * h] = p[sub][n][2 * h + 1] = 0.f;
         }
-        uint32_t line[2][G];  // (scale, offset) of tokens r and r + 8
 #pragma unroll
-        for (int h = 0; h < 2; ++h) lds_words<G>(line[h], key_lines + sub * Shape::kKeyLines + (r + 8 * h) * (4 * G));
-        float s[NT][4];
+      for (int g = 0; g < G; ++g) {
+        float d[SUBS][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int j = 0; j < 2; ++j) {
+          uint4 q[NT];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[n][k] = 0.f;
+          for (int n = 0; n < NT; ++n) q[n] = lds128(queries_at + ((n * G + g) * 2 + j) * 512);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          float d[NT][4];
+          for (int sub = 0; sub < SUBS; ++sub) {
+            const uint32_t w0 = x[sub][0][j * G + g] << 2, w1 = x[sub][1][j * G + g] << 2;
+            const uint32_t v0 = x[sub][0][j * G + g] >> 6, v1 = x[sub][1][j * G + g] >> 6;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              if (j == 0)
+                mma_first(d[sub][n], w0 & kLowCodes, w1 & kLowCodes, w0 & kHighCodes, w1 & kHighCodes, q[n].x, q[n].y);
+              else
+                mma_f16_16816(d[sub][n], w0 & kLowCodes, w1 & kLowCodes, w0 & kHighCodes, w1 & kHighCodes, q[n].x, q[n].y);
+              mma_f16_16816(d[sub][n], v0 & kLowCodes, v1 & kLowCodes, v0 & kHighCodes, v1 & kHighCodes, q[n].z, q[n].w);
+            }
+          }
+        }
+        float2 sums[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint2 v = lds64(sums_at + (n * G + g) * 32);
+          sums[n] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+        }
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 l2 = halves_of(line[sub][h][g]);
+            const float low = fmaf(-8.f, l2.x, l2.y);  // what code 0 stands for
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              p[sub][n][2 * h] = fmaf(d[sub][n][2 * h], l2.x, fmaf(low, sums[n].x, p[sub][n][2 * h]));
+              p[sub][n][2 * h + 1] = fmaf(d[sub][n][2 * h + 1], l2.x, fmaf(low, sums[n].y, p[sub][n][2 * h + 1]));
+            }
+          }
+      }
+      auto each_logit = [&](auto&& f) {
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) d[n][k] = 0.f;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t w0 = x[0][j * G + g] << 2, w1 = x[1][j * G + g] << 2, v0 = x[0][j * G + g] >> 6, v1 = x[1][j * G + g] >> 6;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const uint4 q = sm.queries[((n * G + g) * 2 + j) * 32 + lane];
-              mma_f16_16816(d[n], w0 & kLowCodes, w1 & kLowCodes, w0 & kHighCodes, w1 & kHighCodes, q.x, q.y);
-              mma_f16_16816(d[n], v0 & kLowCodes, v1 & kLowCodes, v0 & kHighCodes, v1 & kHighCodes, q.z, q.w);
-            }
-          }
-          const float2 line0 = halves_of(line[0][g]), line1 = halves_of(line[1][g]);
-          const float low0 = fmaf(-8.f, line0.x, line0.y), low1 = fmaf(-8.f, line1.x, line1.y);  // what code 0 stands for
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const float2 qs = *reinterpret_cast<const float2*>(&sm.query_sums[n][g][2 * c]);
-            s[n][0] = fmaf(d[n][0], line0.x, fmaf(low0, qs.x, s[n][0]));
-            s[n][1] = fmaf(d[n][1], line0.x, fmaf(low0, qs.y, s[n][1]));
-            s[n][2] = fmaf(d[n][2], line1.x, fmaf(low1, qs.x, s[n][2]));
-            s[n][3] = fmaf(d[n][3], line1.x, fmaf(low1, qs.y, s[n][3]));
-          }
-        }
-        const uint32_t exponents = value_lines + sub * Shape::kValueLines + 64 * G;
-        power[sub][0] = lds_half(exponents + 2 * r);
-        power[sub][1] = lds_half(exponents + 2 * r + 16);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (!capped) {
-              p[sub][n][k] = fmaf(s[n][k], row_scale[n][k & 1], power[sub][k >> 1]);
-              continue;
-            }
-            // cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1); the
-            // factor 2 log2(e) / cap is in row_scale. The difference is off by
-            // some 2^-23 of the cap: above kRows4WideCap not taken.
-            float y = s[n][k] * row_scale[n][k & 1];
-            if (wide)
-              y = capped_by(y * (0.5f / kLog2e), a.softcap * kLog2e);
-            else
-              y = a.softcap * kLog2e - __fdividef(2.f * kLog2e * a.softcap, ex2(y) + 1.f);
-            p[sub][n][k] = y + power[sub][k >> 1];
-          }
-      }
-      const bool masked = t0 + CHUNK - 1 > pos_min || (a.window && pos_max - t0 >= a.window);
+            for (int k = 0; k < 4; ++k) p[sub][n][k] = f(p[sub][n][k], row_scale[n][k & 1], power[sub][k >> 1]);
+      };
+      if (!capped)
+        each_logit([&](float x, float scale, float e) { return fmaf(x, scale, e); });
+      else if (!wide)
+        // cap * tanh(x / cap) = cap - 2 cap / (exp(2 x / cap) + 1); the factor
+        // 2 log2(e) / cap is in row_scale. The difference is off by some 2^-23 of
+        // the cap: above kRows4WideCap not taken.
+        each_logit([&](float x, float scale, float e) { return cap2 - __fdividef(2.f * cap2, ex2(x * scale) + 1.f) + e; });
+      else
+        each_logit([&](float x, float scale, float e) { return capped_by(x * scale * (0.5f / kLog2e), cap2) + e; });
+      const bool masked = there != kAll || t0 + CHUNK - 1 > pos_min || (a.window && pos_max - t0 >= a.window);
       if (masked) {
 #pragma unroll
         for (int sub = 0; sub < SUBS; ++sub)
@@ -524,8 +588,15 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const int j = t0 + sub * 16 + r + (k >> 1) * 8, pos = row_pos[n][k & 1];
-              if (j > pos || (a.window && pos - j >= a.window)) p[sub][n][k] = kNegInf;
+              if (j > pos || (a.window && pos - j >= a.window) || !((there >> sub) & 1)) p[sub][n][k] = kNegInf;
             }
+        // E that is no number has made the weights NaN of the rows that see the
+        // token; it does not reach the others (neither does what lies where no token is)
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (!(fabsf(power[sub][h]) <= 64.f)) power[sub][h] = 0.f;
       }
       // raise the references where a weight passes them
       bool passes = false;
@@ -551,7 +622,11 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
             const float f = ex2(mp[n][k] - t);
             mp[n][k] = t;
             l[n][k] *= f;
-            zero[n][k] *= f;
+#pragma unroll
+            for (int z = 0; z < Z; ++z) {
+              zero[n][z][k] *= f;
+              zero[n][z][k + 2] *= f;
+            }
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -563,62 +638,61 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
       }
 #pragma unroll
       for (int sub = 0; sub < SUBS; ++sub) {
-        if (!use[sub]) continue;
         uint32_t pf[NT][2];
         const float back[2] = {ex2(-power[sub][0]), ex2(-power[sub][1])};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const bool hidden = masked && p[sub][n][k] == kNegInf;  // weighs nothing, whatever E is
-            const float w = ex2(p[sub][n][k] - mp[n][k & 1]);
-            p[sub][n][k] = hidden ? 0.f : w;
-            l[n][k & 1] += hidden ? 0.f : w * back[k >> 1];
+            p[sub][n][k] = ex2(p[sub][n][k] - mp[n][k & 1]);
+            l[n][k & 1] = fmaf(p[sub][n][k], back[k >> 1], l[n][k & 1]);
           }
           pf[n][0] = transpose_8x8(half2_bits(__floats2half2_rn(p[sub][n][0], p[sub][n][1])));
           pf[n][1] = transpose_8x8(half2_bits(__floats2half2_rn(p[sub][n][2], p[sub][n][3])));
         }
         // O^T += V^T P^T: lane (r, c) has word r of each group, of the tokens
         // 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-        const uint32_t values = base + (SUBS + sub) * Shape::kBox, lines = value_lines + sub * Shape::kValueLines;
-        uint32_t x[2][2][G];  // [tokens, + 8][first, second to be read][group]
+        const uint32_t values = stage + sub * Shape::kBox, lines = value_line_at + stage + sub * Shape::kValueLines;
+        uint32_t y[2][2][G];  // [tokens, + 8][first, second to be read][group]
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) lds_words<G>(x[h][i], values + value_at[i] + h * (4 * DIM));
-        uint32_t scale[2][G], offset[2];  // of two tokens each; offsets: row min(r, G - 1)
+          for (int i = 0; i < 2; ++i) lds_words<G>(y[h][i], values + value_at[i] + h * (4 * DIM));
+        uint32_t scale[2][G], offset[2][G];  // of two tokens each
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          lds_words<G>(scale[h], lines + (c + 4 * h) * (8 * G));
-          offset[h] = lds32(lines + (c + 4 * h) * (8 * G) + 4 * G + 4 * min(r, G - 1));
+          lds_words<G>(scale[h], lines + h * (32 * G));
+          lds_words<G>(offset[h], lines + h * (32 * G) + 4 * G);
         }
-        const int left = at.w.s.length - (t0 + sub * 16);
-        if (left < 16) {  // lines past the sequence may be anything
+        if (masked) {  // lines past the sequence, or of a page that is not there, may be anything
+          const int left = (there >> sub) & 1 ? at.w.s.length - (t0 + sub * 16) : 0;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int t = 2 * c + 8 * h;
             const uint32_t keep = (t < left ? 0xFFFFu : 0u) | (t + 1 < left ? 0xFFFF0000u : 0u);
-            offset[h] &= keep;
 #pragma unroll
-            for (int g = 0; g < G; ++g) scale[h][g] &= keep;
+            for (int g = 0; g < G; ++g) scale[h][g] &= keep, offset[h][g] &= keep;
           }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16_16816(zero[n], offset[0], 0u, offset[1], 0u, pf[n][0], pf[n][1]);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int z = 0; z < Z; ++z)
+            mma_f16_16816(zero[n][z], offset[0][2 * z], offset[0][2 * z + (G > 1)], offset[1][2 * z], offset[1][2 * z + (G > 1)],
+                          pf[n][0], pf[n][1]);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           uint32_t w[NT][2];
-          const uint32_t minus8 = r == g ? 0xC800C800u : 0u;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             w[n][0] = mul_halves(pf[n][0], scale[0][g]);
             w[n][1] = mul_halves(pf[n][1], scale[1][g]);
-            mma_f16_16816(zero[n], minus8, 0u, minus8, 0u, w[n][0], w[n][1]);
+            mma_f16_16816(zero[n][g >> 1], minus8[g & 1][0], minus8[g & 1][1], minus8[g & 1][2], minus8[g & 1][3], w[n][0], w[n][1]);
           }
 #pragma unroll
           for (int hi = 0; hi < 2; ++hi) {
             const uint32_t pair = hi ? high_pair : low_pair;
-            const uint32_t x0 = prmt(x[0][0][g], x[0][1][g], pair), x1 = prmt(x[1][0][g], x[1][1][g], pair);
+            const uint32_t x0 = prmt(y[0][0][g], y[0][1][g], pair), x1 = prmt(y[1][0][g], y[1][1][g], pair);
             const uint32_t y0 = x0 << 2, y1 = x1 << 2, z0 = x0 >> 6, z1 = x1 >> 6;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -628,7 +702,7 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
           }
         }
       }
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      stage = stage == (STAGES - 1) * Shape::kStage ? 0 : stage + Shape::kStage;
     }
 
     // ---- join the warps
@@ -681,13 +755,12 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
       for (int g0 = 0; g0 < G; g0 += per_pass) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const float z0 = __shfl_sync(0xFFFFFFFFu, zero[n][0], g * 4 + c), z1 = __shfl_sync(0xFFFFFFFFu, zero[n][1], g * 4 + c);
           if (g < g0 || g >= g0 + per_pass) continue;
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const int row = 2 * c + k;
             if (row < rows_n) {
-              const float f = sm.factor[warp][n * 8 + row], z = (k ? z1 : z0) * f;
+              const float f = sm.factor[warp][n * 8 + row], z = zero[n][g >> 1][2 * (g & 1) + k] * f;
               float* to = &sm.deposit[((warp * rows_n + row) * per_pass + g - g0) * 64 + r * 8];
 #pragma unroll
               for (int hi = 0; hi < 2; ++hi)
@@ -774,16 +847,20 @@ size_t kv_attend4_partial_bytes(int sm_count) {
 
 template <int DIM, int NT, int CTAS>
 cudaError_t launch_attend4_rows(const AttendArgs& a, int sm_count, cudaStream_t stream) {
+  using Shape = Rows4Shape<DIM>;
   static_assert(CTAS <= kRows4MaxCtas, "workspace slots");
   const size_t smem = 128 + sizeof(Rows4Smem<DIM>) + a.t.seqs * sizeof(int);
-  return launch_overlapped(attend4_rows_kernel<DIM, NT, CTAS>, dim3(sm_count * CTAS), kRows4Threads, smem, stream, a);
+  const auto kernel = Shape::kSubs == 1 || a.c.page_size >= Shape::kChunk
+                          ? attend4_rows_kernel<DIM, NT, CTAS, true>
+                          : attend4_rows_kernel<DIM, NT, CTAS, Shape::kSubs == 1>;
+  return launch_overlapped(kernel, dim3(sm_count * CTAS), kRows4Threads, smem, stream, a);
 }
 
 cudaError_t launch_attend4(const AttendArgs& a, int max_query, int sm_count, cudaStream_t stream) {
   const bool one = static_cast<long long>(max_query) * a.group <= 8;  // query rows per KV head in one n-tile
   switch (a.c.dim) {
     case 64: return one ? launch_attend4_rows<64, 1, 3>(a, sm_count, stream) : launch_attend4_rows<64, 2, 3>(a, sm_count, stream);
-    case 128: return one ? launch_attend4_rows<128, 1, 3>(a, sm_count, stream) : launch_attend4_rows<128, 2, 3>(a, sm_count, stream);
+    case 128: return one ? launch_attend4_rows<128, 1, 3>(a, sm_count, stream) : launch_attend4_rows<128, 2, 2>(a, sm_count, stream);
     default: return one ? launch_attend4_rows<256, 1, 3>(a, sm_count, stream) : launch_attend4_rows<256, 2, 2>(a, sm_count, stream);
   }
 }
