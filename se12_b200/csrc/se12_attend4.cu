@@ -841,7 +841,10 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
 
 // ------------------------------------------------------------------ launch
 
-size_t kv_attend4_partial_bytes(int sm_count) {
+bool kv_attend4_takes_tiles(int max_query, int group, int dim) { return static_cast<long long>(max_query) * group > 16; }
+
+size_t kv_attend4_partial_bytes(int sm_count, bool tile) {
+  if (tile) return kv_attend_tile_partial_bytes(sm_count);
   return static_cast<size_t>(sm_count) * kRows4MaxCtas * 2 * kRows4SlotFloats * 4;
 }
 
@@ -857,6 +860,7 @@ cudaError_t launch_attend4_rows(const AttendArgs& a, int sm_count, cudaStream_t 
 }
 
 cudaError_t launch_attend4(const AttendArgs& a, int max_query, int sm_count, cudaStream_t stream) {
+  if (kv_attend4_takes_tiles(max_query, a.group, a.c.dim)) return launch_attend_tile(a, sm_count, stream);
   const bool one = static_cast<long long>(max_query) * a.group <= 8;  // query rows per KV head in one n-tile
   switch (a.c.dim) {
     case 64: return one ? launch_attend4_rows<64, 1, 3>(a, sm_count, stream) : launch_attend4_rows<64, 2, 3>(a, sm_count, stream);

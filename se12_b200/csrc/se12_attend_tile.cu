@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       mbar_init(&sm.p_full[i], kTileSoftmaxWarps);
       mbar_init(&sm.pv_done[i], 1);
     }
-    for (int i = 0; i < kTileMeta; ++i) mbar_init(&sm.meta_full[i], 1);
+    for (int i = 0; i < kTileMeta; ++i) mbar_init(&sm.meta_full[i], KIND == kKvInt4 ? kTileLoaderWarps : 1);
     mbar_init(&sm.q_free, 1);
     mbar_init(&sm.q_full[0], kTileQueryWarps);
     mbar_init(&sm.q_full[1], kTileQueryWarps);
@@ -774,14 +774,15 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
     const uint8_t* codes = keys ? a.c.k_codes : a.c.v_codes;
     unsigned char* tiles = keys ? k_tiles : v_tiles;
     constexpr int kHalf = 4;  // 16-byte vectors per thread and half tile
+    constexpr bool kFour = KIND == kKvInt4;
     // A warp's vector: 8 tokens x 64 bytes. The 8 lanes of a shared-memory
     // phase hold one column of 8 tokens: all banks, in the swizzled layout.
     constexpr int kStep = Shape::kTokens / 8;  // tokens between a thread's vectors: 8 or 16
     const int w4 = tid >> 5;
-    const int panel = w4 % PANELS, sub = (w4 / PANELS) * 8 + (lane & 7);  // panel of 64 dimensions, token of a vector
+    const int panel = w4 % PANELS, sub = kFour ? 0 : (w4 / PANELS) * 8 + (lane & 7);  // panel of 64 dimensions, token of a vector
     const int column = panel * 64 + (lane >> 3) * 16;
     const int dim = a.c.dim;
-    const bool wanted = column < dim;
+    const bool wanted = kFour || column < dim;
     const uint8_t* source = codes + column;
     const int place = panel * Shape::kPanelBytes + sub * 128;
     const int place0 = place + ((((lane >> 3) * 2) ^ (lane & 7)) << 4), place1 = place + ((((lane >> 3) * 2 + 1) ^ (lane & 7)) << 4);
@@ -848,13 +849,153 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
         *reinterpret_cast<uint4*>(tile + place1 + (first + v) * kStep * 128) = h;
       }
     };
-    // Two halves per tile, each loaded a tile ahead: 32 KB per SM on the way.
-    uint4 ra[kHalf], rb[kHalf];
     fetch_pages();
     take_tile();
+    const int tiles_all = g1 - g0;
+    if constexpr (kFour) {
+      // ---- 4 bits. A warp has two cells of 16 tokens of a tile (256 dimensions:
+      // half of each row's codes), four vectors of 8 tokens x 64 bytes of codes.
+      // Keys become FP16 values; values become FP16 times 2^-X, X the largest E of
+      // the cell's tokens that count, which takes the place of a block's scale. A
+      // token whose E is no number has NaN for a key and zero for a value: the
+      // rows that see it are NaN, as their weights are.
+      const bool narrow = dim == 64;
+      const int groups = DP == 256 ? 4 : narrow ? 1 : 2;
+      const int part = DP == 256 ? (w4 & 1) * 4 + (lane >> 3) : lane >> 3;  // 16 bytes of a row's codes
+      const bool mine = !narrow || part < 2;
+      const int row_codes = dim / 2, key_lines = 4 * groups, cell_bytes = 64 * groups + 32;
+      constexpr int kWords = DP == 256 ? 8 : 4;  // of a vector's lines (keys: the first half of them)
+      const uint8_t* lines_of = static_cast<const uint8_t*>(keys ? a.c.k_scales : a.c.v_scales);
+      const uint8_t* cells = static_cast<const uint8_t*>(a.c.v_scales);
+      auto cell_of = [&](int v) { return DP == 256 ? (v >> 1) * 2 + (w4 >> 1) : (v >> 1) * 4 + w4; };
+      // Where word w of a vector goes: the 64 dimensions of a panel, 8 per column.
+      auto place_of = [&](int v, int w) {
+        const int to_panel = DP == 256 ? w : narrow ? part >> 1 : w & 1;
+        const int to_column = DP == 256 ? part : narrow ? (part & 1) * 4 + w : 2 * part + (w >> 1);
+        const int token = cell_of(v) * 16 + (v & 1) * 8 + (lane & 7);
+        return to_panel * Shape::kPanelBytes + token * 128 + ((to_column ^ (lane & 7)) << 4);
+      };
+      struct Vector {
+        uint4 codes;
+        uint32_t lines[kWords];  // keys: (scale, offset) of each group; values: scales, then offsets, of two tokens each
+        uint32_t power;          // E
+      };
+      Vector r[4];
+      auto load4 = [&](int v) {
+        const int row = __shfl_sync(0xFFFFFFFFu, rows_at, cell_of(v));
+        const int in_cell = (v & 1) * 8 + (lane & 7);
+        const bool use = row >= 0 && cell_of(v) * 16 + in_cell < limit;
+        r[v].codes = load_or_zero(codes + static_cast<long long>(row + in_cell) * row_codes + part * 16, use && mine);
+        const uint8_t* line = keys ? lines_of + static_cast<long long>(row + in_cell) * key_lines
+                                   : lines_of + static_cast<long long>(row >> 4) * cell_bytes + (in_cell >> 1) * (8 * groups);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) r[v].lines[i] = 0;
+        if (use && mine) {
+          if (DP == 256) {
+            const uint4 x = *reinterpret_cast<const uint4*>(line);
+            r[v].lines[0] = x.x, r[v].lines[1] = x.y, r[v].lines[2] = x.z, r[v].lines[3] = x.w;
+            if (!keys) {
+              const uint4 y = *reinterpret_cast<const uint4*>(line + 16);
+              r[v].lines[kWords - 4] = y.x, r[v].lines[kWords - 3] = y.y, r[v].lines[kWords - 2] = y.z, r[v].lines[kWords - 1] = y.w;
+            }
+          } else if (narrow) {
+            r[v].lines[0] = r[v].lines[1] = *reinterpret_cast<const uint32_t*>(line);
+            if (!keys) r[v].lines[2] = r[v].lines[3] = *reinterpret_cast<const uint32_t*>(line + 4);
+          } else if (keys) {
+            const uint2 x = *reinterpret_cast<const uint2*>(line);
+            r[v].lines[0] = x.x, r[v].lines[1] = x.y;
+          } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(line);
+            r[v].lines[0] = x.x, r[v].lines[1] = x.y, r[v].lines[2] = x.z, r[v].lines[3] = x.w;
+          }
+        }
+        r[v].power = 0xFC00u;  // -inf: a token that does not count
+        if (use)
+          r[v].power = *reinterpret_cast<const uint16_t*>(cells + static_cast<long long>(row >> 4) * cell_bytes + 64 * groups + 2 * in_cell);
+      };
+      // A vector's codes on their lines, to the tile.
+      auto store4 = [&](int v, unsigned char* tile, float cell_power) {
+        const float e = __half2float(__ushort_as_half(static_cast<unsigned short>(r[v].power)));
+        const bool number = e == e;
+        // (2^(E - X) of a token: what it takes from FP16's subnormals weighs nothing beside the cell's largest)
+        const uint32_t down = half2_bits(__half2half2(__float2half_rn(number ? ex2(e - cell_power) : 0.f)));
+        const uint32_t side = (lane & 1) ? 0x3232u : 0x1010u;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int g = DP == 256 ? w : w & 1;
+          uint32_t scale, offset;
+          if (keys) {
+            scale = prmt(r[v].lines[g], 0u, 0x1010u);
+            offset = prmt(r[v].lines[g], 0u, 0x3232u);
+            if (!number) scale = offset = 0x7FFF7FFFu;
+          } else {
+            const __half2 d = *reinterpret_cast<const __half2*>(&down);
+            const uint32_t s = prmt(r[v].lines[g], 0u, side), o = prmt(r[v].lines[kWords / 2 + g], 0u, side);
+            scale = half2_bits(__hmul2(*reinterpret_cast<const __half2*>(&s), d));
+            offset = half2_bits(__hmul2(*reinterpret_cast<const __half2*>(&o), d));
+          }
+          const uint32_t x = word_of(r[v].codes, w), y = x >> 8;
+          // u + 1024 and u + 64 in FP16, codes 0 and 4, 1 and 5, 2 and 6, 3 and 7
+          uint32_t h[4] = {(x & 0x000F000Fu) | 0x64006400u, (x & 0x00F000F0u) | 0x54005400u, (y & 0x000F000Fu) | 0x64006400u,
+                           (y & 0x00F000F0u) | 0x54005400u};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            asm("sub.f16x2 %0, %0, %1;" : "+r"(h[k]) : "r"(k & 1 ? 0x54805480u : 0x64086408u));
+            asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h[k]) : "r"(scale), "r"(offset));
+          }
+          *reinterpret_cast<uint4*>(tile + place_of(v, w)) =
+              make_uint4(prmt(h[0], h[1], 0x5410u), prmt(h[2], h[3], 0x5410u), prmt(h[0], h[1], 0x7632u), prmt(h[2], h[3], 0x7632u));
+        }
+      };
+#pragma unroll
+      for (int v = 0; v < 4; ++v) load4(v);
+#pragma unroll 1
+      for (int j = 0; j < tiles_all; ++j) {
+        const int stage = j & 1;
+        unsigned char* tile = tiles + stage * kTileKvBytes;
+        float cell_power[2];  // of the warp's cells; 0 where no token counts
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = kNegInf;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float e = __half2float(__ushort_as_half(static_cast<unsigned short>(r[2 * i + h].power)));
+            x = fmaxf(x, e);  // (NaN is left out)
+          }
+#pragma unroll
+          for (int d = 1; d < 8; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
+          cell_power[i] = fabsf(x) <= 64.f ? x : 0.f;
+        }
+        // the tile two before has been read by its products
+        if (j >= 2) wait(keys ? &sm.s_full[stage] : &sm.pv_done[stage], ((j >> 1) + 1) & 1);
+        const bool more = j + 1 < tiles_all;
+        const unsigned missing_groups = __ballot_sync(0xFFFFFFFFu, missing);
+        if (more) take_tile();
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          store4(v, tile, cell_power[v >> 1]);
+          if (more) load4(v);
+        }
+        fence_proxy_async_shared();
+        if (keys) {
+          const int slot = j % kTileMeta;
+          if (lane < 2) {
+            const int cell = cell_of(2 * lane);
+            sm.meta[slot][cell][0] = 1.f;
+            sm.meta[slot][cell][1] = lane == 0 ? cell_power[0] : cell_power[1];
+          }
+          if (tid == 0) sm.meta_missing[slot] = static_cast<int>(missing_groups);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.meta_full[slot]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(keys ? &sm.k_full[stage] : &sm.v_full[stage]);
+      }
+    } else {
+    // Two halves per tile, each loaded a tile ahead: 32 KB per SM on the way.
+    uint4 ra[kHalf], rb[kHalf];
     load(ra, 0);
     load(rb, kHalf);
-    const int tiles_all = g1 - g0;
 #pragma unroll 1
     for (int j = 0; j < tiles_all; ++j) {
       const int stage = j & 1;
@@ -885,6 +1026,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(keys ? &sm.k_full[stage] : &sm.v_full[stage]);
+    }
     }
   } else {
     // ---- softmax: row 32 warp + lane
@@ -1087,6 +1229,9 @@ cudaError_t launch_attend_tile_as(const AttendArgs& a, int sm_count, cudaStream_
 }
 
 cudaError_t launch_attend_tile(const AttendArgs& a, int sm_count, cudaStream_t stream) {
+  if (a.c.kind == kKvInt4)
+    return a.c.dim <= 128 ? launch_attend_tile_as<kKvInt4, 128>(a, sm_count, stream)
+                          : launch_attend_tile_as<kKvInt4, 256>(a, sm_count, stream);
   if (a.c.kind == kKvInt8)
     return a.c.dim <= 128 ? launch_attend_tile_as<kKvInt8, 128>(a, sm_count, stream)
                           : launch_attend_tile_as<kKvInt8, 256>(a, sm_count, stream);

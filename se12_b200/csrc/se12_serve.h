@@ -119,7 +119,8 @@ cudaError_t launch_kv_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, c
                              int sm_count, cudaStream_t stream);
 size_t kv_attend_partial_bytes(int sm_count, bool tile);
 cudaError_t launch_attend4(const AttendArgs& a, int max_query, int sm_count, cudaStream_t stream);
-size_t kv_attend4_partial_bytes(int sm_count);
+size_t kv_attend4_partial_bytes(int sm_count, bool tile);
+bool kv_attend4_takes_tiles(int max_query, int group, int dim);
 bool kv_attend_takes_tiles(int max_query, int group, int dim);
 cudaError_t launch_attend_tile(const AttendArgs& a, int sm_count, cudaStream_t stream);
 size_t kv_attend_tile_partial_bytes(int sm_count);

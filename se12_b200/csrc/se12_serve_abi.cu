@@ -178,14 +178,18 @@ int se12_kv_append_normed(const se12_kv_cache* cache, const se12_kv_batch* batch
 // [arrival counters, zero between calls][partial sums]
 size_t se12_kv_attend_workspace_bytes(const se12_kv_cache* c) {
   if (!c) return 0;
-  return SE12_COUNTER_BYTES + std::max(se12::kv_attend_partial_bytes(c->sm_count, false),
-                                       se12::kv_attend_partial_bytes(c->sm_count, true));
+  return SE12_COUNTER_BYTES + std::max({se12::kv_attend_partial_bytes(c->sm_count, false),
+                                        se12::kv_attend_partial_bytes(c->sm_count, true),
+                                        se12::kv_attend4_partial_bytes(c->sm_count, false)});
 }
 
 size_t se12_kv_attend_call_bytes(const se12_kv_cache* c, int q_heads, int max_query) {
   if (!c || q_heads < 1 || max_query < 1) return 0;
-  if (c->view.kind == SE12_KV_INT4) return SE12_COUNTER_BYTES + se12::kv_attend4_partial_bytes(c->sm_count);
-  const bool tiles = se12::kv_attend_takes_tiles(max_query, std::max(q_heads / c->view.heads, 1), c->view.dim);
+  const int group = std::max(q_heads / c->view.heads, 1);
+  if (c->view.kind == SE12_KV_INT4)
+    return SE12_COUNTER_BYTES +
+           se12::kv_attend4_partial_bytes(c->sm_count, se12::kv_attend4_takes_tiles(max_query, group, c->view.dim));
+  const bool tiles = se12::kv_attend_takes_tiles(max_query, group, c->view.dim);
   return SE12_COUNTER_BYTES + se12::kv_attend_partial_bytes(c->sm_count, tiles);
 }
 
