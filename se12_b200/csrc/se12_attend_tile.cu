@@ -182,6 +182,42 @@ __device__ __forceinline__ uint4 load_or_zero(const uint8_t* p, bool use) {
   return v;
 }
 
+__device__ __forceinline__ uint32_t load_word_or(const uint8_t* p, bool use, uint32_t other) {
+  uint32_t v;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, %3;\n\t@p ld.global.u32 %0, [%1];\n\t}"
+               : "=&r"(v)
+               : "l"(p), "r"(static_cast<uint32_t>(use)), "r"(other)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ uint32_t load_half_or(const uint8_t* p, bool use, uint32_t other) {
+  uint32_t v;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, %3;\n\t@p ld.global.u16 %0, [%1];\n\t}"
+               : "=&r"(v)
+               : "l"(p), "r"(static_cast<uint32_t>(use)), "r"(other)
+               : "memory");
+  return v;
+}
+
+// 4 bits: tiles hold the 8 dimensions of a word in the order 0 4 1 5 2 6 3 7, as
+// its codes are unpacked. Where dimension d of 8 is, and 8 halves put in that order.
+template <int KIND>
+__device__ __forceinline__ constexpr int of_eight(int d) {
+  return KIND == kKvInt4 ? (d & 3) * 2 + (d >> 2) : d;
+}
+template <int KIND>
+__device__ __forceinline__ uint4 unpacked_order(uint32_t x01, uint32_t x23, uint32_t x45, uint32_t x67) {
+  if constexpr (KIND == kKvInt4)
+    return make_uint4(prmt(x01, x45, 0x5410u), prmt(x01, x45, 0x7632u), prmt(x23, x67, 0x5410u), prmt(x23, x67, 0x7632u));
+  return make_uint4(x01, x23, x45, x67);
+}
+
+template <int N>
+__device__ __forceinline__ void to_words(uint32_t (&w)[N], int at, const uint4& v) {
+  w[at] = v.x, w[at + 1] = v.y, w[at + 2] = v.z, w[at + 3] = v.w;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -563,7 +599,8 @@ __device__ __forceinline__ void store_8(uint16_t* out, int d, int dim, int vec, 
 
 // ------------------------------------------------------------------ kernel
 
-template <int KIND, int DP>
+// NARROW: 64 dimensions (of 4-bit codes; 8-bit ones take any number in their stride).
+template <int KIND, int DP, bool NARROW>
 __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(const AttendArgs a) {
   using Shape = TileShape<KIND, DP>;
   constexpr int TT = Shape::kTokens, PANELS = Shape::kPanels, GROUPS = Shape::kGroups;
@@ -754,7 +791,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
 #pragma unroll
             for (int j = 0; j < kVectors; ++j)
               *reinterpret_cast<uint4*>(q_tile + j * Shape::kQueryPanel + q_row * 128 + ((part ^ (q_row & 7)) << 4)) =
-                  make_uint4(halves(raw[j].x), halves(raw[j].y), halves(raw[j].z), halves(raw[j].w));
+                  unpacked_order<KIND>(halves(raw[j].x), halves(raw[j].y), halves(raw[j].z), halves(raw[j].w));
             if (part == 0)
               sm.row_scale[pair & 1][q_row] = __uint_as_float(static_cast<unsigned>(127 + e) << 23) * fabsf(a.scale);
           }
@@ -856,22 +893,22 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       // ---- 4 bits. A warp has two cells of 16 tokens of a tile (256 dimensions:
       // half of each row's codes), four vectors of 8 tokens x 64 bytes of codes.
       // Keys become FP16 values; values become FP16 times 2^-X, X the largest E of
-      // the cell's tokens that count, which takes the place of a block's scale. A
+      // the cell's tokens that count, which takes the place of a block's scale. The 8
+      // of a word stay in the order their codes are unpacked in (of_eight). A
       // token whose E is no number has NaN for a key and zero for a value: the
       // rows that see it are NaN, as their weights are.
-      const bool narrow = dim == 64;
-      const int groups = DP == 256 ? 4 : narrow ? 1 : 2;
+      constexpr int groups = DP == 256 ? 4 : NARROW ? 1 : 2;
       const int part = DP == 256 ? (w4 & 1) * 4 + (lane >> 3) : lane >> 3;  // 16 bytes of a row's codes
-      const bool mine = !narrow || part < 2;
-      const int row_codes = dim / 2, key_lines = 4 * groups, cell_bytes = 64 * groups + 32;
+      const bool mine = !NARROW || part < 2;
+      constexpr int row_codes = 32 * groups, key_lines = 4 * groups, cell_bytes = 64 * groups + 32;
       constexpr int kWords = DP == 256 ? 8 : 4;  // of a vector's lines (keys: the first half of them)
       const uint8_t* lines_of = static_cast<const uint8_t*>(keys ? a.c.k_scales : a.c.v_scales);
       const uint8_t* cells = static_cast<const uint8_t*>(a.c.v_scales);
       auto cell_of = [&](int v) { return DP == 256 ? (v >> 1) * 2 + (w4 >> 1) : (v >> 1) * 4 + w4; };
       // Where word w of a vector goes: the 64 dimensions of a panel, 8 per column.
       auto place_of = [&](int v, int w) {
-        const int to_panel = DP == 256 ? w : narrow ? part >> 1 : w & 1;
-        const int to_column = DP == 256 ? part : narrow ? (part & 1) * 4 + w : 2 * part + (w >> 1);
+        const int to_panel = DP == 256 ? w : NARROW ? part >> 1 : w & 1;
+        const int to_column = DP == 256 ? part : NARROW ? (part & 1) * 4 + w : 2 * part + (w >> 1);
         const int token = cell_of(v) * 16 + (v & 1) * 8 + (lane & 7);
         return to_panel * Shape::kPanelBytes + token * 128 + ((to_column ^ (lane & 7)) << 4);
       };
@@ -881,37 +918,33 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
         uint32_t power;          // E
       };
       Vector r[4];
-      auto load4 = [&](int v) {
-        const int row = __shfl_sync(0xFFFFFFFFu, rows_at, cell_of(v));
-        const int in_cell = (v & 1) * 8 + (lane & 7);
-        const bool use = row >= 0 && cell_of(v) * 16 + in_cell < limit;
-        r[v].codes = load_or_zero(codes + static_cast<long long>(row + in_cell) * row_codes + part * 16, use && mine);
-        const uint8_t* line = keys ? lines_of + static_cast<long long>(row + in_cell) * key_lines
-                                   : lines_of + static_cast<long long>(row >> 4) * cell_bytes + (in_cell >> 1) * (8 * groups);
+      auto load_cell = [&](int i) {  // the i-th of the warp's: vectors 2 i and 2 i + 1
+        const int row = __shfl_sync(0xFFFFFFFFu, rows_at, cell_of(2 * i));
+        const int token = lane & 7, left = row >= 0 ? limit - cell_of(2 * i) * 16 - token : 0;
+        const uint8_t* code = codes + static_cast<long long>(row + token) * row_codes + part * 16;
+        const uint8_t* cell = cells + static_cast<long long>(row >> 4) * cell_bytes;
+        const uint8_t* line = keys ? lines_of + static_cast<long long>(row + token) * key_lines : cell + (token >> 1) * (8 * groups);
+        const uint8_t* power = cell + 64 * groups + 2 * token;
+        const int line_step = keys ? 8 * key_lines : 32 * groups;
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) r[v].lines[i] = 0;
-        if (use && mine) {
-          if (DP == 256) {
-            const uint4 x = *reinterpret_cast<const uint4*>(line);
-            r[v].lines[0] = x.x, r[v].lines[1] = x.y, r[v].lines[2] = x.z, r[v].lines[3] = x.w;
-            if (!keys) {
-              const uint4 y = *reinterpret_cast<const uint4*>(line + 16);
-              r[v].lines[kWords - 4] = y.x, r[v].lines[kWords - 3] = y.y, r[v].lines[kWords - 2] = y.z, r[v].lines[kWords - 1] = y.w;
-            }
-          } else if (narrow) {
-            r[v].lines[0] = r[v].lines[1] = *reinterpret_cast<const uint32_t*>(line);
-            if (!keys) r[v].lines[2] = r[v].lines[3] = *reinterpret_cast<const uint32_t*>(line + 4);
+        for (int h = 0; h < 2; ++h) {
+          Vector& x = r[2 * i + h];
+          const bool use = left > 8 * h, wanted_lines = use && mine;
+          x.codes = load_or_zero(code + h * (8 * row_codes), wanted_lines);
+          if constexpr (DP == 256) {
+            to_words(x.lines, 0, load_or_zero(line + h * line_step, wanted_lines));
+            if (!keys) to_words(x.lines, kWords - 4, load_or_zero(line + h * line_step + 16, wanted_lines));
+          } else if constexpr (NARROW) {
+            x.lines[0] = x.lines[1] = load_word_or(line + h * line_step, wanted_lines, 0u);
+            x.lines[2] = x.lines[3] = load_word_or(line + h * line_step + 4, wanted_lines && !keys, 0u);
           } else if (keys) {
-            const uint2 x = *reinterpret_cast<const uint2*>(line);
-            r[v].lines[0] = x.x, r[v].lines[1] = x.y;
+            x.lines[0] = load_word_or(line + h * line_step, wanted_lines, 0u);
+            x.lines[1] = load_word_or(line + h * line_step + 4, wanted_lines, 0u);
           } else {
-            const uint4 x = *reinterpret_cast<const uint4*>(line);
-            r[v].lines[0] = x.x, r[v].lines[1] = x.y, r[v].lines[2] = x.z, r[v].lines[3] = x.w;
+            to_words(x.lines, 0, load_or_zero(line + h * line_step, wanted_lines));
           }
+          x.power = load_half_or(power + 16 * h, use, 0xFC00u);  // (-inf: a token that does not count)
         }
-        r[v].power = 0xFC00u;  // -inf: a token that does not count
-        if (use)
-          r[v].power = *reinterpret_cast<const uint16_t*>(cells + static_cast<long long>(row >> 4) * cell_bytes + 64 * groups + 2 * in_cell);
       };
       // A vector's codes on their lines, to the tile.
       auto store4 = [&](int v, unsigned char* tile, float cell_power) {
@@ -943,12 +976,11 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
             asm("sub.f16x2 %0, %0, %1;" : "+r"(h[k]) : "r"(k & 1 ? 0x54805480u : 0x64086408u));
             asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h[k]) : "r"(scale), "r"(offset));
           }
-          *reinterpret_cast<uint4*>(tile + place_of(v, w)) =
-              make_uint4(prmt(h[0], h[1], 0x5410u), prmt(h[2], h[3], 0x5410u), prmt(h[0], h[1], 0x7632u), prmt(h[2], h[3], 0x7632u));
+          *reinterpret_cast<uint4*>(tile + place_of(v, w)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
       };
-#pragma unroll
-      for (int v = 0; v < 4; ++v) load4(v);
+      load_cell(0);
+      load_cell(1);
 #pragma unroll 1
       for (int j = 0; j < tiles_all; ++j) {
         const int stage = j & 1;
@@ -972,9 +1004,10 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
         const unsigned missing_groups = __ballot_sync(0xFFFFFFFFu, missing);
         if (more) take_tile();
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          store4(v, tile, cell_power[v >> 1]);
-          if (more) load4(v);
+        for (int i = 0; i < 2; ++i) {
+          store4(2 * i, tile, cell_power[i]);
+          store4(2 * i + 1, tile, cell_power[i]);
+          if (more) load_cell(i);
         }
         fence_proxy_async_shared();
         if (keys) {
@@ -1134,8 +1167,10 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                w[e] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[k + 2 * e]) * f)) |
-                       (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[k + 2 * e + 1]) * f))) << 16);
+                w[e] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[k + of_eight<KIND>(2 * e)]) * f)) |
+                       (static_cast<uint32_t>(__bfloat16_as_ushort(
+                            __float2bfloat16_rn(__uint_as_float(o[k + of_eight<KIND>(2 * e + 1)]) * f)))
+                        << 16);
               store_8(out, d0 + k, a.c.dim, a.o_vec, w);
             }
           }
@@ -1209,8 +1244,8 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            w[e] = __bfloat16_as_ushort(__float2bfloat16_rn(v[k + 2 * e] * f)) |
-                   (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(v[k + 2 * e + 1] * f))) << 16);
+            w[e] = __bfloat16_as_ushort(__float2bfloat16_rn(v[k + of_eight<KIND>(2 * e)] * f)) |
+                   (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(v[k + of_eight<KIND>(2 * e + 1)] * f))) << 16);
           store_8(out, d0 + k, a.c.dim, a.o_vec, w);
         }
       }
@@ -1222,16 +1257,17 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
 
 size_t kv_attend_tile_partial_bytes(int sm_count) { return static_cast<size_t>(sm_count) * 2 * kTileSlotFloats * 4; }
 
-template <int KIND, int DP>
+template <int KIND, int DP, bool NARROW = false>
 cudaError_t launch_attend_tile_as(const AttendArgs& a, int sm_count, cudaStream_t stream) {
   const size_t smem = TileShape<KIND, DP>::kSmem + (2 * a.t.seqs + 1) * sizeof(int);
-  return launch_overlapped(attend_tile_kernel<KIND, DP>, dim3(sm_count), kTileAttendThreads, smem, stream, a);
+  return launch_overlapped(attend_tile_kernel<KIND, DP, NARROW>, dim3(sm_count), kTileAttendThreads, smem, stream, a);
 }
 
 cudaError_t launch_attend_tile(const AttendArgs& a, int sm_count, cudaStream_t stream) {
   if (a.c.kind == kKvInt4)
-    return a.c.dim <= 128 ? launch_attend_tile_as<kKvInt4, 128>(a, sm_count, stream)
-                          : launch_attend_tile_as<kKvInt4, 256>(a, sm_count, stream);
+    return a.c.dim == 64    ? launch_attend_tile_as<kKvInt4, 128, true>(a, sm_count, stream)
+           : a.c.dim == 128 ? launch_attend_tile_as<kKvInt4, 128>(a, sm_count, stream)
+                            : launch_attend_tile_as<kKvInt4, 256>(a, sm_count, stream);
   if (a.c.kind == kKvInt8)
     return a.c.dim <= 128 ? launch_attend_tile_as<kKvInt8, 128>(a, sm_count, stream)
                           : launch_attend_tile_as<kKvInt8, 256>(a, sm_count, stream);
