@@ -126,13 +126,16 @@ __device__ __forceinline__ void load_row(RowOf8& r, const T* row, const RowOrder
 }
 
 template <int DIM, bool VEC>
-__device__ __forceinline__ void normalise_row(RowOf8& r, const RowNorm& norm, double eps, const RowOrder& o, int l) {
-  const float f = norm_factor(team_sum(add_squares<4>(r.b, add_squares<4>(r.a, 0.0)), DIM / 8), DIM, eps);
-  RowOf8 w;
+__device__ __forceinline__ void load_weight_row(RowOf8& w, const RowNorm& norm, const RowOrder& o, int l) {
   if (norm.bf16)
     load_row<DIM, VEC>(w, static_cast<const __nv_bfloat16*>(norm.weight), o, l);
   else
     load_row<DIM, VEC>(w, static_cast<const float*>(norm.weight), o, l);
+}
+
+template <int DIM>
+__device__ __forceinline__ void normalise_row(RowOf8& r, const RowOf8& w, double eps) {
+  const float f = norm_factor(team_sum(add_squares<4>(r.b, add_squares<4>(r.a, 0.0)), DIM / 8), DIM, eps);
   apply_norm<4>(r.a, f, w.a);
   apply_norm<4>(r.b, f, w.b);
 }
@@ -188,18 +191,21 @@ struct GroupLine {
   __device__ __forceinline__ uint32_t codes(const float (&x)[4]) const {
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float u = rintf(__fmul_rn(__fsub_rn(x[j], middle), inverse)) + 8.f;
-      w |= static_cast<uint32_t>(fminf(fmaxf(u, 0.f), 15.f)) << (4 * j);  // (NaN: 0)
+    for (int j = 3; j >= 0; --j) {
+      // rounded to a whole number by an addend of 1.5 2^23 (and 8, the zero point): the code is in the last bits
+      const float u = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], middle), inverse), -8.f), 7.f);  // (NaN: -8)
+      w = w * 16 + __float_as_uint(__fadd_rn(u, 12582920.f));
     }
-    return w;
+    return w & 0xFFFFu;
   }
 };
 
 // A lane's row quantised and stored as token `slot` of a block. All lanes of
-// the warp take part; where `live` is false nothing is stored.
-template <int DIM, bool KEYS>
-__device__ __forceinline__ void store_row(const AppendArgs& a, RowOf8& r, long long block, int slot, int l, bool live) {
+// the warp take part; where `live` is false nothing is stored. (Keys and values
+// by one piece of code: two, unrolled over four rows, were waiting for
+// instructions most of the time, 13 prompt chunks 387 us.)
+template <int DIM>
+__device__ __forceinline__ void store_row(const AppendArgs& a, bool keys, RowOf8& r, long long block, int slot, int l, bool live) {
   constexpr int G = DIM / kKv4Group;
   constexpr int kSpan = DIM >= 128 ? 16 : 8;  // lanes of a group
   float lo_a = min_nan(min_nan(r.a[0], r.a[1]), min_nan(r.a[2], r.a[3])), hi_a = max_nan(max_nan(r.a[0], r.a[1]), max_nan(r.a[2], r.a[3]));
@@ -218,56 +224,48 @@ __device__ __forceinline__ void store_row(const AppendArgs& a, RowOf8& r, long l
     }
   }
   if (DIM < 128) lo_b = lo_a, hi_b = hi_a;
-  GroupLine ga, gb;
+  const float size_a = max_nan(fabsf(lo_a), fabsf(hi_a)), size_b = max_nan(fabsf(lo_b), fabsf(hi_b));
   float exponent = 0.f;
-  if (KEYS) {
-    ga.fit(lo_a, hi_a);
-    gb.fit(lo_b, hi_b);
-    const __half nan = __ushort_as_half(0x7FFFu);
-    if (!(max_nan(fabsf(lo_a), fabsf(hi_a)) <= kKv4KeyLimit)) ga.scale = ga.offset = nan;
-    if (!(max_nan(fabsf(lo_b), fabsf(hi_b)) <= kKv4KeyLimit)) gb.scale = gb.offset = nan;
-  } else {
-    float amax = max_nan(max_nan(fabsf(lo_a), fabsf(hi_a)), max_nan(fabsf(lo_b), fabsf(hi_b)));
+  if (!keys) {
+    float amax = max_nan(size_a, size_b);
     if (DIM == 256) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 16));
-    if (amax < kKv4ValueLimit) {
-      const int e = max(static_cast<int>(__float_as_uint(amax) >> 23) - 130, kKv4MinExponent);
-      exponent = static_cast<float>(e);
-      const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
-      lo_a *= down, hi_a *= down, lo_b *= down, hi_b *= down;
+    const bool fits = amax < kKv4ValueLimit;  // (otherwise, NaN too, the token is NaN through E alone: its line is 0)
+    const int e = fits ? max(static_cast<int>(__float_as_uint(amax) >> 23) - 130, kKv4MinExponent) : 0;
+    exponent = fits ? static_cast<float>(e) : __uint_as_float(0x7FC00000u);
+    const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+    auto scaled = [&](float x) { return fits ? x * down : 0.f; };
+    lo_a = scaled(lo_a), hi_a = scaled(hi_a), lo_b = scaled(lo_b), hi_b = scaled(hi_b);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r.a[j] *= down, r.b[j] *= down;
-    } else {  // (also NaN) the token is NaN through E alone: scales and offsets stay finite
-      exponent = __uint_as_float(0x7FC00000u);
-      lo_a = hi_a = lo_b = hi_b = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) r.a[j] = r.b[j] = 0.f;
-    }
-    ga.fit(lo_a, hi_a);
-    gb.fit(lo_b, hi_b);
+    for (int j = 0; j < 4; ++j) r.a[j] = scaled(r.a[j]), r.b[j] = scaled(r.b[j]);
   }
+  GroupLine ga, gb;
+  ga.fit(lo_a, hi_a);
+  gb.fit(lo_b, hi_b);
   // Words of 8 codes: an even lane completes the first vector's, an odd one the second's.
   const uint32_t wa = ga.codes(r.a), wb = gb.codes(r.b);
   const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, l & 1 ? wa : wb, 1);
   const uint32_t word = l & 1 ? other | (wb << 16) : wa | (other << 16);
   if (!live) return;
   const int n = (l & 1 ? DIM / 16 : 0) + l / 2;  // the word in the row's order
-  uint8_t* codes = KEYS ? a.c.k_codes : a.c.v_codes;
   const long long row = block * a.c.page_size + slot;
-  reinterpret_cast<uint32_t*>(codes + row * (DIM / 2))[(n & 7) * G + (n >> 3)] = word;
+  reinterpret_cast<uint32_t*>((keys ? a.c.k_codes : a.c.v_codes) + row * (DIM / 2))[(n & 7) * G + (n >> 3)] = word;
   // The lanes of span h hold group h of the first half (ga) and group G / 2 + h of the second.
   const int h = l / kSpan, k = l % kSpan;
-  if (KEYS) {
-    __half2* scales = reinterpret_cast<__half2*>(a.c.k_scales) + row * G;
-    if (k == 0) scales[h] = __halves2half2(ga.scale, ga.offset);
-    if (DIM >= 128 && k == 1) scales[G / 2 + h] = __halves2half2(gb.scale, gb.offset);
+  if (keys) {
+    const bool second = k == 1;
+    if (k == 0 || (DIM >= 128 && second)) {
+      const bool fits = (second ? size_b : size_a) <= kKv4KeyLimit;
+      const __half2 line = second ? __halves2half2(gb.scale, gb.offset) : __halves2half2(ga.scale, ga.offset);
+      const __half2 nan = __half2half2(__ushort_as_half(0x7FFFu));
+      reinterpret_cast<__half2*>(a.c.k_scales)[row * G + (second ? G / 2 + h : h)] = fits ? line : nan;
+    }
   } else {
     __half* cell = reinterpret_cast<__half*>(a.c.v_scales) +
                    (block * (a.c.page_size >> 4) + (slot >> 4)) * (32 * G + 16);
-    __half* pair = cell + ((slot & 15) >> 1) * (4 * G) + (slot & 1);
-    if (k == 0) pair[2 * h] = ga.scale;
-    if (k == 1) pair[2 * (G + h)] = ga.offset;
-    if (DIM >= 128 && k == 2) pair[2 * (G / 2 + h)] = gb.scale;
-    if (DIM >= 128 && k == 3) pair[2 * (G + G / 2 + h)] = gb.offset;
+    // lane k of a span: scale, offset of ga, of gb; lane 4 of the row: E
+    const int at = ((slot & 15) >> 1) * (4 * G) + (slot & 1);
+    const __half x = k == 0 ? ga.scale : k == 1 ? ga.offset : k == 2 ? gb.scale : gb.offset;
+    if (k < (DIM >= 128 ? 4 : 2)) cell[at + 2 * ((k & 1 ? G : 0) + (k < 2 ? h : G / 2 + h))] = x;
     if (l == 4) cell[32 * G + (slot & 15)] = __float2half_rn(exponent);
   }
 }
@@ -288,11 +286,12 @@ __device__ __forceinline__ int sequence_at(const TokenBatch& t, int token, int l
 }
 
 // A warp takes a token's queries, keys or values, 32 / (DIM / 8) heads side by
-// side and U of those one after the other (all their loads on the way at once).
+// side and up to `turns` of those one after the other, the next on its way.
 // `q_warps` and `kv_warps`: warps per token for its queries, and for its keys and
 // for its values.
-template <typename T, int DIM, bool VEC, int U>
-__global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArgs a, const int q_warps, const int kv_warps) {
+template <typename T, int DIM, bool VEC>
+__global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArgs a, const int q_warps, const int kv_warps,
+                                                                 const int turns) {
   constexpr int kTeam = DIM / 8, kTeams = 32 / kTeam;
   __shared__ float4 staged[kKv4Threads / 32][kTeams][DIM / 4];
   grid_launch_dependents();
@@ -305,22 +304,15 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArg
   int part = static_cast<int>(item - static_cast<long long>(token) * per_token);
   const bool queries = part < q_warps, keys = !queries && part < q_warps + kv_warps;
   part -= queries ? 0 : keys ? q_warps : q_warps + kv_warps;
-  const int heads = queries ? a.q_heads : a.c.heads, head0 = part * (U * kTeams) + team;
+  const int heads = queries ? a.q_heads : a.c.heads, head0 = part * (turns * kTeams);
+  const int end = min(head0 + turns * kTeams, heads);
   const T* src = static_cast<const T*>(queries ? a.q : keys ? a.k : a.v) + token * (queries ? a.q_ts : keys ? a.k_ts : a.v_ts);
   const long long hs = queries ? a.q_hs : keys ? a.k_hs : a.v_hs;
   const RowOrder order = row_order<DIM>(a, queries || keys);
+  // (teams past the last head take the last one again, and store nothing)
+  RowOf8 next;
+  load_row<DIM, VEC>(next, src + min(head0 + team, heads - 1) * hs, order, l);
 
-  RowOf8 row[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int head = head0 + u * kTeams;
-    if (head < heads) {
-      load_row<DIM, VEC>(row[u], src + head * hs, order, l);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) row[u].a[j] = row[u].b[j] = 0.f;
-    }
-  }
   const ListSizes sizes{a.t.tokens, a.t.max_pages << a.c.page_shift, 1, 0};
   const int b = sequence_at(a.t, token, lane);
   const SeqRows s = a.t.rows_of(b, sizes);
@@ -331,16 +323,11 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArg
     raise_status(kStatusBadArgument);
     pos = -1;
   }
+  uint16_t* out = a.q_out + token * a.o_ts;
   if (pos < 0) {
-    if (!queries) return;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int head = head0 + u * kTeams;
-      if (head < heads) {
-        uint16_t* out = a.q_out + token * a.o_ts + head * a.o_hs;
-        for (int i = l; i < DIM; i += kTeam) out[i] = 0;
-      }
-    }
+    if (queries)
+      for (int head = head0 + team; head < end; head += kTeams)
+        for (int i = l; i < DIM; i += kTeam) out[head * a.o_hs + i] = 0;
     return;
   }
   const int page = queries ? 0 : page_of(a.t, a.c, b, pos);
@@ -348,34 +335,32 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArg
   Angles angles;
   load_angles<DIM, VEC>(angles, a, order, pos, l);
   const RowNorm norm = queries ? a.q_norm : keys ? a.k_norm : RowNorm{};
+  RowOf8 weight;
+  if (norm.weight) load_weight_row<DIM, VEC>(weight, norm, order, l);
+  const int slot = pos & (a.c.page_size - 1);
+#pragma unroll 1
+  for (int first = head0; first < end; first += kTeams) {
+    const int head = first + team;
+    const bool live = head < end;
+    RowOf8 row = next;
+    if (first + kTeams < end) load_row<DIM, VEC>(next, src + min(head + kTeams, heads - 1) * hs, order, l);
+    if (norm.weight) normalise_row<DIM>(row, weight, a.norm_eps);
+    rotate_row(row, angles, order, l, DIM / 4);
+    if (order.apart) reorder_row<DIM, VEC>(row, reinterpret_cast<float*>(staged[warp][team]), order, l);
+    if (!queries) {
+      store_row<DIM>(a, keys, row, static_cast<long long>(page) * a.c.heads + head, slot, l, live);
+    } else if (live) {
+      uint16_t* to = out + head * a.o_hs;
+      if (VEC) {
+        store_bf16<4>(to + 4 * l, row.a);
+        store_bf16<4>(to + DIM / 2 + 4 * l, row.b);
+      } else {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int head = head0 + u * kTeams;
-    const bool live = head < heads;
-    if (norm.weight) normalise_row<DIM, VEC>(row[u], norm, a.norm_eps, order, l);
-    rotate_row(row[u], angles, order, l, DIM / 4);
-    if (order.apart) reorder_row<DIM, VEC>(row[u], reinterpret_cast<float*>(staged[warp][team]), order, l);
-    if (queries) {
-      uint16_t* out = a.q_out + token * a.o_ts + head * a.o_hs;
-      if (live) {
-        if (VEC) {
-          store_bf16<4>(out + 4 * l, row[u].a);
-          store_bf16<4>(out + DIM / 2 + 4 * l, row[u].b);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            out[4 * l + j] = __bfloat16_as_ushort(__float2bfloat16_rn(row[u].a[j]));
-            out[DIM / 2 + 4 * l + j] = __bfloat16_as_ushort(__float2bfloat16_rn(row[u].b[j]));
-          }
+        for (int j = 0; j < 4; ++j) {
+          to[4 * l + j] = __bfloat16_as_ushort(__float2bfloat16_rn(row.a[j]));
+          to[DIM / 2 + 4 * l + j] = __bfloat16_as_ushort(__float2bfloat16_rn(row.b[j]));
         }
       }
-    } else {
-      const long long block = static_cast<long long>(page) * a.c.heads + head;
-      const int slot = pos & (a.c.page_size - 1);
-      if (keys)
-        store_row<DIM, true>(a, row[u], block, slot, l, live);
-      else
-        store_row<DIM, false>(a, row[u], block, slot, l, live);
     }
   }
 }
@@ -437,15 +422,20 @@ __global__ void __launch_bounds__(256) kv4_decode_kernel(const KvView c, const i
 
 // ------------------------------------------------------------------ launches
 
-template <typename T, int DIM, bool VEC, int U>
+template <typename T, int DIM, bool VEC>
 cudaError_t launch_append4_as(const AppendArgs& a, cudaStream_t stream) {
-  constexpr int kHeads = U * (32 / (DIM / 8));  // of a warp
-  const int q_warps = a.q ? (a.q_heads + kHeads - 1) / kHeads : 0, kv_warps = (a.c.heads + kHeads - 1) / kHeads;
+  constexpr int kTeams = 32 / (DIM / 8);
+  // Few rows: one after the other in as many warps; many: up to 8 in one, which
+  // finds the token's place and angles once for them.
+  const long long rows = static_cast<long long>(a.t.tokens) * (2 * a.c.heads + (a.q ? a.q_heads : 0)) / kTeams;
+  const int turns = rows > 16384 ? 8 : 1;
+  const int heads = turns * kTeams;  // of a warp
+  const int q_warps = a.q ? (a.q_heads + heads - 1) / heads : 0, kv_warps = (a.c.heads + heads - 1) / heads;
   const long long warps = static_cast<long long>(a.t.tokens) * (q_warps + 2 * kv_warps);
   const long long ctas = (warps + kKv4Threads / 32 - 1) / (kKv4Threads / 32);
   if (ctas > INT32_MAX) return cudaErrorInvalidConfiguration;
-  return launch_overlapped(kv4_append_kernel<T, DIM, VEC, U>, dim3(static_cast<unsigned>(ctas)), kKv4Threads, 0, stream, a,
-                           q_warps, kv_warps);
+  return launch_overlapped(kv4_append_kernel<T, DIM, VEC>, dim3(static_cast<unsigned>(ctas)), kKv4Threads, 0, stream, a, q_warps,
+                           kv_warps, turns);
 }
 
 template <typename T, int DIM>
@@ -460,9 +450,7 @@ cudaError_t launch_append4_dim(const AppendArgs& a, cudaStream_t stream) {
   if (a.q && (reinterpret_cast<uintptr_t>(a.q_out) % 8 || a.o_ts % 4 || a.o_hs % 4)) vec = false;
   for (const RowNorm& n : {a.q_norm, a.k_norm})
     if (reinterpret_cast<uintptr_t>(n.weight) % (n.bf16 ? 8 : 16)) vec = false;
-  if (!vec) return launch_append4_as<T, DIM, false, 1>(a, stream);
-  const long long rows = static_cast<long long>(a.t.tokens) * (2 * a.c.heads + (a.q ? a.q_heads : 0));
-  return rows > 16384 ? launch_append4_as<T, DIM, true, 4>(a, stream) : launch_append4_as<T, DIM, true, 1>(a, stream);
+  return vec ? launch_append4_as<T, DIM, true>(a, stream) : launch_append4_as<T, DIM, false>(a, stream);
 }
 
 cudaError_t launch_kv4_append(bool bf16, const AppendArgs& a, cudaStream_t stream) {
