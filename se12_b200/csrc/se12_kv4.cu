@@ -33,10 +33,10 @@ constexpr float kKv4KeyLimit = 65000.f;         // larger keys do not fit FP16's
 constexpr float kKv4ValueLimit = 17179869184.f;  // 2^34: E is at most 30
 constexpr int kKv4Threads = 128;
 
-// How a head's row is spread over its team of DIM / 8 lanes. In order: lane l
-// has the dimensions 4 l .. 4 l + 3 and DIM / 2 + 4 l .. + 3. Read: the members
-// of the pairs 4 l .. 4 l + 3 that are turned together, which are the same
-// dimensions unless part of the row is turned in halves.
+// How a head's row is spread over its team of DIM / 16 lanes. In order: lane l
+// has the dimensions 8 l .. 8 l + 7 and DIM / 2 + 8 l .. + 7, a word of codes
+// each. Read: the members of the pairs 8 l .. 8 l + 7 that are turned together,
+// which are the same dimensions unless part of the row is turned in halves.
 struct RowOrder {
   int mode;    // 0: not turned; 1: pairs (i, i + half); 2: neighbours
   int turned;  // pairs that are
@@ -65,117 +65,211 @@ __device__ __forceinline__ RowOrder row_order(const AppendArgs& a, bool turned) 
   return o;
 }
 
-// A lane's part of a row.
-struct RowOf8 {
-  float a[4], b[4];
+// Eight values, two by two.
+struct Eight {
+  unsigned long long v[4];
+
+  __device__ __forceinline__ void set(int j, float x) {  // (j known at compile time)
+    float lo, hi;
+    unpair(v[j >> 1], lo, hi);
+    v[j >> 1] = j & 1 ? pair_of(lo, x) : pair_of(x, hi);
+  }
+  __device__ __forceinline__ float get(int j) const {
+    float lo, hi;
+    unpair(v[j >> 1], lo, hi);
+    return j & 1 ? hi : lo;
+  }
 };
 
-// The cosines and sines that a lane needs at one position.
-struct Angles {
-  float c[4], s[4];
-};
+__device__ __forceinline__ unsigned long long both(float x) { return pair_of(x, x); }
 
-// VEC: every vector of four elements (and the angles' vectors) is aligned, and
-// halves are multiples of four.
-template <int DIM, bool VEC>
-__device__ __forceinline__ void load_angles(Angles& t, const AppendArgs& a, const RowOrder& o, int pos, int l) {
+// x + y and x - y, each rounded by itself also where x and y are products: of
+// mul.rn.f32x2 and add.rn.f32x2 the assembler makes one fma, of this it does not.
+__device__ __forceinline__ unsigned long long add_apart(unsigned long long x, unsigned long long y) {
+  float a, b, c, d;
+  unpair(x, a, b);
+  unpair(y, c, d);
+  return pair_of(__fadd_rn(a, c), __fadd_rn(b, d));
+}
+__device__ __forceinline__ unsigned long long sub_apart(unsigned long long x, unsigned long long y) {
+  float a, b, c, d;
+  unpair(x, a, b);
+  unpair(y, c, d);
+  return pair_of(__fsub_rn(a, c), __fsub_rn(b, d));
+}
+
+__device__ __forceinline__ void load_eight(Eight& x, const float* p) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) t.c[j] = 1.f, t.s[j] = 0.f;
+  for (int i = 0; i < 2; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(p + 4 * i);
+    x.v[2 * i] = pair_of(v.x, v.y);
+    x.v[2 * i + 1] = pair_of(v.z, v.w);
+  }
+}
+__device__ __forceinline__ void load_eight(Eight& x, const __nv_bfloat16* p) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x.v[i] = pair_of(__uint_as_float(word_of(v, i) << 16), __uint_as_float(word_of(v, i) & 0xFFFF0000u));
+}
+
+// A lane's part of a row.
+struct RowPart16 {
+  Eight a, b;
+};
+
+// How rows are read. kSimple: vectors of eight aligned elements, turned in halves
+// as a whole or not at all; kVector: such vectors, halves multiples of eight or
+// neighbours; kSingle: anything, element by element.
+enum RowKind { kSimple, kVector, kSingle };
+
+template <int DIM, RowKind HOW, typename T>
+__device__ __forceinline__ void load_row(RowPart16& r, const T* row, const RowOrder& o, int l) {
+  if (HOW != kSingle) {
+    int ia = 8 * l, ib = DIM / 2 + 8 * l;
+    if (HOW == kVector && o.apart) {
+      ia = 8 * l < o.half ? 8 * l : 16 * l;
+      ib = 8 * l < o.half ? 8 * l + o.half : 16 * l + 8;
+    }
+    load_eight(r.a, row + ia);
+    load_eight(r.b, row + ib);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      int ia = 8 * l + j, ib = DIM / 2 + 8 * l + j;
+      if (o.apart) o.at(8 * l + j, ia, ib);
+      r.a.set(j, load_value(row + ia));
+      r.b.set(j, load_value(row + ib));
+    }
+  }
+}
+
+// The cosines and sines that a lane needs at one position: of the pairs 8 l ..
+// 8 l + 7, or of the neighbours in its two vectors.
+template <int DIM, RowKind HOW>
+__device__ __forceinline__ void load_angles(RowPart16& t, const AppendArgs& a, const RowOrder& o, int pos, int l) {
   if (o.mode == 0) return;
   const float* cos = a.cos + pos * a.rope_stride;
   const float* sin = a.sin + pos * a.rope_stride;
-  if (o.mode == 1) {  // pairs 4 l .. 4 l + 3
-    if (VEC) {
-      if (4 * l < o.turned) {
-        load_vector<4>(t.c, cos + 4 * l);
-        load_vector<4>(t.s, sin + 4 * l);
-      }
-    } else {
+  if (HOW == kSimple) {
+    load_eight(t.a, cos + 8 * l);
+    load_eight(t.b, sin + 8 * l);
+    return;
+  }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (4 * l + j < o.turned) t.c[j] = cos[4 * l + j], t.s[j] = sin[4 * l + j];
-    }
-  } else {  // neighbours: two pairs in each of the lane's vectors
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int p = (j < 2 ? 2 * l : DIM / 4 + 2 * l - 2) + j;
-      if (p < o.turned) t.c[j] = cos[p], t.s[j] = sin[p];
-    }
+  for (int j = 0; j < 8; ++j) {
+    const int p = o.mode == 1 ? 8 * l + j : (j < 4 ? 4 * l : DIM / 4 + 4 * l - 4) + j;
+    t.a.set(j, p < o.turned ? cos[p] : 1.f);
+    t.b.set(j, p < o.turned ? sin[p] : 0.f);
   }
 }
 
-template <int DIM, bool VEC, typename T>
-__device__ __forceinline__ void load_row(RowOf8& r, const T* row, const RowOrder& o, int l) {
-  if (VEC) {
-    int ia = 4 * l, ib = DIM / 2 + 4 * l;
-    if (o.apart) {
-      ia = 4 * l < o.half ? 4 * l : 8 * l;
-      ib = 4 * l < o.half ? 4 * l + o.half : 8 * l + 4;
-    }
-    load_vector<4>(r.a, row + ia);
-    load_vector<4>(r.b, row + ib);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int ia = 4 * l + j, ib = DIM / 2 + 4 * l + j;
-      if (o.apart) o.at(4 * l + j, ia, ib);
-      r.a[j] = load_value(row + ia);
-      r.b[j] = load_value(row + ib);
-    }
-  }
-}
-
-template <int DIM, bool VEC>
-__device__ __forceinline__ void load_weight_row(RowOf8& w, const RowNorm& norm, const RowOrder& o, int l) {
+template <int DIM, RowKind HOW>
+__device__ __forceinline__ void load_weights_row(RowPart16& w, const RowNorm& norm, const RowOrder& o, int l) {
   if (norm.bf16)
-    load_row<DIM, VEC>(w, static_cast<const __nv_bfloat16*>(norm.weight), o, l);
+    load_row<DIM, HOW>(w, static_cast<const __nv_bfloat16*>(norm.weight), o, l);
   else
-    load_row<DIM, VEC>(w, static_cast<const float*>(norm.weight), o, l);
+    load_row<DIM, HOW>(w, static_cast<const float*>(norm.weight), o, l);
 }
 
 template <int DIM>
-__device__ __forceinline__ void normalise_row(RowOf8& r, const RowOf8& w, double eps) {
-  const float f = norm_factor(team_sum(add_squares<4>(r.b, add_squares<4>(r.a, 0.0)), DIM / 8), DIM, eps);
-  apply_norm<4>(r.a, f, w.a);
-  apply_norm<4>(r.b, f, w.b);
+__device__ __forceinline__ void normalise_row(RowPart16& r, const RowPart16& w, double eps) {
+  double sum[2] = {0.0, 0.0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const double x = r.a.get(j), y = r.b.get(j);
+    sum[0] = fma(x, x, sum[0]);
+    sum[1] = fma(y, y, sum[1]);
+  }
+  const unsigned long long f = both(norm_factor(team_sum(sum[0] + sum[1], DIM / 16), DIM, eps));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r.a.v[i] = mul_pair(mul_pair(r.a.v[i], f), w.a.v[i]);
+    r.b.v[i] = mul_pair(mul_pair(r.b.v[i], f), w.b.v[i]);
+  }
 }
 
-__device__ __forceinline__ void rotate_row(RowOf8& r, const Angles& t, const RowOrder& o, int l, int quarter) {
-  if (o.mode == 1) {
+template <int DIM, RowKind HOW>
+__device__ __forceinline__ void rotate_row(RowPart16& r, const RowPart16& t, const RowOrder& o, int l) {
+  if (o.mode == 0) return;
+  if (HOW == kSimple) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (4 * l + j < o.turned) turn(r.a[j], r.b[j], t.c[j], t.s[j]);
-  } else if (o.mode == 2) {
+    for (int i = 0; i < 4; ++i) {  // as turn(): each product and each sum rounded by itself
+      const unsigned long long x = sub_apart(mul_pair(r.a.v[i], t.a.v[i]), mul_pair(r.b.v[i], t.b.v[i]));
+      r.b.v[i] = add_apart(mul_pair(r.b.v[i], t.a.v[i]), mul_pair(r.a.v[i], t.b.v[i]));
+      r.a.v[i] = x;
+    }
+  } else if (o.mode == 1) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (2 * l + j < o.turned) turn(r.a[2 * j], r.a[2 * j + 1], t.c[j], t.s[j]);
-      if (quarter + 2 * l + j < o.turned) turn(r.b[2 * j], r.b[2 * j + 1], t.c[2 + j], t.s[2 + j]);
+    for (int j = 0; j < 8; ++j) {
+      float x = r.a.get(j), y = r.b.get(j);
+      if (8 * l + j < o.turned) turn(x, y, t.a.get(j), t.b.get(j));
+      r.a.set(j, x);
+      r.b.set(j, y);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x = r.a.get(2 * j), y = r.a.get(2 * j + 1);
+      if (4 * l + j < o.turned) turn(x, y, t.a.get(j), t.b.get(j));
+      r.a.set(2 * j, x);
+      r.a.set(2 * j + 1, y);
+      x = r.b.get(2 * j), y = r.b.get(2 * j + 1);
+      if (DIM / 4 + 4 * l + j < o.turned) turn(x, y, t.a.get(4 + j), t.b.get(4 + j));
+      r.b.set(2 * j, x);
+      r.b.set(2 * j + 1, y);
     }
   }
 }
 
 // A row read apart put in order, through the team's row of shared memory.
-template <int DIM, bool VEC>
-__device__ __forceinline__ void reorder_row(RowOf8& r, float* staged, const RowOrder& o, int l) {
+template <int DIM, RowKind HOW>
+__device__ __forceinline__ void reorder_row(RowPart16& r, float* staged, const RowOrder& o, int l) {
   __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 8; ++j) {
     int ia, ib;
-    if (VEC) {
-      ia = (4 * l < o.half ? 4 * l : 8 * l) + j;
-      ib = (4 * l < o.half ? 4 * l + o.half : 8 * l + 4) + j;
+    if (HOW == kVector) {
+      ia = (8 * l < o.half ? 8 * l : 16 * l) + j;
+      ib = (8 * l < o.half ? 8 * l + o.half : 16 * l + 8) + j;
     } else {
-      o.at(4 * l + j, ia, ib);
+      o.at(8 * l + j, ia, ib);
     }
-    staged[ia] = r.a[j];
-    staged[ib] = r.b[j];
+    staged[ia] = r.a.get(j);
+    staged[ib] = r.b.get(j);
   }
   __syncwarp();
-  load_vector<4>(r.a, staged + 4 * l);
-  load_vector<4>(r.b, staged + DIM / 2 + 4 * l);
+  load_eight(r.a, staged + 8 * l);
+  load_eight(r.b, staged + DIM / 2 + 8 * l);
 }
 
-// A group's scale and offset, and the codes of a lane's four values in 16 bits.
+template <bool VEC>
+__device__ __forceinline__ void store_eight(uint16_t* p, const Eight& x) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = __bfloat16_as_ushort(__float2bfloat16_rn(x.get(2 * i))) |
+           (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(x.get(2 * i + 1)))) << 16);
+  if (VEC) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[2 * i] = static_cast<uint16_t>(w[i]);
+      p[2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
+    }
+  }
+}
+
+__device__ __forceinline__ void extremes(const Eight& x, float& lo, float& hi) {
+  lo = hi = x.get(0);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) {
+    lo = min_nan(lo, x.get(j));
+    hi = max_nan(hi, x.get(j));
+  }
+}
+
+// A group's scale and offset, and the word of eight values' codes.
 struct GroupLine {
   __half scale, offset;
   float middle, inverse;
@@ -188,15 +282,21 @@ struct GroupLine {
     inverse = s > 0.f ? __frcp_rn(s) : 0.f;
   }
 
-  __device__ __forceinline__ uint32_t codes(const float (&x)[4]) const {
+  // Rounded to whole numbers by an addend of 1.5 2^23 (and 8, the zero point): the
+  // code is in the last bits, under what eight of the addend's bits sum up to.
+  __device__ __forceinline__ uint32_t word(const Eight& x) const {
+    const unsigned long long m = both(middle), f = both(inverse), up = both(12582920.f);
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 3; j >= 0; --j) {
-      // rounded to a whole number by an addend of 1.5 2^23 (and 8, the zero point): the code is in the last bits
-      const float u = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], middle), inverse), -8.f), 7.f);  // (NaN: -8)
-      w = w * 16 + __float_as_uint(__fadd_rn(u, 12582920.f));
+    for (int i = 3; i >= 0; --i) {
+      float lo, hi;
+      unpair(mul_pair(sub_apart(x.v[i], m), f), lo, hi);
+      lo = fminf(fmaxf(lo, -8.f), 7.f);  // (NaN: -8)
+      hi = fminf(fmaxf(hi, -8.f), 7.f);
+      unpair(add_pair(pair_of(lo, hi), up), lo, hi);
+      w = (w * 16 + __float_as_uint(hi)) * 16 + __float_as_uint(lo);
     }
-    return w & 0xFFFFu;
+    return w - 0x4B400000u * 0x11111111u;
   }
 };
 
@@ -205,11 +305,12 @@ struct GroupLine {
 // by one piece of code: two, unrolled over four rows, were waiting for
 // instructions most of the time, 13 prompt chunks 387 us.)
 template <int DIM>
-__device__ __forceinline__ void store_row(const AppendArgs& a, bool keys, RowOf8& r, long long block, int slot, int l, bool live) {
+__device__ __forceinline__ void store_row(const AppendArgs& a, bool keys, RowPart16& r, long long block, int slot, int l, bool live) {
   constexpr int G = DIM / kKv4Group;
-  constexpr int kSpan = DIM >= 128 ? 16 : 8;  // lanes of a group
-  float lo_a = min_nan(min_nan(r.a[0], r.a[1]), min_nan(r.a[2], r.a[3])), hi_a = max_nan(max_nan(r.a[0], r.a[1]), max_nan(r.a[2], r.a[3]));
-  float lo_b = min_nan(min_nan(r.b[0], r.b[1]), min_nan(r.b[2], r.b[3])), hi_b = max_nan(max_nan(r.b[0], r.b[1]), max_nan(r.b[2], r.b[3]));
+  constexpr int kSpan = DIM >= 128 ? 8 : 4;  // lanes of a group
+  float lo_a, hi_a, lo_b, hi_b;
+  extremes(r.a, lo_a, hi_a);
+  extremes(r.b, lo_b, hi_b);
   if (DIM < 128) {
     lo_a = min_nan(lo_a, lo_b);
     hi_a = max_nan(hi_a, hi_b);
@@ -228,27 +329,33 @@ __device__ __forceinline__ void store_row(const AppendArgs& a, bool keys, RowOf8
   float exponent = 0.f;
   if (!keys) {
     float amax = max_nan(size_a, size_b);
-    if (DIM == 256) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 16));
+    if (DIM == 256) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 8));
     const bool fits = amax < kKv4ValueLimit;  // (otherwise, NaN too, the token is NaN through E alone: its line is 0)
     const int e = fits ? max(static_cast<int>(__float_as_uint(amax) >> 23) - 130, kKv4MinExponent) : 0;
     exponent = fits ? static_cast<float>(e) : __uint_as_float(0x7FC00000u);
     const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
-    auto scaled = [&](float x) { return fits ? x * down : 0.f; };
-    lo_a = scaled(lo_a), hi_a = scaled(hi_a), lo_b = scaled(lo_b), hi_b = scaled(hi_b);
+    if (!fits) {
+      lo_a = hi_a = lo_b = hi_b = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r.a[j] = scaled(r.a[j]), r.b[j] = scaled(r.b[j]);
+      for (int i = 0; i < 4; ++i) r.a.v[i] = r.b.v[i] = 0;
+    }
+    lo_a *= down, hi_a *= down, lo_b *= down, hi_b *= down;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r.a.v[i] = mul_pair(r.a.v[i], both(down));
+      r.b.v[i] = mul_pair(r.b.v[i], both(down));
+    }
   }
   GroupLine ga, gb;
   ga.fit(lo_a, hi_a);
   gb.fit(lo_b, hi_b);
-  // Words of 8 codes: an even lane completes the first vector's, an odd one the second's.
-  const uint32_t wa = ga.codes(r.a), wb = gb.codes(r.b);
-  const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, l & 1 ? wa : wb, 1);
-  const uint32_t word = l & 1 ? other | (wb << 16) : wa | (other << 16);
+  const uint32_t wa = ga.word(r.a), wb = gb.word(r.b);
   if (!live) return;
-  const int n = (l & 1 ? DIM / 16 : 0) + l / 2;  // the word in the row's order
   const long long row = block * a.c.page_size + slot;
-  reinterpret_cast<uint32_t*>((keys ? a.c.k_codes : a.c.v_codes) + row * (DIM / 2))[(n & 7) * G + (n >> 3)] = word;
+  uint32_t* words = reinterpret_cast<uint32_t*>((keys ? a.c.k_codes : a.c.v_codes) + row * (DIM / 2));
+  const int n = DIM / 16 + l;
+  words[(l & 7) * G + (l >> 3)] = wa;
+  words[(n & 7) * G + (n >> 3)] = wb;
   // The lanes of span h hold group h of the first half (ga) and group G / 2 + h of the second.
   const int h = l / kSpan, k = l % kSpan;
   if (keys) {
@@ -262,11 +369,11 @@ __device__ __forceinline__ void store_row(const AppendArgs& a, bool keys, RowOf8
   } else {
     __half* cell = reinterpret_cast<__half*>(a.c.v_scales) +
                    (block * (a.c.page_size >> 4) + (slot >> 4)) * (32 * G + 16);
-    // lane k of a span: scale, offset of ga, of gb; lane 4 of the row: E
+    // lane k of a span: scale, offset of ga, of gb; the row's last lane: E
     const int at = ((slot & 15) >> 1) * (4 * G) + (slot & 1);
     const __half x = k == 0 ? ga.scale : k == 1 ? ga.offset : k == 2 ? gb.scale : gb.offset;
     if (k < (DIM >= 128 ? 4 : 2)) cell[at + 2 * ((k & 1 ? G : 0) + (k < 2 ? h : G / 2 + h))] = x;
-    if (l == 4) cell[32 * G + (slot & 15)] = __float2half_rn(exponent);
+    if (l == DIM / 16 - 1) cell[32 * G + (slot & 15)] = __float2half_rn(exponent);
   }
 }
 
@@ -285,15 +392,15 @@ __device__ __forceinline__ int sequence_at(const TokenBatch& t, int token, int l
   return low;
 }
 
-// A warp takes a token's queries, keys or values, 32 / (DIM / 8) heads side by
+// A warp takes a token's queries, keys or values, 32 / (DIM / 16) heads side by
 // side and up to `turns` of those one after the other, the next on its way.
 // `q_warps` and `kv_warps`: warps per token for its queries, and for its keys and
 // for its values.
-template <typename T, int DIM, bool VEC>
+template <typename T, int DIM, RowKind HOW>
 __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArgs a, const int q_warps, const int kv_warps,
                                                                  const int turns) {
-  constexpr int kTeam = DIM / 8, kTeams = 32 / kTeam;
-  __shared__ float4 staged[kKv4Threads / 32][kTeams][DIM / 4];
+  constexpr int kTeam = DIM / 16, kTeams = 32 / kTeam;
+  __shared__ float4 staged[HOW == kSimple ? 1 : kKv4Threads / 32][HOW == kSimple ? 1 : kTeams][HOW == kSimple ? 1 : DIM / 4];
   grid_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kTeam, team = lane / kTeam;
   const int per_token = q_warps + 2 * kv_warps;
@@ -310,8 +417,8 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArg
   const long long hs = queries ? a.q_hs : keys ? a.k_hs : a.v_hs;
   const RowOrder order = row_order<DIM>(a, queries || keys);
   // (teams past the last head take the last one again, and store nothing)
-  RowOf8 next;
-  load_row<DIM, VEC>(next, src + min(head0 + team, heads - 1) * hs, order, l);
+  RowPart16 next;
+  load_row<DIM, HOW>(next, src + min(head0 + team, heads - 1) * hs, order, l);
 
   const ListSizes sizes{a.t.tokens, a.t.max_pages << a.c.page_shift, 1, 0};
   const int b = sequence_at(a.t, token, lane);
@@ -332,35 +439,27 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArg
   }
   const int page = queries ? 0 : page_of(a.t, a.c, b, pos);
   if (page < 0) return;
-  Angles angles;
-  load_angles<DIM, VEC>(angles, a, order, pos, l);
+  RowPart16 angles;
+  load_angles<DIM, HOW>(angles, a, order, pos, l);
   const RowNorm norm = queries ? a.q_norm : keys ? a.k_norm : RowNorm{};
-  RowOf8 weight;
-  if (norm.weight) load_weight_row<DIM, VEC>(weight, norm, order, l);
+  RowPart16 weight;
+  if (norm.weight) load_weights_row<DIM, HOW>(weight, norm, order, l);
   const int slot = pos & (a.c.page_size - 1);
 #pragma unroll 1
   for (int first = head0; first < end; first += kTeams) {
     const int head = first + team;
     const bool live = head < end;
-    RowOf8 row = next;
-    if (first + kTeams < end) load_row<DIM, VEC>(next, src + min(head + kTeams, heads - 1) * hs, order, l);
+    RowPart16 row = next;
+    if (first + kTeams < end) load_row<DIM, HOW>(next, src + min(head + kTeams, heads - 1) * hs, order, l);
     if (norm.weight) normalise_row<DIM>(row, weight, a.norm_eps);
-    rotate_row(row, angles, order, l, DIM / 4);
-    if (order.apart) reorder_row<DIM, VEC>(row, reinterpret_cast<float*>(staged[warp][team]), order, l);
+    rotate_row<DIM, HOW>(row, angles, order, l);
+    if (HOW != kSimple && order.apart) reorder_row<DIM, HOW>(row, reinterpret_cast<float*>(staged[warp][team]), order, l);
     if (!queries) {
       store_row<DIM>(a, keys, row, static_cast<long long>(page) * a.c.heads + head, slot, l, live);
     } else if (live) {
       uint16_t* to = out + head * a.o_hs;
-      if (VEC) {
-        store_bf16<4>(to + 4 * l, row.a);
-        store_bf16<4>(to + DIM / 2 + 4 * l, row.b);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          to[4 * l + j] = __bfloat16_as_ushort(__float2bfloat16_rn(row.a[j]));
-          to[DIM / 2 + 4 * l + j] = __bfloat16_as_ushort(__float2bfloat16_rn(row.b[j]));
-        }
-      }
+      store_eight<HOW != kSingle>(to + 8 * l, row.a);
+      store_eight<HOW != kSingle>(to + DIM / 2 + 8 * l, row.b);
     }
   }
 }
@@ -422,35 +521,40 @@ __global__ void __launch_bounds__(256) kv4_decode_kernel(const KvView c, const i
 
 // ------------------------------------------------------------------ launches
 
-template <typename T, int DIM, bool VEC>
+inline bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+template <typename T, int DIM, RowKind HOW>
 cudaError_t launch_append4_as(const AppendArgs& a, cudaStream_t stream) {
-  constexpr int kTeams = 32 / (DIM / 8);
-  // Few rows: one after the other in as many warps; many: up to 8 in one, which
-  // finds the token's place and angles once for them.
+  constexpr int kTeams = 32 / (DIM / 16);
+  // Few rows: a warp for every kTeams of a token; many: up to four times as many
+  // in one, which finds the token's place and angles once for them.
   const long long rows = static_cast<long long>(a.t.tokens) * (2 * a.c.heads + (a.q ? a.q_heads : 0)) / kTeams;
-  const int turns = rows > 16384 ? 8 : 1;
+  const int turns = rows > 16384 ? 4 : 1;
   const int heads = turns * kTeams;  // of a warp
   const int q_warps = a.q ? (a.q_heads + heads - 1) / heads : 0, kv_warps = (a.c.heads + heads - 1) / heads;
   const long long warps = static_cast<long long>(a.t.tokens) * (q_warps + 2 * kv_warps);
   const long long ctas = (warps + kKv4Threads / 32 - 1) / (kKv4Threads / 32);
   if (ctas > INT32_MAX) return cudaErrorInvalidConfiguration;
-  return launch_overlapped(kv4_append_kernel<T, DIM, VEC>, dim3(static_cast<unsigned>(ctas)), kKv4Threads, 0, stream, a, q_warps,
+  return launch_overlapped(kv4_append_kernel<T, DIM, HOW>, dim3(static_cast<unsigned>(ctas)), kKv4Threads, 0, stream, a, q_warps,
                            kv_warps, turns);
 }
 
 template <typename T, int DIM>
 cudaError_t launch_append4_dim(const AppendArgs& a, cudaStream_t stream) {
-  // vectors of four elements: every row, angle and weight address a multiple of four of its elements
-  bool vec = !a.cos || (a.rotary % 8 == 0 && a.rope_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.cos) % 16 == 0 &&
-                        reinterpret_cast<uintptr_t>(a.sin) % 16 == 0);
+  // vectors of eight elements: every row, angle and weight address 16-byte aligned
+  const bool turned = a.cos != nullptr, simple = !turned || (!a.interleaved && a.rotary == DIM);
+  bool vec = !turned || a.interleaved || a.rotary % 16 == 0;
+  if (turned && simple) vec = vec && a.rope_stride % 4 == 0 && aligned_to(a.cos, 16) && aligned_to(a.sin, 16);
+  constexpr int kElements = 16 / sizeof(T);
   const void* ptr[3] = {a.k, a.v, a.q};
   const long long stride[6] = {a.k_ts, a.k_hs, a.v_ts, a.v_hs, a.q_ts, a.q_hs};
   for (int i = 0; i < 3; ++i)
-    if (ptr[i] && (reinterpret_cast<uintptr_t>(ptr[i]) % (4 * sizeof(T)) || stride[2 * i] % 4 || stride[2 * i + 1] % 4)) vec = false;
-  if (a.q && (reinterpret_cast<uintptr_t>(a.q_out) % 8 || a.o_ts % 4 || a.o_hs % 4)) vec = false;
+    if (ptr[i] && (!aligned_to(ptr[i], 16) || stride[2 * i] % kElements || stride[2 * i + 1] % kElements)) vec = false;
+  if (a.q && (!aligned_to(a.q_out, 16) || a.o_ts % 8 || a.o_hs % 8)) vec = false;
   for (const RowNorm& n : {a.q_norm, a.k_norm})
-    if (reinterpret_cast<uintptr_t>(n.weight) % (n.bf16 ? 8 : 16)) vec = false;
-  return vec ? launch_append4_as<T, DIM, true>(a, stream) : launch_append4_as<T, DIM, false>(a, stream);
+    if (!aligned_to(n.weight, 16)) vec = false;
+  if (!vec) return launch_append4_as<T, DIM, kSingle>(a, stream);
+  return simple ? launch_append4_as<T, DIM, kSimple>(a, stream) : launch_append4_as<T, DIM, kVector>(a, stream);
 }
 
 cudaError_t launch_kv4_append(bool bf16, const AppendArgs& a, cudaStream_t stream) {
