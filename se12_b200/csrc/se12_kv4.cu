@@ -122,14 +122,21 @@ struct RowPart16 {
 // neighbours; kSingle: anything, element by element.
 enum RowKind { kSimple, kVector, kSingle };
 
+// Where in a row the two vectors of lane l begin.
+template <int DIM, RowKind HOW>
+__device__ __forceinline__ void vectors_at(const RowOrder& o, int l, int& ia, int& ib) {
+  ia = 8 * l, ib = DIM / 2 + 8 * l;
+  if (HOW == kVector && o.apart) {
+    ia = 8 * l < o.half ? 8 * l : 16 * l;
+    ib = 8 * l < o.half ? 8 * l + o.half : 16 * l + 8;
+  }
+}
+
 template <int DIM, RowKind HOW, typename T>
 __device__ __forceinline__ void load_row(RowPart16& r, const T* row, const RowOrder& o, int l) {
   if (HOW != kSingle) {
-    int ia = 8 * l, ib = DIM / 2 + 8 * l;
-    if (HOW == kVector && o.apart) {
-      ia = 8 * l < o.half ? 8 * l : 16 * l;
-      ib = 8 * l < o.half ? 8 * l + o.half : 16 * l + 8;
-    }
+    int ia, ib;
+    vectors_at<DIM, HOW>(o, l, ia, ib);
     load_eight(r.a, row + ia);
     load_eight(r.b, row + ib);
   } else {
@@ -142,6 +149,45 @@ __device__ __forceinline__ void load_row(RowPart16& r, const T* row, const RowOr
     }
   }
 }
+
+// A row on its way: as it lies in memory, so that nothing is moved when it is taken.
+template <typename T, int DIM, RowKind HOW>
+struct RowAhead {
+  static constexpr int kVectors = sizeof(T) / 2;  // of 16 bytes, of eight elements
+  uint4 a[kVectors], b[kVectors];
+  RowPart16 single;
+
+  __device__ __forceinline__ void load(const T* row, const RowOrder& o, int l) {
+    if (HOW == kSingle) {
+      load_row<DIM, HOW>(single, row, o, l);
+      return;
+    }
+    int ia, ib;
+    vectors_at<DIM, HOW>(o, l, ia, ib);
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      a[i] = reinterpret_cast<const uint4*>(row + ia)[i];
+      b[i] = reinterpret_cast<const uint4*>(row + ib)[i];
+    }
+  }
+  __device__ __forceinline__ static void eight_of(Eight& x, const uint4 (&v)[kVectors]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(T) == 4)
+        x.v[i] = pair_of(__uint_as_float(word_of(v[i / 2 % kVectors], 2 * (i & 1))), __uint_as_float(word_of(v[i / 2 % kVectors], 2 * (i & 1) + 1)));
+      else
+        x.v[i] = pair_of(__uint_as_float(word_of(v[0], i) << 16), __uint_as_float(word_of(v[0], i) & 0xFFFF0000u));
+    }
+  }
+  __device__ __forceinline__ void take(RowPart16& r) const {
+    if (HOW == kSingle) {
+      r = single;
+      return;
+    }
+    eight_of(r.a, a);
+    eight_of(r.b, b);
+  }
+};
 
 // The cosines and sines that a lane needs at one position: of the pairs 8 l ..
 // 8 l + 7, or of the neighbours in its two vectors.
@@ -397,7 +443,7 @@ __device__ __forceinline__ int sequence_at(const TokenBatch& t, int token, int l
 // `q_warps` and `kv_warps`: warps per token for its queries, and for its keys and
 // for its values.
 template <typename T, int DIM, RowKind HOW>
-__global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArgs a, const int q_warps, const int kv_warps,
+__global__ void __launch_bounds__(kKv4Threads, HOW == kSingle ? 3 : 5) kv4_append_kernel(const AppendArgs a, const int q_warps, const int kv_warps,
                                                                  const int turns) {
   constexpr int kTeam = DIM / 16, kTeams = 32 / kTeam;
   __shared__ float4 staged[HOW == kSimple ? 1 : kKv4Threads / 32][HOW == kSimple ? 1 : kTeams][HOW == kSimple ? 1 : DIM / 4];
@@ -417,8 +463,8 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArg
   const long long hs = queries ? a.q_hs : keys ? a.k_hs : a.v_hs;
   const RowOrder order = row_order<DIM>(a, queries || keys);
   // (teams past the last head take the last one again, and store nothing)
-  RowPart16 next;
-  load_row<DIM, HOW>(next, src + min(head0 + team, heads - 1) * hs, order, l);
+  RowAhead<T, DIM, HOW> next;
+  next.load(src + min(head0 + team, heads - 1) * hs, order, l);
 
   const ListSizes sizes{a.t.tokens, a.t.max_pages << a.c.page_shift, 1, 0};
   const int b = sequence_at(a.t, token, lane);
@@ -449,8 +495,9 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const AppendArg
   for (int first = head0; first < end; first += kTeams) {
     const int head = first + team;
     const bool live = head < end;
-    RowPart16 row = next;
-    if (first + kTeams < end) load_row<DIM, HOW>(next, src + min(head + kTeams, heads - 1) * hs, order, l);
+    RowPart16 row;
+    next.take(row);
+    if (first + kTeams < end) next.load(src + min(head + kTeams, heads - 1) * hs, order, l);
     if (norm.weight) normalise_row<DIM>(row, weight, a.norm_eps);
     rotate_row<DIM, HOW>(row, angles, order, l);
     if (HOW != kSimple && order.apart) reorder_row<DIM, HOW>(row, reinterpret_cast<float*>(staged[warp][team]), order, l);
