@@ -23,6 +23,7 @@
 // Both kernels are bound by memory and, for few tokens, by their latency.
 #include "se12_kv.cuh"
 
+#include <algorithm>
 #include <cuda_fp16.h>
 
 namespace se12 {
@@ -511,58 +512,74 @@ __global__ void __launch_bounds__(kKv4Threads, HOW == kSingle ? 3 : 5) kv4_appen
   }
 }
 
-// Pages read back as BF16, a CTA per block (page of a head), keys and values by
-// blockIdx.y, a thread per word of 8 values.
+// Pages read back as BF16, keys and values by blockIdx.y. A thread takes 16 bytes
+// of codes of each of two neighbouring tokens, which share a cell's lines: 64
+// values. (A thread per word of 8: 14000 tokens of 8 heads of 256 46 us.)
 template <int DIM>
-__global__ void __launch_bounds__(256) kv4_decode_kernel(const KvView c, const int32_t* pages, int count, uint16_t* k_out,
+__global__ void __launch_bounds__(256) kv4_decode_kernel(const KvView c, const int32_t* pages, unsigned blocks, uint16_t* k_out,
                                                          uint16_t* v_out) {
-  constexpr int G = DIM / kKv4Group, kWords = DIM / 8;
+  constexpr int G = DIM / kKv4Group, kParts = DIM / 32;  // 16 bytes of codes: words 4 part .. + 3
   grid_launch_dependents();
   grid_dependency_wait();
   const bool keys = blockIdx.y == 0;
-  const long long blocks = static_cast<long long>(count) * c.heads;
-  const int words = c.page_size * kWords;
-  for (long long n = blockIdx.x; n < blocks; n += gridDim.x) {
-    const int nth = static_cast<int>(n / c.heads), head = static_cast<int>(n - static_cast<long long>(nth) * c.heads);
-    const int page = pages ? pages[nth] : nth;
-    uint4* out = reinterpret_cast<uint4*>((keys ? k_out : v_out) + n * (static_cast<long long>(c.page_size) * DIM));
+  const int shift = c.page_shift - 1 + (DIM == 64 ? 1 : DIM == 128 ? 2 : 3);  // items of a block, a power of two
+  const unsigned long long items = static_cast<unsigned long long>(blocks) << shift;
+  for (unsigned long long at = blockIdx.x * 256ull + threadIdx.x; at < items; at += gridDim.x * 256ull) {
+    const unsigned n = static_cast<unsigned>(at >> shift), nth = n / c.heads, head = n - nth * c.heads;
+    const int item = static_cast<int>(at) & ((1 << shift) - 1), part = item % kParts, token = item / kParts * 2;
+    const int page = pages ? pages[nth] : static_cast<int>(nth);
+    uint16_t* out = (keys ? k_out : v_out) + (static_cast<unsigned long long>(n) * c.page_size + token) * DIM;
+    // dimension where word w of the 16 bytes begins
+    auto dim_of = [&](int w) { return (4 * part + w) % G * kKv4Group + (4 * part + w) / G * 8; };
     if (page < 0 || page >= c.pages) {
       raise_status(kStatusBadArgument);
-      for (int i = threadIdx.x; i < words; i += 256) out[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) *reinterpret_cast<uint4*>(out + (w >> 2) * DIM + dim_of(w & 3)) = make_uint4(0, 0, 0, 0);
       continue;
     }
-    const long long block = static_cast<long long>(page) * c.heads + head;
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>((keys ? c.k_codes : c.v_codes) + block * c.page_size * (DIM / 2));
-    const __half2* key_scales = reinterpret_cast<const __half2*>(c.k_scales) + block * c.page_size * G;
-    const __half* value_scales = reinterpret_cast<const __half*>(c.v_scales) + block * (c.page_size >> 4) * (32 * G + 16);
-#pragma unroll 4
-    for (int i = threadIdx.x; i < words; i += 256) {
-      const int token = i / kWords, w = i % kWords, g = w / 8;
-      const uint32_t u = codes[token * kWords + (w & 7) * G + g];
-      float scale, offset, power = 1.f;
-      if (keys) {
-        const float2 line = __half22float2(key_scales[token * G + g]);
-        scale = line.x, offset = line.y;
-      } else {
-        const __half* cell = value_scales + (token >> 4) * (32 * G + 16);
-        const __half* pair = cell + ((token & 15) >> 1) * (4 * G) + (token & 1);
-        scale = __half2float(pair[2 * g]);
-        offset = __half2float(pair[2 * (G + g)]);
-        const float e = __half2float(cell[32 * G + (token & 15)]);  // a whole number, or NaN
-        power = e == e ? __uint_as_float(static_cast<unsigned>(static_cast<int>(e) + 127) << 23) : e;
-      }
-      uint32_t o[4];
+    const long long row = (static_cast<long long>(page) * c.heads + head) * c.page_size + token;
+    const uint4* codes = reinterpret_cast<const uint4*>((keys ? c.k_codes : c.v_codes) + row * (DIM / 2)) + part;
+    const uint4 x[2] = {codes[0], codes[kParts]};
+    float scale[2][G], offset[2][G], power[2] = {1.f, 1.f};
+    if (keys) {
+      const __half2* line = reinterpret_cast<const __half2*>(c.k_scales) + row * G;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float x[2];
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          x[k] = fmaf(static_cast<float>(static_cast<int>((u >> (8 * j + 4 * k)) & 15u) - 8), scale, offset) * power;
-        o[j] = __bfloat16_as_ushort(__float2bfloat16_rn(x[0])) |
-               (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(x[1]))) << 16);
+        for (int g = 0; g < G; ++g) {
+          const float2 v = __half22float2(line[t * G + g]);
+          scale[t][g] = v.x, offset[t][g] = v.y;
+        }
+    } else {
+      const __half* cell = reinterpret_cast<const __half*>(c.v_scales) + (row >> 4) * (32 * G + 16);
+      const __half2* pair = reinterpret_cast<const __half2*>(cell) + (token & 15) * G;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float2 s = __half22float2(pair[g]), o = __half22float2(pair[G + g]);
+        scale[0][g] = s.x, scale[1][g] = s.y, offset[0][g] = o.x, offset[1][g] = o.y;
       }
-      out[i] = make_uint4(o[0], o[1], o[2], o[3]);
+      const float2 e = __half22float2(*reinterpret_cast<const __half2*>(cell + 32 * G + (token & 15)));  // whole numbers, or NaN
+      power[0] = e.x == e.x ? __uint_as_float(static_cast<unsigned>(static_cast<int>(e.x) + 127) << 23) : e.x;
+      power[1] = e.y == e.y ? __uint_as_float(static_cast<unsigned>(static_cast<int>(e.y) + 127) << 23) : e.y;
     }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int g = w % G;  // (four words, G of 1, 2 or 4)
+        const uint32_t u = word_of(x[t], w);
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k)  // the code under 2^23's last bits is u + 2^23
+            v[k] = fmaf(__uint_as_float(((u >> (8 * j + 4 * k)) & 15u) | 0x4B000000u) - 8388616.f, scale[t][g], offset[t][g]) * power[t];
+          o[j] = __bfloat16_as_ushort(__float2bfloat16_rn(v[0])) |
+                 (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(v[1]))) << 16);
+        }
+        *reinterpret_cast<uint4*>(out + t * DIM + dim_of(w)) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
   }
 }
 
@@ -614,10 +631,11 @@ cudaError_t launch_kv4_append(bool bf16, const AppendArgs& a, cudaStream_t strea
 
 cudaError_t launch_kv4_decode(const KvView& c, const int32_t* pages, int count, uint16_t* k_out, uint16_t* v_out,
                               cudaStream_t stream) {
-  const long long blocks = static_cast<long long>(count) * c.heads;
-  const dim3 grid(static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20)), 2);
+  const unsigned blocks = static_cast<unsigned>(count) * static_cast<unsigned>(c.heads);  // (their output has to fit the memory)
+  const unsigned long long items = static_cast<unsigned long long>(blocks) * (c.page_size / 2) * (c.dim / 32);
+  const dim3 grid(static_cast<unsigned>(std::min(items / 256 + 1, 1ull << 20)), 2);
   return launch_overlapped(c.dim == 64 ? kv4_decode_kernel<64> : c.dim == 128 ? kv4_decode_kernel<128> : kv4_decode_kernel<256>,
-                           grid, 256, 0, stream, c, pages, count, k_out, v_out);
+                           grid, 256, 0, stream, c, pages, blocks, k_out, v_out);
 }
 
 }  // namespace se12
