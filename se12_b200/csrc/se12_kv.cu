@@ -136,13 +136,9 @@ struct RowPart {
     load_vector<VP>(b, row + 32 * VP + lane * VP);
   }
 
-  __device__ __forceinline__ void normalise(const RowNorm& norm, int dim, double eps, int lane) {
-    const float factor = norm_factor(team_sum(add_squares<VP>(b, add_squares<VP>(a, 0.0)), 32), dim, eps);
-    float w[VP];
-    load_weights<VP>(w, norm, lane * VP);
-    apply_norm<VP>(a, factor, w);
-    load_weights<VP>(w, norm, 32 * VP + lane * VP);
-    apply_norm<VP>(b, factor, w);
+  __device__ __forceinline__ void normalise(float factor, const float (&wa)[VP], const float (&wb)[VP]) {
+    apply_norm<VP>(a, factor, wa);
+    apply_norm<VP>(b, factor, wb);
   }
 
   __device__ __forceinline__ void rotate(const float (&c)[VP], const float (&s)[VP]) {
@@ -198,6 +194,34 @@ __device__ __forceinline__ float joined_scale(float before, bool older, unsigned
   }
   return before;
 }
+
+// A norm's weights in a lane, and rows normalised with them: the sums of all N at
+// once (also of rows that hold nothing, whose results nobody reads).
+template <int VP>
+struct NormOfRows {
+  RowNorm norm;
+  float wa[VP], wb[VP];
+
+  __device__ __forceinline__ NormOfRows(const RowNorm& n, int lane) : norm(n) {
+    if (norm.weight) {
+      load_weights<VP>(wa, norm, lane * VP);
+      load_weights<VP>(wb, norm, 32 * VP + lane * VP);
+    }
+  }
+  template <int N>
+  __device__ __forceinline__ void apply(RowPart<VP> (&row)[N], int dim, double eps) const {
+    if (!norm.weight) return;
+    double sum[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) sum[k] = add_squares<VP>(row[k].b, add_squares<VP>(row[k].a, 0.0));
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1)
+#pragma unroll
+      for (int k = 0; k < N; ++k) sum[k] += __shfl_xor_sync(0xFFFFFFFFu, sum[k], d);
+#pragma unroll
+    for (int k = 0; k < N; ++k) row[k].normalise(norm_factor(sum[k], dim, eps), wa, wb);
+  }
+};
 
 // How a row of queries or keys (turned) or values (not) splits into pairs.
 // Vector lanes (vp > 1) serve rows that are turned in halves, whole or not
@@ -319,8 +343,8 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, cons
   const bool held = VP > 1 && count <= 8 * kHeld;
   RowPart<VP> row[kHeld];
   const RowNorm norm = NORM && keys ? a.k_norm : RowNorm{};
+  const NormOfRows<VP> norms(VP > 1 ? norm : RowNorm{}, lane);
   auto rotate = [&](RowPart<VP>& r, int i) {
-    if (NORM && norm.weight) r.normalise(norm, dim, a.norm_eps, lane);
     if (turned) {
       float c[VP], s[VP];
       load_vector<VP>(c, a.cos + (pos + i) * a.rope_stride + lane * VP);
@@ -345,6 +369,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, cons
     if constexpr (VP > 1) {
       for (int i0 = warp; i0 < count; i0 += 8 * kHeld) {
         if (!held) load(h, i0);
+        if (NORM) norms.apply(row, dim, a.norm_eps);
 #pragma unroll
         for (int k = 0; k < kHeld; ++k)
           if (i0 + 8 * k < count) {
@@ -385,6 +410,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, bool keys, cons
       for (int i0 = warp; i0 < count; i0 += 8 * kHeld) {
         if (!held) {
           load(h, i0);
+          if (NORM) norms.apply(row, dim, a.norm_eps);
 #pragma unroll
           for (int k = 0; k < kHeld; ++k)
             if (i0 + 8 * k < count) rotate(row[k], i0 + 8 * k);
@@ -428,16 +454,17 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int token, i
   }
   const T* src = static_cast<const T*>(a.q) + token * a.q_ts;
   uint16_t* out = a.q_out + token * a.o_ts;
+  const NormOfRows<VP> norms(NORM ? a.q_norm : RowNorm{}, lane);
   constexpr int kHeads = 4;  // on their way together
   for (int h0 = 0; h0 < a.q_heads; h0 += kHeads) {
     RowPart<VP> row[kHeads];
 #pragma unroll
     for (int k = 0; k < kHeads; ++k)
       if (h0 + k < a.q_heads) row[k].load(src + (h0 + k) * a.q_hs, lane);
+    if (NORM) norms.apply(row, a.c.dim, a.norm_eps);
 #pragma unroll
     for (int k = 0; k < kHeads; ++k)
       if (h0 + k < a.q_heads) {
-        if (NORM && a.q_norm.weight) row[k].normalise(a.q_norm, a.c.dim, a.norm_eps, lane);
         if (a.cos) row[k].rotate(c, s);
         store_bf16<VP>(out + (h0 + k) * a.o_hs + lane * VP, row[k].a);
         store_bf16<VP>(out + (h0 + k) * a.o_hs + 32 * VP + lane * VP, row[k].b);
@@ -453,7 +480,7 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int token, i
 // read again from L2. The last blockIdx.y rotates the queries, a warp per
 // token.
 template <typename T, int KIND, int VP, bool NORM>
-__global__ void __launch_bounds__(256, 3) kv_append_prompt_kernel(const AppendArgs a, const int span, const int heads_each) {
+__global__ void __launch_bounds__(256, NORM && VP == 4 ? 2 : 3) kv_append_prompt_kernel(const AppendArgs a, const int span, const int heads_each) {
   __shared__ unsigned s_amax[2][8];
   grid_launch_dependents();
   grid_dependency_wait();
@@ -584,10 +611,23 @@ cudaError_t launch_append_kind(const AppendArgs& a, cudaStream_t stream) {
   return vp == 4 ? launch_append_as<T, KIND, 4, NORM>(a, stream) : launch_append_as<T, KIND, 2, NORM>(a, stream);
 }
 
+// Normalised queries of many tokens go through the 4-bit cache's row kernel, in a
+// launch of their own: half the lanes per row and a warp per few heads instead of
+// one per token (7 prompt chunks, 64 query heads of 128, BF16, with the pages read
+// back: 114 us by one launch, 72 by two).
 template <typename T, int KIND>
 cudaError_t launch_append_normed(const AppendArgs& a, cudaStream_t stream) {
-  return a.q_norm.weight || a.k_norm.weight ? launch_append_kind<T, KIND, true>(a, stream)
-                                            : launch_append_kind<T, KIND, false>(a, stream);
+  if (!a.q_norm.weight && !a.k_norm.weight) return launch_append_kind<T, KIND, false>(a, stream);
+  AppendArgs rest = a;
+  if (a.q && a.q_norm.weight && a.t.query_start && a.t.tokens > 256 && kv4_rows_take(a.c.dim)) {
+    AppendArgs queries = a;
+    queries.k = queries.v = nullptr;
+    const cudaError_t err = launch_kv4_append(sizeof(T) == 2, queries, stream);
+    if (err != cudaSuccess) return err;
+    rest.q = nullptr;
+  }
+  return rest.k_norm.weight || rest.q ? launch_append_kind<T, KIND, true>(rest, stream)
+                                      : launch_append_kind<T, KIND, false>(rest, stream);
 }
 
 cudaError_t launch_kv_append(bool bf16, const AppendArgs& a, cudaStream_t stream) {

@@ -595,7 +595,7 @@ cudaError_t launch_append4_as(const AppendArgs& a, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.t.tokens) * (2 * a.c.heads + (a.q ? a.q_heads : 0)) / kTeams;
   const int turns = rows > 16384 ? 4 : 1;
   const int heads = turns * kTeams;  // of a warp
-  const int q_warps = a.q ? (a.q_heads + heads - 1) / heads : 0, kv_warps = (a.c.heads + heads - 1) / heads;
+  const int q_warps = a.q ? (a.q_heads + heads - 1) / heads : 0, kv_warps = a.k ? (a.c.heads + heads - 1) / heads : 0;
   const long long warps = static_cast<long long>(a.t.tokens) * (q_warps + 2 * kv_warps);
   const long long ctas = (warps + kKv4Threads / 32 - 1) / (kKv4Threads / 32);
   if (ctas > INT32_MAX) return cudaErrorInvalidConfiguration;
@@ -620,6 +620,9 @@ cudaError_t launch_append4_dim(const AppendArgs& a, cudaStream_t stream) {
   if (!vec) return launch_append4_as<T, DIM, kSingle>(a, stream);
   return simple ? launch_append4_as<T, DIM, kSimple>(a, stream) : launch_append4_as<T, DIM, kVector>(a, stream);
 }
+
+// a.k null: the queries alone (for caches of any kind, head dimensions as here).
+bool kv4_rows_take(int dim) { return dim == 64 || dim == 128 || dim == 256; }
 
 cudaError_t launch_kv4_append(bool bf16, const AppendArgs& a, cudaStream_t stream) {
   switch (a.c.dim) {

@@ -112,6 +112,7 @@ struct LogprobArgs {
 cudaError_t launch_kv_append(bool bf16, const AppendArgs& a, cudaStream_t stream);
 cudaError_t launch_kv_decode(const KvView& c, const int32_t* pages, int count, uint16_t* k_out, uint16_t* v_out,
                              cudaStream_t stream);
+bool kv4_rows_take(int dim);
 cudaError_t launch_kv4_append(bool bf16, const AppendArgs& a, cudaStream_t stream);
 cudaError_t launch_kv4_decode(const KvView& c, const int32_t* pages, int count, uint16_t* k_out, uint16_t* v_out,
                               cudaStream_t stream);
