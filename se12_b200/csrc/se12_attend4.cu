@@ -32,7 +32,7 @@ constexpr int kRows4Threads = kRows4Warps * 32;
 constexpr int kRows4SlotRows = 16;
 constexpr int kRows4SlotFloats = kRows4SlotRows * (256 + 4);  // sums, then (mp, l) per row
 constexpr int kRows4MaxCtas = 3;       // per SM
-constexpr int kRows4PairCost = 8;      // what a pair's queries, joins and output cost, in chunks
+constexpr int kRows4PairCost = 16;      // what a pair's queries, joins and output cost, in chunks
 constexpr float kRows4WideCap = 128.f;  // as kAttendWideCap
 
 template <int DIM>
@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
     // masks pair the codes. Every second one of a word's pairs is a sixteenth.
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      if ((n & (kRows4Warps - 1)) != warp) continue;
+      // (a warp takes every fourth group of the n-tiles)
+      if (G < kRows4Warps && (warp < n * G % kRows4Warps || warp >= n * G % kRows4Warps + G)) continue;
       const int row = tile * ROWS + n * 8 + r;
       uint4 raw[G][2];
       unsigned big = 0;
@@ -426,6 +427,7 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
       const float down = __uint_as_float(static_cast<unsigned>(127 + 14 - e) << 23);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
+        if (((n * G + g) & (kRows4Warps - 1)) != warp) continue;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -841,7 +843,23 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
 
 // ------------------------------------------------------------------ launch
 
-bool kv_attend4_takes_tiles(int max_query, int group, int dim) { return static_cast<long long>(max_query) * group > 16; }
+// This file's kernel reads and widens the codes again for every 16 query rows of a
+// sequence, attend_tile_kernel for every 128, at a cost that hardly depends on how
+// many of them there are. us by this kernel and by that one, 8 KV heads (small
+// ones: 2), sequences of 77 to 4093, 1000, 100 to 3000, 2000 to 8000 tokens:
+//   128 dimensions  24 seqs      1       64       4
+//     32 rows       75, 93    17, 31  139, 191  38, 49
+//     48            99, 96    17, 31  208, 194  45, 50
+//     64           130, 98    23, 31  258, 194  51, 50
+//   256 dimensions, capped
+//     32           192, 158   33, 53  298, 305  72, 82
+//     48           281, 167   36, 54  443, 321  86, 81
+//   64 dimensions, capped
+//     64            35, 57    16, 33   51, 84   27, 56
+//    128            52, 58    17, 33   85, 85   30, 54
+bool kv_attend4_takes_tiles(int max_query, int group, int dim) {
+  return static_cast<long long>(max_query) * group > (dim == 64 ? 128 : dim == 128 ? 48 : 32);
+}
 
 size_t kv_attend4_partial_bytes(int sm_count, bool tile) {
   if (tile) return kv_attend_tile_partial_bytes(sm_count);
