@@ -1,5 +1,5 @@
 """A small decoder served from SE12 weights: prompts in chunks, then one token
-at a time, with a paged 8-bit cache and log probabilities.
+at a time, with a paged 8-bit or 4-bit cache and log probabilities.
 
 Everything between the input ids and the log probabilities that is not a
 norm, an activation or a sum runs in this package's kernels:
@@ -46,6 +46,7 @@ class Shape:
     window: int = 64  # of every other layer
     page: int = 16
     kind: str = "int8"
+    qk_norm: bool = False  # queries and keys normalised per head before the rotation
 
 
 class Layer:
@@ -57,6 +58,7 @@ class Layer:
         self.down = encode_device(weights(s.hidden, s.intermediate))
         self.cache = PagedKvCache(pages, s.page, s.kv_heads, s.head_dim, s.kind)
         self.window = window
+        self.q_norm, self.k_norm = (1 + weights(2, s.head_dim)).unbind() if s.qk_norm else (None, None)
 
 
 def norm(x: torch.Tensor) -> torch.Tensor:
@@ -92,7 +94,8 @@ class Decoder:
         for layer in self.layers:
             y = layer.qkv.gemv(norm(x)).view(-1, s.q_heads + 2 * s.kv_heads, s.head_dim)
             q = layer.cache.append(y[:, s.q_heads : s.q_heads + s.kv_heads], y[:, s.q_heads + s.kv_heads :], self.table, lens,
-                                   q=y[:, : s.q_heads], cos=self.cos, sin=self.sin, query_start=query_start)
+                                   q=y[:, : s.q_heads], cos=self.cos, sin=self.sin, query_start=query_start,
+                                   q_norm=layer.q_norm, k_norm=layer.k_norm)
             a = layer.cache.attend(q, self.table, lens, query_start=query_start, max_query=max_query,
                                    softcap=s.attn_softcap, window=layer.window)
             x = x + layer.o.gemv(a.view(-1, s.q_heads * s.head_dim))
@@ -162,10 +165,11 @@ def main() -> None:
     p = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     p.add_argument("--layers", type=int, default=2)
     p.add_argument("--new", type=int, default=12)
-    p.add_argument("--kind", choices=("int8", "e4m3"), default="int8")
+    p.add_argument("--kind", choices=("int8", "e4m3", "int4"), default="int8")
+    p.add_argument("--qk-norm", action="store_true", help="normalise queries and keys per head")
     p.add_argument("--graph", action="store_true", help="replay the decode step as one CUDA graph")
     a = p.parse_args()
-    model = Decoder(Shape(layers=a.layers, kind=a.kind))
+    model = Decoder(Shape(layers=a.layers, kind=a.kind, qk_norm=a.qk_norm))
     prompts = [[(7 * i + 3 * j) % 4096 for j in range(n)] for i, n in enumerate((5, 100, 33, 1))]
     ids, scores = generate(model, prompts, a.new, graph=a.graph)
     for i, prompt in enumerate(prompts):

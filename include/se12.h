@@ -501,7 +501,8 @@ typedef struct se12_kv_attend_args {
 } se12_kv_attend_args;
 
 /* Enough for any call on the cache; enough for calls of these sizes (a third
- * for up to 16 query rows per KV head, 32 for head dimensions up to 128). */
+ * for few query rows per KV head: up to 16, 32 for head dimensions up to 128;
+ * int4: up to 128, 48 and 32 for head dimensions of 64, 128 and 256). */
 size_t se12_kv_attend_workspace_bytes(const se12_kv_cache* cache);
 size_t se12_kv_attend_call_bytes(const se12_kv_cache* cache, int q_heads, int max_query);
 int se12_kv_attend(const se12_kv_cache* cache, const se12_kv_batch* batch, const se12_kv_attend_args* args,

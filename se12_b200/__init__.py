@@ -7,7 +7,7 @@ GEMV. The package keeps the interface of the reference implementation
 domain codec (``se12_b200.codec``), the GEMV entry point
 (``se12_b200.gemv``), the GPU decoder (``se12_b200.decoder``) and the
 runtime Linear replacement (``se12_b200.runtime``). Around the GEMVs a
-decode step has the paged 8-bit key/value cache with its attention
+decode step has the paged 8-bit or 4-bit key/value cache with its attention
 (``se12_b200.kv_cache``) and log probabilities of the LM head's rows
 (``se12_b200.logprobs``).
 """

@@ -1,9 +1,10 @@
-"""A paged key/value cache in 8 bits, and attention over it.
+"""A paged key/value cache in 8 or 4 bits, and attention over it.
 
 ``PagedKvCache`` holds one layer's keys and values as 8-bit codes (int8 or
-e4m3) with one fp32 scale per block (a page of one KV head). ``append``
-stores a step's new keys and values, rotated to their positions, and rotates
-the queries in the same launch; ``attend`` is the attention of those queries
+e4m3) with one fp32 scale per block (a page of one KV head), or as 4-bit codes
+with a scale and an offset per token and 64 dimensions. ``append`` stores a
+step's new keys and values, normalised and rotated to their positions, and does
+the same to the queries in the same pass; ``attend`` is the attention of those queries
 over the sequences' pages; ``decode`` reads pages back as BF16. They take the
 grouped q/k/v GEMV's fp32 output as it is and give the BF16 rows the o
 projection's GEMV takes, so that a decode step is
