@@ -5,21 +5,32 @@
 //   o_id = sum_j p_ij (vs_jg (u_jd - 8) + vo_jg),  p_ij = 2^(s_ij + E_j) / sum_j 2^s_ij
 //
 // for groups g of 64 dimensions, u the codes, ks, ko, vs, vo scales and
-// offsets. A code never becomes a value: its four bits, masked where they lie,
-// are the FP16 subnormal u 2^-24 (or 16 u 2^-24, four bits higher, met by a
-// query's or a sum's factor of 1/16), which mma.sync multiplies exactly. So 8
-// keys take six instructions and 8 values seven, where widening to signed
-// numbers takes nine more, at a rate of codes at which issue slots are what runs
-// out. Zero points are put right afterwards: keys' with the sums of the query's
-// groups, values' by the products of one more instruction per group, whose
-// second operand is the same rounded weights that the codes were multiplied by
-// (a difference of roundings would not cancel where weights are equal).
+// offsets. A code never becomes a value: its four bits, shifted and masked, are
+// the FP16 subnormal u 2^-22 (or u 2^-18, four bits higher, met by a query's or a
+// sum's factor of 1/16), which mma.sync multiplies exactly. So 8 keys take six
+// instructions and 8 values seven; subtracting the zero point from each pair of
+// them would take four more. Zero points are put right afterwards: keys' with
+// the sums of the query's groups, values' by the products of one more instruction
+// per group, whose second operand is the same rounded weights that the codes were
+// multiplied by (a difference of roundings would not cancel where weights are
+// equal).
 //
 // A group's products are scaled in fp32 (keys) or through its weights
 // p vs in FP16 (values; the scales are relative to 2^E, so that both factors
 // have FP16's full precision whatever the values' size).
 //
-// Work list, warps' pipelines, joins: as attend_rows_kernel, see there.
+// Work list, warps' parts of a run, joins: as attend_rows_kernel, see there. A
+// warp's chunks come by asynchronous copies of 16 bytes per lane, three chunks
+// (of 2048 codes of keys and of values) deep: a whole chunk takes ten copies, where
+// boxes copied by one lane each are a loop over the lanes (206 us for the first case
+// below, 190 with copies by all).
+//
+// 64 sequences of 1000 to 16384 tokens, 64 query and 8 KV heads of 128: 156 us,
+// 4.2 TB/s (copies alone 114; with the keys' products 131); one of 131071, 32 and
+// 16 heads of 128, capped: 81 us, 3.8 TB/s. What bounds it is the issue of 305
+// instructions per 16 tokens and head at 2.1 of 4 a cycle with 12 warps per SM. 16
+// warps of 128 registers work out again what they cannot hold (351 instructions,
+// 174 us); a warp that copies for four others does not keep up (183 us).
 #include "se12_attend.cuh"
 
 #include <cuda_bf16.h>
@@ -32,7 +43,10 @@ constexpr int kRows4Threads = kRows4Warps * 32;
 constexpr int kRows4SlotRows = 16;
 constexpr int kRows4SlotFloats = kRows4SlotRows * (256 + 4);  // sums, then (mp, l) per row
 constexpr int kRows4MaxCtas = 3;       // per SM
-constexpr int kRows4PairCost = 16;      // what a pair's queries, joins and output cost, in chunks
+// What a pair's queries, joins and output cost, in chunks. (4, 8, 12, 16 and 24: 24
+// sequences with drafted tokens 87, 77, 68, 68 and 71 us; 16 with a window 53, 48,
+// 46, 45 and 45; equal lengths do not care.)
+constexpr int kRows4PairCost = 16;
 constexpr float kRows4WideCap = 128.f;  // as kAttendWideCap
 
 template <int DIM>

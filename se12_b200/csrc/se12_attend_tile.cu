@@ -1,4 +1,4 @@
-// Attention over the paged 8-bit cache for many query rows per KV head
+// Attention over the paged cache for many query rows per KV head
 // (prompt chunks, drafted tokens of wide groups): tiles of 128 query rows on
 // the tensor cores.
 //
@@ -31,6 +31,10 @@
 // usual tile's second pass takes a handful of instructions per logit; the sum l
 // comes from the weights, by a factor per 16 tokens. Other tiles take the slow
 // way, eight tokens at a time.
+//
+// 4-bit pages differ in the loaders alone, which widen the codes on their lines
+// (about 380 instructions of each loading warp per tile instead of 200): 2 x 509
+// queries over 5000 to 8191 tokens, 256 dimensions, capped, 259 us instead of 213.
 //
 // The work list (sequences, KV heads, row tiles, KV tiles) is cut into runs of
 // equal cost, one per CTA, and a tile's CTAs are joined as in attend_rows_kernel.

@@ -586,7 +586,15 @@ cudaError_t launch_append_as(const AppendArgs& a, cudaStream_t stream) {
   // of 128, 64 query heads of 128, 2100 tokens 41 -> 62; 16000 170 -> 183 (four heads).
   const int span = a.t.tokens <= 256 ? 1 : 16;
   const long long blocks = static_cast<long long>(a.t.tokens) / a.c.page_size * 2 * a.c.heads;
-  const int heads_each = a.t.tokens <= 256 ? 1 : a.c.page_size <= 32 ? 4 : blocks >= 900 ? 2 : 1;
+  // With norms a head takes longer, and few blocks are better spread: one, two and
+  // four heads, 8 KV heads, without queries: 300 tokens, pages of 32 of 128 9, 13,
+  // 20; 600 of 256 10, 14, 21; 3000, pages of 16 of 256 40, 33, 34; 7000, pages of
+  // 32 of 128 44, 35, 33; 16100 100, 78, 69.
+  const int heads_each = a.t.tokens <= 256 || (NORM && blocks < 900) ? 1
+                         : NORM && blocks < 2500                     ? 2
+                         : a.c.page_size <= 32                       ? 4
+                         : blocks >= 900                             ? 2
+                                                                     : 1;
   const dim3 grid((a.t.tokens + span - 1) / span, 2 * ((a.c.heads + heads_each - 1) / heads_each) + (a.q ? 1 : 0));
   return launch_overlapped(kv_append_prompt_kernel<T, KIND, VP, NORM>, grid, 256, 0, stream, a, span, heads_each);
 }
@@ -614,7 +622,7 @@ cudaError_t launch_append_kind(const AppendArgs& a, cudaStream_t stream) {
 // Normalised queries of many tokens go through the 4-bit cache's row kernel, in a
 // launch of their own: half the lanes per row and a warp per few heads instead of
 // one per token (7 prompt chunks, 64 query heads of 128, BF16, with the pages read
-// back: 114 us by one launch, 72 by two).
+// back: 114 us by one launch, 72 by two; 62 with fewer heads per CTA).
 template <typename T, int KIND>
 cudaError_t launch_append_normed(const AppendArgs& a, cudaStream_t stream) {
   if (!a.q_norm.weight && !a.k_norm.weight) return launch_append_kind<T, KIND, false>(a, stream);

@@ -20,7 +20,11 @@
 // of neighbouring tokens in cells of 16: [8 pairs][groups scales, groups
 // offsets][2], then the 16 E.
 //
-// Both kernels are bound by memory and, for few tokens, by their latency.
+// 13 prompt chunks of 301 to 2043 tokens, 16 query and 8 KV heads of 256, BF16,
+// with norms: 118 us, 3.0 TB/s of what has to move; what bounds it is the issue of
+// some 180 instructions per row at 2.5 of 4 a cycle (20 warps per SM). Their pages
+// read back: 24 us, 6.2 TB/s. For few tokens both are bound by their latency (64
+// tokens of 80 heads: 5 us).
 #include "se12_kv.cuh"
 
 #include <algorithm>
