@@ -390,7 +390,8 @@ int se12_encode_raw(const uint16_t* w_dev, int rows, int cols, int ldw, const in
  *   k_scales: [pages][kv_heads][page_size][groups][scale, offset] fp16
  *   v_scales: [pages][kv_heads][page_size / 16] cells of 32 * groups + 16 fp16:
  *             [8 pairs of tokens][groups scales, groups offsets][2 tokens], [16] E
- * both 16-byte aligned, scales and offsets of values finite.
+ * both 16-byte aligned, scales and offsets of values finite, E a whole number
+ * from -30 to 30, or NaN (the token's values are).
  */
 #define SE12_KV_INT8 0
 #define SE12_KV_E4M3 1

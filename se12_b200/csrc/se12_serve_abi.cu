@@ -17,7 +17,8 @@ namespace {
 
 // A launch has at most kAttendMaxCtas CTAs per SM, each with a counter.
 constexpr int kMaxSms = 160;
-static_assert(kMaxSms * se12::kAttendMaxCtas * sizeof(int) <= SE12_COUNTER_BYTES, "the counters of a launch");
+static_assert(kMaxSms * std::max(se12::kAttendMaxCtas, se12::kRows4MaxCtas) * sizeof(int) <= SE12_COUNTER_BYTES,
+              "the counters of a launch");
 
 // Codes as [pages * heads * page_size rows][dim bytes], one box = 16 tokens x
 // 128 bytes (a page is a multiple of 16 tokens, so a box never leaves it;
@@ -150,6 +151,9 @@ int se12_kv_append_normed(const se12_kv_cache* cache, const se12_kv_batch* batch
   if (norms) {
     if (!(norms->eps >= 0.0) || std::isinf(norms->eps))
       return fail(SE12_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+    if (reinterpret_cast<uintptr_t>(norms->q_weight) % (norms->q_bf16 ? 2 : 4) ||
+        reinterpret_cast<uintptr_t>(norms->k_weight) % (norms->k_bf16 ? 2 : 4))
+      return fail(SE12_ERR_MISALIGNED, "norm weights must be aligned to their type");
     a.q_norm = {p->q ? norms->q_weight : nullptr, norms->q_bf16};
     a.k_norm = {norms->k_weight, norms->k_bf16};
     a.norm_eps = norms->eps;

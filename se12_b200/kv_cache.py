@@ -117,9 +117,9 @@ class PagedKvCache:
     page_size, groups, 2] (scale, offset); ``v_scales`` fp16 [pages, kv_heads,
     page_size / 16, 32 * groups + 16]: of 16 tokens, for each two neighbours
     the groups' scales and then their offsets (the two tokens' side by side),
-    then a whole number E per token: its values are 2^E times what scale and
-    offset give. Scales and offsets of values are finite; E is NaN for a token
-    whose values were not."""
+    then a whole number E per token, -30 to 30: its values are 2^E times what
+    scale and offset give. Scales and offsets of values are finite; E is NaN for
+    a token whose values were not."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, kind: str = "int8", device="cuda"):
         self._check(pages, page_size, kv_heads, head_dim, kind)

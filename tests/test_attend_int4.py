@@ -433,3 +433,54 @@ def test_offsets_past_32_bits():
         a, b = (c.attend(q, where, lens, query_start=at) for c, where in ((cache, table), (small, near)))
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
     assert torch.equal(cache.decode(table[0])[1], small.decode()[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 60])
+def test_calls_at_once_on_two_streams(n):
+    """Long and short batches side by side, again and again, each on a stream of
+    its own and one of them as a graph besides: the bits of calls one by one."""
+    cases = []
+    for seed, lens in ((1, [9000, 3, 700]), (2, [40, 5000, 5000])):
+        g = torch.Generator().manual_seed(seed)
+        lens = [max(ln, n) for ln in lens]
+        table, pool = random_tables(g, lens, 32)
+        f = Filled(g, pool, 32, 2, 128)
+        q = torch.randn(3 * n, 8, 128, generator=g).to(torch.bfloat16).cuda()
+        start = torch.arange(0, 3 * n + 1, n, dtype=torch.int32).cuda()
+        table, lens = table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+
+        def call(f=f, q=q, table=table, lens=lens, start=start):
+            return f.cache.attend(q, table, lens, query_start=start, max_query=n, window=4000)
+
+        cases.append((call, call(), torch.cuda.Stream()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = cases[0][0]()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        graph.replay()
+        outs = []
+        for call, want, stream in cases:
+            with torch.cuda.stream(stream):
+                outs.append((call(), want))
+        torch.cuda.synchronize()
+        assert torch.equal(held.view(torch.int16), cases[0][1].view(torch.int16))
+        for got, want in outs:
+            assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 3, 70])
+def test_rows_of_no_sequence_stay_as_they_are(dim, n):
+    g = torch.Generator().manual_seed(dim + n)
+    lens = [100, n + 7]
+    table, pool = random_tables(g, lens, 16)
+    f = Filled(g, pool, 16, 1, dim)
+    q = torch.randn(2 * n + 9, 4, dim, generator=g).to(torch.bfloat16)
+    start = torch.tensor([4, 4 + n, 4 + 2 * n], dtype=torch.int32).cuda()
+    out = torch.full(q.shape, 3.0, dtype=torch.bfloat16, device="cuda")
+    f.cache.attend(q.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), query_start=start, max_query=n, out=out)
+    assert bool((out[:4] == 3).all()) and bool((out[4 + 2 * n :] == 3).all())
+    f.check(q[4 : 4 + 2 * n], table, lens, [n, n], out[4 : 4 + 2 * n], many=n * 4 > 16)

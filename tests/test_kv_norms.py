@@ -139,3 +139,49 @@ def test_abi_refuses_bad_norms():
     lib = _lib.load()
     assert lib.se12_kv_append_normed(None, None, None, None, None) == 1
     assert _lib.KV_NORMS.size == 32
+
+
+def test_abi_refuses_misaligned_weights():
+    """Before anything else of the call is looked at on the device: the handle is
+    one made without a GPU's work (its pointers are never followed)."""
+    from se12_b200 import _build, _lib
+
+    _build.build()
+    lib = _lib.load()
+    if torch.cuda.is_available():
+        from se12_b200.kv_cache import PagedKvCache
+
+        x = torch.zeros(1, 1, 64, device="cuda")
+        cache, ints = PagedKvCache(1, 16, 1, 64), torch.ones(1, 1, dtype=torch.int32, device="cuda")
+        batch = _lib.KV_BATCH.pack(1, 1, ints.data_ptr(), 0, ints.data_ptr(), 1, 1)
+        args = _lib.KV_APPEND.pack(False, 1, x.data_ptr(), x.data_ptr(), x.data_ptr(), *[64] * 6, 0, 0, 0, 0, 0, False, x.data_ptr(), 64, 64)
+        for q, k, bf16, want in ((x.data_ptr() + 2, 0, 0, 3), (0, x.data_ptr() + 1, 1, 3)):
+            norms = _lib.KV_NORMS.pack(q, k, bf16, bf16, 1e-6)
+            assert lib.se12_kv_append_normed(cache.handle, batch, args, norms, None) == want
+        assert lib.se12_kv_append_normed(cache.handle, batch, args, _lib.KV_NORMS.pack(0, 0, 0, 0, -1.0), None) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3", "int4"])
+@pytest.mark.parametrize("tokens", [40, 300])
+def test_rows_behind_the_last_sequence_are_not_stored(kind, tokens):
+    """query_start ends before the batch does, and begins after its first rows:
+    those rows' queries are zeros, their keys and values are nowhere."""
+    from se12_b200.kv_cache import PagedKvCache
+
+    g = torch.Generator().manual_seed(tokens)
+    dim, heads, page = 128, 2, 16
+    n = tokens - 13
+    table = torch.arange(40, dtype=torch.int32).view(2, 20).cuda()
+    lens = torch.tensor([n - 5, 5], dtype=torch.int32).cuda()
+    start = torch.tensor([3, n - 2, n + 3], dtype=torch.int32).cuda()
+    x = torch.randn(tokens, heads, dim, generator=g).cuda()
+    w = torch.randn(dim, generator=g).cuda()
+    cos, sin = (t.cuda() for t in rope(g, 400, dim // 2))
+    whole, part = (PagedKvCache(40, page, heads, dim, kind) for _ in range(2))
+    q = whole.append(x, x, table, lens, q=x, query_start=start, cos=cos, sin=sin, q_norm=w, k_norm=w)
+    rows = slice(3, n + 3)
+    again = part.append(x[rows], x[rows], table, lens, q=x[rows], query_start=start - 3, cos=cos, sin=sin, q_norm=w, k_norm=w)
+    assert torch.equal(q[rows], again) and not q[:3].any() and not q[n + 3 :].any()
+    assert torch.equal(whole.k_codes, part.k_codes) and torch.equal(whole.v_codes, part.v_codes)
+    assert torch.equal(whole.k_scales, part.k_scales) and torch.equal(whole.v_scales, part.v_scales)
