@@ -32,9 +32,14 @@
 // comes from the weights, by a factor per 16 tokens. Other tiles take the slow
 // way, eight tokens at a time.
 //
-// 4-bit pages differ in the loaders alone, which widen the codes on their lines
+// 4-bit pages differ in the loaders, which widen the codes on their lines
 // (about 380 instructions of each loading warp per tile instead of 200): 2 x 509
-// queries over 5000 to 8191 tokens, 256 dimensions, capped, 259 us instead of 213.
+// queries over 5000 to 8191 tokens, 256 dimensions, capped, 259 us instead of 211.
+// Their tokens have a power of two each. Where those of 16 tokens are close to each
+// other they share one, as a block's scale; tiles with others go the slow way, in
+// which every token has its own. With every hundredth token, at random, 2^6 below
+// the rest: 345 us (700 queries of 700, 3000 and 9000, 128 dimensions, group 4, no
+// cap: 380 us, and 489).
 //
 // The work list (sequences, KV heads, row tiles, KV tiles) is cut into runs of
 // equal cost, one per CTA, and a tile's CTAs are joined as in attend_rows_kernel.
@@ -55,6 +60,11 @@ constexpr int kTileSoftmaxRegs = 208, kTileLoaderRegs = 104, kTileIssuerRegs = 8
 static_assert(kTileSoftmaxRegs + 2 * kTileLoaderRegs + kTileIssuerRegs <= 4 * 128, "more registers than the launch has");
 constexpr int kTileKvBytes = 32768;   // an FP16 tile of keys or values
 constexpr int kTileMeta = 4;          // tiles whose block scales are kept
+// 4 bits: the most that the E of a cell's tokens may differ by for their values to
+// stand beside the largest, so that one factor serves the cell. A row that does not
+// see the largest, or gives it no weight, loses that many of the 14 powers of two
+// that FP16 has below 1 for its weights, and scales and offsets for theirs.
+constexpr int kTileSpread = 6;
 // What a pair's queries, first loads and output cost, in KV tiles. (Calls
 // repeated in a graph, before later checks added a few per cent: 24 sequences
 // of 77 to 4093 tokens, 2 to 6 new ones of 8 rows: uncounted 105 us, the SMs
@@ -331,7 +341,10 @@ __device__ __forceinline__ int tile_boundary(const AttendArgs& a, const int* bef
 }
 
 struct TileSmem {
-  float meta[kTileMeta][8][2];        // [16 tokens of the tile][scale of keys, log2 of values' scale]
+  // [16 tokens of the tile][scale of keys, log2 of values' scale (4 bits: NaN where each
+  // token has its own, in `power`)]
+  float meta[kTileMeta][8][2];
+  float power[kTileMeta][128];
   int meta_missing[kTileMeta];        // bit g: those tokens' page is not there
   float row_scale[2][kTileAttendRows];  // of this pair and the next
   // Pairs shared with other CTAs (a run's first and last) that this CTA
@@ -369,6 +382,7 @@ struct RowSoftmax {
 struct TileLogits {
   uint32_t from, to;        // S and P of this tile in tensor memory, this warp's lanes
   const float (*meta)[2];   // per 16 tokens: scale of keys, log2 of values' scale
+  const float* power;       // per token, where that is NaN (4 bits)
   float row_scale;          // logits per product (capped: logits / cap)
   float cap2;               // cap * log2(e)
   int low, high;            // this row sees the tile's tokens low .. high
@@ -539,7 +553,7 @@ __device__ __forceinline__ bool usual_tile(RowSoftmax& r, const TileLogits& z, S
 
 // Any tile, eight tokens at a time. `missing`: bit q set where the 16 tokens'
 // page is not there; masked and missing tokens weigh nothing.
-template <int TT, typename ScaleSums>
+template <int KIND, int TT, typename ScaleSums>
 __device__ __forceinline__ void any_tile(RowSoftmax& r, const TileLogits& z, int missing, ScaleSums&& scale_sums) {
   auto logits = [&](float (&y)[8], int k0) {
     uint32_t s[8];
@@ -554,16 +568,22 @@ __device__ __forceinline__ void any_tile(RowSoftmax& r, const TileLogits& z, int
       y[k] = k0 + k < z.low || k0 + k > z.high || !there ? kNegInf : v;
     }
   };
+  auto value_scales = [&](float (&lv)[8], int k0) {
+    const float of_all = z.meta[k0 >> 4][1];
+    const bool own = KIND == kKvInt4 && of_all != of_all;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) lv[k] = own ? z.power[k0 + k] : of_all;
+  };
   float top = r.m, top_v = r.mp;
 #pragma unroll 1
   for (int k0 = 0; k0 < TT; k0 += 8) {
-    float y[8];
+    float y[8], lv[8];
     logits(y, k0);
-    const float lv = z.meta[k0 >> 4][1];
+    value_scales(lv, k0);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       top = fmaxf(top, y[k]);
-      if (y[k] != kNegInf) top_v = fmaxf(top_v, y[k] + lv);
+      if (y[k] != kNegInf) top_v = fmaxf(top_v, y[k] + lv[k]);
     }
   }
   r.l *= ex2(r.m - top);
@@ -572,14 +592,14 @@ __device__ __forceinline__ void any_tile(RowSoftmax& r, const TileLogits& z, int
   r.mp = top_v;
 #pragma unroll 1
   for (int k0 = 0; k0 < TT; k0 += 8) {
-    float y[8];
+    float y[8], lv[8];
     logits(y, k0);
-    const float shift = z.meta[k0 >> 4][1] - r.mp;
+    value_scales(lv, k0);
     uint32_t p[4];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       r.l += ex2(y[k] - r.m);
-      y[k] = y[k] == kNegInf ? 0.f : ex2(y[k] + shift);
+      y[k] = y[k] == kNegInf ? 0.f : ex2(y[k] + (lv[k] - r.mp));
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) p[k] = half2_bits(__floats2half2_rn(y[2 * k], y[2 * k + 1]));
@@ -897,7 +917,9 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       // ---- 4 bits. A warp has two cells of 16 tokens of a tile (256 dimensions:
       // half of each row's codes), four vectors of 8 tokens x 64 bytes of codes.
       // Keys become FP16 values; values become FP16 times 2^-X, X the largest E of
-      // the cell's tokens that count, which takes the place of a block's scale. The 8
+      // the cell's tokens that count, which takes the place of a block's scale; where
+      // a token's E is more than kTileSpread below it, FP16 times 2^-E of their own,
+      // and the tile goes the slow way. (A token of zeros may have any E.) The 8
       // of a word stay in the order their codes are unpacked in (of_eight). A
       // token whose E is no number has NaN for a key and zero for a value: the
       // rows that see it are NaN, as their weights are.
@@ -950,12 +972,28 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
           x.power = load_half_or(power + 16 * h, use, 0xFC00u);  // (-inf: a token that does not count)
         }
       };
-      // A vector's codes on their lines, to the tile.
+      auto power_of = [&](int v) { return __half2float(__ushort_as_half(static_cast<unsigned short>(r[v].power))); };
+      // Whether a token of the warp's cells (in `far`, a bit per vector, its own lanes)
+      // has a line that is not zeros: bits of the cells. (Seldom asked: small.)
+      auto cells_with_lines = [&](unsigned far) {
+        unsigned found = 0;
+#pragma unroll 1
+        for (int v = 0; v < 4; ++v) {
+          const int row = __shfl_sync(0xFFFFFFFFu, rows_at, cell_of(v & 2));
+          const uint8_t* pair = cells + static_cast<long long>(row >> 4) * cell_bytes + ((lane & 7) >> 1) * (8 * groups) + (v & 1) * (32 * groups);
+          uint32_t any = 0;
+#pragma unroll 1
+          for (int w = lane >> 3; w < 2 * groups; w += 4) any |= load_word_or(pair + 4 * w, (far >> v) & 1, 0u);
+          if (__any_sync(0xFFFFFFFFu, (any & ((lane & 1) ? 0x7FFF0000u : 0x7FFFu)) != 0)) found |= 1u << (v >> 1);
+        }
+        return found;
+      };
+      // A vector's codes on their lines, to the tile. `cell_power`: X, or NaN.
       auto store4 = [&](int v, unsigned char* tile, float cell_power) {
-        const float e = __half2float(__ushort_as_half(static_cast<unsigned short>(r[v].power)));
+        const float e = power_of(v);
         const bool number = e == e;
-        // (2^(E - X) of a token: what it takes from FP16's subnormals weighs nothing beside the cell's largest)
-        const uint32_t down = half2_bits(__half2half2(__float2half_rn(number ? ex2(e - cell_power) : 0.f)));
+        const float to_cell = cell_power == cell_power ? ex2(e - cell_power) : 1.f;
+        const uint32_t down = half2_bits(__half2half2(__float2half_rn(number ? to_cell : 0.f)));
         const uint32_t side = (lane & 1) ? 0x3232u : 0x1010u;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -989,23 +1027,51 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
       for (int j = 0; j < tiles_all; ++j) {
         const int stage = j & 1;
         unsigned char* tile = tiles + stage * kTileKvBytes;
-        float cell_power[2];  // of the warp's cells; 0 where no token counts
+        float cell_power[2];  // of the warp's cells: X (0 where no token counts), or NaN
+        unsigned far = 0;     // this lane's tokens that are too far below X
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float x = kNegInf;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float e = __half2float(__ushort_as_half(static_cast<unsigned short>(r[2 * i + h].power)));
-            x = fmaxf(x, e);  // (NaN is left out)
-          }
+          float x = fmaxf(power_of(2 * i), power_of(2 * i + 1));  // (NaN is left out)
 #pragma unroll
           for (int d = 1; d < 8; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
           cell_power[i] = fabsf(x) <= 64.f ? x : 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float below = cell_power[i] - power_of(2 * i + h);
+            if (below > kTileSpread && below < 1000.f) far |= 1u << (2 * i + h);  // (not -inf: no token)
+          }
+        }
+        if (__any_sync(0xFFFFFFFFu, far != 0)) {
+          far = cells_with_lines(far);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if ((far >> i) & 1) cell_power[i] = __uint_as_float(0x7FC00000u);
         }
         // the tile two before has been read by its products
         if (j >= 2) wait(keys ? &sm.s_full[stage] : &sm.pv_done[stage], ((j >> 1) + 1) & 1);
         const bool more = j + 1 < tiles_all;
         const unsigned missing_groups = __ballot_sync(0xFFFFFFFFu, missing);
+        if (keys) {
+          const int slot = j % kTileMeta;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int cell = cell_of(2 * i);
+            if (lane == 0) {
+              sm.meta[slot][cell][0] = 1.f;
+              sm.meta[slot][cell][1] = cell_power[i];
+            }
+            if (cell_power[i] != cell_power[i] && lane < 8) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float e = power_of(2 * i + h);
+                sm.power[slot][cell * 16 + h * 8 + lane] = fabsf(e) <= 64.f ? e : 0.f;
+              }
+            }
+          }
+          if (tid == 0) sm.meta_missing[slot] = static_cast<int>(missing_groups);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.meta_full[slot]);
+        }
         if (more) take_tile();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -1014,17 +1080,6 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
           if (more) load_cell(i);
         }
         fence_proxy_async_shared();
-        if (keys) {
-          const int slot = j % kTileMeta;
-          if (lane < 2) {
-            const int cell = cell_of(2 * lane);
-            sm.meta[slot][cell][0] = 1.f;
-            sm.meta[slot][cell][1] = lane == 0 ? cell_power[0] : cell_power[1];
-          }
-          if (tid == 0) sm.meta_missing[slot] = static_cast<int>(missing_groups);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.meta_full[slot]);
-        }
         __syncwarp();
         if (lane == 0) mbar_arrive(keys ? &sm.k_full[stage] : &sm.v_full[stage]);
       }
@@ -1100,6 +1155,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
           z.from = tmem + lanes + Shape::kColS + (j & 1) * TT;
           z.to = tmem + lanes + Shape::kColP + (j & 1) * (TT / 2);
           z.meta = sm.meta[slot];
+          z.power = sm.power[slot];
           z.row_scale = row_scale;
           z.cap2 = cap2;
           z.low = a.window ? pos - t0 - (a.window - 1) : 0;
@@ -1129,7 +1185,7 @@ __global__ void __launch_bounds__(kTileAttendThreads, 1) attend_tile_kernel(cons
             else
               finished = masked ? usual_tile<TT, false, true>(r, z, scale_sums) : usual_tile<TT, false, false>(r, z, scale_sums);
           }
-          if (!finished) any_tile<TT>(r, z, missing, scale_sums);
+          if (!finished) any_tile<KIND, TT>(r, z, missing, scale_sums);
           tmem_wait_store();
         }
         tc_fence_before();
