@@ -891,7 +891,7 @@ struct se12_chain {
 
 namespace {
 
-constexpr size_t kChainSmemLimit = 227 * 1024;
+constexpr size_t kChainSmemLimit = se12::kMaxSmemPerCta;
 constexpr int kChainMinConsumers = 12;
 
 // x budget: what is left of shared memory with kChainMinConsumers warps.

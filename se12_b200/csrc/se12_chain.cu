@@ -792,7 +792,7 @@ cudaError_t launch_chain(bool raw, const ChainParams& p, int grid, size_t smem, 
   using Kernel = void (*)(const ChainParams);
   const Kernel kernel = raw ? (p.batch <= 8 ? chain_kernel<1, true> : chain_kernel<2, true>)
                             : (p.batch <= 8 ? chain_kernel<1, false> : chain_kernel<2, false>);
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  cudaError_t err = allow_shared_memory(kernel);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);

@@ -1222,7 +1222,8 @@ cudaError_t launch_gemv(bool raw, const CUtensorMap& map0, const CUtensorMap& ma
                         : ar   ? table_ar[blocks][kind][a.x_resident ? 1 : 0]
                                : table[blocks][kind][a.x_resident ? 1 : 0];
   if (!kernel) return cudaErrorInvalidValue;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // (the decode tables are 64 bytes, which the compiler aligns to 1024 in front of the rest)
+  cudaError_t err = allow_shared_memory(kernel, raw ? 0 : 1024);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.grid);

@@ -7,6 +7,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "se12_launch.h"
+
 namespace se12 {
 
 // One SE12 matrix on the device, as the kernels see it.
@@ -133,7 +135,6 @@ constexpr int kRecFbOffset = kRecEscOffset + kRecGroupTiles * 16;
 constexpr int kRecFbTiles = kRecGroupTiles + 4;  // copied from the 4-tile-aligned tile at or before the group
 constexpr int kRecSlotBytes = kRecFbOffset + kRecFbTiles * 4;
 constexpr size_t kCoResidentSmem = 112 * 1024;  // two CTAs fit on one SM
-constexpr size_t kMaxSmemPerCta = 227 * 1024;   // one CTA per SM (sm_100 opt-in maximum)
 
 // Bytes per batch row of resident x: K rounded up to whole tiles (256
 // columns; the columns past K hold zeros), plus 64 so consecutive rows start

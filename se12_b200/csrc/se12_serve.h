@@ -9,6 +9,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "se12_launch.h"
 #include "se12_worklist.h"
 
 namespace se12 {
@@ -134,8 +135,7 @@ template <typename... Params, typename... Args>
 inline cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
                                      Args&&... args) {
   if (smem > 48 * 1024) {
-    const cudaError_t err =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t err = allow_shared_memory(kernel);
     if (err != cudaSuccess) return err;
   }
   cudaLaunchConfig_t cfg{};
