@@ -67,13 +67,12 @@ PFN_cuMemGetAddressRange_v3020 address_range_query() {
 }
 
 int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
-               const cuuint64_t* strides, const cuuint32_t* box,
-               CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+               const cuuint64_t* strides, const cuuint32_t* box) {
   auto fn = tensor_map_encoder();
   if (!fn) return fail(SE12_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint32_t estride[3] = {1, 1, 1};
   CUresult r = fn(map, type, rank, const_cast<void*>(base), dims, strides, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(SE12_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(int(r)));
   return SE12_OK;
 }

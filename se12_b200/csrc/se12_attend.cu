@@ -92,6 +92,16 @@ struct AttendSmem {
   int before[1];  // [seqs + 1] units of the sequences before (per KV head)
 };
 
+// A place in the work list: chunk `chunk` of pair `pair` (KV head x row
+// tile) of sequence b. The list counts units: a pair's are kAttendPairCost for
+// its beginning and end, from `start` on, and one per chunk.
+struct Place {
+  int b, pair, chunk;
+  int start;
+  SeqWork w;
+  __device__ __forceinline__ int unit() const { return start + kAttendPairCost + chunk; }
+};
+
 template <int KIND, int DP, int NT, int CTAS>
 __global__ void __launch_bounds__(kAttendThreads, CTAS)
     attend_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -150,7 +160,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
       if (static_cast<long long>(sm.before[mid]) * heads <= u) lo = mid;
       else hi = mid - 1;
     }
-    Place<kAttendPairCost> p;
+    Place p;
     p.b = lo;
     p.w = sequence_work<CHUNK, ROWS>(a, lo);
     const int x = u - sm.before[lo] * heads, each = p.w.chunks + kAttendPairCost;
@@ -161,7 +171,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
     return p;
   };
   // To the place `by` chunks on; false where that is past this CTA's run.
-  auto advance = [&](Place<kAttendPairCost>& p, int by) {
+  auto advance = [&](Place& p, int by) {
     p.chunk += by;
     while (p.chunk >= p.w.chunks) {
       p.chunk -= p.w.chunks;
@@ -183,7 +193,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
   unsigned char* pipe = pipes + warp * (kAttendStages * kAttendStageBytes);
   const uint32_t pipe_addr = smem_addr(pipe);
   const uint64_t policy = policy_evict_first();
-  Place<kAttendPairCost> next = locate(u0);
+  Place next = locate(u0);
   bool more = advance(next, warp);  // `next` is a chunk of the run
   int next_page = -1;  // this lane's (lane < SUBS) page for the next chunk to issue
   auto fetch_page = [&]() {
@@ -240,7 +250,7 @@ __global__ void __launch_bounds__(kAttendThreads, CTAS)
   bool dead = false;  // a wait ran out: skip the rest (status raised)
 
   // ---- the pairs of this CTA's run
-  Place<kAttendPairCost> at = locate(u0);
+  Place at = locate(u0);
   int done = 0;  // chunks of the run before this pair
   for (bool here = advance(at, 0); here;) {
     const int run = min(at.w.chunks - at.chunk, u1 - at.unit());  // chunks of this pair here

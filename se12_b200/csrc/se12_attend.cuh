@@ -88,15 +88,4 @@ __device__ __forceinline__ SeqWork sequence_work(const AttendArgs& a, int b) {
   return sequence_work(a.t.rows_of(b, list_sizes(a)), list_sizes(a), CHUNK, ROWS);
 }
 
-// A place in the work list: chunk `chunk` of pair `pair` (KV head x row
-// tile) of sequence b. The list counts units: a pair's are COST for its beginning
-// and end, from `start` on, and one per chunk.
-template <int COST>
-struct Place {
-  int b, pair, chunk;
-  int start;
-  SeqWork w;
-  __device__ __forceinline__ int unit() const { return start + COST + chunk; }
-};
-
 }  // namespace se12

@@ -144,7 +144,7 @@ __device__ __forceinline__ float2 halves_of(uint32_t w) { return __half22float2(
 // its sum as if a subnormal began at 2^-14: two bits more are worth a shift.)
 constexpr uint32_t kLowCodes = 0x003C003Cu, kHighCodes = 0x03C003C0u;
 
-// 16 bytes, asynchronously (where `use`).
+// 16 bytes, asynchronously; the second only where `use`.
 __device__ __forceinline__ void copy_16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -184,8 +184,9 @@ template <int DIM, int NT, int CTAS, bool ONE>
 __global__ void __launch_bounds__(kRows4Threads, CTAS)
     attend4_rows_kernel(const AttendArgs a) {
   using Shape = Rows4Shape<DIM>;
-  // A place in the work list, as Place: KV head, row tile and chunk; the pair's
-  // chunks in this CTA's run end before `stop`.
+  // A place in the work list, which counts units: a pair's (KV head x row tile) are
+  // kRows4PairCost for its beginning and end, from `start` on, and one per chunk. The
+  // pair's chunks in this CTA's run end before `stop`.
   struct Spot {
     int b, head, tile, chunk, stop;
     int start;

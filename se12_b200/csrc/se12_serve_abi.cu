@@ -1,5 +1,5 @@
-// C-ABI layer of the decode-step operators around the GEMVs: the paged 8-bit
-// key/value cache, attention over it and token log probabilities (argument
+// C-ABI layer of the decode-step operators around the GEMVs: the paged 8-bit or
+// 4-bit key/value cache, attention over it and token log probabilities (argument
 // checks, TMA descriptors, launches). See include/se12.h.
 #include "se12_serve.h"
 
@@ -8,7 +8,7 @@
 
 struct se12_kv_cache {
   se12::KvView view;
-  alignas(64) CUtensorMap k_map;
+  alignas(64) CUtensorMap k_map;  // 8 bits (4-bit codes are read without)
   alignas(64) CUtensorMap v_map;
   int sm_count;
 };
@@ -24,15 +24,11 @@ static_assert(kMaxSms * std::max(se12::kAttendMaxCtas, se12::kRows4MaxCtas) * si
 // 128 bytes (a page is a multiple of 16 tokens, so a box never leaves it;
 // columns past dim read as zero codes, which stand for zero).
 int encode_kv_map(CUtensorMap* map, const void* codes, const se12::KvView& v) {
-  const bool four = v.kind == se12::kKvInt4;  // a box is 16 whole rows, swizzled as their length allows
-  const cuuint64_t row = four ? v.dim / 2 : v.dim;
-  const cuuint64_t dims[2] = {row, static_cast<cuuint64_t>(v.pages) * v.heads * v.page_size};
-  const cuuint64_t strides[1] = {row};
-  const cuuint32_t box[2] = {four ? static_cast<cuuint32_t>(row) : 128, 16};
-  const CUtensorMapSwizzle swizzle = !four || row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                                     : row == 64         ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                         : CU_TENSOR_MAP_SWIZZLE_NONE;
-  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box, swizzle);
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(v.dim),
+                              static_cast<cuuint64_t>(v.pages) * v.heads * v.page_size};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(v.dim)};
+  const cuuint32_t box[2] = {128, 16};
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box);
 }
 
 // SMs of the current device, at most kMaxSms; asked once per device.
@@ -118,8 +114,8 @@ int se12_kv_cache_create(const se12_kv_pages* p, se12_kv_cache** out) {
   v.dim = p->head_dim;
   v.kind = p->kind;
   c->sm_count = std::min(sm_count, kMaxSms);
-  st = encode_kv_map(&c->k_map, p->k_codes, v);
-  if (st == SE12_OK) st = encode_kv_map(&c->v_map, p->v_codes, v);
+  if (!four) st = encode_kv_map(&c->k_map, p->k_codes, v);
+  if (!four && st == SE12_OK) st = encode_kv_map(&c->v_map, p->v_codes, v);
   if (st != SE12_OK) {
     delete c;
     return st;
