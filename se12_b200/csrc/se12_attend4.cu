@@ -25,8 +25,8 @@
 // boxes copied by one lane each are a loop over the lanes (206 us for the first case
 // below, 190 with copies by all).
 //
-// 64 sequences of 1000 to 16384 tokens, 64 query and 8 KV heads of 128: 156 us,
-// 4.2 TB/s (copies alone 114; with the keys' products 131); one of 131071, 32 and
+// 64 sequences of 1000 to 16384 tokens, 64 query and 8 KV heads of 128: 166 us,
+// 3.9 TB/s (copies alone 114; with the keys' products 131); one of 131071, 32 and
 // 16 heads of 128, capped: 81 us, 3.8 TB/s. What bounds it is the issue of 305
 // instructions per 16 tokens and head at 2.1 of 4 a cycle with 12 warps per SM. 16
 // warps of 128 registers work out again what they cannot hold (351 instructions,
@@ -863,15 +863,16 @@ __global__ void __launch_bounds__(kRows4Threads, CTAS)
 // many of them there are. us by this kernel and by that one, 8 KV heads (small
 // ones: 2), sequences of 77 to 4093, 1000, 100 to 3000, 2000 to 8000 tokens:
 //   128 dimensions  24 seqs      1       64       4
-//     32 rows       75, 93    17, 31  139, 191  38, 49
-//     48            99, 96    17, 31  208, 194  45, 50
-//     64           130, 98    23, 31  258, 194  51, 50
+//     32 rows       62, 102   17, 31  116, 205  36, 52
+//     48            85, 104   18, 32  166, 206  43, 53
+//     64           108, 105   23, 32  209, 207  49, 53
 //   256 dimensions, capped
-//     32           192, 158   33, 53  298, 305  72, 82
-//     48           281, 167   36, 54  443, 321  86, 81
+//     32           160, 166   42, 55  298, 317  70, 79
+//     48           231, 172   35, 55  444, 328  87, 81
 //   64 dimensions, capped
-//     64            35, 57    16, 33   51, 84   27, 56
-//    128            52, 58    17, 33   85, 85   30, 54
+//     64            36, 58    16, 35   55, 86   25, 56
+//    128            54, 59    16, 36   91, 89   30, 55
+//    192            70, 81    16, 35  123, 143  35, 56
 bool kv_attend4_takes_tiles(int max_query, int group, int dim) {
   return static_cast<long long>(max_query) * group > (dim == 64 ? 128 : dim == 128 ? 48 : 32);
 }

@@ -619,10 +619,14 @@ cudaError_t launch_append_kind(const AppendArgs& a, cudaStream_t stream) {
   return vp == 4 ? launch_append_as<T, KIND, 4, NORM>(a, stream) : launch_append_as<T, KIND, 2, NORM>(a, stream);
 }
 
-// Normalised queries of many tokens go through the 4-bit cache's row kernel, in a
-// launch of their own: half the lanes per row and a warp per few heads instead of
-// one per token (7 prompt chunks, 64 query heads of 128, BF16, with the pages read
-// back: 114 us by one launch, 72 by two; 62 with fewer heads per CTA).
+// Normalised queries of many tokens go through the 4-bit cache's row
+// kernel, in a launch of their own: half the lanes per row and a warp per few heads
+// instead of one per token. us by one launch and by two, BF16 with rotation, in a
+// graph: 64 query and 8 KV heads of 128, 300 tokens 53, 12; 1000 61, 22; 5000 104,
+// 88. 16 and 8 of 256: 22, 10; 28, 19; 74, 74. 32 and 8 of 64: 56, 14; 67, 17; 104,
+// 59. With fewer tokens the second launch costs an eager call 2 us of the host's time
+// (16 heads of 256, 256 tokens: 21.7, 23.9), which it wins back in a graph or with
+// many heads only (64 heads of 128, 256 tokens: in a graph 29, 15; eager 28.6, 23.9).
 template <typename T, int KIND>
 cudaError_t launch_append_normed(const AppendArgs& a, cudaStream_t stream) {
   if (!a.q_norm.weight && !a.k_norm.weight) return launch_append_kind<T, KIND, false>(a, stream);
