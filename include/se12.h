@@ -390,8 +390,11 @@ int se12_encode_raw(const uint16_t* w_dev, int rows, int cols, int ldw, const in
  *   k_scales: [pages][kv_heads][page_size][groups][scale, offset] fp16
  *   v_scales: [pages][kv_heads][page_size / 16] cells of 32 * groups + 16 fp16:
  *             [8 pairs of tokens][groups scales, groups offsets][2 tokens], [16] E
- * both 16-byte aligned, scales and offsets of values finite, E a whole number
- * from -30 to 30, or NaN (the token's values are).
+ * both 16-byte aligned. (u - 8) * scale + offset is in FP16's range for every u,
+ * scales of values are finite and below 128 and their offsets finite, also where
+ * no row looks; E is a whole number from -30 to 30, or NaN (the token's values are).
+ * Keys have no E: a group whose values differ by less than 2^-10 keeps fewer bits,
+ * by less than 2^-21 its offset alone, and offsets end at 2^-24.
  */
 #define SE12_KV_INT8 0
 #define SE12_KV_E4M3 1
@@ -468,7 +471,8 @@ int se12_kv_append(const se12_kv_cache* cache, const se12_kv_batch* batch, const
 
 /* The same with norms of the queries and keys of each head before the
  * rotation: a row x becomes x / sqrt(mean(x^2) + eps) * weight, its squares
- * summed in 64 bits. A null weight, or norms null: none for those rows. */
+ * summed in 64 bits (where a checkpoint multiplies by 1 + w, pass 1 + w). A null
+ * weight, or norms null: none for those rows. */
 typedef struct se12_kv_norms {
   const void* q_weight;        /* device [head_dim], fp32 or BF16 */
   const void* k_weight;

@@ -118,8 +118,14 @@ class PagedKvCache:
     page_size / 16, 32 * groups + 16]: of 16 tokens, for each two neighbours
     the groups' scales and then their offsets (the two tokens' side by side),
     then a whole number E per token, -30 to 30: its values are 2^E times what
-    scale and offset give. Scales and offsets of values are finite; E is NaN for
-    a token whose values were not."""
+    scale and offset give. E is NaN for a token whose values are not finite or
+    reach 2^34, a key group's scale and offset where it is not finite or passes
+    65000. Keys have no E: a group whose values differ by less than 2^-10 keeps
+    fewer bits, by less than 2^-21 its offset alone, and offsets end at 2^-24.
+
+    Attention takes any scales and offsets (``from_tensors``) with which every
+    code's (u - 8) * scale + offset is in FP16's range, values' scales below 128;
+    those of hidden values have to be finite too."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, kind: str = "int8", device="cuda"):
         self._check(pages, page_size, kv_heads, head_dim, kind)
@@ -266,7 +272,8 @@ class PagedKvCache:
         ``q_norm`` and ``k_norm`` (fp32 or BF16 [head_dim] weights) normalise
         each head's queries or keys before that: x / sqrt(mean(x^2) +
         ``norm_eps``) * weight, in fp32 (the mean from 64-bit sums) without a
-        rounding in between."""
+        rounding in between. (Of a checkpoint whose norms multiply by 1 + w the
+        caller passes 1 + w.)"""
         dtype = k.dtype
         k_strides = self._row_strides(k, "k", self.kv_heads, None, _FLOATS)
         tokens = k.shape[0]

@@ -223,3 +223,34 @@ def test_several_tiles_of_few_rows(dim, group, n, pattern, softcap, window):
     f = Sized(g, 16 if dim == 256 else 64, 2, dim, [sizes(pattern, g, max(length, n)) for length in (700, 61, 17, n)])
     q = (2 * torch.randn(sum(counts), 2 * group, dim, generator=g)).to(torch.bfloat16)
     f.check(q, counts, f.attend(q, counts, softcap=softcap, window=window), softcap, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 70])
+def test_the_largest_scales_and_offsets(dim, n):
+    """Of tensors that append did not write: scales up to 128, offsets beside which
+    the codes stay in FP16's range, and weights up to 2^8 of the reference."""
+    g = torch.Generator().manual_seed(dim + n)
+    length = 300
+    f = Sized(g, 16, 1, dim, [torch.zeros(length)])
+    ids = f.table[0].long()
+    plain = f.plain
+    plain.scale["v"][ids] = (127.9 * torch.rand(plain.scale["v"][ids].shape, generator=g) ** 4).half()
+    plain.offset["v"][ids] = (30000 * (2 * torch.rand(plain.offset["v"][ids].shape, generator=g) - 1)).half()
+    plain.e[ids] = -12.0
+    # the first tokens' logits are 5 below the rest: weights pass the reference without raising it
+    plain.u["k"][ids[0]], plain.scale["k"][ids[0]] = 8, 0
+    plain.offset["k"][ids[0]] = -5 * dim**-0.5
+    plain.u["k"][ids[1:]], plain.scale["k"][ids[1:]], plain.offset["k"][ids[1:]] = 8, 0, 0
+    flat = lambda t: t[ids, 0].flatten(0, 1)[:length]  # noqa: E731
+    power = 2.0**-12
+    f.k[0][0] = flat(plain.values("k"))
+    steps = (flat(plain.u["v"]).double().unflatten(-1, (-1, GROUP)) - 8) * flat(plain.scale["v"]).double()[..., None]
+    f.s[0][0] = steps.flatten(-2) * power
+    f.o[0][0] = flat(plain.offset["v"]).double().repeat_interleave(GROUP, -1) * power
+    f.step[0][0] = flat(plain.scale["v"]).double().repeat_interleave(GROUP, -1) * power
+    f.e[0][0] = -12.0
+    f.cache = type(f.cache).from_tensors(*(t.cuda() for t in plain.tensors()), "int4")
+    q = torch.ones(n, 2, dim).to(torch.bfloat16)
+    f.check(q, [n], f.attend(q, [n]))
